@@ -288,6 +288,88 @@ int tessera_hip_attend_step(const ts_step_args *a, void *stream);
 int tessera_hip_flash_rows(const ts_rows_args *a, void *stream);
 
 /* ----------------------------------------------------------------------------
+ * Kept blocks: kept rows in 8 bits. A block is 16 positions of one kv head, e4m3 codes times
+ * a power of two 2^e (-100 <= e <= 119) for K and another for V:
+ *   k       [pages * page / 16][kv_heads][16 positions][width] codes
+ *   v       [pages * page / 16][kv_heads][width][16 positions] codes
+ *   scales  [pages * page / 16][kv_heads rounded up to even][2] f32, K's then V's
+ * The key at position j of slot s is position j % 16 of block
+ * table[s * kept_pages + (j >> log2 page)] * (page / 16) + j % page / 16, or of block
+ * (s * keys + j) / 16 when kept_table is NULL (keys a multiple of 16). Pages copy whole
+ * (tessera_hip_kv_copy with page = 1 and a page's bytes as the row).
+ * No counterpart in the reference, whose kept rows are bf16.
+ * ------------------------------------------------------------------------- */
+
+/* Device-side refusals beside TS_STATUS_POSITION (`status` of the calls below). */
+#define TS_STATUS_PAGE 4u   /* a slot >= slot_count, or a table entry >= pages */
+#define TS_STATUS_TWICE 8u  /* rows of one call that meet in a block and do not stand together */
+
+/* New rows into the kept rows: q and k through RmsNorm per head (q_gain / k_gain, or neither
+ * where the gain is NULL) and the rotation of their position (pairs (j, j + width / 2), or
+ * (2j, 2j + 1) without `halves`; no rotation where rope_table is NULL), q to q_out; k and v
+ * kept at (slot, position), in bf16 rows (as tessera_hip_qk_norm_rope_append keeps them) or in
+ * e4m3 blocks:
+ *  - A call that writes a block's first position starts the block: its scales are the least
+ *    powers of two that hold the call's values of it (amax <= 448 * 2^e, over finite values),
+ *    and positions that the call does not write keep their bytes and mean nothing.
+ *  - Any other call lets a block's scales only grow, and moves the codes already there to the
+ *    grown scale (exact, but for codes that turn subnormal). What a block holds thus depends on
+ *    how its positions were divided among calls.
+ *  - Codes are rounded to nearest even; infinities and NaN become NaN codes and take no part in
+ *    the scale; values past 448 * 2^119 become the largest.
+ *  - Rows of one call that fall into one block (16 positions of a slot) stand together and in
+ *    order; a later run of rows of the same block is kept nowhere and sets TS_STATUS_TWICE. Two
+ *    slots of a call never share the page they append to (Pool::grow sees to it).
+ *  - A row past its slot's positions is kept nowhere (its q is NaN) and sets
+ *    TS_STATUS_POSITION, one whose page the buffers do not hold TS_STATUS_PAGE.
+ * No counterpart in the reference (its append follows separate norm and rotation stages,
+ * engine/models/src/shared.rs:109-145, engine/ir/interp/src/run.rs:122-198). */
+typedef struct {
+    const void *q, *k, *v;         /* rows; q may be NULL: only k and v */
+    const float *q_gain, *k_gain;  /* [width] or NULL */
+    const float *rope_table;       /* [rope_rows][width / 2][2] (cos, sin), or NULL */
+    void *q_out;                   /* [rows, heads, width]; may be q where that is laid out so */
+    void *k_kept, *v_kept;
+    float *scales;                 /* e4m3 blocks only */
+    const uint32_t *slots, *positions; /* [rows] */
+    const uint32_t *kept_table;    /* [slot_count * kept_pages], or NULL for dense */
+    uint32_t *status;              /* device word or NULL: TS_STATUS_* bits are OR-ed in */
+    uint32_t rows, heads, kv_heads;
+    uint32_t width;                /* 128 */
+    uint32_t q_stride, k_stride, v_stride; /* elements from a row to the next, whole 16-byte pieces */
+    uint32_t keys;                 /* positions a slot may hold */
+    uint32_t slot_count, kept_pages;
+    uint32_t page, pages;          /* rows a page (power of two >= 16), pages the kept rows hold */
+    uint32_t rope_rows;            /* >= keys */
+    int32_t halves;
+    int32_t x_dtype, q_out_dtype;  /* f32 or bf16 */
+    int32_t kv_dtype;              /* TS_BF16 rows or TS_E4M3 blocks */
+    float eps;
+} ts_append_args;
+int tessera_hip_append_rows(const ts_append_args *a, void *stream);
+
+/* Ragged-row attention over kept blocks: attend_rows' and flash_rows' semantics (row r sees keys
+ * [max(0, p - back), p] of its slot), q f32 or bf16, out f32 or bf16. rows.k, rows.v: the
+ * blocks; rows.kv_dtype TS_E4M3. Codes enter the products exactly, times their scale; sums and
+ * softmax in f32; f32 q and, with f32 q, the softmax weights enter as two bf16 parts, with bf16 q
+ * the weights as one.
+ *  - `run`: how many rows of a slot stand together (1: a decode step; the drafted rows of a
+ *    sequence; a prompt chunk's rows; an average serves for ragged ones). It decides how rows are
+ *    grouped and which kernel runs, never what is computed.
+ *  - Refused rows (a position as for attend_rows; a slot >= slot_count; a page >= pages among the
+ *    row's keys) write NaN and set their status bit.
+ *  - A NaN among a row's own keys reaches that row alone; codes past a sequence's last position
+ *    may be anything.
+ * At most 64 q heads a kv head. */
+typedef struct {
+    ts_rows_args rows;
+    const float *scales;
+    uint32_t slot_count, pages, run;
+} ts_kept8_args;
+int tessera_hip_attend_kept8(const ts_kept8_args *a, void *stream);
+size_t tessera_hip_attend_kept8_workspace(const ts_kept8_args *a);
+
+/* ----------------------------------------------------------------------------
  * Elementwise chains not fused into a product.
  * out[i] = chain(x[i], operands at i) for i < len, with `after` as above (read
  * `after.sum` is x; operands with spans repeat). out may alias x or an operand.
@@ -476,6 +558,47 @@ typedef struct {
     uint32_t rows, width, k;
 } ts_top_k_args;
 int tessera_hip_top_k(const ts_top_k_args *a, void *stream);
+
+/* Verification of drafted tokens. Sequence s has counts[s] drafts (at most `most`) and
+ * counts[s] + 1 rows of target logits, first[s] .. first[s] + counts[s] (row t: the
+ * distribution at draft t; the last: after every draft).
+ *  p_t = softmax(logits_t / temperature), q_t the drafter's probabilities (draft_probs, or 1 at
+ *  the drafted token when NULL).
+ *  - Drafts are taken from the first on while u[s, t] * q_t(draft) < p_t(draft); accepted[s] is
+ *    how many.
+ *  - The token after them is picked by u[s, most]: after a refused draft from max(p_t - q_t, 0)
+ *    (from p_t, should that be zero everywhere), after the last draft from p: the first index
+ *    whose running sum, in index order, exceeds u times the whole.
+ *  - temperature <= 0 (or NaN), or uniforms NULL: greedy. Drafts are taken while they are
+ *    tessera_hip_argmax's pick of their row, and the next token is that pick.
+ *  tokens[s]: the accepted drafts, the picked token, then `width` in the rest.
+ * NaN and -inf logits have probability 0; a row of nothing else refuses its draft and picks
+ * `width`. +inf logits share the whole. Probabilities of the drafter that are NaN or negative
+ * count as 0. A sequence with counts[s] > most or rows past `rows` gets accepted 0 and `width`
+ * throughout, and sets TS_STATUS_POSITION. Exponentials and sums are in f64: over a vocabulary
+ * of 150,000 the running sum's borders in f32 would move by more than they are apart.
+ * No counterpart in the reference (its engine decodes greedily, one token a step,
+ * engine/engine/src/lib.rs:401-470). */
+typedef struct {
+    const void *logits;          /* [rows, width], `stride` elements apart */
+    const uint32_t *drafts;      /* [seqs, most] */
+    const float *uniforms;       /* [seqs, most + 1] in [0, 1), or NULL: greedy */
+    const float *draft_probs;    /* [seqs, most, width], or NULL */
+    const float *temperatures;   /* [seqs], or NULL: `temperature` for all */
+    const uint32_t *counts;      /* [seqs], or NULL: `most` each */
+    const uint32_t *first;       /* [seqs], or NULL: s * (most + 1) */
+    uint32_t *tokens;            /* [seqs, most + 1] */
+    uint32_t *accepted;          /* [seqs] */
+    void *workspace;
+    size_t workspace_bytes;
+    uint32_t *status;            /* device word or NULL */
+    uint32_t seqs, most, rows, width;
+    uint32_t stride;             /* elements from a row of logits to the next, >= width */
+    int32_t logits_dtype;        /* f32 or bf16 */
+    float temperature;
+} ts_verify_args;
+int tessera_hip_verify(const ts_verify_args *a, void *stream);
+size_t tessera_hip_verify_workspace(const ts_verify_args *a);
 
 #ifdef __cplusplus
 }

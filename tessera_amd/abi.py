@@ -21,6 +21,8 @@ TS_ERR_ARCH = -2
 TS_ERR_WORKSPACE = -3
 
 TS_STATUS_POSITION = 1  # ts_rows_args.status: a row's position was refused
+TS_STATUS_PAGE = 4      # a slot or a page that the kept rows do not hold
+TS_STATUS_TWICE = 8     # rows of one append that meet in a block without standing together
 
 TS_F32, TS_BF16, TS_E4M3, TS_U32 = 0, 1, 2, 3
 TS_Q8_0, TS_MXFP8, TS_INT4_G32, TS_Q4_0 = 4, 5, 6, 7  # block forms (engine/ir/mem/src/block.rs:251-291)
@@ -136,6 +138,21 @@ StepArgs = _args("StepArgs", "ts_step_args", [
     ("rows", RowsArgs), ("qkv", _v), ("q_gain", _v), ("k_gain", _v), ("rope_table", _v),
     ("rope_rows", _u), ("eps", _f)])
 
+AppendArgs = _args("AppendArgs", "ts_append_args", [
+    ("q", _v), ("k", _v), ("v", _v), ("q_gain", _v), ("k_gain", _v), ("rope_table", _v), ("q_out", _v),
+    ("k_kept", _v), ("v_kept", _v), ("scales", _v), ("slots", _v), ("positions", _v), ("kept_table", _v),
+    ("status", _v), ("rows", _u), ("heads", _u), ("kv_heads", _u), ("width", _u), ("q_stride", _u),
+    ("k_stride", _u), ("v_stride", _u), ("keys", _u), ("slot_count", _u), ("kept_pages", _u), ("page", _u),
+    ("pages", _u), ("rope_rows", _u), ("halves", C.c_int32), ("x_dtype", C.c_int32),
+    ("q_out_dtype", C.c_int32), ("kv_dtype", C.c_int32), ("eps", _f)])
+Kept8Args = _args("Kept8Args", "ts_kept8_args", [
+    ("rows", RowsArgs), ("scales", _v), ("slot_count", _u), ("pages", _u), ("run", _u)])
+VerifyArgs = _args("VerifyArgs", "ts_verify_args", [
+    ("logits", _v), ("drafts", _v), ("uniforms", _v), ("draft_probs", _v), ("temperatures", _v), ("counts", _v),
+    ("first", _v), ("tokens", _v), ("accepted", _v), ("workspace", _v), ("workspace_bytes", C.c_size_t),
+    ("status", _v), ("seqs", _u), ("most", _u), ("rows", _u), ("width", _u), ("stride", _u),
+    ("logits_dtype", C.c_int32), ("temperature", _f)])
+
 
 _P = C.c_void_p
 _U = C.c_uint32
@@ -175,6 +192,11 @@ SIGNATURES = {
     "tessera_hip_map": (C.c_int, [C.POINTER(MapArgs), _P]),
     "tessera_hip_flash": (C.c_int, [C.POINTER(FlashArgs), _P]),
     "tessera_hip_pack_f32": (C.c_int, [C.POINTER(PackArgs), _P]),
+    "tessera_hip_append_rows": (C.c_int, [C.POINTER(AppendArgs), _P]),
+    "tessera_hip_attend_kept8": (C.c_int, [C.POINTER(Kept8Args), _P]),
+    "tessera_hip_attend_kept8_workspace": (C.c_size_t, [C.POINTER(Kept8Args)]),
+    "tessera_hip_verify": (C.c_int, [C.POINTER(VerifyArgs), _P]),
+    "tessera_hip_verify_workspace": (C.c_size_t, [C.POINTER(VerifyArgs)]),
 }
 
 

@@ -1,0 +1,568 @@
+// Attention over kept blocks (kept8.h): decode rows, several drafted rows of a sequence, prompts.
+//
+// Row r (slot s, position p) sees the keys at [max(0, p - back), p] of its slot: w = softmax(q . k *
+// scale), out = sum of w v (engine/ir/interp/src/cpu.rs:293-351 over bf16 rows; no counterpart in the
+// reference for blocks).
+//
+// A tile is the q heads of one kv head for R rows that stand together, its (row, head) pairs the columns
+// of 16-wide matrix products: S^T = K q^T and O^T = V^T P^T, so the scores of a column stay in its
+// lanes and P^T is the second product's operand as it stands. Each wave takes steps of 64 keys, four
+// blocks:
+//  * K: tile t of the four 16-key tiles takes positions 4t .. 4t + 3 of each block, so that a lane's
+//    16 scores are the 16 positions of one block (block lane / 16), the order V's operand has them in.
+//    A lane reads 16 bytes of a key (d 64 s + 16 (lane / 16) ..), two operands' worth.
+//  * V: 16 bytes are the 16 positions of one d of block lane / 16, again two operands.
+//  Nothing passes through LDS: codes go from memory to registers, through the conversion that applies
+//  the block's scale, into the matrix unit; the next step's are asked for as soon as this step's are used.
+//  The four waves of a group, and the groups that share a tile's keys, are joined by their maxima and
+//  sums, the former in LDS, the latter by a second kernel.
+#include <algorithm>
+
+#include "kept8.h"
+
+namespace {
+
+using namespace kept8;
+
+constexpr uint32_t kStep = 64;           // keys a wave takes at a time
+constexpr uint32_t kWaves = 4;
+constexpr uint32_t kRound = kStep * kWaves;
+constexpr uint32_t kPart = 132;          // floats of a column's partial result: max, sum, 2 unused, 128
+constexpr float kSlack = 8.0f;           // base-2 headroom of the softmax reference point
+
+struct AttendParams {
+    const void *q;
+    const uint8_t *k, *v;
+    const float *scales;
+    void *out;
+    float *partials;  // [tile][kv head][part][16 NT][kPart], or NULL: one part
+    const uint32_t *slots, *positions;
+    uint32_t *status;
+    Place place;
+    uint32_t rows, heads, kv_heads, group, back, max_position;
+    uint32_t tile_rows, chunk, parts;  // rows a tile; keys of a part at a time (a multiple of kRound)
+    float scale;
+    int out_bf16;
+};
+
+TS_DEV float rows4_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+TS_DEV float rows4_max(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+TS_DEV void store4(const AttendParams &p, size_t at, f32x4 v) {
+    if (p.out_bf16)
+        *(u32x2 *)((uint16_t *)p.out + at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    else
+        *(f32x4 *)((float *)p.out + at) = v;
+}
+
+// Bytes of a word of four positions pos .. pos + 3 that lie in [lo, hi].
+TS_DEV uint32_t within4(uint32_t w, uint32_t pos, uint32_t lo, uint32_t hi) {
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) m |= (pos + i >= lo && pos + i <= hi) ? 0xffu << (8 * i) : 0u;
+    return w & m;
+}
+
+// The place of a step's block: its page looked up, or the page's own row of a dense slot.
+struct BlockAt {
+    uint32_t block;
+    bool ok;
+};
+TS_DEV BlockAt block_at(const Place &p, uint32_t slot, uint32_t block) {
+    uint64_t row;
+    const bool ok = row_of(p, slot, block * kBlock, row);
+    return {(uint32_t)(row / kBlock), ok};
+}
+
+template <int NT, bool QF32>
+__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(AttendParams p) {
+    constexpr uint32_t kCols = 16 * NT, kParts = QF32 ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) float joined[];  // [kWaves][kCols][kPart]
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t col = lane & 15, grp = lane >> 4;
+    const uint32_t part = blockIdx.x % p.parts, gi = blockIdx.x / p.parts;
+    const uint32_t kvh = gi % p.kv_heads, tile = gi / p.kv_heads, G = p.group;
+
+    // Columns: (row, head) pairs of the tile, row by row.
+    uint32_t pos[NT], from[NT], slot[NT];
+    bool live[NT];
+    bf16x8 q[NT][4][kParts];
+    const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes into q, exactly
+    const float sl = p.scale == 0.0f ? 0x1p-100f : fabsf(p.scale) * 1.4426950408889634f;  // to base 2
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const uint32_t c = 16 * nt + col, ri = c / G, r = tile * p.tile_rows + ri;
+        const bool there = ri < p.tile_rows && r < p.rows;
+        pos[nt] = there ? p.positions[r] : 0;
+        slot[nt] = there ? p.slots[r] : 0;
+        live[nt] = there && pos[nt] <= p.max_position && holds(p.place, slot[nt], pos[nt]);
+        if (there && !live[nt] && p.status && part == 0 && kvh == 0 && wave == 0 && grp == 0)
+            atomicOr(p.status, slot[nt] >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
+        from[nt] = pos[nt] > p.back ? pos[nt] - p.back : 0;
+        const size_t at = ((size_t)(live[nt] ? r : 0) * p.heads + kvh * G + (live[nt] ? c % G : 0)) * 128;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {  // operand j: d 64 (j / 2) + 16 grp + 8 (j % 2) ..
+            const uint32_t d = 64 * (j >> 1) + 16 * grp + 8 * (j & 1);
+            if (!QF32) {
+                u32x4 w = *(const u32x4 *)((const uint16_t *)p.q + at + d);
+                w = live[nt] ? w ^ qsign : u32x4{0, 0, 0, 0};
+                q[nt][j][0] = as_bf16x8(w);
+            } else {
+                const f32x4 x = *(const f32x4 *)((const float *)p.q + at + d);
+                const f32x4 y = *(const f32x4 *)((const float *)p.q + at + d + 4);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float a = e < 2 ? x[2 * e] : y[2 * e - 4], b = e < 2 ? x[2 * e + 1] : y[2 * e - 3];
+                    if (qsign) { a = -a; b = -b; }
+                    if (!live[nt]) a = b = 0.0f;
+                    const float ha = bf16_round(a), hb = bf16_round(b);
+                    hi[e] = pack_bf16x2(ha, hb);
+                    lo[e] = pack_bf16x2(a - ha, b - hb);
+                }
+                q[nt][j][0] = as_bf16x8(u32x4{hi[0], hi[1], hi[2], hi[3]});
+                q[nt][j][kParts - 1] = as_bf16x8(u32x4{lo[0], lo[1], lo[2], lo[3]});
+            }
+        }
+    }
+
+    float m[NT], l[NT];
+    f32x4 o[NT][8];  // O^T: lane's column, d 16 dt + 4 grp + i
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 8; dt++) o[nt][dt] = f32x4{0, 0, 0, 0};
+    }
+    bool worked = false;
+
+    // A pass over the keys for each slot among the columns (one, where rows of a slot stand together).
+    bool wait[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) wait[nt] = live[nt];
+    for (;;) {
+        uint32_t now = 0;
+        bool any = false;
+#pragma unroll
+        for (int nt = NT - 1; nt >= 0; nt--) {
+            const uint64_t b = __builtin_amdgcn_ballot_w64(wait[nt]);
+            if (b) {
+                now = __builtin_amdgcn_readlane(slot[nt], __builtin_ctzll(b));
+                any = true;
+            }
+        }
+        if (!any) break;
+        bool act[NT];
+        uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            act[nt] = wait[nt] && slot[nt] == now;
+            wait[nt] = wait[nt] && !act[nt];
+            if (act[nt]) {
+                lo = min(lo, from[nt]);
+                hi = max(hi, pos[nt]);
+            }
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+            lo = min(lo, (uint32_t)__shfl_xor((int)lo, x, 64));
+            hi = max(hi, (uint32_t)__shfl_xor((int)hi, x, 64));
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock;
+        bool lost = false, gone = false;  // the lane's block of this step, or of any, is on a page not held
+
+        // Step i of this wave: the keys from step_base(i) on; parts take chunks in turn.
+        const uint32_t per = p.chunk / kRound;
+        auto step_off = [&](uint32_t i) -> uint64_t {
+            return ((uint64_t)(i / per) * p.parts + part) * p.chunk + (i % per) * kRound + wave * kStep;
+        };
+        uint32_t i = 0;
+        // The first step at or after i that begins within the keys (chunks ascend; none: done).
+        auto inside_keys = [&](uint32_t i) { return step_off(i) <= hi - base0; };
+        u32x4 kf[4][2], vf[8];
+        float ks = 0.0f, vs = 0.0f;
+        auto load_k = [&](uint32_t base) {
+            const BlockAt b = block_at(p.place, now, min(base / kBlock + (col >> 2), last));
+            ks = p.scales[((size_t)b.block * scale_heads(p.kv_heads) + kvh) * 2];
+            const uint8_t *at = p.k + ((size_t)b.block * p.kv_heads + kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) kf[t][s] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * s);
+        };
+        auto load_v = [&](uint32_t base) {
+            const BlockAt b = block_at(p.place, now, min(base / kBlock + grp, last));
+            lost = !b.ok;
+            vs = p.scales[((size_t)b.block * scale_heads(p.kv_heads) + kvh) * 2 + 1];
+            const uint8_t *at = p.v + ((size_t)b.block * p.kv_heads + kvh) * kBlockBytes + col * kBlock;
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++) vf[dt] = *(const u32x4 *)(at + dt * 16 * kBlock);
+        };
+        if (inside_keys(0)) {
+            worked = true;
+            load_k(base0 + (uint32_t)step_off(0));
+            load_v(base0 + (uint32_t)step_off(0));
+        } else if (step_off(0) - wave * kStep <= hi - base0) {
+            worked = true;  // another wave of the group
+        }
+        for (; inside_keys(i); i++) {
+            const uint32_t base = base0 + (uint32_t)step_off(i);
+            const bool more = inside_keys(i + 1);
+            const uint32_t next = more ? base0 + (uint32_t)step_off(i + 1) : 0;
+            f32x4 s[4][NT];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) s[t][nt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const u32x4 w = kf[t][j >> 1];
+                    const bf16x8 kc = codes8(j & 1 ? w.z : w.x, j & 1 ? w.w : w.y, ks);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (uint32_t e = 0; e < kParts; e++) s[t][nt] = mfma16(kc, q[nt][j][e], s[t][nt]);
+                }
+            }
+            if (more) load_k(next);
+            if (__builtin_amdgcn_ballot_w64(lost) != 0) {  // a page that the buffers do not hold: NaN scores
+                gone |= lost;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[t][nt][e] = lost ? __builtin_nanf("") : s[t][nt][e];
+            }
+
+            // A step wholly inside every column's window skips the masks.
+            bool inside = true;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                inside &= act[nt] ? (base + kStep - 1 <= pos[nt] && base >= from[nt]) : !live[nt];
+            inside = __builtin_amdgcn_ballot_w64(!inside) == 0;
+            uint32_t seen[NT];  // a bit for each of the lane's 16 keys
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) seen[nt] = 0xffffu;
+            if (!inside) {
+                const uint32_t key0 = base + kBlock * grp;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    seen[nt] = 0;
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t key = key0 + 4 * t + e;
+                            const bool ok = act[nt] & (key <= pos[nt]) & (key >= from[nt]);
+                            s[t][nt][e] = ok ? s[t][nt][e] : -INFINITY;
+                            seen[nt] |= ok ? 1u << (4 * t + e) : 0u;
+                        }
+                }
+                // Codes outside [lo, hi] may be anything: as zeros they add nothing.
+#pragma unroll
+                for (int dt = 0; dt < 8; dt++)
+                    vf[dt] = u32x4{within4(vf[dt].x, key0, lo, hi), within4(vf[dt].y, key0 + 4, lo, hi),
+                                   within4(vf[dt].z, key0 + 8, lo, hi), within4(vf[dt].w, key0 + 12, lo, hi)};
+            }
+            bf16x8 w[NT][2][kParts];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float mx = s[0][nt][0];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[t][nt][e]);
+                mx = rows4_max(mx) * sl;
+                // The reference point moves only when a score passes it by 2^kSlack: most steps leave
+                // the sums and O unscaled, and no weight passes 2^kSlack.
+                const bool raise = mx > m[nt] + kSlack;
+                const float mn = raise ? mx : m[nt];
+                const float alpha = raise ? __builtin_amdgcn_exp2f(m[nt] - mn) : 1.0f;
+                const float mo = mn == -INFINITY ? 0.0f : mn;
+                float sum = 0.0f;
+                uint32_t hw[8], lw[8];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float a = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e], sl, -mo));
+                        const float b = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e + 1], sl, -mo));
+                        sum += a + b;
+                        hw[2 * t + e / 2] = pack_bf16x2(a, b);
+                        if (QF32)
+                            lw[2 * t + e / 2] = pack_bf16x2(a - lo_bf16(hw[2 * t + e / 2]), b - hi_bf16(hw[2 * t + e / 2]));
+                    }
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    w[nt][x][0] = as_bf16x8(u32x4{hw[4 * x], hw[4 * x + 1], hw[4 * x + 2], hw[4 * x + 3]});
+                    if (QF32) w[nt][x][kParts - 1] = as_bf16x8(u32x4{lw[4 * x], lw[4 * x + 1], lw[4 * x + 2], lw[4 * x + 3]});
+                }
+                l[nt] = l[nt] * alpha + rows4_sum(sum);
+                m[nt] = mn;
+                if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+#pragma unroll
+                    for (int dt = 0; dt < 8; dt++) o[nt][dt] *= alpha;
+                }
+            }
+            // A NaN code at a key that some columns see and some do not: a weight of 0 times NaN must
+            // not reach the latter. Such codes become 0, and what they reach is marked by a product of
+            // (code is NaN) with (column sees the key).
+            if (!inside) {
+                uint32_t nan = 0;
+#pragma unroll
+                for (int dt = 0; dt < 8; dt++)
+                    nan |= nan_codes(vf[dt].x) | nan_codes(vf[dt].y) | nan_codes(vf[dt].z) | nan_codes(vf[dt].w);
+                if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+#pragma unroll
+                    for (int dt = 0; dt < 8; dt++) {
+                        uint32_t ones[4];  // e4m3 1.0 (0x38) at each NaN code
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t b = nan_codes(vf[dt][e]) >> 7;
+                            ones[e] = b * 0x38u;
+                            vf[dt][e] &= ~(b * 0xffu);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            f32x4 hit = f32x4{0, 0, 0, 0};
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                uint32_t sw[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t two = seen[nt] >> (8 * x + 2 * e);
+                                    sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
+                                }
+                                hit = mfma16(codes8(ones[2 * x], ones[2 * x + 1], 1.0f),
+                                             as_bf16x8(u32x4{sw[0], sw[1], sw[2], sw[3]}), hit);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (hit[e] > 0.0f) o[nt][dt][e] = __builtin_nanf("");
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const bf16x8 vc = codes8(x ? vf[dt].z : vf[dt].x, x ? vf[dt].w : vf[dt].y, vs);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (uint32_t e = 0; e < kParts; e++) o[nt][dt] = mfma16(vc, w[nt][x][e], o[nt][dt]);
+                }
+            if (more) load_v(next);
+        }
+        if (p.status && __builtin_amdgcn_ballot_w64(gone) != 0 && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+    }
+
+    // The waves' results joined, a thread four d of a column at a time.
+    float *mine = p.partials ? p.partials + ((size_t)gi * p.parts + part) * kCols * kPart : nullptr;
+    if (mine && !worked) {  // nothing to join (uniform over the group)
+        for (uint32_t c = threadIdx.x; c < kCols; c += 256) {
+            mine[c * kPart] = -INFINITY;
+            mine[c * kPart + 1] = 0.0f;
+        }
+        return;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float *at = joined + (wave * kCols + 16 * nt + col) * kPart;
+        if (grp == 0) {
+            at[0] = m[nt];
+            at[1] = live[nt] ? l[nt] : __builtin_nanf("");  // a refused column passed unmasked with the others
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[nt][dt];
+    }
+    __syncthreads();
+    const uint32_t used = min(p.tile_rows, p.rows - tile * p.tile_rows) * G;
+    for (uint32_t e = threadIdx.x; e < used * 32; e += 256) {
+        const uint32_t c = e / 32, d = e % 32 * 4;
+        float M = -INFINITY;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) M = fmaxf(M, joined[(w * kCols + c) * kPart]);
+        float L = 0.0f;
+        f32x4 O = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) {
+            const float *at = joined + (w * kCols + c) * kPart;
+            const float f = at[0] == -INFINITY ? (at[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(at[0] - M);
+            L += at[1] * f;
+            O += *(const f32x4 *)(at + 4 + d) * f;
+        }
+        if (mine) {
+            if (d == 0) {
+                mine[c * kPart] = M;
+                mine[c * kPart + 1] = L;
+            }
+            *(f32x4 *)(mine + c * kPart + 4 + d) = O;
+        } else {
+            const size_t r = tile * p.tile_rows + c / G;
+            store4(p, (r * p.heads + kvh * G + c % G) * 128 + d, O / L);  // 0 / 0 of a refused row: NaN
+        }
+    }
+}
+
+// The parts of a tile's columns joined in their order, a thread four d of a column.
+__global__ __launch_bounds__(64) void join_kept8_kernel(AttendParams p, uint32_t cols, uint32_t pieces) {
+    const uint32_t gi = blockIdx.x / pieces, kvh = gi % p.kv_heads, tile = gi / p.kv_heads, G = p.group;
+    const uint32_t used = min(p.tile_rows, p.rows - tile * p.tile_rows) * G;
+    const uint32_t c = blockIdx.x % pieces * 2 + threadIdx.x / 32, d = threadIdx.x % 32 * 4;
+    if (c >= used) return;
+    const float *all = p.partials + ((size_t)gi * p.parts * cols + c) * kPart;
+    const size_t next = (size_t)cols * kPart;
+    constexpr uint32_t kBatch = 8;
+    float M = -INFINITY;
+    for (uint32_t j0 = 0; j0 < p.parts; j0 += kBatch) {
+        float mq[kBatch];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) mq[j] = all[min(j0 + j, p.parts - 1) * next];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) M = fmaxf(M, mq[j]);
+    }
+    float L = 0.0f;
+    f32x4 O = f32x4{0, 0, 0, 0};
+    for (uint32_t j0 = 0; j0 < p.parts; j0 += kBatch) {
+        float mq[kBatch], lq[kBatch];
+        f32x4 oq[kBatch];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) {  // past the end: read, not used
+            const float *at = all + min(j0 + j, p.parts - 1) * next;
+            mq[j] = at[0];
+            lq[j] = at[1];
+            oq[j] = *(const f32x4 *)(at + 4 + d);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) {
+            // An empty part (max -inf, sum 0) has no O.
+            if (j0 + j >= p.parts || (mq[j] == -INFINITY && lq[j] == 0.0f)) continue;
+            const float f = mq[j] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mq[j] - M);
+            L += lq[j] * f;
+            O += oq[j] * f;
+        }
+    }
+    const size_t r = tile * p.tile_rows + c / G;
+    store4(p, (r * p.heads + kvh * G + c % G) * 128 + d, O / L);
+}
+
+struct Plan {
+    uint32_t tile_rows, nt, tiles, parts, chunk;
+};
+
+Plan plan(const ts_kept8_args *k) {
+    const ts_rows_args *a = &k->rows;
+    const uint32_t G = a->heads / a->kv_heads;
+    Plan s;
+    const uint32_t most = std::max(1u, 64 / G);  // rows that 64 columns take
+    const uint32_t run = std::max(1u, std::min(k->run, a->rows));
+    s.tile_rows = std::min(run, most);
+    const uint32_t cols = s.tile_rows * G;
+    s.nt = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
+    s.tiles = (a->rows + s.tile_rows - 1) / s.tile_rows;
+    // Keys are split into parts until the groups cover the chip about twice over (four waves of two a
+    // SIMD, 512 groups at a time), a part no less than one round of a group's waves.
+    const uint64_t groups = (uint64_t)s.tiles * a->kv_heads;
+    const uint64_t span = std::min<uint64_t>((uint64_t)a->max_position + 1, (uint64_t)a->back + s.tile_rows + kBlock);
+    const uint64_t rounds = (span + kRound - 1) / kRound;
+    s.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rounds, (1024 + groups - 1) / groups));
+    s.chunk = (uint32_t)((rounds + s.parts - 1) / s.parts) * kRound;
+    s.parts = (uint32_t)std::max<uint64_t>(1, (span + s.chunk - 1) / s.chunk);
+    return s;
+}
+
+size_t partial_bytes(const ts_kept8_args *k, const Plan &s) {
+    return s.parts <= 1 ? 0 : (size_t)s.tiles * k->rows.kv_heads * s.parts * 16 * s.nt * kPart * sizeof(float);
+}
+
+int check(const ts_kept8_args *k) {
+    TS_REQUIRE(k, "attend_kept8: null args");
+    const ts_rows_args *a = &k->rows;
+    TS_REQUIRE(a->q && a->k && a->v && a->out && a->slots && a->positions && k->scales, "attend_kept8: null pointer");
+    TS_REQUIRE(a->width == 128, "attend_kept8: head width %u (128 supported)", a->width);
+    TS_REQUIRE(a->kv_heads >= 1 && a->kv_heads <= 1024 && a->heads >= 1 && a->heads % a->kv_heads == 0 &&
+                   a->heads / a->kv_heads <= 64,
+               "attend_kept8: %u heads over %u kv heads (at most 64 each)", a->heads, a->kv_heads);
+    TS_REQUIRE((a->q_dtype == TS_F32 || a->q_dtype == TS_BF16) && a->kv_dtype == TS_E4M3 &&
+                   (a->out_dtype == TS_F32 || a->out_dtype == TS_BF16),
+               "attend_kept8: q and out f32 or bf16, kept rows e4m3 blocks supported");
+    int rc = ts::kept_check("attend_kept8", a->kept_table, a->page, a->keys, k->slot_count, a->kept_pages, k->pages, true);
+    if (rc) return rc;
+    TS_REQUIRE(a->keys <= 1u << 30, "attend_kept8: %u positions a slot", a->keys);
+    TS_REQUIRE((uint64_t)k->pages * a->page <= 1ull << 36, "attend_kept8: %u pages of %u rows", k->pages, a->page);
+    TS_REQUIRE(ts::aligned(a->k, 16) && ts::aligned(a->v, 16) && ts::aligned(a->q, 16) && ts::aligned(a->out, 16) &&
+                   ts::aligned(k->scales, 16),
+               "attend_kept8: q, k, v, scales and out must be 16-byte aligned");
+    return TS_OK;
+}
+
+template <int NT, bool QF32>
+int launch(const AttendParams &p, uint32_t groups, void *stream) {
+    constexpr uint32_t kLds = kWaves * 16 * NT * kPart * sizeof(float);
+    static const hipError_t attr = hipFuncSetAttribute((const void *)attend_kept8_kernel<NT, QF32>,
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (attr != hipSuccess) return ts::hip_status(attr, "attend_kept8: shared memory attribute");
+    hipLaunchKernelGGL((attend_kept8_kernel<NT, QF32>), dim3(groups), dim3(256), kLds, (hipStream_t)stream, p);
+    TS_CHECK_LAUNCH("attend_kept8 launch");
+    return TS_OK;
+}
+
+}  // namespace
+
+extern "C" size_t tessera_hip_attend_kept8_workspace(const ts_kept8_args *k) {
+    if (!k || k->rows.kv_heads == 0 || k->rows.heads == 0 || k->rows.heads % k->rows.kv_heads ||
+        k->rows.heads / k->rows.kv_heads > 64 || k->rows.rows == 0)
+        return 0;
+    return partial_bytes(k, plan(k));
+}
+
+extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
+    int rc = check(k);
+    if (rc) return rc;
+    const ts_rows_args *a = &k->rows;
+    if (a->rows == 0) return TS_OK;
+    const Plan s = plan(k);
+    TS_REQUIRE((uint64_t)s.tiles * a->kv_heads * s.parts <= 0x7fffffffull / 64, "attend_kept8: %u rows in one launch", a->rows);
+    const size_t need = partial_bytes(k, s);
+    if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
+        return ts::fail(TS_ERR_WORKSPACE, "attend_kept8: workspace of %zu bytes, 16-byte aligned, needed", need);
+    AttendParams p;
+    p.q = a->q; p.k = (const uint8_t *)a->k; p.v = (const uint8_t *)a->v; p.scales = k->scales; p.out = a->out;
+    p.partials = need ? (float *)a->workspace : nullptr;
+    p.slots = a->slots; p.positions = a->positions; p.status = a->status;
+    p.place.table = a->kept_table; p.place.keys = a->keys; p.place.slot_count = k->slot_count;
+    p.place.kept_pages = a->kept_pages; p.place.page_shift = (uint32_t)__builtin_ctz(a->page); p.place.pages = k->pages;
+    p.rows = a->rows; p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads;
+    p.back = a->back; p.max_position = a->max_position;
+    p.tile_rows = s.tile_rows; p.chunk = s.chunk; p.parts = s.parts;
+    p.scale = a->scale; p.out_bf16 = a->out_dtype == TS_BF16;
+    const uint32_t groups = s.tiles * a->kv_heads * s.parts;
+    const bool f32 = a->q_dtype == TS_F32;
+    switch (s.nt) {
+    case 1: rc = f32 ? launch<1, true>(p, groups, stream) : launch<1, false>(p, groups, stream); break;
+    case 2: rc = f32 ? launch<2, true>(p, groups, stream) : launch<2, false>(p, groups, stream); break;
+    default: rc = f32 ? launch<4, true>(p, groups, stream) : launch<4, false>(p, groups, stream); break;
+    }
+    if (rc || s.parts == 1) return rc;
+    const uint32_t pieces = (s.tile_rows * p.group + 1) / 2;
+    hipLaunchKernelGGL(join_kept8_kernel, dim3(s.tiles * a->kv_heads * pieces), dim3(64), 0, (hipStream_t)stream, p,
+                       16 * s.nt, pieces);
+    TS_CHECK_LAUNCH("attend_kept8 join launch");
+    return TS_OK;
+}

@@ -201,3 +201,12 @@ def copy_pages(buffers, copies, *, page, pages, status=None, check=True):
     a.status = status.data_ptr() if status is not None else None
     rc = lib().tessera_hip_kv_copy(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream))
     abi.check(rc, "tessera_hip_kv_copy")
+
+
+def copy_kept8(k, v, scales, copies, *, page, status=None):
+    """Pool.grow's copies over kept8() blocks, in stream order: whole pages (a block's positions share
+    their scales, so a page copies with all of them). copies: [(from, to, rows), ...]."""
+    pages = k.shape[0] * 16 // page
+    whole = [(f, t, 1) for f, t, _ in copies]
+    copy_pages([k.view(pages, -1), v.view(pages, -1)], whole, page=1, pages=pages, status=status)
+    copy_pages([scales.view(pages, -1)], whole, page=1, pages=pages, status=status)

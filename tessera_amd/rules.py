@@ -2,7 +2,8 @@
 
 Each function is named for the reference rule whose kernel it launches
 (``tiled``, ``lanes``, ``linear``, ``attend_rows``, ``flash_rows``, ``rms_norm``,
-``rope``, ``argmax``, ``top_k``, ``gather``) and takes the same operands in the
+``rope``, ``argmax``, ``top_k``, ``gather``; ``append_rows``, ``attend_kept8`` and ``verify``
+have no rule of the reference beside them) and takes the same operands in the
 same order as that rule's Launch (reads, epilogue operands, output, counts:
 engine/plan/lower/src/abi.rs:148-153, product.rs:70-76, rule.rs:92-110).
 torch only provides device memory and the current stream; every computation is
@@ -397,3 +398,193 @@ def top_k(x, k, ids=None):
         ids = torch.empty((rows, k), dtype=torch.int32, device=x.device)
     abi.call("tessera_hip_top_k", C.byref(abi.TopKArgs(_ptr(x), _ptr(ids), rows, width, k)), _stream())
     return ids
+
+
+# ---------------------------------------------------------------------------------------------
+# Speculative decoding over an 8-bit cache: kept blocks, appends, attention, verification.
+# ---------------------------------------------------------------------------------------------
+
+KEPT_BLOCK = 16  # positions a kept block holds
+_INTS = (torch.int32, torch.uint32)
+
+
+def _checked(what, device, **tensors):
+    """Contiguous tensors on `device`, the one that the call is made on; None passes."""
+    if device.type != "cuda":
+        raise ValueError(f"{what}: tensors on {device}, not on a GPU")
+    for name, t in tensors.items():
+        if t is not None and (t.device != device or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous and on {device}")
+
+
+def _indices(what, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.dtype not in _INTS:
+            raise ValueError(f"{what}: {name} must be 32-bit integers")
+
+
+def _call_on(device, name, args):
+    """The call on `device`'s current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        abi.call(name, C.byref(args), _stream())
+    else:
+        with torch.cuda.device(device):
+            abi.call(name, C.byref(args), _stream())
+
+
+def kept8(pages, kv_heads, page=16, device="cuda"):
+    """Kept blocks of `pages` pages, all zero: (k, v, scales) as include/tessera_hip.h lays them out
+    (16 positions of one kv head a block: e4m3 codes times a power of two)."""
+    blocks = pages * page // KEPT_BLOCK
+    k = torch.zeros((blocks, kv_heads, KEPT_BLOCK, 128), dtype=torch.uint8, device=device)
+    v = torch.zeros((blocks, kv_heads, 128, KEPT_BLOCK), dtype=torch.uint8, device=device)
+    return k, v, torch.zeros((blocks, (kv_heads + 1) // 2 * 2, 2), dtype=torch.float32, device=device)
+
+
+def _kept8_sizes(what, k, v, scales, kv_heads, page):
+    """Pages that the blocks hold."""
+    blocks = k.shape[0]
+    if k.shape != (blocks, kv_heads, KEPT_BLOCK, 128) or v.shape != (blocks, kv_heads, 128, KEPT_BLOCK) or \
+            scales.shape != (blocks, (kv_heads + 1) // 2 * 2, 2) or scales.dtype != torch.float32 or \
+            _DT.get(k.dtype) != abi.TS_E4M3 or _DT.get(v.dtype) != abi.TS_E4M3:
+        raise ValueError(f"{what}: kept blocks of {kv_heads} heads as kept8() makes them")
+    return blocks * KEPT_BLOCK // page
+
+
+def _slots(what, table, kept_pages, slot_rows, keys):
+    """Slots that the table (or the dense kept rows) holds."""
+    if table is None:
+        return slot_rows // keys
+    if kept_pages < 1 or table.numel() % kept_pages:
+        raise ValueError(f"{what}: a table of {table.numel()} entries is not whole slots of {kept_pages}")
+    return table.numel() // kept_pages
+
+
+def _row_stride(x):
+    """Elements from a row of x [rows, heads, 128] to the next (one row: any will do)."""
+    return 0 if x is None else x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+
+
+def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=None, k_gain=None, angles=None,
+                halves=True, eps=1e-6, scales=None, table=None, kept_pages=0, page=16, q_out=None, status=None):
+    """New rows k, v [rows, kv_heads, 128] (views of a product's rows serve: only the rows' distance is
+    free) into the kept rows, q [rows, heads, 128] rotated to q_out (of q's type unless given). With
+    gains q / k pass through RmsNorm, with `angles` (rope_table's, at least `keys` positions) through the
+    rotation. `scales` given: k_kept, v_kept are kept8() blocks; else bf16 rows [*, kv_heads, 128].
+    Rows of one call that fall into one block of 16 positions stand together, in order. status: int32
+    device word, TS_STATUS_* bits of rows that were not kept. Returns q_out."""
+    rows, kv_heads, width = k.shape
+    heads = q.shape[1] if q is not None else 0
+    x = _DT.get(k.dtype)
+    if v.shape != k.shape or v.dtype != k.dtype or (q is not None and (q.dtype != k.dtype or q.shape != (rows, heads, width))):
+        raise ValueError("append_rows: q, k and v must be rows of one type and width")
+    for t in (q, k, v):
+        if t is not None and (t.stride(2) != 1 or t.stride(1) != width or t.device != k.device):
+            raise ValueError("append_rows: a row's heads must lie back to back, on one device")
+    _checked("append_rows", k.device, k_kept=k_kept, v_kept=v_kept, slots=slots, positions=positions, table=table,
+             scales=scales, q_gain=q_gain, k_gain=k_gain, angles=angles, q_out=q_out, status=status)
+    _indices("append_rows", slots=slots, positions=positions, table=table, status=status)
+    if slots.numel() != rows or positions.numel() != rows:
+        raise ValueError(f"append_rows: {rows} rows need as many slots and positions")
+    for g in (q_gain, k_gain):
+        if g is not None and (g.dtype != torch.float32 or g.numel() != width):
+            raise ValueError("append_rows: gains are f32, one a column")
+    if angles is not None and (angles.dtype != torch.float32 or angles.numel() != angles.shape[0] * width):
+        raise ValueError("append_rows: angles as rope_table makes them")
+    if scales is not None:
+        pages = _kept8_sizes("append_rows", k_kept, v_kept, scales, kv_heads, page)
+        held, kv = k_kept.shape[0] * KEPT_BLOCK, abi.TS_E4M3
+    else:
+        held, kv = k_kept.numel() // (kv_heads * width) if kv_heads else 0, abi.TS_BF16
+        if k_kept.dtype != torch.bfloat16 or v_kept.dtype != torch.bfloat16 or v_kept.numel() != k_kept.numel() or \
+                k_kept.shape[-2:] != (kv_heads, width):
+            raise ValueError("append_rows: kept rows are bf16 [rows, kv_heads, 128], or blocks with their scales")
+        pages = held // page
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty((rows, heads, width), dtype=q.dtype, device=q.device)
+        elif q_out.shape != q.shape:
+            raise ValueError("append_rows: q_out must have q's shape")
+    a = abi.AppendArgs(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_gain), _ptr(k_gain), _ptr(angles), _ptr(q_out),
+                       k_kept.data_ptr(), v_kept.data_ptr(), _ptr(scales), slots.data_ptr(), positions.data_ptr(),
+                       _ptr(table), _ptr(status), rows, heads, kv_heads, width, _row_stride(q), _row_stride(k),
+                       _row_stride(v), keys, _slots("append_rows", table, kept_pages, held, keys), kept_pages, page, pages,
+                       angles.shape[0] if angles is not None else 0, 1 if halves else 0, -1 if x is None else x,
+                       -1 if q_out is None else _DT.get(q_out.dtype, -1), kv, eps)
+    _call_on(k.device, "tessera_hip_append_rows", a)
+    return q_out
+
+
+def attend_kept8(q, k, v, scales, slots, positions, *, keys, scale, table=None, kept_pages=0, page=16,
+                 back=abi.U32_MAX, run=1, max_position=None, out=None, out_dtype=torch.float32, status=None):
+    """Attention of q [rows, heads, 128] (f32 or bf16) over kept8() blocks: decode rows, several drafted
+    rows of a sequence, prompts. run: how many rows of a slot stand together (a hint: it groups rows and
+    picks the kernel). max_position (an upper bound on positions) defaults to their maximum (a host
+    read: pass it when capturing a graph). out f32 or bf16."""
+    rows, heads, width = q.shape
+    kv_heads = k.shape[1]
+    pages = _kept8_sizes("attend_kept8", k, v, scales, kv_heads, page)
+    if out is None:
+        out = torch.empty((rows, heads, width), dtype=out_dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("attend_kept8: out must have q's shape")
+    _checked("attend_kept8", q.device, q=q, k=k, v=v, scales=scales, slots=slots, positions=positions, table=table,
+             out=out, status=status)
+    _indices("attend_kept8", slots=slots, positions=positions, table=table, status=status)
+    if slots.numel() != rows or positions.numel() != rows:
+        raise ValueError(f"attend_kept8: {rows} rows need as many slots and positions")
+    if max_position is None:
+        max_position = int(positions.max().item()) if rows else 0
+    r = abi.RowsArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+                     _ptr(table), None, 0, rows, keys, heads, kv_heads, width, back, kept_pages, page, scale,
+                     _DT.get(q.dtype, -1), abi.TS_E4M3, _DT.get(out.dtype, -1), max_position, _ptr(status))
+    a = abi.Kept8Args(r, scales.data_ptr(), _slots("attend_kept8", table, kept_pages, k.shape[0] * KEPT_BLOCK, keys),
+                      pages, run)
+    need = abi.load().tessera_hip_attend_kept8_workspace(C.byref(a))
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.rows.workspace, a.rows.workspace_bytes = scratch.data_ptr(), need
+    _call_on(q.device, "tessera_hip_attend_kept8", a)
+    return out
+
+
+def verify(logits, drafts, uniforms=None, *, counts=None, first=None, draft_probs=None, temperature=1.0, tokens=None,
+           accepted=None, status=None):
+    """Drafted tokens [seqs, most] against the target's logits [rows, width] (f32 or bf16; rows any
+    distance apart): sequence s's rows are first[s] .. first[s] + counts[s] (without them s * (most + 1)
+    and most). uniforms [seqs, most + 1] f32 in [0, 1): one a draft, the last for the token after the
+    accepted ones; None: greedy. draft_probs f32 [seqs, most, width]: the drafter's probabilities; None: it
+    had only the one token. temperature: a number or f32 [seqs] (<= 0: greedy).
+    Returns (tokens [seqs, most + 1], accepted [seqs]) int32: the accepted drafts, the next token, then
+    `width`."""
+    rows, width = logits.shape
+    seqs, most = drafts.shape
+    per = temperature if isinstance(temperature, torch.Tensor) else None
+    stride = logits.stride(0) if rows > 1 else width
+    if (logits.stride(1) != 1 and width > 1) or stride < width:
+        raise ValueError("verify: a row's logits must lie back to back, rows apart")
+    if tokens is None:
+        tokens = torch.empty((seqs, most + 1), dtype=torch.int32, device=logits.device)
+    if accepted is None:
+        accepted = torch.empty(seqs, dtype=torch.int32, device=logits.device)
+    _checked("verify", logits.device, drafts=drafts, uniforms=uniforms, draft_probs=draft_probs, temperature=per,
+             counts=counts, first=first, tokens=tokens, accepted=accepted, status=status)
+    _indices("verify", drafts=drafts, counts=counts, first=first, tokens=tokens, accepted=accepted, status=status)
+    for name, t, shape in (("uniforms", uniforms, (seqs, most + 1)), ("draft_probs", draft_probs, (seqs, most, width)),
+                           ("temperature", per, (seqs,))):
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape):
+            raise ValueError(f"verify: {name} must be f32 {list(shape)}")
+    for name, t, shape in (("counts", counts, (seqs,)), ("first", first, (seqs,)), ("tokens", tokens, (seqs, most + 1)),
+                           ("accepted", accepted, (seqs,))):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"verify: {name} must be {list(shape)}")
+    a = abi.VerifyArgs(logits.data_ptr(), _ptr(drafts), _ptr(uniforms), _ptr(draft_probs), _ptr(per), _ptr(counts),
+                       _ptr(first), tokens.data_ptr(), accepted.data_ptr(), None, 0, _ptr(status), seqs, most, rows,
+                       width, stride, _DT.get(logits.dtype, -1),
+                       0.0 if per is not None else temperature)
+    need = abi.load().tessera_hip_verify_workspace(C.byref(a))
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+    _call_on(logits.device, "tessera_hip_verify", a)
+    return tokens, accepted
