@@ -40,10 +40,32 @@ struct AttendParams {
     uint32_t *status;
     Place place;
     uint32_t rows, heads, kv_heads, group, back, max_position;
-    uint32_t tile_rows, chunk, parts;  // rows a tile; keys of a part at a time (a multiple of kRound)
+    uint32_t tile_rows, tile_heads, splits;  // rows and q heads a tile; tiles a kv head's q heads take
+    uint32_t chunk, parts;                   // keys of a part at a time (a multiple of kRound); parts
     float scale;
     int out_bf16;
 };
+
+// Tile gi: rows from row0, q heads from head0 of one kv head.
+struct Tile {
+    uint32_t row0, head0, end, kvh;
+    // Column c's row and q head; false where it has none.
+    TS_DEV bool column(const AttendParams &p, uint32_t c, uint32_t &r, uint32_t &h) const {
+        const uint32_t ri = c / p.tile_heads;
+        r = row0 + ri;
+        h = head0 + c % p.tile_heads;
+        return ri < p.tile_rows && r < p.rows && h < end;
+    }
+};
+TS_DEV Tile tile_of(const AttendParams &p, uint32_t gi) {
+    Tile t;
+    const uint32_t split = gi % p.splits;
+    t.kvh = gi / p.splits % p.kv_heads;
+    t.row0 = gi / (p.splits * p.kv_heads) * p.tile_rows;
+    t.head0 = t.kvh * p.group + split * p.tile_heads;
+    t.end = (t.kvh + 1) * p.group;
+    return t;
+}
 
 TS_DEV float rows4_sum(float x) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -73,25 +95,42 @@ TS_DEV uint32_t within4(uint32_t w, uint32_t pos, uint32_t lo, uint32_t hi) {
     return w & m;
 }
 
-// The place of a step's block: its page looked up, or the page's own row of a dense slot.
-struct BlockAt {
-    uint32_t block;
-    bool ok;
-};
-TS_DEV BlockAt block_at(const Place &p, uint32_t slot, uint32_t block) {
-    uint64_t row;
-    const bool ok = row_of(p, slot, block * kBlock, row);
-    return {(uint32_t)(row / kBlock), ok};
+// Two f32 as packed bf16, rounded to nearest even; NaN stays NaN.
+TS_DEV uint32_t bf16_pair(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(ts_f32x2{a, b}, ts_bf16x2));
 }
+// P parts of two f32 values: bf16 values that add up to them (24 bits in three parts, 8 in one).
+template <uint32_t P>
+TS_DEV void split_pair(float a, float b, uint32_t (&w)[P]) {
+#pragma unroll
+    for (uint32_t e = 0; e < P; e++) {
+        w[e] = bf16_pair(a, b);
+        if (e + 1 < P) {
+            a -= lo_bf16(w[e]);
+            b -= hi_bf16(w[e]);
+        }
+    }
+}
+
+// The table and the scales are read by scalar loads (their addresses are uniform), which return
+// beside the codes' vector loads instead of behind them.
+typedef const __attribute__((address_space(4))) uint32_t const_u32;
+typedef const __attribute__((address_space(4))) float const_f32;
+template <class T>
+TS_DEV T in_constant(const void *p) { return (T)(uintptr_t)p; }
+
+// Keeps what follows from being computed earlier: eight registers of codes at a time are widened,
+// where the compiler would widen all of a step's and spill.
+TS_DEV void pin(u32x4 &v) { asm volatile("" : "+v"(v)); }
 
 template <int NT, bool QF32>
 __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(AttendParams p) {
-    constexpr uint32_t kCols = 16 * NT, kParts = QF32 ? 2 : 1;
+    constexpr uint32_t kCols = 16 * NT, kParts = QF32 ? 3 : 1;
     extern __shared__ __attribute__((aligned(16))) float joined[];  // [kWaves][kCols][kPart]
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4;
     const uint32_t part = blockIdx.x % p.parts, gi = blockIdx.x / p.parts;
-    const uint32_t kvh = gi % p.kv_heads, tile = gi / p.kv_heads, G = p.group;
+    const Tile tile = tile_of(p, gi);
 
     // Columns: (row, head) pairs of the tile, row by row.
     uint32_t pos[NT], from[NT], slot[NT];
@@ -101,15 +140,15 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
     const float sl = p.scale == 0.0f ? 0x1p-100f : fabsf(p.scale) * 1.4426950408889634f;  // to base 2
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const uint32_t c = 16 * nt + col, ri = c / G, r = tile * p.tile_rows + ri;
-        const bool there = ri < p.tile_rows && r < p.rows;
+        uint32_t r, h;
+        const bool there = tile.column(p, 16 * nt + col, r, h);
         pos[nt] = there ? p.positions[r] : 0;
         slot[nt] = there ? p.slots[r] : 0;
         live[nt] = there && pos[nt] <= p.max_position && holds(p.place, slot[nt], pos[nt]);
-        if (there && !live[nt] && p.status && part == 0 && kvh == 0 && wave == 0 && grp == 0)
+        if (there && !live[nt] && p.status && part == 0 && wave == 0 && grp == 0)
             atomicOr(p.status, slot[nt] >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
         from[nt] = pos[nt] > p.back ? pos[nt] - p.back : 0;
-        const size_t at = ((size_t)(live[nt] ? r : 0) * p.heads + kvh * G + (live[nt] ? c % G : 0)) * 128;
+        const size_t at = live[nt] ? ((size_t)r * p.heads + h) * 128 : 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {  // operand j: d 64 (j / 2) + 16 grp + 8 (j % 2) ..
             const uint32_t d = 64 * (j >> 1) + 16 * grp + 8 * (j & 1);
@@ -120,18 +159,15 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
             } else {
                 const f32x4 x = *(const f32x4 *)((const float *)p.q + at + d);
                 const f32x4 y = *(const f32x4 *)((const float *)p.q + at + d + 4);
-                uint32_t hi[4], lo[4];
+                uint32_t w[4][kParts];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float a = e < 2 ? x[2 * e] : y[2 * e - 4], b = e < 2 ? x[2 * e + 1] : y[2 * e - 3];
                     if (qsign) { a = -a; b = -b; }
-                    if (!live[nt]) a = b = 0.0f;
-                    const float ha = bf16_round(a), hb = bf16_round(b);
-                    hi[e] = pack_bf16x2(ha, hb);
-                    lo[e] = pack_bf16x2(a - ha, b - hb);
+                    split_pair<kParts>(live[nt] ? a : 0.0f, live[nt] ? b : 0.0f, w[e]);
                 }
-                q[nt][j][0] = as_bf16x8(u32x4{hi[0], hi[1], hi[2], hi[3]});
-                q[nt][j][kParts - 1] = as_bf16x8(u32x4{lo[0], lo[1], lo[2], lo[3]});
+#pragma unroll
+                for (uint32_t e = 0; e < kParts; e++) q[nt][j][e] = as_bf16x8(u32x4{w[0][e], w[1][e], w[2][e], w[3][e]});
             }
         }
     }
@@ -174,57 +210,109 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
                 hi = max(hi, pos[nt]);
             }
         }
+        // Keys every active column sees: [all_lo, all_hi]. A column not active sees none.
+        uint32_t all_lo = 0, all_hi = 0xffffffffu;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            if (act[nt]) {
+                all_lo = max(all_lo, from[nt]);
+                all_hi = min(all_hi, pos[nt]);
+            } else if (live[nt]) {
+                all_lo = 0xffffffffu;
+            }
+        }
 #pragma unroll
         for (int x = 1; x < 16; x <<= 1) {
             lo = min(lo, (uint32_t)__shfl_xor((int)lo, x, 64));
             hi = max(hi, (uint32_t)__shfl_xor((int)hi, x, 64));
+            all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, x, 64));
+            all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, x, 64));
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
-        const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock;
-        bool lost = false, gone = false;  // the lane's block of this step, or of any, is on a page not held
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, span = hi - base0;
+        worked |= (uint64_t)part * p.chunk <= span;
 
-        // Step i of this wave: the keys from step_base(i) on; parts take chunks in turn.
-        const uint32_t per = p.chunk / kRound;
-        auto step_off = [&](uint32_t i) -> uint64_t {
-            return ((uint64_t)(i / per) * p.parts + part) * p.chunk + (i % per) * kRound + wave * kStep;
+        // The blocks of a step, block j of it by its page (one whose page is not held: bit j of `lost`,
+        // read as page 0), and the scales of them.
+        struct Blocks {
+            uint32_t at[4], lost;
         };
-        uint32_t i = 0;
-        // The first step at or after i that begins within the keys (chunks ascend; none: done).
-        auto inside_keys = [&](uint32_t i) { return step_off(i) <= hi - base0; };
+        auto look = [&](uint32_t base) {
+            Blocks b;
+            b.lost = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t key = min(base / kBlock + j, last) * kBlock;
+                if (p.place.table) {
+                    const_u32 *t = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
+                    uint32_t id = t[key >> p.place.page_shift];
+                    if (id >= p.place.pages) {
+                        id = 0;
+                        b.lost |= 1u << j;
+                    }
+                    const uint32_t in = key & ((1u << p.place.page_shift) - 1);
+                    b.at[j] = (id << (p.place.page_shift - 4)) + in / kBlock;
+                } else {
+                    b.at[j] = now * (p.place.keys / kBlock) + key / kBlock;
+                }
+            }
+            return b;
+        };
+        // Lane value j of four uniform ones.
+        auto choose = [](uint32_t j, auto a, auto b, auto c, auto d) {
+            const auto x = j & 1 ? b : a, y = j & 1 ? d : c;
+            return j & 2 ? y : x;
+        };
         u32x4 kf[4][2], vf[8];
         float ks = 0.0f, vs = 0.0f;
-        auto load_k = [&](uint32_t base) {
-            const BlockAt b = block_at(p.place, now, min(base / kBlock + (col >> 2), last));
-            ks = p.scales[((size_t)b.block * scale_heads(p.kv_heads) + kvh) * 2];
-            const uint8_t *at = p.k + ((size_t)b.block * p.kv_heads + kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
+        const_f32 *scales = in_constant<const_f32 *>(p.scales + tile.kvh * 2);
+        const size_t scale_row = scale_heads(p.kv_heads) * 2;
+        auto load_k = [&](const Blocks &b) {
+            const uint32_t block = choose(col >> 2, b.at[0], b.at[1], b.at[2], b.at[3]);
+            const uint8_t *at = p.k + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int s = 0; s < 2; s++) kf[t][s] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * s);
+                for (int x = 0; x < 2; x++) kf[t][x] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * x);
+            ks = choose(col >> 2, scales[b.at[0] * scale_row], scales[b.at[1] * scale_row], scales[b.at[2] * scale_row],
+                        scales[b.at[3] * scale_row]);
         };
-        auto load_v = [&](uint32_t base) {
-            const BlockAt b = block_at(p.place, now, min(base / kBlock + grp, last));
-            lost = !b.ok;
-            vs = p.scales[((size_t)b.block * scale_heads(p.kv_heads) + kvh) * 2 + 1];
-            const uint8_t *at = p.v + ((size_t)b.block * p.kv_heads + kvh) * kBlockBytes + col * kBlock;
+        auto load_v = [&](const Blocks &b) {
+            const uint32_t block = choose(grp, b.at[0], b.at[1], b.at[2], b.at[3]);
+            const uint8_t *at = p.v + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + col * kBlock;
 #pragma unroll
             for (int dt = 0; dt < 8; dt++) vf[dt] = *(const u32x4 *)(at + dt * 16 * kBlock);
+            vs = choose(grp, scales[b.at[0] * scale_row + 1], scales[b.at[1] * scale_row + 1],
+                        scales[b.at[2] * scale_row + 1], scales[b.at[3] * scale_row + 1]);
         };
-        if (inside_keys(0)) {
-            worked = true;
-            load_k(base0 + (uint32_t)step_off(0));
-            load_v(base0 + (uint32_t)step_off(0));
-        } else if (step_off(0) - wave * kStep <= hi - base0) {
-            worked = true;  // another wave of the group
-        }
-        for (; inside_keys(i); i++) {
-            const uint32_t base = base0 + (uint32_t)step_off(i);
-            const bool more = inside_keys(i + 1);
-            const uint32_t next = more ? base0 + (uint32_t)step_off(i + 1) : 0;
+
+        // Keys from base0 + off on are this wave's next step: a part takes chunks in turn, its waves the
+        // steps of a chunk.
+        uint64_t off = (uint64_t)part * p.chunk + wave * kStep;
+        uint32_t left = p.chunk / kRound;  // steps of the chunk
+        if (off > span) continue;
+        Blocks b = look(base0 + (uint32_t)off);
+        load_k(b);
+        load_v(b);
+        for (bool more = true; more;) {
+            const uint32_t base = base0 + (uint32_t)off, lost = b.lost;
+            off += kRound;
+            if (--left == 0) {
+                left = p.chunk / kRound;
+                off += (uint64_t)(p.parts - 1) * p.chunk;
+            }
+            more = off <= span;
+            // (The last step's codes are asked for once more, from the caches: a branch around the
+            // loads would keep two copies of them in registers.)
+            b = look(more ? base0 + (uint32_t)off : base);
             f32x4 s[4][NT];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
+                pin(kf[t][0]);
+                pin(kf[t][1]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) s[t][nt] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -237,104 +325,48 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
                         for (uint32_t e = 0; e < kParts; e++) s[t][nt] = mfma16(kc, q[nt][j][e], s[t][nt]);
                 }
             }
-            if (more) load_k(next);
-            if (__builtin_amdgcn_ballot_w64(lost) != 0) {  // a page that the buffers do not hold: NaN scores
-                gone |= lost;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) s[t][nt][e] = lost ? __builtin_nanf("") : s[t][nt][e];
-            }
+            load_k(b);
 
-            // A step wholly inside every column's window skips the masks.
-            bool inside = true;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                inside &= act[nt] ? (base + kStep - 1 <= pos[nt] && base >= from[nt]) : !live[nt];
-            inside = __builtin_amdgcn_ballot_w64(!inside) == 0;
-            uint32_t seen[NT];  // a bit for each of the lane's 16 keys
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) seen[nt] = 0xffffu;
-            if (!inside) {
+            // A step that meets a window's edge, or a block that is lost.
+            if (base < all_lo || base + (kStep - 1) > all_hi || lost) {
                 const uint32_t key0 = base + kBlock * grp;
+                const bool gone = lost >> grp & 1;
+                if (lost && p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+                uint32_t seen[NT];  // a bit for each of the lane's 16 keys
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    seen[nt] = 0;
+                    // Keys e of the lane with from <= key0 + e <= pos.
+                    const int first = max((int)(from[nt] - key0), 0), end = min((int)(pos[nt] - key0) + 1, 16);
+                    const uint32_t upto = end <= 0 ? 0u : (1u << end) - 1;
+                    seen[nt] = act[nt] && first < 16 ? upto & (0xffffu << first) : 0u;
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const uint32_t key = key0 + 4 * t + e;
-                            const bool ok = act[nt] & (key <= pos[nt]) & (key >= from[nt]);
-                            s[t][nt][e] = ok ? s[t][nt][e] : -INFINITY;
-                            seen[nt] |= ok ? 1u << (4 * t + e) : 0u;
+                            const float x = gone ? __builtin_nanf("") : s[t][nt][e];
+                            s[t][nt][e] = seen[nt] >> (4 * t + e) & 1 ? x : -INFINITY;
                         }
                 }
                 // Codes outside [lo, hi] may be anything: as zeros they add nothing.
-#pragma unroll
-                for (int dt = 0; dt < 8; dt++)
-                    vf[dt] = u32x4{within4(vf[dt].x, key0, lo, hi), within4(vf[dt].y, key0 + 4, lo, hi),
-                                   within4(vf[dt].z, key0 + 8, lo, hi), within4(vf[dt].w, key0 + 12, lo, hi)};
-            }
-            bf16x8 w[NT][2][kParts];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float mx = s[0][nt][0];
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[t][nt][e]);
-                mx = rows4_max(mx) * sl;
-                // The reference point moves only when a score passes it by 2^kSlack: most steps leave
-                // the sums and O unscaled, and no weight passes 2^kSlack.
-                const bool raise = mx > m[nt] + kSlack;
-                const float mn = raise ? mx : m[nt];
-                const float alpha = raise ? __builtin_amdgcn_exp2f(m[nt] - mn) : 1.0f;
-                const float mo = mn == -INFINITY ? 0.0f : mn;
-                float sum = 0.0f;
-                uint32_t hw[8], lw[8];
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const float a = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e], sl, -mo));
-                        const float b = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e + 1], sl, -mo));
-                        sum += a + b;
-                        hw[2 * t + e / 2] = pack_bf16x2(a, b);
-                        if (QF32)
-                            lw[2 * t + e / 2] = pack_bf16x2(a - lo_bf16(hw[2 * t + e / 2]), b - hi_bf16(hw[2 * t + e / 2]));
-                    }
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    w[nt][x][0] = as_bf16x8(u32x4{hw[4 * x], hw[4 * x + 1], hw[4 * x + 2], hw[4 * x + 3]});
-                    if (QF32) w[nt][x][kParts - 1] = as_bf16x8(u32x4{lw[4 * x], lw[4 * x + 1], lw[4 * x + 2], lw[4 * x + 3]});
-                }
-                l[nt] = l[nt] * alpha + rows4_sum(sum);
-                m[nt] = mn;
-                if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-#pragma unroll
-                    for (int dt = 0; dt < 8; dt++) o[nt][dt] *= alpha;
-                }
-            }
-            // A NaN code at a key that some columns see and some do not: a weight of 0 times NaN must
-            // not reach the latter. Such codes become 0, and what they reach is marked by a product of
-            // (code is NaN) with (column sees the key).
-            if (!inside) {
                 uint32_t nan = 0;
 #pragma unroll
-                for (int dt = 0; dt < 8; dt++)
+                for (int dt = 0; dt < 8; dt++) {
+                    vf[dt] = u32x4{within4(vf[dt].x, key0, lo, hi), within4(vf[dt].y, key0 + 4, lo, hi),
+                                   within4(vf[dt].z, key0 + 8, lo, hi), within4(vf[dt].w, key0 + 12, lo, hi)};
                     nan |= nan_codes(vf[dt].x) | nan_codes(vf[dt].y) | nan_codes(vf[dt].z) | nan_codes(vf[dt].w);
+                }
+                // A NaN code at a key that some columns see and some do not: a weight of 0 times NaN
+                // must not reach the latter. Such codes become 0, and what they reach is marked by a
+                // product of (code is NaN) with (column sees the key).
                 if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
 #pragma unroll
                     for (int dt = 0; dt < 8; dt++) {
                         uint32_t ones[4];  // e4m3 1.0 (0x38) at each NaN code
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const uint32_t b = nan_codes(vf[dt][e]) >> 7;
-                            ones[e] = b * 0x38u;
-                            vf[dt][e] &= ~(b * 0xffu);
+                            const uint32_t at = nan_codes(vf[dt][e]) >> 7;
+                            ones[e] = at * 0x38u;
+                            vf[dt][e] &= ~(at * 0xffu);
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
@@ -357,8 +389,48 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
                     }
                 }
             }
+            bf16x8 w[NT][2][kParts];
 #pragma unroll
-            for (int dt = 0; dt < 8; dt++)
+            for (int nt = 0; nt < NT; nt++) {
+                float mx = s[0][nt][0];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[t][nt][e]);
+                mx = rows4_max(mx) * sl;
+                // The reference point moves only when a score passes it by 2^kSlack: most steps leave
+                // the sums and O unscaled, and no weight passes 2^kSlack.
+                const bool raise = mx > m[nt] + kSlack;
+                const float mn = raise ? mx : m[nt];
+                const float mo = mn == -INFINITY ? 0.0f : mn;
+                float sum = 0.0f;
+                uint32_t pw[8][kParts];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float a = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e], sl, -mo));
+                        const float c = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e + 1], sl, -mo));
+                        sum += a + c;
+                        split_pair<kParts>(a, c, pw[2 * t + e / 2]);
+                    }
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (uint32_t e = 0; e < kParts; e++)
+                        w[nt][x][e] = as_bf16x8(u32x4{pw[4 * x][e], pw[4 * x + 1][e], pw[4 * x + 2][e], pw[4 * x + 3][e]});
+                if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+                    const float alpha = raise ? __builtin_amdgcn_exp2f(m[nt] - mn) : 1.0f;
+                    l[nt] *= alpha;
+                    m[nt] = mn;
+#pragma unroll
+                    for (int dt = 0; dt < 8; dt++) o[nt][dt] *= alpha;
+                }
+                l[nt] += sum;  // of the lane's keys: the column's four lanes are added at the end
+            }
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++) {
+                pin(vf[dt]);
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     const bf16x8 vc = codes8(x ? vf[dt].z : vf[dt].x, x ? vf[dt].w : vf[dt].y, vs);
@@ -367,9 +439,9 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
 #pragma unroll
                         for (uint32_t e = 0; e < kParts; e++) o[nt][dt] = mfma16(vc, w[nt][x][e], o[nt][dt]);
                 }
-            if (more) load_v(next);
+            }
+            load_v(b);
         }
-        if (p.status && __builtin_amdgcn_ballot_w64(gone) != 0 && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
     }
 
     // The waves' results joined, a thread four d of a column at a time.
@@ -384,17 +456,19 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         float *at = joined + (wave * kCols + 16 * nt + col) * kPart;
+        const float sum = rows4_sum(l[nt]);
         if (grp == 0) {
             at[0] = m[nt];
-            at[1] = live[nt] ? l[nt] : __builtin_nanf("");  // a refused column passed unmasked with the others
+            at[1] = live[nt] ? sum : __builtin_nanf("");  // a refused column passed unmasked with the others
         }
 #pragma unroll
         for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[nt][dt];
     }
     __syncthreads();
-    const uint32_t used = min(p.tile_rows, p.rows - tile * p.tile_rows) * G;
-    for (uint32_t e = threadIdx.x; e < used * 32; e += 256) {
+    for (uint32_t e = threadIdx.x; e < kCols * 32; e += 256) {
         const uint32_t c = e / 32, d = e % 32 * 4;
+        uint32_t r, h;
+        if (!tile.column(p, c, r, h)) continue;
         float M = -INFINITY;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; w++) M = fmaxf(M, joined[(w * kCols + c) * kPart]);
@@ -414,18 +488,18 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
             }
             *(f32x4 *)(mine + c * kPart + 4 + d) = O;
         } else {
-            const size_t r = tile * p.tile_rows + c / G;
-            store4(p, (r * p.heads + kvh * G + c % G) * 128 + d, O / L);  // 0 / 0 of a refused row: NaN
+            store4(p, ((size_t)r * p.heads + h) * 128 + d, O / L);  // 0 / 0 of a refused row: NaN
         }
     }
 }
 
 // The parts of a tile's columns joined in their order, a thread four d of a column.
 __global__ __launch_bounds__(64) void join_kept8_kernel(AttendParams p, uint32_t cols, uint32_t pieces) {
-    const uint32_t gi = blockIdx.x / pieces, kvh = gi % p.kv_heads, tile = gi / p.kv_heads, G = p.group;
-    const uint32_t used = min(p.tile_rows, p.rows - tile * p.tile_rows) * G;
+    const uint32_t gi = blockIdx.x / pieces;
+    const Tile tile = tile_of(p, gi);
     const uint32_t c = blockIdx.x % pieces * 2 + threadIdx.x / 32, d = threadIdx.x % 32 * 4;
-    if (c >= used) return;
+    uint32_t r, h;
+    if (!tile.column(p, c, r, h)) return;
     const float *all = p.partials + ((size_t)gi * p.parts * cols + c) * kPart;
     const size_t next = (size_t)cols * kPart;
     constexpr uint32_t kBatch = 8;
@@ -458,29 +532,31 @@ __global__ __launch_bounds__(64) void join_kept8_kernel(AttendParams p, uint32_t
             O += oq[j] * f;
         }
     }
-    const size_t r = tile * p.tile_rows + c / G;
-    store4(p, (r * p.heads + kvh * G + c % G) * 128 + d, O / L);
+    store4(p, ((size_t)r * p.heads + h) * 128 + d, O / L);
 }
 
 struct Plan {
-    uint32_t tile_rows, nt, tiles, parts, chunk;
+    uint32_t tile_rows, tile_heads, splits, nt, groups, parts, chunk;  // groups: tiles times kv heads
 };
 
 Plan plan(const ts_kept8_args *k) {
     const ts_rows_args *a = &k->rows;
     const uint32_t G = a->heads / a->kv_heads;
     Plan s;
-    const uint32_t most = std::max(1u, 64 / G);  // rows that 64 columns take
+    // 64 columns at most, 32 of f32 q (three parts of q and of the weights take the registers).
+    const uint32_t most = a->q_dtype == TS_F32 ? 32 : 64;
+    s.tile_heads = std::min(G, most);
+    s.splits = (G + s.tile_heads - 1) / s.tile_heads;
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
-    s.tile_rows = std::min(run, most);
-    const uint32_t cols = s.tile_rows * G;
+    s.tile_rows = std::min(run, most / s.tile_heads);
+    const uint32_t cols = s.tile_rows * s.tile_heads;
     s.nt = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-    s.tiles = (a->rows + s.tile_rows - 1) / s.tile_rows;
     // Keys are split into parts until the groups cover the chip about twice over (four waves of two a
     // SIMD, 512 groups at a time), a part no less than one round of a group's waves.
-    const uint64_t groups = (uint64_t)s.tiles * a->kv_heads;
+    const uint64_t groups = (uint64_t)((a->rows + s.tile_rows - 1) / s.tile_rows) * a->kv_heads * s.splits;
     const uint64_t span = std::min<uint64_t>((uint64_t)a->max_position + 1, (uint64_t)a->back + s.tile_rows + kBlock);
     const uint64_t rounds = (span + kRound - 1) / kRound;
+    s.groups = (uint32_t)std::min<uint64_t>(groups, 0xffffffffu);
     s.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rounds, (1024 + groups - 1) / groups));
     s.chunk = (uint32_t)((rounds + s.parts - 1) / s.parts) * kRound;
     s.parts = (uint32_t)std::max<uint64_t>(1, (span + s.chunk - 1) / s.chunk);
@@ -488,7 +564,7 @@ Plan plan(const ts_kept8_args *k) {
 }
 
 size_t partial_bytes(const ts_kept8_args *k, const Plan &s) {
-    return s.parts <= 1 ? 0 : (size_t)s.tiles * k->rows.kv_heads * s.parts * 16 * s.nt * kPart * sizeof(float);
+    return s.parts <= 1 ? 0 : (size_t)s.groups * s.parts * 16 * s.nt * kPart * sizeof(float);
 }
 
 int check(const ts_kept8_args *k) {
@@ -538,7 +614,7 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     const ts_rows_args *a = &k->rows;
     if (a->rows == 0) return TS_OK;
     const Plan s = plan(k);
-    TS_REQUIRE((uint64_t)s.tiles * a->kv_heads * s.parts <= 0x7fffffffull / 64, "attend_kept8: %u rows in one launch", a->rows);
+    TS_REQUIRE((uint64_t)s.groups * s.parts <= 0x7fffffffull / 32, "attend_kept8: %u rows in one launch", a->rows);
     const size_t need = partial_bytes(k, s);
     if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
         return ts::fail(TS_ERR_WORKSPACE, "attend_kept8: workspace of %zu bytes, 16-byte aligned, needed", need);
@@ -552,16 +628,17 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     p.back = a->back; p.max_position = a->max_position;
     p.tile_rows = s.tile_rows; p.chunk = s.chunk; p.parts = s.parts;
     p.scale = a->scale; p.out_bf16 = a->out_dtype == TS_BF16;
-    const uint32_t groups = s.tiles * a->kv_heads * s.parts;
+    p.tile_heads = s.tile_heads; p.splits = s.splits;
+    const uint32_t groups = s.groups * s.parts;
     const bool f32 = a->q_dtype == TS_F32;
     switch (s.nt) {
     case 1: rc = f32 ? launch<1, true>(p, groups, stream) : launch<1, false>(p, groups, stream); break;
     case 2: rc = f32 ? launch<2, true>(p, groups, stream) : launch<2, false>(p, groups, stream); break;
-    default: rc = f32 ? launch<4, true>(p, groups, stream) : launch<4, false>(p, groups, stream); break;
+    default: rc = launch<4, false>(p, groups, stream); break;
     }
     if (rc || s.parts == 1) return rc;
-    const uint32_t pieces = (s.tile_rows * p.group + 1) / 2;
-    hipLaunchKernelGGL(join_kept8_kernel, dim3(s.tiles * a->kv_heads * pieces), dim3(64), 0, (hipStream_t)stream, p,
+    const uint32_t pieces = (s.tile_rows * s.tile_heads + 1) / 2;
+    hipLaunchKernelGGL(join_kept8_kernel, dim3(s.groups * pieces), dim3(64), 0, (hipStream_t)stream, p,
                        16 * s.nt, pieces);
     TS_CHECK_LAUNCH("attend_kept8 join launch");
     return TS_OK;
