@@ -18,113 +18,17 @@
 //  sums, the former in LDS, the latter by a second kernel.
 #include <algorithm>
 
-#include "kept8.h"
+#include "kept8_attend.h"
 
 namespace {
 
 using namespace kept8;
 
-constexpr uint32_t kStep = 64;           // keys a wave takes at a time
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kRound = kStep * kWaves;
-constexpr uint32_t kPart = 132;          // floats of a column's partial result: max, sum, 2 unused, 128
-constexpr float kSlack = 8.0f;           // base-2 headroom of the softmax reference point
-
-struct AttendParams {
-    const void *q;
-    const uint8_t *k, *v;
-    const float *scales;
-    void *out;
-    float *partials;  // [tile][kv head][part][16 NT][kPart], or NULL: one part
-    const uint32_t *slots, *positions;
-    uint32_t *status;
-    Place place;
-    uint32_t rows, heads, kv_heads, group, back, max_position;
-    uint32_t tile_rows, tile_heads, splits;  // rows and q heads a tile; tiles a kv head's q heads take
-    uint32_t chunk, parts;                   // keys of a part at a time (a multiple of kRound); parts
-    float scale;
-    int out_bf16;
-};
-
-// Tile gi: rows from row0, q heads from head0 of one kv head.
-struct Tile {
-    uint32_t row0, head0, end, kvh;
-    // Column c's row and q head; false where it has none.
-    TS_DEV bool column(const AttendParams &p, uint32_t c, uint32_t &r, uint32_t &h) const {
-        const uint32_t ri = c / p.tile_heads;
-        r = row0 + ri;
-        h = head0 + c % p.tile_heads;
-        return ri < p.tile_rows && r < p.rows && h < end;
-    }
-};
-TS_DEV Tile tile_of(const AttendParams &p, uint32_t gi) {
-    Tile t;
-    const uint32_t split = gi % p.splits;
-    t.kvh = gi / p.splits % p.kv_heads;
-    t.row0 = gi / (p.splits * p.kv_heads) * p.tile_rows;
-    t.head0 = t.kvh * p.group + split * p.tile_heads;
-    t.end = (t.kvh + 1) * p.group;
-    return t;
-}
-
-TS_DEV float rows4_sum(float x) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-TS_DEV float rows4_max(float x) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-TS_DEV void store4(const AttendParams &p, size_t at, f32x4 v) {
-    if (p.out_bf16)
-        *(u32x2 *)((uint16_t *)p.out + at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    else
-        *(f32x4 *)((float *)p.out + at) = v;
-}
-
-// Bytes of a word of four positions pos .. pos + 3 that lie in [lo, hi].
-TS_DEV uint32_t within4(uint32_t w, uint32_t pos, uint32_t lo, uint32_t hi) {
-    uint32_t m = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; i++) m |= (pos + i >= lo && pos + i <= hi) ? 0xffu << (8 * i) : 0u;
-    return w & m;
-}
-
-// Two f32 as packed bf16, rounded to nearest even; NaN stays NaN.
-TS_DEV uint32_t bf16_pair(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(ts_f32x2{a, b}, ts_bf16x2));
-}
-// P parts of two f32 values: bf16 values that add up to them (24 bits in three parts, 8 in one).
-template <uint32_t P>
-TS_DEV void split_pair(float a, float b, uint32_t (&w)[P]) {
-#pragma unroll
-    for (uint32_t e = 0; e < P; e++) {
-        w[e] = bf16_pair(a, b);
-        if (e + 1 < P) {
-            a -= lo_bf16(w[e]);
-            b -= hi_bf16(w[e]);
-        }
-    }
-}
-
-// The table and the scales are read by scalar loads (their addresses are uniform), which return
-// beside the codes' vector loads instead of behind them.
-typedef const __attribute__((address_space(4))) uint32_t const_u32;
-typedef const __attribute__((address_space(4))) float const_f32;
-template <class T>
-TS_DEV T in_constant(const void *p) { return (T)(uintptr_t)p; }
-
-// Keeps what follows from being computed earlier: eight registers of codes at a time are widened,
-// where the compiler would widen all of a step's and spill.
-TS_DEV void pin(u32x4 &v) { asm volatile("" : "+v"(v)); }
 
 template <int NT, bool QF32>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(AttendParams p) {
+__global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
     constexpr uint32_t kCols = 16 * NT, kParts = QF32 ? 3 : 1;
     extern __shared__ __attribute__((aligned(16))) float joined[];  // [kWaves][kCols][kPart]
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -136,8 +40,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
     uint32_t pos[NT], from[NT], slot[NT];
     bool live[NT];
     bf16x8 q[NT][4][kParts];
-    const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes into q, exactly
-    const float sl = p.scale == 0.0f ? 0x1p-100f : fabsf(p.scale) * 1.4426950408889634f;  // to base 2
+    const float sl = base2_scale(p.scale);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         uint32_t r, h;
@@ -149,27 +52,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
             atomicOr(p.status, slot[nt] >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
         from[nt] = pos[nt] > p.back ? pos[nt] - p.back : 0;
         const size_t at = live[nt] ? ((size_t)r * p.heads + h) * 128 : 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {  // operand j: d 64 (j / 2) + 16 grp + 8 (j % 2) ..
-            const uint32_t d = 64 * (j >> 1) + 16 * grp + 8 * (j & 1);
-            if (!QF32) {
-                u32x4 w = *(const u32x4 *)((const uint16_t *)p.q + at + d);
-                w = live[nt] ? w ^ qsign : u32x4{0, 0, 0, 0};
-                q[nt][j][0] = as_bf16x8(w);
-            } else {
-                const f32x4 x = *(const f32x4 *)((const float *)p.q + at + d);
-                const f32x4 y = *(const f32x4 *)((const float *)p.q + at + d + 4);
-                uint32_t w[4][kParts];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float a = e < 2 ? x[2 * e] : y[2 * e - 4], b = e < 2 ? x[2 * e + 1] : y[2 * e - 3];
-                    if (qsign) { a = -a; b = -b; }
-                    split_pair<kParts>(live[nt] ? a : 0.0f, live[nt] ? b : 0.0f, w[e]);
-                }
-#pragma unroll
-                for (uint32_t e = 0; e < kParts; e++) q[nt][j][e] = as_bf16x8(u32x4{w[0][e], w[1][e], w[2][e], w[3][e]});
-            }
-        }
+        load_q<QF32, kParts>(p, live[nt], at, grp, q[nt]);
     }
 
     float m[NT], l[NT];
@@ -235,8 +118,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
         const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, span = hi - base0;
         worked |= (uint64_t)part * p.chunk <= span;
 
-        // The blocks of a step, block j of it by its page (one whose page is not held: bit j of `lost`,
-        // read as page 0), and the scales of them.
+        // The blocks of a step; bit j of `lost`: block j's page is not held.
         struct Blocks {
             uint32_t at[4], lost;
         };
@@ -245,19 +127,9 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
             b.lost = 0;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t key = min(base / kBlock + j, last) * kBlock;
-                if (p.place.table) {
-                    const_u32 *t = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
-                    uint32_t id = t[key >> p.place.page_shift];
-                    if (id >= p.place.pages) {
-                        id = 0;
-                        b.lost |= 1u << j;
-                    }
-                    const uint32_t in = key & ((1u << p.place.page_shift) - 1);
-                    b.at[j] = (id << (p.place.page_shift - 4)) + in / kBlock;
-                } else {
-                    b.at[j] = now * (p.place.keys / kBlock) + key / kBlock;
-                }
+                bool gone;
+                b.at[j] = block_of(p.place, now, min(base / kBlock + j, last) * kBlock, gone);
+                b.lost |= gone ? 1u << j : 0u;
             }
             return b;
         };
@@ -308,13 +180,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
             // (The last step's codes are asked for once more, from the caches: a branch around the
             // loads would keep two copies of them in registers.)
             b = look(more ? base0 + (uint32_t)off : base);
-            f32x4 s[4][NT];
+            f32x4 s[NT][4];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 pin(kf[t][0]);
                 pin(kf[t][1]);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[t][nt] = f32x4{0, 0, 0, 0};
+                for (int nt = 0; nt < NT; nt++) s[nt][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const u32x4 w = kf[t][j >> 1];
@@ -322,7 +194,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (uint32_t e = 0; e < kParts; e++) s[t][nt] = mfma16(kc, q[nt][j][e], s[t][nt]);
+                        for (uint32_t e = 0; e < kParts; e++) s[nt][t] = mfma16(kc, q[nt][j][e], s[nt][t]);
                 }
             }
             load_k(b);
@@ -335,16 +207,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
                 uint32_t seen[NT];  // a bit for each of the lane's 16 keys
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    // Keys e of the lane with from <= key0 + e <= pos.
-                    const int first = max((int)(from[nt] - key0), 0), end = min((int)(pos[nt] - key0) + 1, 16);
-                    const uint32_t upto = end <= 0 ? 0u : (1u << end) - 1;
-                    seen[nt] = act[nt] && first < 16 ? upto & (0xffffu << first) : 0u;
+                    seen[nt] = act[nt] ? seen_keys(key0, from[nt], pos[nt]) : 0u;
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const float x = gone ? __builtin_nanf("") : s[t][nt][e];
-                            s[t][nt][e] = seen[nt] >> (4 * t + e) & 1 ? x : -INFINITY;
+                            const float x = gone ? __builtin_nanf("") : s[nt][t][e];
+                            s[nt][t][e] = seen[nt] >> (4 * t + e) & 1 ? x : -INFINITY;
                         }
                 }
                 // Codes outside [lo, hi] may be anything: as zeros they add nothing.
@@ -391,43 +260,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attend_kept8_kernel(Atte
             }
             bf16x8 w[NT][2][kParts];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float mx = s[0][nt][0];
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[t][nt][e]);
-                mx = rows4_max(mx) * sl;
-                // The reference point moves only when a score passes it by 2^kSlack: most steps leave
-                // the sums and O unscaled, and no weight passes 2^kSlack.
-                const bool raise = mx > m[nt] + kSlack;
-                const float mn = raise ? mx : m[nt];
-                const float mo = mn == -INFINITY ? 0.0f : mn;
-                float sum = 0.0f;
-                uint32_t pw[8][kParts];
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const float a = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e], sl, -mo));
-                        const float c = __builtin_amdgcn_exp2f(fmaf(s[t][nt][e + 1], sl, -mo));
-                        sum += a + c;
-                        split_pair<kParts>(a, c, pw[2 * t + e / 2]);
-                    }
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (uint32_t e = 0; e < kParts; e++)
-                        w[nt][x][e] = as_bf16x8(u32x4{pw[4 * x][e], pw[4 * x + 1][e], pw[4 * x + 2][e], pw[4 * x + 3][e]});
-                if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-                    const float alpha = raise ? __builtin_amdgcn_exp2f(m[nt] - mn) : 1.0f;
-                    l[nt] *= alpha;
-                    m[nt] = mn;
-#pragma unroll
-                    for (int dt = 0; dt < 8; dt++) o[nt][dt] *= alpha;
-                }
-                l[nt] += sum;  // of the lane's keys: the column's four lanes are added at the end
-            }
+            for (int nt = 0; nt < NT; nt++) weigh<kParts, 8>(s[nt], sl, m[nt], l[nt], o[nt], w[nt]);
 #pragma unroll
             for (int dt = 0; dt < 8; dt++) {
                 pin(vf[dt]);
@@ -535,36 +368,37 @@ __global__ __launch_bounds__(64) void join_kept8_kernel(AttendParams p, uint32_t
     store4(p, ((size_t)r * p.heads + h) * 128 + d, O / L);
 }
 
+// How a call runs: `columns` (row, q head) pairs a tile; 16: the kernel above, more: kept8_rows.hip's.
 struct Plan {
-    uint32_t tile_rows, tile_heads, splits, nt, groups, parts, chunk;  // groups: tiles times kv heads
+    uint32_t columns, tile_rows, groups, parts, chunk;  // groups: tiles times kv heads
 };
 
 Plan plan(const ts_kept8_args *k) {
     const ts_rows_args *a = &k->rows;
     const uint32_t G = a->heads / a->kv_heads;
+    const bool f32 = a->q_dtype == TS_F32;
     Plan s;
-    // 64 columns at most, 32 of f32 q (three parts of q and of the weights take the registers).
-    const uint32_t most = a->q_dtype == TS_F32 ? 32 : 64;
-    s.tile_heads = std::min(G, most);
-    s.splits = (G + s.tile_heads - 1) / s.tile_heads;
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
-    s.tile_rows = std::min(run, most / s.tile_heads);
-    const uint32_t cols = s.tile_rows * s.tile_heads;
-    s.nt = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-    // Keys are split into parts until the groups cover the chip about twice over (four waves of two a
-    // SIMD, 512 groups at a time), a part no less than one round of a group's waves.
-    const uint64_t groups = (uint64_t)((a->rows + s.tile_rows - 1) / s.tile_rows) * a->kv_heads * s.splits;
-    const uint64_t span = std::min<uint64_t>((uint64_t)a->max_position + 1, (uint64_t)a->back + s.tile_rows + kBlock);
-    const uint64_t rounds = (span + kRound - 1) / kRound;
+    const uint64_t wanted = (uint64_t)run * G;
+    // f32 q, in three parts, leaves a wave of the shared kernel 16 columns.
+    s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 ? 128 : 256;
+    s.tile_rows = std::min(run, s.columns / G);
+    const uint64_t groups = (uint64_t)((a->rows + s.tile_rows - 1) / s.tile_rows) * a->kv_heads;
     s.groups = (uint32_t)std::min<uint64_t>(groups, 0xffffffffu);
-    s.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rounds, (1024 + groups - 1) / groups));
-    s.chunk = (uint32_t)((rounds + s.parts - 1) / s.parts) * kRound;
+    // Keys are split into parts until the groups cover the chip about twice over (groups of four waves
+    // of two a SIMD: 512 at a time; of eight: 256), a part no less than a round of a group's waves.
+    const uint32_t least = s.columns == 16 ? kRound : 4 * kStep;
+    const uint64_t want = s.columns <= 64 ? 1024 : 512;
+    const uint64_t span = std::min<uint64_t>((uint64_t)a->max_position + 1, (uint64_t)a->back + s.tile_rows + kBlock);
+    const uint64_t rounds = (span + least - 1) / least;
+    s.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rounds, (want + groups - 1) / groups));
+    s.chunk = (uint32_t)((rounds + s.parts - 1) / s.parts) * least;
     s.parts = (uint32_t)std::max<uint64_t>(1, (span + s.chunk - 1) / s.chunk);
     return s;
 }
 
 size_t partial_bytes(const ts_kept8_args *k, const Plan &s) {
-    return s.parts <= 1 ? 0 : (size_t)s.groups * s.parts * 16 * s.nt * kPart * sizeof(float);
+    return s.parts <= 1 ? 0 : (size_t)s.groups * s.parts * s.columns * kPart * sizeof(float);
 }
 
 int check(const ts_kept8_args *k) {
@@ -614,7 +448,7 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     const ts_rows_args *a = &k->rows;
     if (a->rows == 0) return TS_OK;
     const Plan s = plan(k);
-    TS_REQUIRE((uint64_t)s.groups * s.parts <= 0x7fffffffull / 32, "attend_kept8: %u rows in one launch", a->rows);
+    TS_REQUIRE((uint64_t)s.groups * s.parts <= 0x7fffffffull / 128, "attend_kept8: %u rows in one launch", a->rows);
     const size_t need = partial_bytes(k, s);
     if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
         return ts::fail(TS_ERR_WORKSPACE, "attend_kept8: workspace of %zu bytes, 16-byte aligned, needed", need);
@@ -628,18 +462,15 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     p.back = a->back; p.max_position = a->max_position;
     p.tile_rows = s.tile_rows; p.chunk = s.chunk; p.parts = s.parts;
     p.scale = a->scale; p.out_bf16 = a->out_dtype == TS_BF16;
-    p.tile_heads = s.tile_heads; p.splits = s.splits;
     const uint32_t groups = s.groups * s.parts;
     const bool f32 = a->q_dtype == TS_F32;
-    switch (s.nt) {
-    case 1: rc = f32 ? launch<1, true>(p, groups, stream) : launch<1, false>(p, groups, stream); break;
-    case 2: rc = f32 ? launch<2, true>(p, groups, stream) : launch<2, false>(p, groups, stream); break;
-    default: rc = launch<4, false>(p, groups, stream); break;
-    }
+    if (s.columns > 16)
+        rc = ts::kept8_rows_launch(p, s.columns, f32, groups, stream);
+    else
+        rc = f32 ? launch<1, true>(p, groups, stream) : launch<1, false>(p, groups, stream);
     if (rc || s.parts == 1) return rc;
-    const uint32_t pieces = (s.tile_rows * s.tile_heads + 1) / 2;
-    hipLaunchKernelGGL(join_kept8_kernel, dim3(s.groups * pieces), dim3(64), 0, (hipStream_t)stream, p,
-                       16 * s.nt, pieces);
+    const uint32_t pieces = (s.tile_rows * p.group + 1) / 2;
+    hipLaunchKernelGGL(join_kept8_kernel, dim3(s.groups * pieces), dim3(64), 0, (hipStream_t)stream, p, s.columns, pieces);
     TS_CHECK_LAUNCH("attend_kept8 join launch");
     return TS_OK;
 }
