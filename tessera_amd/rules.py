@@ -406,30 +406,34 @@ def top_k(x, k, ids=None):
 
 KEPT_BLOCK = 16  # positions a kept block holds
 _INTS = (torch.int32, torch.uint32)
+_CODES = (torch.uint8, torch.float8_e4m3fn)
+_F32 = (torch.float32,)
+_ROWS = (torch.float32, torch.bfloat16)
 
 
-def _checked(what, device, **tensors):
-    """Contiguous tensors on `device`, the one that the call is made on; None passes."""
-    if device.type != "cuda":
-        raise ValueError(f"{what}: tensors on {device}, not on a GPU")
-    for name, t in tensors.items():
-        if t is not None and (t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be contiguous and on {device}")
+def _checked(what, on, *tensors):
+    """Each (name, tensor, its types, its elements or -1): contiguous and on GPU `on`; None passes. (The
+    operators below look at their tensors in one expression, and come here to say what is wrong: a loop
+    over ten tensors costs as much as the launch.)"""
+    if on < 0:
+        raise ValueError(f"{what}: tensors not on a GPU")
+    for name, t, types, count in tensors:
+        if t is not None and (t.get_device() != on or t.dtype not in types or not t.is_contiguous() or
+                              (count >= 0 and t.numel() != count)):
+            raise ValueError(f"{what}: {name} must be contiguous, on GPU {on}, of " +
+                             " or ".join(str(d).replace("torch.", "") for d in types) +
+                             (f", {count} elements" if count >= 0 else ""))
 
 
-def _indices(what, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.dtype not in _INTS:
-            raise ValueError(f"{what}: {name} must be 32-bit integers")
-
-
-def _call_on(device, name, args):
-    """The call on `device`'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        abi.call(name, C.byref(args), _stream())
+def _call_on(on, fn, args):
+    """The call on GPU `on`'s current stream, whichever device is current."""
+    if on == torch.cuda.current_device():
+        code = fn(args, _stream() if _raw_stream is None else _raw_stream(on))
     else:
-        with torch.cuda.device(device):
-            abi.call(name, C.byref(args), _stream())
+        with torch.cuda.device(on):
+            code = fn(args, _stream())
+    if code:
+        abi.check(code, fn.__name__)
 
 
 def kept8(pages, kv_heads, page=16, device="cuda"):
@@ -441,28 +445,23 @@ def kept8(pages, kv_heads, page=16, device="cuda"):
     return k, v, torch.zeros((blocks, (kv_heads + 1) // 2 * 2, 2), dtype=torch.float32, device=device)
 
 
-def _kept8_sizes(what, k, v, scales, kv_heads, page):
-    """Pages that the blocks hold."""
-    blocks = k.shape[0]
-    if k.shape != (blocks, kv_heads, KEPT_BLOCK, 128) or v.shape != (blocks, kv_heads, 128, KEPT_BLOCK) or \
-            scales.shape != (blocks, (kv_heads + 1) // 2 * 2, 2) or scales.dtype != torch.float32 or \
-            _DT.get(k.dtype) != abi.TS_E4M3 or _DT.get(v.dtype) != abi.TS_E4M3:
+def _kept8_blocks(what, k, v, scales, kv_heads):
+    """How many blocks there are; the shapes are kept8()'s."""
+    blocks, *one = k.shape
+    if one != [kv_heads, KEPT_BLOCK, 128] or v.shape != (blocks, kv_heads, 128, KEPT_BLOCK) or \
+            scales.shape != (blocks, (kv_heads + 1) // 2 * 2, 2):
         raise ValueError(f"{what}: kept blocks of {kv_heads} heads as kept8() makes them")
-    return blocks * KEPT_BLOCK // page
+    return blocks
 
 
-def _slots(what, table, kept_pages, slot_rows, keys):
+def _slots(what, table, kept_pages, held, keys):
     """Slots that the table (or the dense kept rows) holds."""
     if table is None:
-        return slot_rows // keys
-    if kept_pages < 1 or table.numel() % kept_pages:
+        return held // keys if keys else 0
+    slots, rest = divmod(table.numel(), kept_pages) if kept_pages > 0 else (0, 1)
+    if rest:
         raise ValueError(f"{what}: a table of {table.numel()} entries is not whole slots of {kept_pages}")
-    return table.numel() // kept_pages
-
-
-def _row_stride(x):
-    """Elements from a row of x [rows, heads, 128] to the next (one row: any will do)."""
-    return 0 if x is None else x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+    return slots
 
 
 def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=None, k_gain=None, angles=None,
@@ -473,45 +472,60 @@ def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=
     rotation. `scales` given: k_kept, v_kept are kept8() blocks; else bf16 rows [*, kv_heads, 128].
     Rows of one call that fall into one block of 16 positions stand together, in order. status: int32
     device word, TS_STATUS_* bits of rows that were not kept. Returns q_out."""
-    rows, kv_heads, width = k.shape
-    heads = q.shape[1] if q is not None else 0
-    x = _DT.get(k.dtype)
-    if v.shape != k.shape or v.dtype != k.dtype or (q is not None and (q.dtype != k.dtype or q.shape != (rows, heads, width))):
-        raise ValueError("append_rows: q, k and v must be rows of one type and width")
-    for t in (q, k, v):
-        if t is not None and (t.stride(2) != 1 or t.stride(1) != width or t.device != k.device):
-            raise ValueError("append_rows: a row's heads must lie back to back, on one device")
-    _checked("append_rows", k.device, k_kept=k_kept, v_kept=v_kept, slots=slots, positions=positions, table=table,
-             scales=scales, q_gain=q_gain, k_gain=k_gain, angles=angles, q_out=q_out, status=status)
-    _indices("append_rows", slots=slots, positions=positions, table=table, status=status)
-    if slots.numel() != rows or positions.numel() != rows:
-        raise ValueError(f"append_rows: {rows} rows need as many slots and positions")
-    for g in (q_gain, k_gain):
-        if g is not None and (g.dtype != torch.float32 or g.numel() != width):
-            raise ValueError("append_rows: gains are f32, one a column")
-    if angles is not None and (angles.dtype != torch.float32 or angles.numel() != angles.shape[0] * width):
-        raise ValueError("append_rows: angles as rope_table makes them")
-    if scales is not None:
-        pages = _kept8_sizes("append_rows", k_kept, v_kept, scales, kv_heads, page)
-        held, kv = k_kept.shape[0] * KEPT_BLOCK, abi.TS_E4M3
-    else:
-        held, kv = k_kept.numel() // (kv_heads * width) if kv_heads else 0, abi.TS_BF16
-        if k_kept.dtype != torch.bfloat16 or v_kept.dtype != torch.bfloat16 or v_kept.numel() != k_kept.numel() or \
-                k_kept.shape[-2:] != (kv_heads, width):
-            raise ValueError("append_rows: kept rows are bf16 [rows, kv_heads, 128], or blocks with their scales")
-        pages = held // page
+    what = "append_rows"
+    rows, kv_heads, width = shape = k.shape
+    on, x = k.get_device(), k.dtype
+    (k_stride, k_head, k_one), (v_stride, v_head, v_one) = k.stride(), v.stride()
+    if x not in _ROWS or v.dtype is not x or v.shape != shape or v.get_device() != on or k_one != 1 or v_one != 1 or \
+            ((k_head != width or v_head != width) and kv_heads > 1):
+        raise ValueError("append_rows: k and v must be rows of one type (f32 or bf16), width and device, a row's "
+                         "heads back to back")
+    heads = q_stride = q_type = 0
     if q is not None:
+        heads = q.size(1)
+        q_stride, q_head, q_one = q.stride()
+        if q.dtype is not x or q.shape != (rows, heads, width) or q.get_device() != on or q_one != 1 or \
+                (q_head != width and heads > 1):
+            raise ValueError("append_rows: q must be rows as k's, a row's heads back to back")
         if q_out is None:
-            q_out = torch.empty((rows, heads, width), dtype=q.dtype, device=q.device)
-        elif q_out.shape != q.shape:
-            raise ValueError("append_rows: q_out must have q's shape")
-    a = abi.AppendArgs(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_gain), _ptr(k_gain), _ptr(angles), _ptr(q_out),
-                       k_kept.data_ptr(), v_kept.data_ptr(), _ptr(scales), slots.data_ptr(), positions.data_ptr(),
-                       _ptr(table), _ptr(status), rows, heads, kv_heads, width, _row_stride(q), _row_stride(k),
-                       _row_stride(v), keys, _slots("append_rows", table, kept_pages, held, keys), kept_pages, page, pages,
-                       angles.shape[0] if angles is not None else 0, 1 if halves else 0, -1 if x is None else x,
-                       -1 if q_out is None else _DT.get(q_out.dtype, -1), kv, eps)
-    _call_on(k.device, "tessera_hip_append_rows", a)
+            q_out = q.new_empty(rows, heads, width)
+        else:
+            _checked(what, on, ("q_out", q_out, _ROWS, rows * heads * width))
+        q_type = _DT[q_out.dtype]
+    if rows == 1:  # any distance will do
+        q_stride, k_stride, v_stride = heads * width, kv_heads * width, kv_heads * width
+    if scales is not None:
+        held = _kept8_blocks(what, k_kept, v_kept, scales, kv_heads) * KEPT_BLOCK
+        kept, kv = _CODES, abi.TS_E4M3
+    else:
+        held = k_kept.numel() // (kv_heads * width) if kv_heads else 0
+        kept, kv = (torch.bfloat16,), abi.TS_BF16
+        if k_kept.shape != v_kept.shape or k_kept.shape[-2:] != (kv_heads, width):
+            raise ValueError("append_rows: kept rows are bf16 [rows, kv_heads, 128], or blocks with their scales")
+    f32 = torch.float32
+    if not (on >= 0 and k_kept.get_device() == v_kept.get_device() == slots.get_device() == positions.get_device() == on
+            and k_kept.dtype in kept and v_kept.dtype in kept and slots.dtype in _INTS and positions.dtype in _INTS
+            and slots.numel() == positions.numel() == rows and k_kept.is_contiguous() and v_kept.is_contiguous()
+            and slots.is_contiguous() and positions.is_contiguous()
+            and (table is None or table.get_device() == on and table.dtype in _INTS and table.is_contiguous())
+            and (scales is None or scales.get_device() == on and scales.dtype is f32 and scales.is_contiguous())
+            and (angles is None or angles.get_device() == on and angles.dtype is f32 and angles.is_contiguous())
+            and (q_gain is None or q_gain.get_device() == on and q_gain.dtype is f32 and q_gain.numel() == width and q_gain.is_contiguous())
+            and (k_gain is None or k_gain.get_device() == on and k_gain.dtype is f32 and k_gain.numel() == width and k_gain.is_contiguous())
+            and (status is None or status.get_device() == on and status.dtype in _INTS)):
+        _checked(what, on, ("k_kept", k_kept, kept, -1), ("v_kept", v_kept, kept, -1), ("slots", slots, _INTS, rows),
+                 ("positions", positions, _INTS, rows), ("table", table, _INTS, -1), ("scales", scales, _F32, -1),
+                 ("angles", angles, _F32, -1), ("q_gain", q_gain, _F32, width), ("k_gain", k_gain, _F32, width),
+                 ("status", status, _INTS, -1))
+    a = abi.AppendArgs(None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                       None if q_gain is None else q_gain.data_ptr(), None if k_gain is None else k_gain.data_ptr(),
+                       None if angles is None else angles.data_ptr(), None if q is None else q_out.data_ptr(),
+                       k_kept.data_ptr(), v_kept.data_ptr(), None if scales is None else scales.data_ptr(),
+                       slots.data_ptr(), positions.data_ptr(), None if table is None else table.data_ptr(),
+                       None if status is None else status.data_ptr(), rows, heads, kv_heads, width, q_stride,
+                       k_stride, v_stride, keys, _slots(what, table, kept_pages, held, keys), kept_pages, page, held // page,
+                       0 if angles is None else angles.numel() // width, halves, _DT[x], q_type, kv, eps)
+    _call_on(on, abi.load().tessera_hip_append_rows, a)
     return q_out
 
 
@@ -521,30 +535,39 @@ def attend_kept8(q, k, v, scales, slots, positions, *, keys, scale, table=None, 
     rows of a sequence, prompts. run: how many rows of a slot stand together (a hint: it groups rows and
     picks the kernel). max_position (an upper bound on positions) defaults to their maximum (a host
     read: pass it when capturing a graph). out f32 or bf16."""
+    what = "attend_kept8"
     rows, heads, width = q.shape
-    kv_heads = k.shape[1]
-    pages = _kept8_sizes("attend_kept8", k, v, scales, kv_heads, page)
+    kv_heads, on = k.shape[1], q.get_device()
+    held = _kept8_blocks(what, k, v, scales, kv_heads) * KEPT_BLOCK
     if out is None:
-        out = torch.empty((rows, heads, width), dtype=out_dtype, device=q.device)
+        out = q.new_empty(rows, heads, width) if out_dtype is q.dtype else q.new_empty(q.shape, dtype=out_dtype)
     elif out.shape != q.shape:
         raise ValueError("attend_kept8: out must have q's shape")
-    _checked("attend_kept8", q.device, q=q, k=k, v=v, scales=scales, slots=slots, positions=positions, table=table,
-             out=out, status=status)
-    _indices("attend_kept8", slots=slots, positions=positions, table=table, status=status)
-    if slots.numel() != rows or positions.numel() != rows:
-        raise ValueError(f"attend_kept8: {rows} rows need as many slots and positions")
+    if not (on >= 0 and k.get_device() == v.get_device() == scales.get_device() == slots.get_device()
+            == positions.get_device() == out.get_device() == on and q.dtype in _ROWS and out.dtype in _ROWS
+            and k.dtype in _CODES and v.dtype in _CODES and scales.dtype is torch.float32 and slots.dtype in _INTS
+            and positions.dtype in _INTS and slots.numel() == positions.numel() == rows and q.is_contiguous()
+            and k.is_contiguous() and v.is_contiguous() and scales.is_contiguous() and slots.is_contiguous()
+            and positions.is_contiguous() and out.is_contiguous()
+            and (table is None or table.get_device() == on and table.dtype in _INTS and table.is_contiguous())
+            and (status is None or status.get_device() == on and status.dtype in _INTS)):
+        _checked(what, on, ("q", q, _ROWS, -1), ("k", k, _CODES, -1), ("v", v, _CODES, -1),
+                 ("scales", scales, _F32, -1), ("slots", slots, _INTS, rows), ("positions", positions, _INTS, rows),
+                 ("table", table, _INTS, -1), ("out", out, _ROWS, -1), ("status", status, _INTS, -1))
     if max_position is None:
         max_position = int(positions.max().item()) if rows else 0
-    r = abi.RowsArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                     _ptr(table), None, 0, rows, keys, heads, kv_heads, width, back, kept_pages, page, scale,
-                     _DT.get(q.dtype, -1), abi.TS_E4M3, _DT.get(out.dtype, -1), max_position, _ptr(status))
-    a = abi.Kept8Args(r, scales.data_ptr(), _slots("attend_kept8", table, kept_pages, k.shape[0] * KEPT_BLOCK, keys),
-                      pages, run)
-    need = abi.load().tessera_hip_attend_kept8_workspace(C.byref(a))
+    a = abi.Kept8Args(abi.RowsArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), slots.data_ptr(),
+                                   positions.data_ptr(), None if table is None else table.data_ptr(), None, 0, rows,
+                                   keys, heads, kv_heads, width, back, kept_pages, page, scale, _DT[q.dtype],
+                                   abi.TS_E4M3, _DT[out.dtype], max_position,
+                                   None if status is None else status.data_ptr()),
+                      scales.data_ptr(), _slots(what, table, kept_pages, held, keys), held // page, run)
+    lib = abi.load()
+    need = lib.tessera_hip_attend_kept8_workspace(a)
     if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        scratch = slots.new_empty((need + 3) // 4)
         a.rows.workspace, a.rows.workspace_bytes = scratch.data_ptr(), need
-    _call_on(q.device, "tessera_hip_attend_kept8", a)
+    _call_on(on, lib.tessera_hip_attend_kept8, a)
     return out
 
 
@@ -555,36 +578,53 @@ def verify(logits, drafts, uniforms=None, *, counts=None, first=None, draft_prob
     and most). uniforms [seqs, most + 1] f32 in [0, 1): one a draft, the last for the token after the
     accepted ones; None: greedy. draft_probs f32 [seqs, most, width]: the drafter's probabilities; None: it
     had only the one token. temperature: a number or f32 [seqs] (<= 0: greedy).
-    Returns (tokens [seqs, most + 1], accepted [seqs]) int32: the accepted drafts, the next token, then
-    `width`."""
+    Returns (tokens [seqs, most + 1], accepted [seqs]) of drafts' type: the accepted drafts, the next token,
+    then `width`."""
+    what = "verify"
     rows, width = logits.shape
     seqs, most = drafts.shape
+    on = logits.get_device()
     per = temperature if isinstance(temperature, torch.Tensor) else None
-    stride = logits.stride(0) if rows > 1 else width
-    if (logits.stride(1) != 1 and width > 1) or stride < width:
-        raise ValueError("verify: a row's logits must lie back to back, rows apart")
+    stride, inner = logits.stride()
+    if rows <= 1:
+        stride = width
+    if (inner != 1 and width > 1) or stride < width or logits.dtype not in _ROWS:
+        raise ValueError("verify: logits are f32 or bf16, a row's back to back, rows apart")
     if tokens is None:
-        tokens = torch.empty((seqs, most + 1), dtype=torch.int32, device=logits.device)
+        tokens = drafts.new_empty(seqs, most + 1)
     if accepted is None:
-        accepted = torch.empty(seqs, dtype=torch.int32, device=logits.device)
-    _checked("verify", logits.device, drafts=drafts, uniforms=uniforms, draft_probs=draft_probs, temperature=per,
-             counts=counts, first=first, tokens=tokens, accepted=accepted, status=status)
-    _indices("verify", drafts=drafts, counts=counts, first=first, tokens=tokens, accepted=accepted, status=status)
-    for name, t, shape in (("uniforms", uniforms, (seqs, most + 1)), ("draft_probs", draft_probs, (seqs, most, width)),
-                           ("temperature", per, (seqs,))):
-        if t is not None and (t.dtype != torch.float32 or t.shape != shape):
-            raise ValueError(f"verify: {name} must be f32 {list(shape)}")
-    for name, t, shape in (("counts", counts, (seqs,)), ("first", first, (seqs,)), ("tokens", tokens, (seqs, most + 1)),
-                           ("accepted", accepted, (seqs,))):
-        if t is not None and t.shape != shape:
-            raise ValueError(f"verify: {name} must be {list(shape)}")
-    a = abi.VerifyArgs(logits.data_ptr(), _ptr(drafts), _ptr(uniforms), _ptr(draft_probs), _ptr(per), _ptr(counts),
-                       _ptr(first), tokens.data_ptr(), accepted.data_ptr(), None, 0, _ptr(status), seqs, most, rows,
-                       width, stride, _DT.get(logits.dtype, -1),
-                       0.0 if per is not None else temperature)
-    need = abi.load().tessera_hip_verify_workspace(C.byref(a))
+        accepted = drafts.new_empty(seqs)
+    if draft_probs is not None and draft_probs.shape != (seqs, most, width):
+        raise ValueError(f"verify: draft_probs must be f32 {[seqs, most, width]}")
+    f32, each = torch.float32, seqs * (most + 1)
+    if not (on >= 0 and drafts.get_device() == tokens.get_device() == accepted.get_device() == on
+            and drafts.dtype in _INTS and tokens.dtype in _INTS and accepted.dtype in _INTS and drafts.is_contiguous()
+            and tokens.is_contiguous() and accepted.is_contiguous() and tokens.numel() == each
+            and accepted.numel() == seqs
+            and (uniforms is None or uniforms.get_device() == on and uniforms.dtype is f32
+                 and uniforms.numel() == each and uniforms.is_contiguous())
+            and (draft_probs is None or draft_probs.get_device() == on and draft_probs.dtype is f32
+                 and draft_probs.is_contiguous())
+            and (counts is None or counts.get_device() == on and counts.dtype in _INTS and counts.numel() == seqs
+                 and counts.is_contiguous())
+            and (first is None or first.get_device() == on and first.dtype in _INTS and first.numel() == seqs
+                 and first.is_contiguous())
+            and (per is None or per.get_device() == on and per.dtype is f32 and per.numel() == seqs
+                 and per.is_contiguous())
+            and (status is None or status.get_device() == on and status.dtype in _INTS)):
+        _checked(what, on, ("drafts", drafts, _INTS, -1), ("uniforms", uniforms, _F32, each),
+                 ("draft_probs", draft_probs, _F32, -1), ("temperature", per, _F32, seqs),
+                 ("counts", counts, _INTS, seqs), ("first", first, _INTS, seqs), ("tokens", tokens, _INTS, each),
+                 ("accepted", accepted, _INTS, seqs), ("status", status, _INTS, -1))
+    a = abi.VerifyArgs(logits.data_ptr(), drafts.data_ptr(), None if uniforms is None else uniforms.data_ptr(),
+                       None if draft_probs is None else draft_probs.data_ptr(), None if per is None else per.data_ptr(),
+                       None if counts is None else counts.data_ptr(), None if first is None else first.data_ptr(),
+                       tokens.data_ptr(), accepted.data_ptr(), None, 0, None if status is None else status.data_ptr(),
+                       seqs, most, rows, width, stride, _DT[logits.dtype], 0.0 if per is not None else temperature)
+    lib = abi.load()
+    need = lib.tessera_hip_verify_workspace(a)
     if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        scratch = drafts.new_empty((need + 3) // 4)
         a.workspace, a.workspace_bytes = scratch.data_ptr(), need
-    _call_on(logits.device, "tessera_hip_verify", a)
+    _call_on(on, lib.tessera_hip_verify, a)
     return tokens, accepted
