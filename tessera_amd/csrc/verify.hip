@@ -6,25 +6,26 @@
 //
 //   p_i = e_i / Z,  e_i = exp((x_i - M) / temperature),  M = max x,  Z = sum of e
 //
-// The vocabulary is cut into chunks of 2048, a group each:
-//   1. every row's chunks: maximum, its first index, and the sum of e against the chunk's own maximum;
-//   2. each sequence's decision, from its rows' chunk results (every group of a sequence works it out
-//      for itself: a few hundred values), the weights' sum over each chunk of the row to draw from, and,
-//      by the group that is last to leave its sum, the draw: the chunk by the chunks' sums, then the
-//      index within it.
+// Two launches:
+//   1. rows: every row in chunks of a few pieces of 2048, a group each: the chunk's maximum, its first
+//      index, and its sum of e against that maximum;
+//   2. draw: each group works out its sequence's verdict from the rows' chunks (a few hundred values, 3 us),
+//      then weighs its share of the row to draw from, a wave a run of 256 indices at a time. The
+//      group that is last of a sequence to do so finds the run where the running sum passes u times the
+//      whole, and one wave the index in it.
+// Code that runs once costs its fetch (about 1 KiB a microsecond), so nothing here is unrolled or inlined
+// twice that need not be.
 // Exponentials and sums are in f64 (the vector unit's f64 rate is f32's here): the draw compares u with
 // running sums whose borders lie 1 / 150,000 apart and closer, and f32 would move them by 1e-7 of the whole.
+#include <algorithm>
+
 #include "common.h"
 
 namespace {
 
-constexpr uint32_t kWaves = 4, kThreads = 64 * kWaves, kEach = 8, kChunk = kThreads * kEach;
-constexpr uint32_t kRuns = kEach / 4;  // runs of 256 indices a wave takes of a chunk
-// A lane has four consecutive indices of each run: its value j is index place(wave, lane, j) of the chunk,
-// in index order by (wave, j / 4, lane, j % 4).
-TS_DEV uint32_t place(uint32_t wave, uint32_t lane, uint32_t j) {
-    return (wave * kRuns + j / 4) * 256 + lane * 4 + j % 4;
-}
+constexpr uint32_t kEach = 8, kWaves = 4, kPiece = 64 * kWaves * kEach;  // the rows' kernel: 2048 indices a piece
+constexpr uint32_t kMostPieces = 8;                // pieces a chunk at most
+constexpr uint32_t kRun = 256, kDrawWaves = 16;    // the draw's: indices a run, waves a group
 
 struct Chunk {  // of one row
     double sum;
@@ -47,9 +48,11 @@ struct VerifyParams {
     const float *uniforms, *probs, *temperatures;
     uint32_t *tokens, *accepted, *status;
     Chunk *chunks;      // [seqs][most + 1][parts]
-    double *sums;       // [seqs][parts]
+    double *sums;       // [seqs][runs]: weights of runs of 256 indices
     uint32_t *done;     // [seqs]: groups of the second kernel that have left their sum
-    uint32_t seqs, most, rows, width, stride, parts;
+    uint32_t seqs, most, rows, width, stride;
+    uint32_t pieces, parts;  // of the rows' kernel: pieces a chunk, chunks a row
+    uint32_t runs, groups;   // of the draw's: runs a row, groups a sequence
     float temperature;
     int whole_x, whole_q;  // four consecutive logits, or probabilities, are one aligned load
 };
@@ -60,10 +63,9 @@ TS_DEV double scalar(double c) {
     return c;
 }
 
-// 2^t for t <= 0: t = n + f, |f| <= 1/2, the series of 2^f = e^(f ln 2) up to the 10th power (the 11th is
-// 3e-13 at most, at |f| = 1/2). 0 for NaN and t below -1074.
+// 2^t for -1200 < t <= 0: t = n + f, |f| <= 1/2, the series of 2^f = e^(f ln 2) up to the 10th power (the
+// 11th is 3e-13 at most, at |f| = 1/2).
 TS_DEV double exp2_neg(double t) {
-    t = fmax(t, -1500.0);
     const double n = __builtin_rint(t), f = t - n;
     double r = __builtin_fma(f, scalar(7.054911620801123e-09), scalar(1.01780860092397e-07));
     r = __builtin_fma(r, f, scalar(1.321548679014431e-06));
@@ -75,26 +77,20 @@ TS_DEV double exp2_neg(double t) {
     r = __builtin_fma(r, f, scalar(0.24022650695910072));
     r = __builtin_fma(r, f, scalar(0.6931471805599453));
     r = __builtin_fma(r, f, 1.0);
-    return __builtin_amdgcn_ldexp(r, (int)n);
+    return __builtin_amdgcn_ldexp(r, (int)n);  // (0 below 2^-1074)
 }
 
-// e of logit x against the maximum: 1 at the maximum (+inf too), 0 for NaN and -inf. `by`: log2(e) /
-// temperature.
-TS_DEV double weight(float x, float most, double by) {
-    if (!(most < __builtin_inff())) return x == most ? 1.0 : 0.0;
-    const double e = exp2_neg(((double)x - (double)most) * by);
-    return x > -__builtin_inff() ? e : 0.0;
-}
-// Of a thread's logits side by side (x as load_logits leaves them, `most` finite or +inf; -inf gives 0).
+// e of logits side by side, `by` = log2(e) / temperature: 1 at the maximum (+inf too), 0 for NaN and -inf
+// (whose t is -inf or NaN; fmax takes its other operand).
 template <int N>
-TS_DEV void weights(const float (&x)[N], float most, double by, double (&w)[N]) {
-    if (!(most < __builtin_inff())) {
+TS_DEV void weights(float (&x)[N], float most, double by, double (&w)[N]) {
+    if (most == __builtin_inff()) {
+        most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < N; j++) w[j] = x[j] == most ? 1.0 : 0.0;
-        return;
+        for (int j = 0; j < N; j++) x[j] = x[j] == __builtin_inff() ? 0.0f : -__builtin_inff();
     }
 #pragma unroll
-    for (int j = 0; j < N; j++) w[j] = exp2_neg(((double)x[j] - (double)most) * by);
+    for (int j = 0; j < N; j++) w[j] = exp2_neg(fmax(((double)x[j] - (double)most) * by, -1100.0));
 }
 TS_DEV double per_unit(float temperature) { return 1.4426950408889634 / (double)temperature; }
 
@@ -104,54 +100,26 @@ TS_DEV float logit(const VerifyParams &p, uint32_t row, uint32_t i) {
     return BF16 ? bf16_float(((const uint16_t *)p.logits)[at]) : ((const float *)p.logits)[at];
 }
 
-// The thread's 16 logits of a chunk, NaN and indices past the row as -inf.
+// Four consecutive logits of a row, NaN and indices past the row as -inf.
 template <bool BF16>
-TS_DEV void load_logits(const VerifyParams &p, uint32_t row, uint32_t chunk, float (&x)[kEach]) {
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-#pragma unroll
-    for (uint32_t v = 0; v < kEach; v += 4) {
-        const uint32_t i = chunk * kChunk + place(wave, lane, v);
-        if (p.whole_x && i + 3 < p.width) {
-            const size_t at = (size_t)row * p.stride + i;
-            if (BF16) {
-                const u32x2 w = *(const u32x2 *)((const uint16_t *)p.logits + at);
-                x[v] = lo_bf16(w.x);
-                x[v + 1] = hi_bf16(w.x);
-                x[v + 2] = lo_bf16(w.y);
-                x[v + 3] = hi_bf16(w.y);
-            } else {
-                const f32x4 w = *(const f32x4 *)((const float *)p.logits + at);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[v + e] = w[e];
-            }
+TS_DEV void load4(const VerifyParams &p, uint32_t row, uint32_t i, float *x) {
+    if (p.whole_x && i + 3 < p.width) {
+        const size_t at = (size_t)row * p.stride + i;
+        if (BF16) {
+            const u32x2 w = *(const u32x2 *)((const uint16_t *)p.logits + at);
+            x[0] = lo_bf16(w.x);
+            x[1] = hi_bf16(w.x);
+            x[2] = lo_bf16(w.y);
+            x[3] = hi_bf16(w.y);
         } else {
+            const f32x4 w = *(const f32x4 *)((const float *)p.logits + at);
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++)
-                x[v + e] = i + e < p.width ? logit<BF16>(p, row, i + e) : -__builtin_inff();
+            for (int e = 0; e < 4; e++) x[e] = w[e];
         }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) x[e] = i + e < p.width ? logit<BF16>(p, row, i + e) : -__builtin_inff();
     }
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; j++) x[j] = x[j] > -__builtin_inff() ? x[j] : -__builtin_inff();
-}
-
-// The drafter's probabilities at the same indices, NaN and negative ones as 0.
-TS_DEV void load_probs(const VerifyParams &p, size_t row, uint32_t chunk, float (&q)[kEach]) {
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float *from = p.probs + row * p.width;
-#pragma unroll
-    for (uint32_t v = 0; v < kEach; v += 4) {
-        const uint32_t i = chunk * kChunk + place(wave, lane, v);
-        if (p.whole_q && i + 3 < p.width) {
-            const f32x4 w = *(const f32x4 *)(from + i);
-#pragma unroll
-            for (int e = 0; e < 4; e++) q[v + e] = w[e];
-        } else {
-#pragma unroll
-            for (uint32_t e = 0; e < 4; e++) q[v + e] = i + e < p.width ? from[i + e] : 0.0f;
-        }
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; j++) q[j] = q[j] > 0.0f ? q[j] : 0.0f;
 }
 
 // A sequence's drafts, first row of logits and temperature (<= 0: greedy); false where it is out of range.
@@ -170,70 +138,111 @@ TS_DEV Seq seq_of(const VerifyParams &p, uint32_t s) {
     return q;
 }
 
-TS_DEV double wave_total(double v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+// Sums over the wave, in every lane: DPP moves within rows of 16 lanes, then the permlane swaps across them
+// (through LDS, two exchanges a step of a double, the six steps take five times as long).
+template <int CTRL>
+TS_DEV double dpp_double(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+TS_DEV double row16_total(double v) {
+    v += dpp_double<0xB1>(v);   // lane ^ 1
+    v += dpp_double<0x4E>(v);   // lane ^ 2
+    v += dpp_double<0x141>(v);  // 7 - lane of each 8
+    v += dpp_double<0x140>(v);  // 15 - lane
     return v;
 }
-
-TS_DEV double group_total(double v) {
-    __shared__ double ss[4];
-    v = wave_total(v);
-    if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (ss[0] + ss[1]) + (ss[2] + ss[3]);
+TS_DEV double wave_total(double v) {
+    v = row16_total(v);
+    uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const auto l32 = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+    const auto h32 = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    v = __builtin_bit_cast(double, (uint64_t)h32[0] << 32 | l32[0]) + __builtin_bit_cast(double, (uint64_t)h32[1] << 32 | l32[1]);
+    b = __builtin_bit_cast(uint64_t, v);
+    const auto l16 = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+    const auto h16 = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)h16[0] << 32 | l16[0]) + __builtin_bit_cast(double, (uint64_t)h16[1] << 32 | l16[1]);
 }
 
-// The larger value, at equal ones the lower index, over the wave.
-TS_DEV void wave_best(float &v, uint32_t &at) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const float w = __shfl_xor(v, o, 64);
-        const uint32_t b = __shfl_xor(at, o, 64);
-        if (w > v || (w == v && b < at)) { v = w; at = b; }
-    }
-}
-
-// A wave takes its maximum and sums against it by itself; the four meet once, at the end.
+// A chunk's pieces, the next one's logits asked for before this one's are weighed. Each lane keeps a
+// maximum and a sum of its own; they meet once, at the end. A lane has two fours of consecutive indices
+// of a piece, 256 apart.
 template <bool BF16>
-__global__ __launch_bounds__(256) void verify_rows_kernel(VerifyParams p) {
-    __shared__ Chunk waves[4];
+__global__ __launch_bounds__(64 * kWaves) void verify_rows_kernel(VerifyParams p) {
+    __shared__ Chunk waves[kWaves];
     const uint32_t part = blockIdx.x % p.parts, sr = blockIdx.x / p.parts;
     const uint32_t s = sr / (p.most + 1), t = sr % (p.most + 1), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const Seq q = seq_of(p, s);
     if (!q.good || t > q.count) return;
     if (p.done && part == 0 && t == 0 && threadIdx.x == 0) p.done[s] = 0;
-    float x[kEach];
-    load_logits<BF16>(p, q.first + t, part, x);
     const double by = per_unit(q.temperature);
-    float most = x[0];
-#pragma unroll
-    for (uint32_t j = 1; j < kEach; j++) most = fmaxf(most, x[j]);
-    most = wave_max(most);
+    const uint32_t first = part * p.pieces, end = min(first + p.pieces, (p.width + kPiece - 1) / kPiece);
+    const uint32_t mine = wave * (kPiece / kWaves) + lane * 4;
+    float x[kEach], most = -__builtin_inff();
     uint32_t at = p.width;
+    double sum = 0.0;
+    auto load = [&](uint32_t piece, float (&to)[kEach]) {
+        load4<BF16>(p, q.first + t, piece * kPiece + mine, to);
+        load4<BF16>(p, q.first + t, piece * kPiece + mine + 256, to + 4);
+    };
+    load(first, x);
+    for (uint32_t piece = first; piece < end; piece++) {
+        float next[kEach];
+        load(min(piece + 1, end - 1), next);  // (the last piece's again, not used)
+        float top = x[0];
 #pragma unroll
-    for (int j = kEach - 1; j >= 0; j--)
-        if (x[j] == most) at = part * kChunk + place(wave, lane, j);  // the lane's first (its places ascend)
-    if (!(most > -__builtin_inff())) at = p.width;
+        for (uint32_t j = 1; j < kEach; j++) top = fmaxf(top, x[j]);  // (NaN: the other operand)
+        float was[1] = {most};
+        const bool raise = top > most;
+        most = raise ? top : most;
+        if (q.greedy) {
+            if (raise) {
+#pragma unroll
+                for (int j = kEach - 1; j >= 0; j--)  // the first: the lane's places ascend
+                    if (x[j] == most) at = piece * kPiece + mine + (j / 4) * 256 + j % 4;
+            }
+        } else {
+            double w[kEach];
+            if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+                double f[1];
+                weights(was, most, by, f);
+                sum *= f[0];
+            }
+            weights(x, most, by, w);
+#pragma unroll
+            for (uint32_t j = 0; j < kEach; j++) sum += w[j];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++) x[j] = next[j];
+    }
+    float own[1] = {most};
+    double scale[1];
+    most = wave_max(most);
+    at = own[0] == most ? at : p.width;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) at = min(at, (uint32_t)__shfl_xor((int)at, o, 64));
-    double sum = 0.0;
     if (!q.greedy) {
-        double w[kEach];
-        weights(x, most, by, w);
-#pragma unroll
-        for (uint32_t j = 0; j < kEach; j++) sum += w[j];
-        sum = most > -__builtin_inff() ? wave_total(sum) : 0.0;
+        weights(own, most, by, scale);
+        sum = wave_total(sum * scale[0]);
     }
     if (lane == 0) waves[wave] = Chunk{sum, most, at};
     __syncthreads();
     if (threadIdx.x == 0) {
         Chunk c = waves[0];
-        for (int w = 1; w < 4; w++)
-            if (waves[w].most > c.most) { c.most = waves[w].most; c.at = waves[w].at; }  // ties: the lower wave's
+        for (uint32_t w = 1; w < kWaves; w++)
+            if (waves[w].most > c.most || (waves[w].most == c.most && waves[w].at < c.at)) {
+                c.most = waves[w].most;
+                c.at = waves[w].at;
+            }
         if (!q.greedy) {
+            float m[kWaves];
+            double f[kWaves];
             c.sum = 0.0;
-            for (int w = 0; w < 4; w++) c.sum += waves[w].sum * weight(waves[w].most, c.most, by);
+            for (uint32_t w = 0; w < kWaves; w++) m[w] = waves[w].most;
+            weights(m, c.most, by, f);
+            for (uint32_t w = 0; w < kWaves; w++) c.sum += waves[w].sum * f[w];
         }
         p.chunks[(size_t)sr * p.parts + part] = c;
     }
@@ -248,7 +257,7 @@ TS_DEV Verdict decide(const VerifyParams &p, uint32_t s, const Seq &q) {
     __shared__ uint32_t taken[kMostDrafts + 1];
     const uint32_t l16 = threadIdx.x & 15;
     const double by = per_unit(q.temperature);
-    for (uint32_t t = threadIdx.x >> 4; t <= q.count; t += kThreads / 16) {
+    for (uint32_t t = threadIdx.x >> 4; t <= q.count; t += blockDim.x / 16) {
         const size_t sr = (size_t)s * (p.most + 1) + t;
         // What the test of the draft needs is asked for before the row's chunks.
         const uint32_t draft = t < q.count ? p.drafts[(size_t)s * p.most + t] : p.width;
@@ -266,15 +275,19 @@ TS_DEV Verdict decide(const VerifyParams &p, uint32_t s, const Seq &q) {
             Chunk four[4];
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) four[j] = c[min(j0 + 16 * j, p.parts - 1)];  // past the end: not used
-            const float was = most;
+            float m[5];
+            double f[5];
+            m[4] = most;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
-                if (j0 + 16 * j < p.parts && four[j].most > most) { most = four[j].most; at = four[j].at; }
+            for (uint32_t j = 0; j < 4; j++) {
+                m[j] = j0 + 16 * j < p.parts ? four[j].most : -__builtin_inff();
+                if (m[j] > most) { most = m[j]; at = four[j].at; }
+            }
             if (q.greedy) continue;
-            z *= weight(was, most, by);
+            weights(m, most, by, f);
+            z *= f[4];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
-                if (j0 + 16 * j < p.parts) z += four[j].sum * weight(four[j].most, most, by);
+            for (uint32_t j = 0; j < 4; j++) z += f[j] > 0.0 ? four[j].sum * f[j] : 0.0;
         }
         float whole = most;
 #pragma unroll
@@ -283,14 +296,18 @@ TS_DEV Verdict decide(const VerifyParams &p, uint32_t s, const Seq &q) {
             const uint32_t b = __shfl_xor(at, o, 64);
             if (w > whole || (w == whole && b < at)) { whole = w; at = b; }
         }
+        double e = 0.0;
         if (!q.greedy) {
-            z *= weight(most, whole, by);
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) z += __shfl_xor(z, o, 64);
+            float m[2] = {most, x};
+            double f[2];
+            weights(m, whole, by, f);
+            z *= f[0];
+            e = f[1];
+            z = row16_total(z);
         }
         if (l16 == 0) {
             chance = chance > 0.0f ? chance : 0.0f;
-            taken[t] = draft < p.width && (q.greedy ? draft == at : (double)u * (double)chance * z < weight(x, whole, by));
+            taken[t] = draft < p.width && (q.greedy ? draft == at : (double)u * (double)chance * z < e);
             rows[t] = Verdict{z, whole, q.first + t, t, t < q.count, at};
         }
     }
@@ -300,56 +317,15 @@ TS_DEV Verdict decide(const VerifyParams &p, uint32_t s, const Seq &q) {
     return rows[n];
 }
 
-// The weights that a draw gives the thread's 16 indices of a chunk of the verdict's row.
-template <bool BF16>
-TS_DEV void draw_weights(const VerifyParams &p, uint32_t s, const Verdict &v, double by, bool residual, uint32_t draft,
-                         uint32_t chunk, double (&w)[kEach]) {
-    float x[kEach], q[kEach];
-    load_logits<BF16>(p, v.row, chunk, x);
-    const bool probs = residual && p.probs;
-    if (probs) load_probs(p, (size_t)s * p.most + v.accepted, chunk, q);
-    weights(x, v.most, by, w);
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; j++) {
-        if (probs) {
-            w[j] -= (double)q[j] * v.whole;
-            w[j] = w[j] > 0.0 ? w[j] : 0.0;
-        } else if (residual && chunk * kChunk + place(threadIdx.x >> 6, threadIdx.x & 63, j) == draft) {
-            w[j] = 0.0;
-        }
-    }
-}
-
 // The sequence's tokens: the accepted drafts, the pick, `width` in the rest.
 TS_DEV void answer(const VerifyParams &p, uint32_t s, bool good, uint32_t accepted, uint32_t pick) {
-    for (uint32_t t = threadIdx.x; t <= p.most; t += kThreads)
+    for (uint32_t t = threadIdx.x; t <= p.most; t += blockDim.x)
         p.tokens[(size_t)s * (p.most + 1) + t] = !good           ? p.width
                                                  : t < accepted  ? p.drafts[(size_t)s * p.most + t]
                                                  : t == accepted ? pick
                                                                  : p.width;
     if (threadIdx.x == 0) p.accepted[s] = good ? accepted : 0;
     if (threadIdx.x == 0 && !good && p.status) atomicOr(p.status, TS_STATUS_POSITION);
-}
-
-// Inclusive running sums over the 256 threads' values in thread order, and the whole.
-TS_DEV double running(double v, double &whole) {
-    __shared__ double ends[4];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double w = __shfl_up(v, o, 64);
-        if ((int)lane >= o) v += w;
-    }
-    __syncthreads();
-    if (lane == 63) ends[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    whole = 0.0;
-    for (uint32_t w = 0; w < 4; w++) {
-        if (w < wave) before += ends[w];
-        whole += ends[w];
-    }
-    return before + v;
 }
 
 // All greedy: the verdict is the answer.
@@ -365,13 +341,13 @@ __global__ __launch_bounds__(256) void verify_greedy_kernel(VerifyParams p) {
     answer(p, s, true, v.accepted, v.pick);
 }
 
-// The draw: a group a chunk leaves its chunk's weight, the last of a sequence to do so picks the token.
+// The draw. Runs of 256 indices, four consecutive ones a lane.
 template <bool BF16>
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyParams p) {
-    __shared__ uint32_t found, last, before;
-    __shared__ double under, runs[kWaves * kRuns];
-    const uint32_t part = blockIdx.x % p.parts, s = blockIdx.x / p.parts;
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyParams p) {
+    __shared__ uint32_t before, found[2];
+    __shared__ double ends[kDrawWaves], starts[2];
+    const uint32_t part = blockIdx.x % p.groups, s = blockIdx.x / p.groups;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const Seq q = seq_of(p, s);
     if (!q.good) {
         if (part == 0) answer(p, s, false, 0, 0);
@@ -383,118 +359,187 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyParams p) {
         return;
     }
     const double by = per_unit(q.temperature);
-    bool residual = v.refused;
     const uint32_t draft = v.refused ? p.drafts[(size_t)s * p.most + v.accepted] : 0;
-    const Chunk *own = p.chunks + ((size_t)s * (p.most + 1) + v.accepted) * p.parts;
-    if (!residual) {  // from p itself: its chunks' weights are there
-        if (part != 0) return;
-    } else {
-        double w[kEach], sum = 0.0;
-        draw_weights<BF16>(p, s, v, by, true, draft, part, w);
+    const float *probs = p.probs ? p.probs + ((size_t)s * p.most + v.accepted) * p.width : nullptr;
+    const double u = (double)p.uniforms[(size_t)s * (p.most + 1) + p.most];
+    double *sums = p.sums + (size_t)s * p.runs;
+    // The weights are max(e - q Z, 0) after a refusal, e otherwise; one pass over the runs for all
+    // groups together, and should the former all be zero, one for e by the last group alone.
+    bool residual = v.refused;
+    uint32_t r0 = part * kDrawWaves + wave, apart = p.groups * kDrawWaves, run = 0xffffffffu;
+    double w[4], target = 0.0, start = 0.0;
+    bool alone = false, searching = false;
+    auto load = [&](uint32_t r, float (&x)[4], float (&c)[4]) {
+        const uint32_t i = r * kRun + lane * 4;
+        load4<BF16>(p, v.row, i, x);
 #pragma unroll
-        for (uint32_t j = 0; j < kEach; j++) sum += w[j];
-        sum = group_total(sum);
-        // The sum is stored and counted past the XCDs' own L2s; the last group sees every one.
-        if (threadIdx.x == 0) {
-            __hip_atomic_store(p.sums + (size_t)s * p.parts + part, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            before = __hip_atomic_fetch_add(p.done + s, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (before + 1 != p.parts) return;
-    }
-    // Chunk sums: of the residual, or of p should the residual be zero everywhere.
-    auto chunk_sum = [&](uint32_t j) {
-        return residual ? __hip_atomic_load(p.sums + (size_t)s * p.parts + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                        : own[j].sum * weight(own[j].most, v.most, by);
-    };
-    const uint32_t per = (p.parts + kThreads - 1) / kThreads, j0 = threadIdx.x * per, j1 = min(j0 + per, p.parts);
-    double whole, mine, upto;
-    auto total = [&] {
-        mine = 0.0;
-        for (uint32_t j = j0; j < j1; j++) mine += chunk_sum(j);
-        upto = running(mine, whole);
-    };
-    total();
-    if (residual && !(whole > 0.0)) {
-        residual = false;
-        total();
-    }
-    // The first chunk whose running sum passes the target; without one (rounding, or u not below
-    // 1) the last chunk that weighs anything.
-    const double target = (double)p.uniforms[(size_t)s * (p.most + 1) + p.most] * whole;
-    if (threadIdx.x == 0) { found = 0xffffffffu; last = 0; under = 0.0; }
-    __syncthreads();
-    uint32_t over = 0xffffffffu, weighs = 0;  // the thread's own such chunks, and the sums before them
-    double before_over = 0.0, before_weighs = 0.0, c = upto - mine;
-    for (uint32_t j = j0; j < j1; j++) {
-        const double w = chunk_sum(j);
-        if (w > 0.0) {
-            weighs = j;
-            before_weighs = c;
-            if (over == 0xffffffffu && c + w > target) {
-                over = j;
-                before_over = c;
+        for (uint32_t e = 0; e < 4; e++) c[e] = 0.0f;
+        if (residual && probs) {
+            if (p.whole_q && i + 3 < p.width) {
+                const f32x4 y = *(const f32x4 *)(probs + i);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) c[e] = y[e];
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) c[e] = i + e < p.width ? probs[i + e] : 0.0f;
             }
         }
-        c += w;
-    }
-    if (over != 0xffffffffu) atomicMin(&found, over);
-    if (weighs) atomicMax(&last, weighs);
-    __syncthreads();
-    const bool passes = found != 0xffffffffu;
-    const uint32_t chunk = passes ? found : last;
-    if (chunk >= j0 && chunk < j1) under = passes ? before_over : before_weighs;
-    __syncthreads();
-    const double start = under;
-    if (threadIdx.x == 0) { found = 0xffffffffu; last = 0; }
-    __syncthreads();
-    // Within it: the sums of the runs of 256 indices, then each thread's own four of each run.
-    double w[kEach], ends[kRuns];
-    draw_weights<BF16>(p, s, v, by, residual, draft, chunk, w);
+    };
+    for (;;) {
+        float x[4], c[4];
+        uint32_t r = r0;
+        if (r < p.runs) load(r, x, c);
+        while (r < p.runs) {
+            const uint32_t next = searching ? p.runs : r + apart;
+            float nx[4], nc[4];
+            if (next < p.runs) load(next, nx, nc);
+            weights(x, v.most, by, w);
 #pragma unroll
-    for (uint32_t run = 0; run < kRuns; run++) {
-        double c = (w[4 * run] + w[4 * run + 1]) + (w[4 * run + 2] + w[4 * run + 3]);
+            for (uint32_t e = 0; e < 4; e++) {
+                if (residual) {
+                    if (!probs && r * kRun + lane * 4 + e == draft) w[e] = 0.0;
+                    w[e] -= (c[e] > 0.0f ? (double)c[e] : 0.0) * v.whole;
+                    w[e] = w[e] > 0.0 ? w[e] : 0.0;
+                }
+            }
+            if (!searching) {
+                const double sum = wave_total((w[0] + w[1]) + (w[2] + w[3]));
+                // Past the XCD's own L2, where the sequence's last group reads it.
+                if (lane == 0) __hip_atomic_store(sums + r, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            r = next;
 #pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                x[e] = nx[e];
+                c[e] = nc[e];
+            }
+        }
+        if (searching) break;  // wave 0 has the weights of the run found
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the sums have arrived
+        __syncthreads();
+        if (!alone) {
+            if (threadIdx.x == 0) before = __hip_atomic_fetch_add(p.done + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (before + 1 != p.groups) return;
+            alone = true;
+        }
+        // The last group: running sums over the runs, a thread a block of consecutive ones.
+        const uint32_t each = (p.runs + 64 * kDrawWaves - 1) / (64 * kDrawWaves);
+        const uint32_t j0 = threadIdx.x * each, j1 = min(j0 + each, p.runs);
+        double mine = 0.0;
+        for (uint32_t j = j0; j < j1; j++) mine += __hip_atomic_load(sums + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        double upto = mine;
+#pragma unroll 1
         for (int o = 1; o < 64; o <<= 1) {
-            const double up = __shfl_up(c, o, 64);
-            if ((int)lane >= o) c += up;
+            const double up = __shfl_up(upto, o, 64);
+            if ((int)lane >= o) upto += up;
         }
-        ends[run] = c;
-        if (lane == 63) runs[wave * kRuns + run] = c;
-    }
-    __syncthreads();
-    uint32_t first = 0xffffffffu, end = 0;  // end: past the last index that weighs anything
-    upto = start;
-    for (uint32_t run = 0; run < wave * kRuns; run++) upto += runs[run];
-#pragma unroll
-    for (uint32_t run = 0; run < kRuns; run++) {
-        c = __shfl_up(ends[run], 1, 64);
-        c = upto + (lane ? c : 0.0);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t i = chunk * kChunk + place(wave, lane, 4 * run + e);
-            c += w[4 * run + e];
-            if (first == 0xffffffffu && w[4 * run + e] > 0.0 && c > target) first = i;
-            if (w[4 * run + e] > 0.0) end = i + 1;
+        if (lane == 63) ends[wave] = upto;
+        if (threadIdx.x < 2) found[threadIdx.x] = threadIdx.x ? 0u : 0xffffffffu;
+        __syncthreads();
+        double whole = 0.0;
+#pragma unroll 1
+        for (uint32_t j = 0; j < kDrawWaves; j++) {
+            if (j < wave) upto += ends[j];
+            whole += ends[j];
         }
-        upto += runs[wave * kRuns + run];
+        if (residual && !(whole > 0.0)) {  // (uniform over the group)
+            residual = false;
+            r0 = wave;
+            apart = kDrawWaves;
+            continue;
+        }
+        // The first run whose running sum passes the target; without one (rounding, or u not below 1) the
+        // last that weighs anything.
+        target = u * whole;
+        uint32_t over = 0xffffffffu, weighs = 0xffffffffu;
+        double over_start = 0.0, weighs_start = 0.0, at = upto - mine;
+        for (uint32_t j = j0; j < j1; j++) {
+            const double c = __hip_atomic_load(sums + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (c > 0.0) {
+                weighs = j;
+                weighs_start = at;
+                if (over == 0xffffffffu && at + c > target) {
+                    over = j;
+                    over_start = at;
+                }
+            }
+            at += c;
+        }
+        // (One lane a wave: the first with one over, the last that weighs.)
+        const uint64_t overs = __builtin_amdgcn_ballot_w64(over != 0xffffffffu);
+        const uint64_t all = __builtin_amdgcn_ballot_w64(weighs != 0xffffffffu);
+        if (overs && lane == __builtin_ctzll(overs)) atomicMin(&found[0], over);
+        if (all && lane == 63 - __builtin_clzll(all)) atomicMax(&found[1], weighs);
+        __syncthreads();
+        run = found[0] != 0xffffffffu ? found[0] : found[1];
+        if (run == over) starts[0] = over_start;
+        if (run == weighs) starts[1] = weighs_start;
+        __syncthreads();
+        start = found[0] != 0xffffffffu ? starts[0] : starts[1];
+        if (wave != 0) return;
+        searching = true;
+        r0 = run;
     }
-    if (first != 0xffffffffu) atomicMin(&found, first);
-    atomicMax(&last, end);
-    __syncthreads();
-    answer(p, s, true, v.accepted, found != 0xffffffffu ? found : last ? last - 1 : p.width);
+    // The run's index, by one wave: the first whose running sum passes the target, or the last that
+    // weighs anything; `width` where nothing does.
+    double upto = (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(upto, o, 64);
+        if ((int)lane >= o) upto += up;
+    }
+    const double left = __shfl_up(upto, 1, 64);
+    double at = start + (lane ? left : 0.0);
+    uint32_t over = 0xffffffffu, last = 0xffffffffu;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++) {
+        at += w[e];
+        const uint32_t i = run * kRun + lane * 4 + e;
+        if (w[e] > 0.0) {
+            last = i;
+            if (over == 0xffffffffu && at > target) over = i;
+        }
+    }
+    const uint64_t overs = __builtin_amdgcn_ballot_w64(over != 0xffffffffu);
+    const uint64_t lasts = __builtin_amdgcn_ballot_w64(last != 0xffffffffu);
+    const uint32_t pick = overs   ? __builtin_amdgcn_readlane(over, __builtin_ctzll(overs))
+                          : lasts ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(lasts))
+                                  : p.width;
+    for (uint32_t t = lane; t <= p.most; t += 64) {
+        const uint32_t kept = t < v.accepted ? p.drafts[(size_t)s * p.most + t] : p.width;
+        p.tokens[(size_t)s * (p.most + 1) + t] = t == v.accepted ? pick : kept;
+    }
+    if (lane == 0) p.accepted[s] = v.accepted;
+}
+
+// How the rows are cut.
+struct Cut {
+    uint32_t pieces, parts, runs, groups;
+};
+Cut cut(const ts_verify_args *a) {
+    Cut c;
+    // The rows' kernel: pieces a chunk so that the groups fill the chip once (8 of 4 waves a CU), a
+    // chunk's later pieces loading under the work on its earlier ones.
+    const uint32_t all = (a->width + kPiece - 1) / kPiece;
+    const uint64_t rows = (uint64_t)a->seqs * (a->most + 1);
+    c.pieces = (uint32_t)std::min<uint64_t>(kMostPieces, std::max<uint64_t>(1, all * rows / 2048));
+    c.parts = (all + c.pieces - 1) / c.pieces;
+    // The draw: about a group a CU (16 waves, four a SIMD), a run a wave at least.
+    c.runs = (a->width + kRun - 1) / kRun;
+    c.groups = std::min((c.runs + kDrawWaves - 1) / kDrawWaves, std::max(1u, 256 / std::max(1u, a->seqs)));
+    return c;
 }
 
 struct Sizes {
     size_t chunks, sums, done;  // bytes
     size_t whole() const { return chunks + sums + done; }
 };
-
 Sizes sizes(const ts_verify_args *a) {
-    const size_t parts = ((size_t)a->width + kChunk - 1) / kChunk;
+    const Cut c = cut(a);
     Sizes z;
-    z.chunks = (size_t)a->seqs * (a->most + 1) * parts * sizeof(Chunk);
-    z.sums = a->uniforms ? a->seqs * parts * sizeof(double) : 0;
+    z.chunks = (size_t)a->seqs * (a->most + 1) * c.parts * sizeof(Chunk);
+    z.sums = a->uniforms ? (size_t)a->seqs * c.runs * sizeof(double) : 0;
     z.done = a->uniforms ? (size_t)a->seqs * sizeof(uint32_t) : 0;
     return z;
 }
@@ -508,7 +553,7 @@ int check(const ts_verify_args *a) {
                a->width, a->stride);
     TS_REQUIRE(a->first || (uint64_t)a->seqs * (a->most + 1) <= a->rows, "verify: %u sequences of %u rows, %u rows given",
                a->seqs, a->most + 1, a->rows);
-    TS_REQUIRE((uint64_t)a->seqs * (a->most + 1) * ((a->width + kChunk - 1) / kChunk) <= 0x7fffffffull,
+    TS_REQUIRE((uint64_t)a->seqs * (a->most + 1) * ((a->width + kPiece - 1) / kPiece) <= 0x7fffffffull,
                "verify: %u sequences in one launch", a->seqs);
     TS_REQUIRE(ts::aligned(a->logits, 4), "verify: logits must be 4-byte aligned");
     return TS_OK;
@@ -516,19 +561,19 @@ int check(const ts_verify_args *a) {
 
 template <bool BF16>
 int launch(const VerifyParams &p, hipStream_t stream) {
-    hipLaunchKernelGGL(verify_rows_kernel<BF16>, dim3(p.seqs * (p.most + 1) * p.parts), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(verify_rows_kernel<BF16>, dim3(p.seqs * (p.most + 1) * p.parts), dim3(64 * kWaves), 0, stream, p);
     TS_CHECK_LAUNCH("verify rows launch");
     if (p.uniforms)
-        hipLaunchKernelGGL(verify_draw_kernel<BF16>, dim3(p.seqs * p.parts), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL(verify_draw_kernel<BF16>, dim3(p.seqs * p.groups), dim3(64 * kDrawWaves), 0, stream, p);
     else
-        hipLaunchKernelGGL(verify_greedy_kernel<BF16>, dim3(p.seqs), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL(verify_greedy_kernel<BF16>, dim3(p.seqs), dim3(256), 0, stream, p);
     TS_CHECK_LAUNCH("verify draw launch");
     return TS_OK;
 }
 
 }  // namespace
 
-extern "C" size_t tessera_hip_verify_workspace(const ts_verify_args *a) { return a ? sizes(a).whole() : 0; }
+extern "C" size_t tessera_hip_verify_workspace(const ts_verify_args *a) { return a && a->width ? sizes(a).whole() : 0; }
 
 extern "C" int tessera_hip_verify(const ts_verify_args *a, void *stream) {
     int rc = check(a);
@@ -546,7 +591,8 @@ extern "C" int tessera_hip_verify(const ts_verify_args *a, void *stream) {
     p.sums = (double *)(w + z.chunks);
     p.done = a->uniforms ? (uint32_t *)(w + z.chunks + z.sums) : nullptr;
     p.seqs = a->seqs; p.most = a->most; p.rows = a->rows; p.width = a->width; p.stride = a->stride;
-    p.parts = (a->width + kChunk - 1) / kChunk;
+    const Cut c = cut(a);
+    p.pieces = c.pieces; p.parts = c.parts; p.runs = c.runs; p.groups = c.groups;
     p.temperature = a->temperature;
     p.whole_x = a->stride % 4 == 0 && ts::aligned(a->logits, a->logits_dtype == TS_BF16 ? 8 : 16);
     p.whole_q = a->width % 4 == 0 && ts::aligned(a->draft_probs, 16);
