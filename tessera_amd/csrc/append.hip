@@ -9,12 +9,16 @@
 // norm and rotation stages (engine/models/src/shared.rs:109-145, engine/ir/interp/src/
 // run.rs:122-198).
 //
-// The unit of work is a segment: rows r, r + 1, ... of the call that are consecutive positions of
-// one slot within one block of 16. One wave owns a segment's kv head: it sees all new values of
-// the block's head, so the scale, the codes and (where the scale grows) the codes already there
-// are settled without another launch or an atomic. The rows of a call that meet in a block must
-// therefore stand together; a later segment of the same block is refused (TS_STATUS_TWICE), found
-// by looking through the rows before it.
+// A head's row is 16 lanes' work, eight values each (four pairs of the rotation), so a wave takes four rows at
+// once, in 16-byte loads, and a row's sum of squares needs no step across rows of lanes.
+//
+// The unit of work for k and v is a segment: rows r, r + 1, ... of the call that are consecutive positions
+// of one slot within one block of 16. One wave owns a segment's kv head, lane group g (16 lanes) the block's
+// positions 4 g .. 4 g + 3: it sees all new values of the block's head, so the scale, the codes and
+// (where the scale grows) the codes already there are settled without another launch or an atomic, and
+// four positions of a d are one word of V's block. The rows of a call that meet in a block must
+// therefore stand together; a later segment of the same block is refused (TS_STATUS_TWICE), found by
+// looking through the rows before it.
 #include "kept8.h"
 
 namespace {
@@ -31,60 +35,101 @@ struct AppendParams {
     uint32_t *status;
     Place place;
     uint32_t rows, heads, kv_heads, q_stride, k_stride, v_stride;
-    uint32_t window, kv_groups, head_groups;  // rows a kv group looks at; groups of 4 kv heads; of 16 q heads
+    uint32_t window, kv_groups;      // rows a kv group looks at, and how many such groups there are
+    uint32_t q_rows, head_quads;     // rows a wave of q heads takes, fours of q heads a row
     float eps;
     int q_out_bf16;
+    int fours;  // slots and positions are 16-byte aligned
 };
 
-constexpr uint32_t kQBatch = 4;  // q heads a wave
+constexpr uint32_t kQRows = 4;
 
-// The lane's pair of a 128-wide row: (j, j + 64) or (2j, 2j + 1).
+// The lane's eight values of a 128-wide row, in memory order: 4 l .. and 64 + 4 l .. (pairs (j, j + 64)), or
+// 8 l .. (pairs (2j, 2j + 1)); pair k is values pa(k), pb(k), its angle 4 l + k.
+template <bool HALVES>
+struct Lanes {
+    static TS_DEV uint32_t at(uint32_t l, uint32_t half) { return HALVES ? 4 * l + 64 * half : 8 * l + 4 * half; }
+    static TS_DEV constexpr int pa(int k) { return HALVES ? k : 2 * k; }
+    static TS_DEV constexpr int pb(int k) { return HALVES ? k + 4 : 2 * k + 1; }
+};
+
+// The lane's values of a row `row` elements past x (uniform, so that the address is a scalar base and a
+// 32-bit offset).
 template <bool XBF16, bool HALVES>
-TS_DEV void load_pair(const void *x, size_t at, uint32_t lane, float &a, float &b) {
-    if (XBF16) {
-        const uint16_t *r = (const uint16_t *)x + at;
-        if (HALVES) {
-            a = bf16_float(r[lane]);
-            b = bf16_float(r[lane + 64]);
+TS_DEV void load8(const void *x, uint32_t row, uint32_t l, float (&v)[8]) {
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const uint32_t at = row + Lanes<HALVES>::at(l, half);
+        if (XBF16) {
+            const u32x2 w = *(const u32x2 *)((const char *)x + (uint32_t)(at * 2));
+            v[4 * half] = lo_bf16(w.x);
+            v[4 * half + 1] = hi_bf16(w.x);
+            v[4 * half + 2] = lo_bf16(w.y);
+            v[4 * half + 3] = hi_bf16(w.y);
         } else {
-            const uint32_t w = *(const uint32_t *)(r + 2 * lane);
-            a = lo_bf16(w);
-            b = hi_bf16(w);
+            const f32x4 w = *(const f32x4 *)((const char *)x + (uint32_t)(at * 4));
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * half + e] = w[e];
         }
-    } else {
-        const float *r = (const float *)x + at;
-        if (HALVES) {
-            a = r[lane];
-            b = r[lane + 64];
-        } else {
-            const float2 w = *(const float2 *)(r + 2 * lane);
-            a = w.x;
-            b = w.y;
-        }
+    }
+}
+// Element `row` rows of `stride` on, as load8's uniform base.
+template <bool XBF16>
+TS_DEV const void *row_base(const void *x, uint32_t row, uint32_t stride) {
+    return (const char *)x + (size_t)row * stride * (XBF16 ? 2 : 4);
+}
+
+template <bool HALVES>
+TS_DEV void store8_bf16(uint16_t *row, uint32_t l, const float (&v)[8]) {
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+        *(u32x2 *)(row + Lanes<HALVES>::at(l, half)) =
+            u32x2{pack_bf16x2(v[4 * half], v[4 * half + 1]), pack_bf16x2(v[4 * half + 2], v[4 * half + 3])};
+}
+
+// RmsNorm of a head's row over its 16 lanes; of pairs (j, j + 64) in the order, and to the bits, of
+// tessera_hip_qk_norm_rope_append.
+template <bool HALVES>
+TS_DEV void norm8(float (&v)[8], const float (&gain)[8], float eps) {
+    float s[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float a = v[Lanes<HALVES>::pa(k)], b = v[Lanes<HALVES>::pb(k)];
+        s[k] = a * a + b * b;
+    }
+    const float inv = 1.0f / sqrtf(row16_sum((s[0] + s[1]) + (s[2] + s[3])) / 128.0f + eps);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = v[k] * (inv * gain[k]);
+}
+
+// The rotation, each value rounded as tessera_hip_qk_norm_rope_append's.
+template <bool HALVES>
+TS_DEV void turn8(float (&v)[8], const f32x4 (&cs)[2]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float c = cs[k / 2][2 * (k % 2)], sn = cs[k / 2][2 * (k % 2) + 1];
+        float &a = v[Lanes<HALVES>::pa(k)], &b = v[Lanes<HALVES>::pb(k)];
+        const float x = a, y = b;
+        a = fmaf(x, c, -(y * sn));
+        b = fmaf(y, c, x * sn);
     }
 }
 
 template <bool HALVES>
-TS_DEV void store_pair_bf16(uint16_t *r, uint32_t lane, float a, float b) {
-    if (HALVES) {
-        r[lane] = bf16_bits(a);
-        r[lane + 64] = bf16_bits(b);
-    } else {
-        *(uint32_t *)(r + 2 * lane) = pack_bf16x2(a, b);
+TS_DEV void load_gain(const float *gain, uint32_t l, float (&g)[8]) {
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const float *from = gain + Lanes<HALVES>::at(l, half);
+#pragma unroll
+        for (int e = 0; e < 4; e++) g[4 * half + e] = from[e];
     }
 }
 
-TS_DEV void norm_pair(float &a, float &b, float ga, float gb, float eps) {
-    const float inv = 1.0f / sqrtf(wave_sum(a * a + b * b) / 128.0f + eps);
-    a = a * (inv * ga);
-    b = b * (inv * gb);
-}
-
-// Rounded as tessera_hip_qk_norm_rope_append's rotation.
-TS_DEV void turn_pair(float &a, float &b, float2 cs) {
-    const float x = a, y = b;
-    a = fmaf(x, cs.x, -(y * cs.y));
-    b = fmaf(y, cs.x, x * cs.y);
+// The lane's four (cos, sin) `rows` rows past the table's uniform row.
+TS_DEV void load_turns(const float2 *row, uint32_t rows, uint32_t l, f32x4 (&cs)[2]) {
+    const char *from = (const char *)row;
+    cs[0] = *(const f32x4 *)(from + (rows * 512 + l * 32));
+    cs[1] = *(const f32x4 *)(from + (rows * 512 + l * 32 + 16));
 }
 
 TS_DEV float finite_abs(float x) {
@@ -92,211 +137,284 @@ TS_DEV float finite_abs(float x) {
     return a < __builtin_inff() ? a : 0.0f;  // infinities and NaN take no part in the scale
 }
 
-// The code of x / scale, `inv` = 1 / scale: beyond the range the largest, NaN for infinities and NaN
-// (the format has no infinity).
+// Four codes of x * inv, `inv` = 1 / scale: beyond the range the largest, NaN for infinities and NaN (the
+// format has no infinity).
 TS_DEV float coded(float x, float inv) {
     const float y = fminf(fmaxf(x * inv, -448.0f), 448.0f);
     return fabsf(x) < __builtin_inff() ? y : __builtin_nanf("");
 }
-TS_DEV uint32_t code_of(float a) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, a, 0, false) & 0xffu; }
+TS_DEV uint32_t codes4(float a, float b, float c, float d, float inv) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(coded(a, inv), coded(b, inv), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(coded(c, inv), coded(d, inv), w, true);
+}
 
 // Four codes held under one scale as codes under another (factor = old / new, a power of two <= 1).
 TS_DEV uint32_t rebase4(uint32_t w, float factor) {
     float f[4];
     e4m3x4_to_f32(w, f);
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * factor, f[1] * factor, 0, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * factor, f[3] * factor, r, true);
-    return (uint32_t)r;
-}
-TS_DEV u32x4 rebase16(u32x4 w, float factor) {
-    return u32x4{rebase4(w.x, factor), rebase4(w.y, factor), rebase4(w.z, factor), rebase4(w.w, factor)};
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * factor, f[1] * factor, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2] * factor, f[3] * factor, r, true);
 }
 
-// One segment of one kv head: N rows at most (1 or 16), n of them, from row r, the first at kept row
-// `row0`.
-template <bool XBF16, bool KEPT8, bool HALVES, int N>
-TS_DEV void append_segment(const AppendParams &p, uint32_t r, uint32_t n, uint64_t row0, uint32_t pos, uint32_t h,
-                           uint32_t lane) {
-    float ka[N], kb[N], va[N], vb[N];
-    float2 cs[N];
+// The segment's row at block position `at`, or the nearest: rows off .. off + n - 1 are written.
+TS_DEV uint32_t segment_row(uint32_t at, uint32_t off, uint32_t n) {
+    return (uint32_t)min(max((int)at - (int)off, 0), (int)n - 1);
+}
+
+// A segment of one row (a decode step's): 16 lanes a kv head's k or v, four of them a wave. A short way, as a
+// step's few groups spend most of their time fetching code.
+template <bool XBF16, bool KEPT8, bool HALVES>
+TS_DEV void append_one(const AppendParams &p, uint64_t row0, uint32_t pos, uint32_t unit, uint32_t r, uint32_t l) {
+    const uint32_t h = unit >> 1, is_v = unit & 1;
+    if (h >= p.kv_heads) return;  // (16 lanes together)
+    const void *k = row_base<XBF16>(p.k, r, p.k_stride), *from = row_base<XBF16>(p.v, r, p.v_stride);
+    float v[8], x[8];
+    load8<XBF16, HALVES>(is_v ? from : k, h * 128, l, v);
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const size_t row = r + min((uint32_t)i, n - 1);  // past the end: read, not used
-        load_pair<XBF16, HALVES>(p.k, row * p.k_stride + h * 128, lane, ka[i], kb[i]);
-        load_pair<XBF16, HALVES>(p.v, row * p.v_stride + h * 128, lane, va[i], vb[i]);
-        if (p.turns) cs[i] = p.turns[(size_t)(pos + min((uint32_t)i, n - 1)) * 64 + lane];
-    }
+    for (int e = 0; e < 8; e++) x[e] = v[e];
     if (p.k_gain) {
-        const float ga = p.k_gain[HALVES ? lane : 2 * lane], gb = p.k_gain[HALVES ? lane + 64 : 2 * lane + 1];
-#pragma unroll
-        for (int i = 0; i < N; i++) norm_pair(ka[i], kb[i], ga, gb, p.eps);
+        float gain[8];
+        load_gain<HALVES>(p.k_gain, l, gain);
+        norm8<HALVES>(x, gain, p.eps);
     }
     if (p.turns) {
-#pragma unroll
-        for (int i = 0; i < N; i++) turn_pair(ka[i], kb[i], cs[i]);
+        f32x4 cs[2];
+        load_turns(p.turns + (size_t)pos * 64, 0, l, cs);
+        turn8<HALVES>(x, cs);
     }
-    if (!KEPT8) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            if ((uint32_t)i >= n) continue;
-            const size_t at = ((row0 + i) * p.kv_heads + h) * 128;
-            store_pair_bf16<HALVES>((uint16_t *)p.k_kept + at, lane, ka[i], kb[i]);
-            store_pair_bf16<HALVES>((uint16_t *)p.v_kept + at, lane, va[i], vb[i]);
-        }
+    for (int e = 0; e < 8; e++) v[e] = is_v ? v[e] : x[e];
+    if (!KEPT8) {
+        store8_bf16<HALVES>((uint16_t *)(is_v ? p.v_kept : p.k_kept) + (row0 * p.kv_heads + h) * 128, l, v);
         return;
     }
-    float ak = 0.0f, av = 0.0f;
+    float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) {  // rows past the end repeat the last one
-        ak = fmaxf(ak, fmaxf(finite_abs(ka[i]), finite_abs(kb[i])));
-        av = fmaxf(av, fmaxf(finite_abs(va[i]), finite_abs(vb[i])));
-    }
-    ak = wave_max(ak);
-    av = wave_max(av);
-    const uint32_t off = (uint32_t)(row0 & (kBlock - 1));
+    for (int k = 0; k < 8; k++) amax = fmaxf(amax, finite_abs(v[k]));
+    amax = row16_max(amax);
+    const uint32_t off = (uint32_t)row0 & (kBlock - 1);
     const uint64_t block = row0 / kBlock;
-    float2 *scale_at = (float2 *)p.scales + block * scale_heads(p.kv_heads) + h;
-    int ek = scale_exponent(ak), ev = scale_exponent(av), wask = ek, wasv = ev;
-    if (off) {  // rows are there: the scale only grows
-        const float2 was = *scale_at;
-        wask = stored_exponent(was.x);
-        wasv = stored_exponent(was.y);
-        ek = max(ek, wask);
-        ev = max(ev, wasv);
+    float *scale_at = p.scales + (block * scale_heads(p.kv_heads) + h) * 2 + is_v;
+    uint8_t *to = (uint8_t *)(is_v ? p.v_kept : p.k_kept) + (block * p.kv_heads + h) * kBlockBytes;
+    int e = scale_exponent(amax), grow = 0;
+    if (off) {  // positions are there: the scale only grows
+        const int was = stored_exponent(*scale_at);
+        e = max(e, was);
+        grow = e - was;
     }
-    const float ik = two_to(-ek), iv = two_to(-ev);
-    uint8_t *kb8 = (uint8_t *)p.k_kept + (block * p.kv_heads + h) * kBlockBytes;
-    uint8_t *vb8 = (uint8_t *)p.v_kept + (block * p.kv_heads + h) * kBlockBytes;
-    if (off && ek > wask) {  // four lanes a row of K: the rows not written now move to the new scale
-        const uint32_t row = lane >> 2;
-        if (row < off || row >= off + n) {
-            u32x4 *at = (u32x4 *)(kb8 + lane * 32);
-            const u32x4 w0 = at[0], w1 = at[1];
-            const float factor = two_to(wask - ek > -126 ? wask - ek : -126);
-            at[0] = rebase16(w0, factor);
-            at[1] = rebase16(w1, factor);
+    if (grow) {  // all of the block; the new position's bytes are written after it
+        const float factor = two_to(max(-grow, -126));
+        u32x4 *at = (u32x4 *)to + l;
+#pragma unroll 1
+        for (uint32_t i = 0; i < kBlockBytes / 256; i++, at += 16) {
+            const u32x4 w = *at;
+            *at = u32x4{rebase4(w.x, factor), rebase4(w.y, factor), rebase4(w.z, factor), rebase4(w.w, factor)};
         }
+        // Other lanes' words of the new position must be there before its bytes.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    const float inv = two_to(-e);
+    const uint32_t lo = codes4(v[0], v[1], v[2], v[3], inv), hi = codes4(v[4], v[5], v[6], v[7], inv);
+    if (!is_v) {
+        *(uint32_t *)(to + off * kWidth + Lanes<HALVES>::at(l, 0)) = lo;
+        *(uint32_t *)(to + off * kWidth + Lanes<HALVES>::at(l, 1)) = hi;
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        if ((uint32_t)i >= n) continue;
-        uint8_t *at = kb8 + (off + i) * kWidth;
-        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(coded(ka[i], ik), coded(kb[i], ik), 0, false);
-        if (HALVES) {
-            at[lane] = (uint8_t)w;
-            at[lane + 64] = (uint8_t)(w >> 8);
-        } else {
-            *(uint16_t *)(at + 2 * lane) = (uint16_t)w;
-        }
+        for (int k = 0; k < 8; k++)
+            to[(Lanes<HALVES>::at(l, k / 4) + k % 4) * kBlock + off] = (uint8_t)((k < 4 ? lo : hi) >> (8 * (k % 4)));
     }
-    // V: 16 positions of a d are one 16-byte piece; the lane's two.
-    typedef unsigned __int128 u128;
-    const u128 ones = ~(u128)0;
-    const u128 mask = (n == kBlock ? ones : (((u128)1 << (8 * n)) - 1)) << (8 * off);
-    const float fv = two_to(wasv - ev > -126 ? wasv - ev : -126);
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        u128 fresh = 0;
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            fresh |= (u128)code_of(coded(e ? vb[i] : va[i], iv)) << (8 * i);
-        u128 *at = (u128 *)(vb8 + (HALVES ? lane + 64 * e : 2 * lane + e) * kBlock);
-        u128 all = fresh << (8 * off);
-        if (n < kBlock) {
-            u32x4 held = *(const u32x4 *)at;
-            if (off && ev > wasv) held = rebase16(held, fv);
-            all = (all & mask) | (__builtin_bit_cast(u128, held) & ~mask);
-        }
-        *(u32x4 *)at = __builtin_bit_cast(u32x4, all);
-    }
-    if (lane == 0) *scale_at = make_float2(two_to(ek), two_to(ev));
+    if (l == 0) *scale_at = two_to(e);
 }
 
-template <bool XBF16, bool KEPT8, bool HALVES>
-__global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (blockIdx.x >= p.kv_groups) {  // q heads of one row
-        const uint32_t g = blockIdx.x - p.kv_groups, r = g / p.head_groups;
-        const uint32_t h0 = (g % p.head_groups) * 4 * kQBatch + wave;
-        if (h0 >= p.heads) return;
-        const uint32_t pos = p.positions[r];
-        const bool held = pos < p.place.keys;
-        float a[kQBatch], b[kQBatch];
+// One segment of n rows of one kv head's k (or v), rows from r on, the first at kept row `row0`: x[i] is
+// position 4 g + i, of the row's own values where the segment writes it, else of one of its rows (not used).
+template <bool KEPT8, bool HALVES, bool IS_V>
+TS_DEV void append_segment(const AppendParams &p, uint64_t row0, uint32_t pos, uint32_t n, uint32_t h, uint32_t lane,
+                           float (&x)[4][8]) {
+    const uint32_t g = lane >> 4, l = lane & 15, off = pos & (kBlock - 1);
+    const uint32_t mine = (((1u << n) - 1) << off) >> (4 * g) & 15;
+    const uint64_t first = row0 - off;  // kept row of the 16's position 0
+    if (!IS_V) {
+        if (p.k_gain) {
+            float gain[8];
+            load_gain<HALVES>(p.k_gain, l, gain);
 #pragma unroll
-        for (uint32_t i = 0; i < kQBatch; i++)  // past the end: read, not used
-            load_pair<XBF16, HALVES>(p.q, (size_t)r * p.q_stride + min(h0 + 4 * i, p.heads - 1) * 128, lane, a[i], b[i]);
-        float2 cs = make_float2(1.0f, 0.0f);
-        if (p.turns && held) cs = p.turns[(size_t)pos * 64 + lane];
-        float ga = 1.0f, gb = 1.0f;
-        if (p.q_gain) {
-            ga = p.q_gain[HALVES ? lane : 2 * lane];
-            gb = p.q_gain[HALVES ? lane + 64 : 2 * lane + 1];
+            for (uint32_t i = 0; i < 4; i++) norm8<HALVES>(x[i], gain, p.eps);
         }
+        if (p.turns) {
+            const float2 *row = p.turns + (size_t)pos * 64;
 #pragma unroll
-        for (uint32_t i = 0; i < kQBatch; i++) {
-            const uint32_t h = h0 + 4 * i;
-            if (h >= p.heads) break;
-            if (p.q_gain) norm_pair(a[i], b[i], ga, gb, p.eps);
-            if (p.turns) turn_pair(a[i], b[i], cs);
-            if (!held) a[i] = b[i] = __builtin_nanf("");
-            const size_t at = ((size_t)r * p.heads + h) * 128;
+            for (uint32_t i = 0; i < 4; i++) {
+                f32x4 cs[2];
+                load_turns(row, segment_row(4 * g + i, off, n), l, cs);
+                turn8<HALVES>(x[i], cs);
+            }
+        }
+    }
+    if (!KEPT8) {
+        char *to = (char *)(IS_V ? p.v_kept : p.k_kept) + (first * p.kv_heads + h) * 256;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if (mine >> i & 1) store8_bf16<HALVES>((uint16_t *)(to + (4 * g + i) * (p.kv_heads * 256)), l, x[i]);
+        return;
+    }
+    float amax = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++)  // (positions not written hold one of the segment's rows)
+#pragma unroll
+        for (int k = 0; k < 8; k++) amax = fmaxf(amax, finite_abs(x[i][k]));
+    amax = wave_max(amax);
+    const uint64_t block = first / kBlock;
+    float *scale_at = p.scales + (block * scale_heads(p.kv_heads) + h) * 2 + (IS_V ? 1 : 0);
+    int e = scale_exponent(amax), grow = 0;
+    if (off) {  // positions are there: the scale only grows
+        const int was = stored_exponent(*scale_at);
+        e = max(e, was);
+        grow = e - was;
+    }
+    const float inv = two_to(-e), factor = two_to(max(-grow, -126));
+    uint8_t *to = (uint8_t *)(IS_V ? p.v_kept : p.k_kept) + (block * p.kv_heads + h) * kBlockBytes;
+    if (!IS_V) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                uint32_t *at = (uint32_t *)(to + (4 * g + i) * kWidth + Lanes<HALVES>::at(l, half));
+                const float *v = x[i] + 4 * half;
+                const uint32_t w = codes4(v[0], v[1], v[2], v[3], inv);
+                if (mine >> i & 1)
+                    *at = w;
+                else if (grow)
+                    *at = rebase4(*at, factor);
+            }
+    } else if (mine || grow) {  // the lane's eight d, four positions of each a word
+        const uint32_t bytes = (mine & 1 ? 0xffu : 0) | (mine & 2 ? 0xff00u : 0) | (mine & 4 ? 0xff0000u : 0) |
+                               (mine & 8 ? 0xff000000u : 0);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            uint32_t *at = (uint32_t *)(to + (Lanes<HALVES>::at(l, k / 4) + k % 4) * kBlock + 4 * g);
+            uint32_t w = codes4(x[0][k], x[1][k], x[2][k], x[3][k], inv) & bytes;
+            if (mine != 15) {
+                uint32_t held = *at;
+                if (grow) held = rebase4(held, factor);
+                w |= held & ~bytes;
+            }
+            *at = w;
+        }
+    }
+    if (lane == 0) *scale_at = two_to(e);
+}
+
+constexpr uint32_t kWaves = 4;
+
+template <bool XBF16, bool KEPT8, bool HALVES>
+__global__ __launch_bounds__(64 * kWaves, 5) void append_kernel(AppendParams p) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (blockIdx.x >= p.kv_groups) {  // four q heads of q_rows rows a wave
+        const uint32_t u = (blockIdx.x - p.kv_groups) * kWaves + wave, r0 = u / p.head_quads * p.q_rows, l = lane & 15;
+        const uint32_t h = u % p.head_quads * 4 + (lane >> 4);
+        if (r0 >= p.rows || h >= p.heads) return;  // (16 lanes together)
+        float v[kQRows][8], gain[8];
+        f32x4 cs[kQRows][2];
+        bool held[kQRows];
+        const uint32_t n = min(p.q_rows, p.rows - r0);
+#pragma unroll
+        for (uint32_t i = 0; i < kQRows; i++) {
+            if (i >= n) continue;
+            load8<XBF16, HALVES>(row_base<XBF16>(p.q, r0 + i, p.q_stride), h * 128, l, v[i]);
+            const uint32_t pos = p.positions[r0 + i];
+            held[i] = pos < p.place.keys;
+            if (p.turns) load_turns(p.turns + (held[i] ? (size_t)pos * 64 : 0), 0, l, cs[i]);
+        }
+        if (p.q_gain) load_gain<HALVES>(p.q_gain, l, gain);
+#pragma unroll
+        for (uint32_t i = 0; i < kQRows; i++) {
+            if (i >= n) continue;
+            if (p.q_gain) norm8<HALVES>(v[i], gain, p.eps);
+            if (p.turns) turn8<HALVES>(v[i], cs[i]);
+            if (!held[i]) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[i][k] = __builtin_nanf("");
+            }
+            const size_t at = ((size_t)(r0 + i) * p.heads + h) * 128;
             if (p.q_out_bf16) {
-                store_pair_bf16<HALVES>((uint16_t *)p.q_out + at, lane, a[i], b[i]);
+                store8_bf16<HALVES>((uint16_t *)p.q_out + at, l, v[i]);
             } else {
-                float *o = (float *)p.q_out + at;
-                if (HALVES) {
-                    o[lane] = a[i];
-                    o[lane + 64] = b[i];
-                } else {
-                    *(float2 *)(o + 2 * lane) = make_float2(a[i], b[i]);
-                }
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+                    *(f32x4 *)((float *)p.q_out + at + Lanes<HALVES>::at(l, half)) =
+                        f32x4{v[i][4 * half], v[i][4 * half + 1], v[i][4 * half + 2], v[i][4 * half + 3]};
             }
         }
         return;
     }
-    // k and v: the segments that begin among the window's rows, a wave a kv head.
-    const uint32_t groups = (p.kv_heads + 3) / 4, h = blockIdx.x % groups * 4 + wave;
-    const uint32_t w0 = blockIdx.x / groups * p.window;
-    // Lane i looks at row w0 + i: a segment begins where the row does not go on from the one before
-    // it, or begins a block.
-    bool begins = false;
-    if (lane < p.window && w0 + lane < p.rows) {
-        const uint32_t r = w0 + lane, pos = p.positions[r];
-        begins = r == 0 || (pos & (kBlock - 1)) == 0 || p.slots[r - 1] != p.slots[r] || p.positions[r - 1] + 1 != pos;
-    }
-    uint64_t todo = __builtin_amdgcn_ballot_w64(begins);
+    // k and v: the segments that begin among the window's rows, a wave a kv head's k or v.
+    const uint32_t groups = (2 * p.kv_heads + kWaves - 1) / kWaves, first_unit = blockIdx.x % groups * kWaves;
+    const uint32_t unit = first_unit + wave, h = unit >> 1, w0 = blockIdx.x / groups * p.window;
+    const bool is_v = unit & 1, mine = h < p.kv_heads;
+    const void *from = is_v ? p.v : p.k;
+    const uint32_t stride = is_v ? p.v_stride : p.k_stride;
+    // Lane i holds row w0 - 1 + i, of the window, the row before it and the 15 after it. A segment begins
+    // where a row does not go on from the one before it, or begins a block.
+    const uint32_t at = w0 + lane, ri = min(max(at, 1u) - 1, p.rows - 1), si = p.slots[ri], pi = p.positions[ri];
+    const bool there = at >= 1 && at - 1 < p.rows;
+    const uint32_t sb = __shfl_up((int)si, 1, 64), pb = __shfl_up((int)pi, 1, 64);  // (by every lane)
+    const bool goes_on = lane && at >= 2 && sb == si && pb + 1 == pi && (pi & (kBlock - 1)) != 0;
+    const uint64_t begins = __builtin_amdgcn_ballot_w64(there && !goes_on);
+    // Of the window's own rows, lanes 1 .. window.
+    uint64_t todo = begins & (((uint64_t)2 << p.window) - 2);
     while (todo) {
-        const uint32_t r = w0 + __builtin_ctzll(todo);
+        const uint32_t li = __builtin_ctzll(todo), r = w0 + li - 1;
         todo &= todo - 1;
-        const uint32_t slot = __builtin_amdgcn_readfirstlane(p.slots[r]);
-        const uint32_t pos = __builtin_amdgcn_readfirstlane(p.positions[r]);
-        bool on = false;  // lane i: row r + i belongs to the segment
-        if (lane < kBlock && r + lane < p.rows)
-            on = p.slots[r + lane] == slot && p.positions[r + lane] == pos + lane && (pos & (kBlock - 1)) + lane < kBlock;
-        const uint32_t count = __builtin_ctzll(~__builtin_amdgcn_ballot_w64(on));
+        const uint32_t slot = __builtin_amdgcn_readlane(si, li), pos = __builtin_amdgcn_readlane(pi, li);
+        const uint32_t off = pos & (kBlock - 1);
+        // It ends where the next one begins, or the rows do.
+        const uint64_t next = begins >> li >> 1;
+        const uint32_t count = min(next ? __builtin_ctzll(next) + 1 : kBlock, min(p.rows - r, kBlock - off));
         // Rows that a slot cannot hold: nothing is kept of them.
         uint32_t n = holds(p.place, slot, pos) ? min(count, p.place.keys - pos) : 0;
         uint32_t bad = n < count ? TS_STATUS_POSITION : 0;
+        if (slot >= p.place.slot_count) bad = TS_STATUS_PAGE;
+        const bool one = n == 1;  // 16 units a group instead of 4: the first groups do them all
+        if (one && first_unit * 4 >= 2 * p.kv_heads) continue;
+        float x[4][8];
+        if (n && mine && !one) {
+            const void *base = row_base<XBF16>(from, r, stride);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++)
+                load8<XBF16, HALVES>(base, segment_row(4 * (lane >> 4) + i, off, n) * stride + h * 128, lane & 15, x[i]);
+        }
         uint64_t row0 = 0;
         if (n && !row_of(p.place, slot, pos, row0)) {
             bad |= TS_STATUS_PAGE;
             n = 0;
         }
-        if (slot >= p.place.slot_count) bad = TS_STATUS_PAGE;
-        // A segment of the same block before this one in the call: the two would race.
+        // A segment of the same block before this one in the call: the two would race. (Looked for while
+        // the rows come.)
         bool twice = false;
-        for (uint32_t j = threadIdx.x; j < r; j += 256)
-            twice |= p.slots[j] == slot && p.positions[j] / kBlock == pos / kBlock;
-        if (__syncthreads_or(twice)) {
+        auto meets = [&](uint32_t sj, uint32_t pj) { return sj == slot && pj / kBlock == pos / kBlock; };
+        const uint32_t whole = p.fours ? r & ~3u : 0;  // rows looked at four at a time
+#pragma unroll 2
+        for (uint32_t j = threadIdx.x * 4; j < whole; j += 256 * kWaves) {
+            const u32x4 a = *(const u32x4 *)(p.slots + j), b = *(const u32x4 *)(p.positions + j);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) twice |= meets(a[e], b[e]);
+        }
+        for (uint32_t j = whole + threadIdx.x; j < r; j += 64 * kWaves) twice |= meets(p.slots[j], p.positions[j]);
+        if (r && __syncthreads_or(twice)) {
             bad |= TS_STATUS_TWICE;
             n = 0;
         }
         if (bad && p.status && threadIdx.x == 0) atomicOr(p.status, bad);
-        if (n == 0 || h >= p.kv_heads) continue;
-        if (n == 1)
-            append_segment<XBF16, KEPT8, HALVES, 1>(p, r, n, row0, pos, h, lane);
+        if (!n) continue;
+        if (one)
+            append_one<XBF16, KEPT8, HALVES>(p, row0, pos, 4 * unit + (lane >> 4), r, lane & 15);
+        else if (!mine)
+            continue;
+        else if (is_v)
+            append_segment<KEPT8, HALVES, true>(p, row0, pos, n, h, lane, x);
         else
-            append_segment<XBF16, KEPT8, HALVES, 16>(p, r, n, row0, pos, h, lane);
+            append_segment<KEPT8, HALVES, false>(p, row0, pos, n, h, lane, x);
     }
 }
 
@@ -333,6 +451,8 @@ extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
                    a->v_stride % unit == 0,
                "append_rows: rows %u and %u apart must hold %u kv heads and be whole 16-byte pieces", a->k_stride,
                a->v_stride, a->kv_heads);
+    TS_REQUIRE(a->k_stride <= 1u << 26 && a->v_stride <= 1u << 26, "append_rows: rows %u and %u apart", a->k_stride,
+               a->v_stride);  // (16 rows within a 32-bit offset)
     TS_REQUIRE(ts::aligned(a->k, 16) && ts::aligned(a->v, 16) && ts::aligned(a->k_kept, 16) && ts::aligned(a->v_kept, 16) &&
                    ts::aligned(a->scales, 16) && ts::aligned(a->rope_table, 8),
                "append_rows: k, v, kept rows and scales must be 16-byte aligned, the angle table 8");
@@ -359,12 +479,17 @@ extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
     p.rows = a->rows; p.heads = a->heads; p.kv_heads = a->kv_heads;
     p.q_stride = a->q_stride; p.k_stride = a->k_stride; p.v_stride = a->v_stride;
     p.eps = a->eps; p.q_out_bf16 = a->q_out_dtype == TS_BF16;
+    p.fours = ts::aligned(a->slots, 16) && ts::aligned(a->positions, 16);
     // Few rows are taken for a decode step, a segment each: a group looks at one row. Of many, most
-    // go on from the row before them, and a group looks at 16.
-    p.window = a->rows <= 1024 ? 1 : 16;
-    const uint64_t kv = (uint64_t)((a->rows + p.window - 1) / p.window) * ((a->kv_heads + 3) / 4);
-    p.head_groups = (a->heads + 4 * kQBatch - 1) / (4 * kQBatch);
-    const uint64_t all = kv + (q ? (uint64_t)a->rows * p.head_groups : 0);
+    // go on from the row before them, and a group looks at 16; and a wave of q heads takes four rows,
+    // whose loads are in flight together.
+    const bool few = a->rows <= 1024;
+    p.window = few ? 1 : 16;
+    p.q_rows = few ? 1 : kQRows;
+    const uint64_t kv = (uint64_t)((a->rows + p.window - 1) / p.window) * ((2 * a->kv_heads + kWaves - 1) / kWaves);
+    p.head_quads = (a->heads + 3) / 4;
+    const uint64_t units = q ? (uint64_t)((a->rows + p.q_rows - 1) / p.q_rows) * p.head_quads : 0;
+    const uint64_t all = kv + (units + kWaves - 1) / kWaves;
     TS_REQUIRE(all <= 0x7fffffffull, "append_rows: %u rows in one launch", a->rows);
     p.kv_groups = (uint32_t)kv;
     const int pick = (a->x_dtype == TS_BF16 ? 4 : 0) | (blocks ? 2 : 0) | (a->halves ? 1 : 0);
@@ -372,7 +497,7 @@ extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
         append_kernel<false, false, false>, append_kernel<false, false, true>, append_kernel<false, true, false>,
         append_kernel<false, true, true>,   append_kernel<true, false, false>, append_kernel<true, false, true>,
         append_kernel<true, true, false>,   append_kernel<true, true, true>};
-    hipLaunchKernelGGL(kernels[pick], dim3((uint32_t)all), dim3(256), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(kernels[pick], dim3((uint32_t)all), dim3(64 * kWaves), 0, (hipStream_t)stream, p);
     TS_CHECK_LAUNCH("append_rows launch");
     return TS_OK;
 }
