@@ -326,46 +326,64 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
     }
 }
 
-// The parts of a tile's columns joined in their order, a thread four d of a column.
-__global__ __launch_bounds__(64) void join_kept8_kernel(AttendParams p, uint32_t cols, uint32_t pieces) {
-    const uint32_t gi = blockIdx.x / pieces;
+// The parts of a tile's columns joined: S lane groups of 32 (four d a lane) take a column's parts in turn,
+// 8 / S columns a group of 256. (One lane group walking 128 parts by itself waits 20 us.)
+template <uint32_t S>
+__global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_t cols, uint32_t pieces) {
+    __shared__ float smax[8], ssum[8];
+    __shared__ f32x4 so[8][32];
+    constexpr uint32_t kBatch = 4;
+    const uint32_t gi = blockIdx.x / pieces, lg = threadIdx.x / 32, d = threadIdx.x % 32;
     const Tile tile = tile_of(p, gi);
-    const uint32_t c = blockIdx.x % pieces * 2 + threadIdx.x / 32, d = threadIdx.x % 32 * 4;
+    const uint32_t c = blockIdx.x % pieces * (8 / S) + lg / S, j1 = lg % S;
     uint32_t r, h;
-    if (!tile.column(p, c, r, h)) return;
-    const float *all = p.partials + ((size_t)gi * p.parts * cols + c) * kPart;
+    const bool there = c < cols && tile.column(p, c, r, h);
+    const float *all = p.partials + ((size_t)gi * p.parts * cols + (there ? c : 0)) * kPart;
     const size_t next = (size_t)cols * kPart;
-    constexpr uint32_t kBatch = 8;
+    // The maximum: every lane of the lane group looks at parts of its own.
     float M = -INFINITY;
-    for (uint32_t j0 = 0; j0 < p.parts; j0 += kBatch) {
-        float mq[kBatch];
+    for (uint32_t j = j1 + S * d; j < p.parts; j += S * 32) M = fmaxf(M, all[j * next]);
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; j++) mq[j] = all[min(j0 + j, p.parts - 1) * next];
+    for (int x = 1; x < 32; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+    if (S > 1) {
+        if (d == 0) smax[lg] = M;
+        __syncthreads();
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; j++) M = fmaxf(M, mq[j]);
+        for (uint32_t s = 0; s < S; s++) M = fmaxf(M, smax[lg / S * S + s]);
     }
     float L = 0.0f;
     f32x4 O = f32x4{0, 0, 0, 0};
-    for (uint32_t j0 = 0; j0 < p.parts; j0 += kBatch) {
+    for (uint32_t j0 = j1; j0 < p.parts; j0 += S * kBatch) {
         float mq[kBatch], lq[kBatch];
         f32x4 oq[kBatch];
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {  // past the end: read, not used
-            const float *at = all + min(j0 + j, p.parts - 1) * next;
+            const float *at = all + min(j0 + S * j, p.parts - 1) * next;
             mq[j] = at[0];
             lq[j] = at[1];
-            oq[j] = *(const f32x4 *)(at + 4 + d);
+            oq[j] = *(const f32x4 *)(at + 4 + 4 * d);
         }
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {
             // An empty part (max -inf, sum 0) has no O.
-            if (j0 + j >= p.parts || (mq[j] == -INFINITY && lq[j] == 0.0f)) continue;
+            if (j0 + S * j >= p.parts || (mq[j] == -INFINITY && lq[j] == 0.0f)) continue;
             const float f = mq[j] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mq[j] - M);
             L += lq[j] * f;
             O += oq[j] * f;
         }
     }
-    store4(p, ((size_t)r * p.heads + h) * 128 + d, O / L);
+    if (S > 1) {
+        so[lg][d] = O;
+        if (d == 0) ssum[lg] = L;
+        __syncthreads();
+        if (j1) return;
+#pragma unroll
+        for (uint32_t s = 1; s < S; s++) {
+            L += ssum[lg + s];
+            O += so[lg + s][d];
+        }
+    }
+    if (there) store4(p, ((size_t)r * p.heads + h) * 128 + 4 * d, O / L);
 }
 
 // How a call runs: `columns` (row, q head) pairs a tile; 16: the kernel above, more: kept8_rows.hip's.
@@ -469,8 +487,10 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     else
         rc = f32 ? launch<1, true>(p, groups, stream) : launch<1, false>(p, groups, stream);
     if (rc || s.parts == 1) return rc;
-    const uint32_t pieces = (s.tile_rows * p.group + 1) / 2;
-    hipLaunchKernelGGL(join_kept8_kernel, dim3(s.groups * pieces), dim3(64), 0, (hipStream_t)stream, p, s.columns, pieces);
+    const uint32_t used = s.tile_rows * p.group, S = s.parts <= 2 ? 1 : s.parts <= 8 ? 2 : 8;
+    const uint32_t pieces = (used * S + 7) / 8;
+    const auto join = S == 1 ? join_kept8_kernel<1> : S == 2 ? join_kept8_kernel<2> : join_kept8_kernel<8>;
+    hipLaunchKernelGGL(join, dim3(s.groups * pieces), dim3(256), 0, (hipStream_t)stream, p, s.columns, pieces);
     TS_CHECK_LAUNCH("attend_kept8 join launch");
     return TS_OK;
 }
