@@ -27,149 +27,131 @@ using namespace kept8;
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kRound = kStep * kWaves;
 
-template <int NT, bool QF32>
+template <bool QF32>
 __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
-    constexpr uint32_t kCols = 16 * NT, kParts = QF32 ? 3 : 1;
+    constexpr uint32_t kCols = 16, kParts = QF32 ? 3 : 1;
     extern __shared__ __attribute__((aligned(16))) float joined[];  // [kWaves][kCols][kPart]
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4;
     const uint32_t part = blockIdx.x % p.parts, gi = blockIdx.x / p.parts;
     const Tile tile = tile_of(p, gi);
+    float *mine = p.partials ? p.partials + ((size_t)gi * p.parts + part) * kCols * kPart : nullptr;
+    auto nothing = [&] {  // a part without keys
+        if (threadIdx.x < kCols) {
+            mine[threadIdx.x * kPart] = -INFINITY;
+            mine[threadIdx.x * kPart + 1] = 0.0f;
+        }
+    };
 
-    // Columns: (row, head) pairs of the tile, row by row.
-    uint32_t pos[NT], from[NT], slot[NT];
-    bool live[NT];
-    bf16x8 q[NT][4][kParts];
+    // The lane's column, a (row, head) pair of the tile.
+    uint32_t r, h;
+    const bool there = tile.column(p, col, r, h);
+    const uint32_t pos = there ? p.positions[r] : 0, slot = there ? p.slots[r] : 0;
+    const bool live = there && pos <= p.max_position && holds(p.place, slot, pos);
+    if (there && !live && p.status && part == 0 && wave == 0 && grp == 0)
+        atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
+    const uint32_t from = pos > p.back ? pos - p.back : 0;
+    const size_t q_at = live ? ((size_t)r * p.heads + h) * 128 : 0;
+
+    // A pass over the keys for each slot among the columns (one, where rows of a slot stand together): its
+    // active columns see keys in [lo, hi], all of them those in [all_lo, all_hi].
+    struct Pass {
+        uint32_t now, lo, hi, all_lo, all_hi;
+        bool act;
+    } s;
+    bool wait = live;
+    auto next_pass = [&] {
+        const uint64_t b = __builtin_amdgcn_ballot_w64(wait);
+        if (!b) return false;
+        s.now = __builtin_amdgcn_readlane(slot, __builtin_ctzll(b));
+        s.act = wait && slot == s.now;
+        wait = wait && !s.act;
+        s.lo = row16_least(s.act ? from : 0xffffffffu);
+        s.hi = ~row16_least(s.act ? ~pos : 0xffffffffu);
+        s.all_lo = ~row16_least(s.act ? ~from : live ? 0u : 0xffffffffu);  // (a column not active sees none)
+        s.all_hi = row16_least(s.act ? pos : 0xffffffffu);
+        return true;
+    };
+    bool more_passes = next_pass();
+    uint32_t base0 = more_passes ? s.lo & ~(kBlock - 1) : 0, span = more_passes ? s.hi - base0 : 0;
+    bool worked = more_passes && (uint64_t)part * p.chunk <= span;
+    if (mine && !worked && __builtin_amdgcn_ballot_w64(wait) == 0) {  // (uniform over the group)
+        nothing();
+        return;
+    }
+
+    // The blocks of a step; bit j of `lost`: block j's page is not held.
+    struct Blocks {
+        uint32_t at[4], lost;
+    } b;
+    auto look = [&](uint32_t base) {
+        b.lost = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            bool gone;
+            b.at[j] = block_of(p.place, s.now, min(base / kBlock + j, s.hi / kBlock) * kBlock, gone);
+            b.lost |= gone ? 1u << j : 0u;
+        }
+    };
+    // Lane value j of four uniform ones.
+    auto choose = [](uint32_t j, auto a, auto b, auto c, auto d) {
+        const auto x = j & 1 ? b : a, y = j & 1 ? d : c;
+        return j & 2 ? y : x;
+    };
+    u32x4 kf[4][2], vf[8];
+    float ks = 0.0f, vs = 0.0f;
+    const_f32 *scales = in_constant<const_f32 *>(p.scales + tile.kvh * 2);
+    const size_t scale_row = scale_heads(p.kv_heads) * 2;
+    auto load_k = [&] {
+        const uint32_t block = choose(col >> 2, b.at[0], b.at[1], b.at[2], b.at[3]);
+        const uint8_t *at = p.k + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) kf[t][x] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * x);
+        ks = choose(col >> 2, scales[b.at[0] * scale_row], scales[b.at[1] * scale_row], scales[b.at[2] * scale_row],
+                    scales[b.at[3] * scale_row]);
+    };
+    auto load_v = [&] {
+        const uint32_t block = choose(grp, b.at[0], b.at[1], b.at[2], b.at[3]);
+        const uint8_t *at = p.v + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + col * kBlock;
+#pragma unroll
+        for (int dt = 0; dt < 8; dt++) vf[dt] = *(const u32x4 *)(at + dt * 16 * kBlock);
+        vs = choose(grp, scales[b.at[0] * scale_row + 1], scales[b.at[1] * scale_row + 1],
+                    scales[b.at[2] * scale_row + 1], scales[b.at[3] * scale_row + 1]);
+    };
+
+    // Keys from base0 + off on are this wave's next step: a part takes chunks in turn, its waves the steps
+    // of a chunk. The first step's K is asked for before q, its V after.
+    const uint64_t off0 = (uint64_t)part * p.chunk + wave * kStep;
+    const bool early = more_passes && off0 <= span;
+    if (early) {
+        look(base0 + (uint32_t)off0);
+        load_k();
+    }
     const float sl = base2_scale(p.scale);
+    bf16x8 q[4][kParts];
+    load_q<QF32, kParts>(p, live, q_at, grp, q);
+    if (early) load_v();
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[8];  // O^T: lane's column, d 16 dt + 4 grp + i
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        uint32_t r, h;
-        const bool there = tile.column(p, 16 * nt + col, r, h);
-        pos[nt] = there ? p.positions[r] : 0;
-        slot[nt] = there ? p.slots[r] : 0;
-        live[nt] = there && pos[nt] <= p.max_position && holds(p.place, slot[nt], pos[nt]);
-        if (there && !live[nt] && p.status && part == 0 && wave == 0 && grp == 0)
-            atomicOr(p.status, slot[nt] >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
-        from[nt] = pos[nt] > p.back ? pos[nt] - p.back : 0;
-        const size_t at = live[nt] ? ((size_t)r * p.heads + h) * 128 : 0;
-        load_q<QF32, kParts>(p, live[nt], at, grp, q[nt]);
-    }
+    for (int dt = 0; dt < 8; dt++) o[dt] = f32x4{0, 0, 0, 0};
 
-    float m[NT], l[NT];
-    f32x4 o[NT][8];  // O^T: lane's column, d 16 dt + 4 grp + i
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        l[nt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < 8; dt++) o[nt][dt] = f32x4{0, 0, 0, 0};
-    }
-    bool worked = false;
-
-    // A pass over the keys for each slot among the columns (one, where rows of a slot stand together).
-    bool wait[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) wait[nt] = live[nt];
-    for (;;) {
-        uint32_t now = 0;
-        bool any = false;
-#pragma unroll
-        for (int nt = NT - 1; nt >= 0; nt--) {
-            const uint64_t b = __builtin_amdgcn_ballot_w64(wait[nt]);
-            if (b) {
-                now = __builtin_amdgcn_readlane(slot[nt], __builtin_ctzll(b));
-                any = true;
+    for (bool first = true; more_passes; first = false, more_passes = next_pass()) {
+        if (!first) {
+            base0 = s.lo & ~(kBlock - 1);
+            span = s.hi - base0;
+            worked |= (uint64_t)part * p.chunk <= span;
+            if (off0 <= span) {
+                look(base0 + (uint32_t)off0);
+                load_k();
+                load_v();
             }
         }
-        if (!any) break;
-        bool act[NT];
-        uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            act[nt] = wait[nt] && slot[nt] == now;
-            wait[nt] = wait[nt] && !act[nt];
-            if (act[nt]) {
-                lo = min(lo, from[nt]);
-                hi = max(hi, pos[nt]);
-            }
-        }
-        // Keys every active column sees: [all_lo, all_hi]. A column not active sees none.
-        uint32_t all_lo = 0, all_hi = 0xffffffffu;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            if (act[nt]) {
-                all_lo = max(all_lo, from[nt]);
-                all_hi = min(all_hi, pos[nt]);
-            } else if (live[nt]) {
-                all_lo = 0xffffffffu;
-            }
-        }
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) {
-            lo = min(lo, (uint32_t)__shfl_xor((int)lo, x, 64));
-            hi = max(hi, (uint32_t)__shfl_xor((int)hi, x, 64));
-            all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, x, 64));
-            all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, x, 64));
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
-        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-        const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, span = hi - base0;
-        worked |= (uint64_t)part * p.chunk <= span;
-
-        // The blocks of a step; bit j of `lost`: block j's page is not held.
-        struct Blocks {
-            uint32_t at[4], lost;
-        };
-        auto look = [&](uint32_t base) {
-            Blocks b;
-            b.lost = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < 4; j++) {
-                bool gone;
-                b.at[j] = block_of(p.place, now, min(base / kBlock + j, last) * kBlock, gone);
-                b.lost |= gone ? 1u << j : 0u;
-            }
-            return b;
-        };
-        // Lane value j of four uniform ones.
-        auto choose = [](uint32_t j, auto a, auto b, auto c, auto d) {
-            const auto x = j & 1 ? b : a, y = j & 1 ? d : c;
-            return j & 2 ? y : x;
-        };
-        u32x4 kf[4][2], vf[8];
-        float ks = 0.0f, vs = 0.0f;
-        const_f32 *scales = in_constant<const_f32 *>(p.scales + tile.kvh * 2);
-        const size_t scale_row = scale_heads(p.kv_heads) * 2;
-        auto load_k = [&](const Blocks &b) {
-            const uint32_t block = choose(col >> 2, b.at[0], b.at[1], b.at[2], b.at[3]);
-            const uint8_t *at = p.k + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int x = 0; x < 2; x++) kf[t][x] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * x);
-            ks = choose(col >> 2, scales[b.at[0] * scale_row], scales[b.at[1] * scale_row], scales[b.at[2] * scale_row],
-                        scales[b.at[3] * scale_row]);
-        };
-        auto load_v = [&](const Blocks &b) {
-            const uint32_t block = choose(grp, b.at[0], b.at[1], b.at[2], b.at[3]);
-            const uint8_t *at = p.v + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + col * kBlock;
-#pragma unroll
-            for (int dt = 0; dt < 8; dt++) vf[dt] = *(const u32x4 *)(at + dt * 16 * kBlock);
-            vs = choose(grp, scales[b.at[0] * scale_row + 1], scales[b.at[1] * scale_row + 1],
-                        scales[b.at[2] * scale_row + 1], scales[b.at[3] * scale_row + 1]);
-        };
-
-        // Keys from base0 + off on are this wave's next step: a part takes chunks in turn, its waves the
-        // steps of a chunk.
-        uint64_t off = (uint64_t)part * p.chunk + wave * kStep;
+        uint64_t off = off0;
         uint32_t left = p.chunk / kRound;  // steps of the chunk
-        if (off > span) continue;
-        Blocks b = look(base0 + (uint32_t)off);
-        load_k(b);
-        load_v(b);
-        for (bool more = true; more;) {
+        for (bool more = off <= span; more;) {
             const uint32_t base = base0 + (uint32_t)off, lost = b.lost;
             off += kRound;
             if (--left == 0) {
@@ -179,49 +161,42 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
             more = off <= span;
             // (The last step's codes are asked for once more, from the caches: a branch around the
             // loads would keep two copies of them in registers.)
-            b = look(more ? base0 + (uint32_t)off : base);
-            f32x4 s[NT][4];
+            look(more ? base0 + (uint32_t)off : base);
+            f32x4 sc[4];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 pin(kf[t][0]);
                 pin(kf[t][1]);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[nt][t] = f32x4{0, 0, 0, 0};
+                sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const u32x4 w = kf[t][j >> 1];
                     const bf16x8 kc = codes8(j & 1 ? w.z : w.x, j & 1 ? w.w : w.y, ks);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (uint32_t e = 0; e < kParts; e++) s[nt][t] = mfma16(kc, q[nt][j][e], s[nt][t]);
+                    for (uint32_t e = 0; e < kParts; e++) sc[t] = mfma16(kc, q[j][e], sc[t]);
                 }
             }
-            load_k(b);
+            load_k();
 
             // A step that meets a window's edge, or a block that is lost.
-            if (base < all_lo || base + (kStep - 1) > all_hi || lost) {
+            if (base < s.all_lo || base + (kStep - 1) > s.all_hi || lost) {
                 const uint32_t key0 = base + kBlock * grp;
                 const bool gone = lost >> grp & 1;
                 if (lost && p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
-                uint32_t seen[NT];  // a bit for each of the lane's 16 keys
+                const uint32_t seen = s.act ? seen_keys(key0, from, pos) : 0u;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    seen[nt] = act[nt] ? seen_keys(key0, from[nt], pos[nt]) : 0u;
+                for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float x = gone ? __builtin_nanf("") : s[nt][t][e];
-                            s[nt][t][e] = seen[nt] >> (4 * t + e) & 1 ? x : -INFINITY;
-                        }
-                }
+                    for (int e = 0; e < 4; e++) {
+                        const float x = gone ? __builtin_nanf("") : sc[t][e];
+                        sc[t][e] = seen >> (4 * t + e) & 1 ? x : -INFINITY;
+                    }
                 // Codes outside [lo, hi] may be anything: as zeros they add nothing.
                 uint32_t nan = 0;
 #pragma unroll
                 for (int dt = 0; dt < 8; dt++) {
-                    vf[dt] = u32x4{within4(vf[dt].x, key0, lo, hi), within4(vf[dt].y, key0 + 4, lo, hi),
-                                   within4(vf[dt].z, key0 + 8, lo, hi), within4(vf[dt].w, key0 + 12, lo, hi)};
+                    vf[dt] = u32x4{within4(vf[dt].x, key0, s.lo, s.hi), within4(vf[dt].y, key0 + 4, s.lo, s.hi),
+                                   within4(vf[dt].z, key0 + 8, s.lo, s.hi), within4(vf[dt].w, key0 + 12, s.lo, s.hi)};
                     nan |= nan_codes(vf[dt].x) | nan_codes(vf[dt].y) | nan_codes(vf[dt].z) | nan_codes(vf[dt].w);
                 }
                 // A NaN code at a key that some columns see and some do not: a weight of 0 times NaN
@@ -237,30 +212,26 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
                             ones[e] = at * 0x38u;
                             vf[dt][e] &= ~(at * 0xffu);
                         }
+                        f32x4 hit = f32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            f32x4 hit = f32x4{0, 0, 0, 0};
+                        for (int x = 0; x < 2; x++) {
+                            uint32_t sw[4];
 #pragma unroll
-                            for (int x = 0; x < 2; x++) {
-                                uint32_t sw[4];
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const uint32_t two = seen[nt] >> (8 * x + 2 * e);
-                                    sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
-                                }
-                                hit = mfma16(codes8(ones[2 * x], ones[2 * x + 1], 1.0f),
-                                             as_bf16x8(u32x4{sw[0], sw[1], sw[2], sw[3]}), hit);
+                            for (int e = 0; e < 4; e++) {
+                                const uint32_t two = seen >> (8 * x + 2 * e);
+                                sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
                             }
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (hit[e] > 0.0f) o[nt][dt][e] = __builtin_nanf("");
+                            hit = mfma16(codes8(ones[2 * x], ones[2 * x + 1], 1.0f),
+                                         as_bf16x8(u32x4{sw[0], sw[1], sw[2], sw[3]}), hit);
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (hit[e] > 0.0f) o[dt][e] = __builtin_nanf("");
                     }
                 }
             }
-            bf16x8 w[NT][2][kParts];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) weigh<kParts, 8>(s[nt], sl, m[nt], l[nt], o[nt], w[nt]);
+            bf16x8 w[2][kParts];
+            weigh<kParts, 8>(sc, sl, m, l, o, w);
 #pragma unroll
             for (int dt = 0; dt < 8; dt++) {
                 pin(vf[dt]);
@@ -268,39 +239,31 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
                 for (int x = 0; x < 2; x++) {
                     const bf16x8 vc = codes8(x ? vf[dt].z : vf[dt].x, x ? vf[dt].w : vf[dt].y, vs);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (uint32_t e = 0; e < kParts; e++) o[nt][dt] = mfma16(vc, w[nt][x][e], o[nt][dt]);
+                    for (uint32_t e = 0; e < kParts; e++) o[dt] = mfma16(vc, w[x][e], o[dt]);
                 }
             }
-            load_v(b);
+            load_v();
         }
     }
 
     // The waves' results joined, a thread four d of a column at a time.
-    float *mine = p.partials ? p.partials + ((size_t)gi * p.parts + part) * kCols * kPart : nullptr;
-    if (mine && !worked) {  // nothing to join (uniform over the group)
-        for (uint32_t c = threadIdx.x; c < kCols; c += 256) {
-            mine[c * kPart] = -INFINITY;
-            mine[c * kPart + 1] = 0.0f;
-        }
+    if (mine && !worked) {
+        nothing();
         return;
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        float *at = joined + (wave * kCols + 16 * nt + col) * kPart;
-        const float sum = rows4_sum(l[nt]);
+    {
+        float *at = joined + (wave * kCols + col) * kPart;
+        const float sum = rows4_sum(l);
         if (grp == 0) {
-            at[0] = m[nt];
-            at[1] = live[nt] ? sum : __builtin_nanf("");  // a refused column passed unmasked with the others
+            at[0] = m;
+            at[1] = live ? sum : __builtin_nanf("");  // a refused column passed unmasked with the others
         }
 #pragma unroll
-        for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[nt][dt];
+        for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[dt];
     }
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < kCols * 32; e += 256) {
         const uint32_t c = e / 32, d = e % 32 * 4;
-        uint32_t r, h;
         if (!tile.column(p, c, r, h)) continue;
         float M = -INFINITY;
 #pragma unroll
@@ -440,13 +403,10 @@ int check(const ts_kept8_args *k) {
     return TS_OK;
 }
 
-template <int NT, bool QF32>
+template <bool QF32>
 int launch(const AttendParams &p, uint32_t groups, void *stream) {
-    constexpr uint32_t kLds = kWaves * 16 * NT * kPart * sizeof(float);
-    static const hipError_t attr = hipFuncSetAttribute((const void *)attend_kept8_kernel<NT, QF32>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (attr != hipSuccess) return ts::hip_status(attr, "attend_kept8: shared memory attribute");
-    hipLaunchKernelGGL((attend_kept8_kernel<NT, QF32>), dim3(groups), dim3(256), kLds, (hipStream_t)stream, p);
+    constexpr uint32_t kLds = kWaves * 16 * kPart * sizeof(float);
+    hipLaunchKernelGGL(attend_kept8_kernel<QF32>, dim3(groups), dim3(256), kLds, (hipStream_t)stream, p);
     TS_CHECK_LAUNCH("attend_kept8 launch");
     return TS_OK;
 }
@@ -485,7 +445,7 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     if (s.columns > 16)
         rc = ts::kept8_rows_launch(p, s.columns, f32, groups, stream);
     else
-        rc = f32 ? launch<1, true>(p, groups, stream) : launch<1, false>(p, groups, stream);
+        rc = f32 ? launch<true>(p, groups, stream) : launch<false>(p, groups, stream);
     if (rc || s.parts == 1) return rc;
     const uint32_t used = s.tile_rows * p.group, S = s.parts <= 2 ? 1 : s.parts <= 8 ? 2 : 8;
     const uint32_t pieces = (used * S + 7) / 8;

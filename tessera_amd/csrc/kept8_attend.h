@@ -52,6 +52,17 @@ TS_DEV float rows4_max(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// The least of the 16 lanes of a row, by DPP moves; uniform where the four rows hold the same.
+template <int CTRL>
+TS_DEV uint32_t dpp_u(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false); }
+TS_DEV uint32_t row16_least(uint32_t v) {
+    v = min(v, dpp_u<0xB1>(v));
+    v = min(v, dpp_u<0x4E>(v));
+    v = min(v, dpp_u<0x141>(v));
+    v = min(v, dpp_u<0x140>(v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
 TS_DEV void store4(const AttendParams &p, size_t at, f32x4 v) {
     if (p.out_bf16)
         *(u32x2 *)((uint16_t *)p.out + at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};

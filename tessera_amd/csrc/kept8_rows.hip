@@ -128,17 +128,10 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                 all_lo = 0xffffffffu;
             }
         }
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) {
-            lo = min(lo, (uint32_t)__shfl_xor((int)lo, x, 64));
-            hi = max(hi, (uint32_t)__shfl_xor((int)hi, x, 64));
-            all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, x, 64));
-            all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, x, 64));
-        }
         // The wave's own keys [wlo, whi] (none: wlo above whi), the group's [lo, hi].
-        const uint32_t wlo = __builtin_amdgcn_readfirstlane(lo), whi = __builtin_amdgcn_readfirstlane(hi);
-        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        const uint32_t wlo = row16_least(lo), whi = ~row16_least(~hi);
+        all_lo = ~row16_least(~all_lo);
+        all_hi = row16_least(all_hi);
         lo = over_waves<W>(shared_words, wave, wlo, [](uint32_t a, uint32_t b) { return min(a, b); });
         hi = over_waves<W>(shared_words, wave, whi, [](uint32_t a, uint32_t b) { return max(a, b); });
         const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, span = hi - base0;
