@@ -25,7 +25,7 @@ namespace {
 using namespace kept8;
 
 constexpr uint32_t kWaves = 4;
-constexpr uint32_t kRound = kStep * kWaves;
+constexpr uint32_t kRound = kStep * kWaves;  // keys of a group's waves at a time, and its unit of shared keys
 
 template <bool QF32>
 __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
@@ -33,259 +33,252 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
     extern __shared__ __attribute__((aligned(16))) float joined[];  // [kWaves][kCols][kPart]
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4;
-    const uint32_t part = blockIdx.x % p.parts, gi = blockIdx.x / p.parts;
-    const Tile tile = tile_of(p, gi);
-    float *mine = p.partials ? p.partials + ((size_t)gi * p.parts + part) * kCols * kPart : nullptr;
-    auto nothing = [&] {  // a part without keys
-        if (threadIdx.x < kCols) {
-            mine[threadIdx.x * kPart] = -INFINITY;
-            mine[threadIdx.x * kPart + 1] = 0.0f;
-        }
-    };
+    __shared__ uint32_t starts[kMaxShared + 1];
+    const uint32_t u = blockIdx.x / p.kv_heads, kvh = blockIdx.x % p.kv_heads;
+    Share share;
+    if (!share_of<kRound>(p, u, lane, starts, share)) return;
+    for (;;) {
+        const Part part = part_of(p, u, lane, kvh, kCols, starts, share);
+        const Tile tile = {part.row0, kvh};
 
-    // The lane's column, a (row, head) pair of the tile.
-    uint32_t r, h;
-    const bool there = tile.column(p, col, r, h);
-    const uint32_t pos = there ? p.positions[r] : 0, slot = there ? p.slots[r] : 0;
-    const bool live = there && pos <= p.max_position && holds(p.place, slot, pos);
-    if (there && !live && p.status && part == 0 && wave == 0 && grp == 0)
-        atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
-    const uint32_t from = pos > p.back ? pos - p.back : 0;
-    const size_t q_at = live ? ((size_t)r * p.heads + h) * 128 : 0;
+        // The lane's column, a (row, head) pair of the tile.
+        uint32_t r, h;
+        const bool there = tile.column(p, col, r, h);
+        const uint32_t pos = there ? p.positions[r] : 0, slot = there ? p.slots[r] : 0;
+        const bool live = there && pos <= p.max_position && holds(p.place, slot, pos);
+        if (there && !live && p.status && part.a == 0 && wave == 0 && grp == 0)
+            atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
+        const uint32_t from = pos > p.back ? pos - p.back : 0;
+        const size_t q_at = live ? ((size_t)r * p.heads + h) * 128 : 0;
 
-    // A pass over the keys for each slot among the columns (one, where rows of a slot stand together): its
-    // active columns see keys in [lo, hi], all of them those in [all_lo, all_hi].
-    struct Pass {
-        uint32_t now, lo, hi, all_lo, all_hi;
-        bool act;
-    } s;
-    bool wait = live;
-    auto next_pass = [&] {
-        const uint64_t b = __builtin_amdgcn_ballot_w64(wait);
-        if (!b) return false;
-        s.now = __builtin_amdgcn_readlane(slot, __builtin_ctzll(b));
-        s.act = wait && slot == s.now;
-        wait = wait && !s.act;
-        s.lo = row16_least(s.act ? from : 0xffffffffu);
-        s.hi = ~row16_least(s.act ? ~pos : 0xffffffffu);
-        s.all_lo = ~row16_least(s.act ? ~from : live ? 0u : 0xffffffffu);  // (a column not active sees none)
-        s.all_hi = row16_least(s.act ? pos : 0xffffffffu);
-        return true;
-    };
-    bool more_passes = next_pass();
-    uint32_t base0 = more_passes ? s.lo & ~(kBlock - 1) : 0, span = more_passes ? s.hi - base0 : 0;
-    bool worked = more_passes && (uint64_t)part * p.chunk <= span;
-    if (mine && !worked && __builtin_amdgcn_ballot_w64(wait) == 0) {  // (uniform over the group)
-        nothing();
-        return;
-    }
-
-    // The blocks of a step; bit j of `lost`: block j's page is not held.
-    struct Blocks {
-        uint32_t at[4], lost;
-    } b;
-    auto look = [&](uint32_t base) {
-        b.lost = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            bool gone;
-            b.at[j] = block_of(p.place, s.now, min(base / kBlock + j, s.hi / kBlock) * kBlock, gone);
-            b.lost |= gone ? 1u << j : 0u;
-        }
-    };
-    // Lane value j of four uniform ones.
-    auto choose = [](uint32_t j, auto a, auto b, auto c, auto d) {
-        const auto x = j & 1 ? b : a, y = j & 1 ? d : c;
-        return j & 2 ? y : x;
-    };
-    u32x4 kf[4][2], vf[8];
-    float ks = 0.0f, vs = 0.0f;
-    const_f32 *scales = in_constant<const_f32 *>(p.scales + tile.kvh * 2);
-    const size_t scale_row = scale_heads(p.kv_heads) * 2;
-    auto load_k = [&] {
-        const uint32_t block = choose(col >> 2, b.at[0], b.at[1], b.at[2], b.at[3]);
-        const uint8_t *at = p.k + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int x = 0; x < 2; x++) kf[t][x] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * x);
-        ks = choose(col >> 2, scales[b.at[0] * scale_row], scales[b.at[1] * scale_row], scales[b.at[2] * scale_row],
-                    scales[b.at[3] * scale_row]);
-    };
-    auto load_v = [&] {
-        const uint32_t block = choose(grp, b.at[0], b.at[1], b.at[2], b.at[3]);
-        const uint8_t *at = p.v + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + col * kBlock;
-#pragma unroll
-        for (int dt = 0; dt < 8; dt++) vf[dt] = *(const u32x4 *)(at + dt * 16 * kBlock);
-        vs = choose(grp, scales[b.at[0] * scale_row + 1], scales[b.at[1] * scale_row + 1],
-                    scales[b.at[2] * scale_row + 1], scales[b.at[3] * scale_row + 1]);
-    };
-
-    // Keys from base0 + off on are this wave's next step: a part takes chunks in turn, its waves the steps
-    // of a chunk. The first step's K is asked for before q, its V after.
-    const uint64_t off0 = (uint64_t)part * p.chunk + wave * kStep;
-    const bool early = more_passes && off0 <= span;
-    if (early) {
-        look(base0 + (uint32_t)off0);
-        load_k();
-    }
-    const float sl = base2_scale(p.scale);
-    bf16x8 q[4][kParts];
-    load_q<QF32, kParts>(p, live, q_at, grp, q);
-    if (early) load_v();
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o[8];  // O^T: lane's column, d 16 dt + 4 grp + i
-#pragma unroll
-    for (int dt = 0; dt < 8; dt++) o[dt] = f32x4{0, 0, 0, 0};
-
-    for (bool first = true; more_passes; first = false, more_passes = next_pass()) {
-        if (!first) {
+        // A pass over the keys for each slot among the columns (one, where rows of a slot stand together): its
+        // active columns see keys in [lo, hi], all of them those in [all_lo, all_hi].
+        struct Pass {
+            uint32_t now, lo, hi, all_lo, all_hi;
+            bool act;
+        } s;
+        bool wait = live;
+        auto next_pass = [&] {
+            const uint64_t b = __builtin_amdgcn_ballot_w64(wait);
+            if (!b) return false;
+            s.now = __builtin_amdgcn_readlane(slot, __builtin_ctzll(b));
+            s.act = wait && slot == s.now;
+            wait = wait && !s.act;
+            s.lo = row16_least(s.act ? from : 0xffffffffu);
+            s.hi = ~row16_least(s.act ? ~pos : 0xffffffffu);
+            s.all_lo = ~row16_least(s.act ? ~from : live ? 0u : 0xffffffffu);  // (a column not active sees none)
+            s.all_hi = row16_least(s.act ? pos : 0xffffffffu);
+            return true;
+        };
+        // Of a pass, the wave's next step is the keys from base0 + off on, its last one's off at most `last`.
+        uint32_t base0, off, last;
+        auto next_keys = [&] {
+            if (!next_pass()) return false;
             base0 = s.lo & ~(kBlock - 1);
-            span = s.hi - base0;
-            worked |= (uint64_t)part * p.chunk <= span;
-            if (off0 <= span) {
-                look(base0 + (uint32_t)off0);
+            const uint32_t span = s.hi - base0, np = span / kRound + 1;
+            const uint32_t a = pass_unit(part.a, part.n, np), b = pass_unit(part.b, part.n, np);
+            off = a * kRound + wave * kStep;
+            last = a < b ? min(b * kRound - 1, span) : 0;
+            if (a >= b) off = 1;
+            return true;
+        };
+        bool more_passes = next_keys();
+
+        // The blocks of a step; bit j of `lost`: block j's page is not held.
+        struct Blocks {
+            uint32_t at[4], lost;
+        } b;
+        auto look = [&](uint32_t base) {
+            b.lost = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                bool gone;
+                b.at[j] = block_of(p.place, s.now, min(base / kBlock + j, s.hi / kBlock) * kBlock, gone);
+                b.lost |= gone ? 1u << j : 0u;
+            }
+        };
+        // Lane value j of four uniform ones.
+        auto choose = [](uint32_t j, auto a, auto b, auto c, auto d) {
+            const auto x = j & 1 ? b : a, y = j & 1 ? d : c;
+            return j & 2 ? y : x;
+        };
+        u32x4 kf[4][2], vf[8];
+        float ks = 0.0f, vs = 0.0f;
+        const_f32 *scales = in_constant<const_f32 *>(p.scales + tile.kvh * 2);
+        const size_t scale_row = scale_heads(p.kv_heads) * 2;
+        auto load_k = [&] {
+            const uint32_t block = choose(col >> 2, b.at[0], b.at[1], b.at[2], b.at[3]);
+            const uint8_t *at = p.k + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + (col & 3) * kWidth + 16 * grp;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) kf[t][x] = *(const u32x4 *)(at + 4 * t * kWidth + 64 * x);
+            ks = choose(col >> 2, scales[b.at[0] * scale_row], scales[b.at[1] * scale_row], scales[b.at[2] * scale_row],
+                        scales[b.at[3] * scale_row]);
+        };
+        auto load_v = [&] {
+            const uint32_t block = choose(grp, b.at[0], b.at[1], b.at[2], b.at[3]);
+            const uint8_t *at = p.v + ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + col * kBlock;
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++) vf[dt] = *(const u32x4 *)(at + dt * 16 * kBlock);
+            vs = choose(grp, scales[b.at[0] * scale_row + 1], scales[b.at[1] * scale_row + 1],
+                        scales[b.at[2] * scale_row + 1], scales[b.at[3] * scale_row + 1]);
+        };
+
+        // The first step's K is asked for before q, its V after.
+        const bool early = more_passes && off <= last;
+        if (early) {
+            look(base0 + off);
+            load_k();
+        }
+        const float sl = base2_scale(p.scale);
+        bf16x8 q[4][kParts];
+        load_q<QF32, kParts>(p, live, q_at, grp, q);
+        if (early) load_v();
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o[8];  // O^T: lane's column, d 16 dt + 4 grp + i
+#pragma unroll
+        for (int dt = 0; dt < 8; dt++) o[dt] = f32x4{0, 0, 0, 0};
+
+        for (bool first = true; more_passes; first = false, more_passes = next_keys()) {
+            if (!first && off <= last) {
+                look(base0 + off);
                 load_k();
                 load_v();
             }
-        }
-        uint64_t off = off0;
-        uint32_t left = p.chunk / kRound;  // steps of the chunk
-        for (bool more = off <= span; more;) {
-            const uint32_t base = base0 + (uint32_t)off, lost = b.lost;
-            off += kRound;
-            if (--left == 0) {
-                left = p.chunk / kRound;
-                off += (uint64_t)(p.parts - 1) * p.chunk;
-            }
-            more = off <= span;
-            // (The last step's codes are asked for once more, from the caches: a branch around the
-            // loads would keep two copies of them in registers.)
-            look(more ? base0 + (uint32_t)off : base);
-            f32x4 sc[4];
+            for (bool more = off <= last; more;) {
+                const uint32_t base = base0 + off, lost = b.lost;
+                off += kRound;
+                more = off <= last;
+                // (The last step's codes are asked for once more, from the caches: a branch around the
+                // loads would keep two copies of them in registers.)
+                look(more ? base0 + off : base);
+                f32x4 sc[4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                pin(kf[t][0]);
-                pin(kf[t][1]);
-                sc[t] = f32x4{0, 0, 0, 0};
+                for (int t = 0; t < 4; t++) {
+                    pin(kf[t][0]);
+                    pin(kf[t][1]);
+                    sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const u32x4 w = kf[t][j >> 1];
-                    const bf16x8 kc = codes8(j & 1 ? w.z : w.x, j & 1 ? w.w : w.y, ks);
+                    for (int j = 0; j < 4; j++) {
+                        const u32x4 w = kf[t][j >> 1];
+                        const bf16x8 kc = codes8(j & 1 ? w.z : w.x, j & 1 ? w.w : w.y, ks);
 #pragma unroll
-                    for (uint32_t e = 0; e < kParts; e++) sc[t] = mfma16(kc, q[j][e], sc[t]);
-                }
-            }
-            load_k();
-
-            // A step that meets a window's edge, or a block that is lost.
-            if (base < s.all_lo || base + (kStep - 1) > s.all_hi || lost) {
-                const uint32_t key0 = base + kBlock * grp;
-                const bool gone = lost >> grp & 1;
-                if (lost && p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
-                const uint32_t seen = s.act ? seen_keys(key0, from, pos) : 0u;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float x = gone ? __builtin_nanf("") : sc[t][e];
-                        sc[t][e] = seen >> (4 * t + e) & 1 ? x : -INFINITY;
+                        for (uint32_t e = 0; e < kParts; e++) sc[t] = mfma16(kc, q[j][e], sc[t]);
                     }
-                // Codes outside [lo, hi] may be anything: as zeros they add nothing.
-                uint32_t nan = 0;
-#pragma unroll
-                for (int dt = 0; dt < 8; dt++) {
-                    vf[dt] = u32x4{within4(vf[dt].x, key0, s.lo, s.hi), within4(vf[dt].y, key0 + 4, s.lo, s.hi),
-                                   within4(vf[dt].z, key0 + 8, s.lo, s.hi), within4(vf[dt].w, key0 + 12, s.lo, s.hi)};
-                    nan |= nan_codes(vf[dt].x) | nan_codes(vf[dt].y) | nan_codes(vf[dt].z) | nan_codes(vf[dt].w);
                 }
-                // A NaN code at a key that some columns see and some do not: a weight of 0 times NaN
-                // must not reach the latter. Such codes become 0, and what they reach is marked by a
-                // product of (code is NaN) with (column sees the key).
-                if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+                load_k();
+
+                // A step that meets a window's edge, or a block that is lost.
+                if (base < s.all_lo || base + (kStep - 1) > s.all_hi || lost) {
+                    const uint32_t key0 = base + kBlock * grp;
+                    const bool gone = lost >> grp & 1;
+                    if (lost && p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+                    const uint32_t seen = s.act ? seen_keys(key0, from, pos) : 0u;
 #pragma unroll
-                    for (int dt = 0; dt < 8; dt++) {
-                        uint32_t ones[4];  // e4m3 1.0 (0x38) at each NaN code
+                    for (int t = 0; t < 4; t++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const uint32_t at = nan_codes(vf[dt][e]) >> 7;
-                            ones[e] = at * 0x38u;
-                            vf[dt][e] &= ~(at * 0xffu);
+                            const float x = gone ? __builtin_nanf("") : sc[t][e];
+                            sc[t][e] = seen >> (4 * t + e) & 1 ? x : -INFINITY;
                         }
-                        f32x4 hit = f32x4{0, 0, 0, 0};
+                    // Codes outside [lo, hi] may be anything: as zeros they add nothing.
+                    uint32_t nan = 0;
 #pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            uint32_t sw[4];
+                    for (int dt = 0; dt < 8; dt++) {
+                        vf[dt] = u32x4{within4(vf[dt].x, key0, s.lo, s.hi), within4(vf[dt].y, key0 + 4, s.lo, s.hi),
+                                       within4(vf[dt].z, key0 + 8, s.lo, s.hi), within4(vf[dt].w, key0 + 12, s.lo, s.hi)};
+                        nan |= nan_codes(vf[dt].x) | nan_codes(vf[dt].y) | nan_codes(vf[dt].z) | nan_codes(vf[dt].w);
+                    }
+                    // A NaN code at a key that some columns see and some do not: a weight of 0 times NaN
+                    // must not reach the latter. Such codes become 0, and what they reach is marked by a
+                    // product of (code is NaN) with (column sees the key).
+                    if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+#pragma unroll
+                        for (int dt = 0; dt < 8; dt++) {
+                            uint32_t ones[4];  // e4m3 1.0 (0x38) at each NaN code
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const uint32_t two = seen >> (8 * x + 2 * e);
-                                sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
+                                const uint32_t at = nan_codes(vf[dt][e]) >> 7;
+                                ones[e] = at * 0x38u;
+                                vf[dt][e] &= ~(at * 0xffu);
                             }
-                            hit = mfma16(codes8(ones[2 * x], ones[2 * x + 1], 1.0f),
-                                         as_bf16x8(u32x4{sw[0], sw[1], sw[2], sw[3]}), hit);
-                        }
+                            f32x4 hit = f32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (hit[e] > 0.0f) o[dt][e] = __builtin_nanf("");
+                            for (int x = 0; x < 2; x++) {
+                                uint32_t sw[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t two = seen >> (8 * x + 2 * e);
+                                    sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
+                                }
+                                hit = mfma16(codes8(ones[2 * x], ones[2 * x + 1], 1.0f),
+                                             as_bf16x8(u32x4{sw[0], sw[1], sw[2], sw[3]}), hit);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (hit[e] > 0.0f) o[dt][e] = __builtin_nanf("");
+                        }
                     }
                 }
-            }
-            bf16x8 w[2][kParts];
-            weigh<kParts, 8>(sc, sl, m, l, o, w);
+                bf16x8 w[2][kParts];
+                weigh<kParts, 8>(sc, sl, m, l, o, w);
 #pragma unroll
-            for (int dt = 0; dt < 8; dt++) {
-                pin(vf[dt]);
+                for (int dt = 0; dt < 8; dt++) {
+                    pin(vf[dt]);
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const bf16x8 vc = codes8(x ? vf[dt].z : vf[dt].x, x ? vf[dt].w : vf[dt].y, vs);
+                    for (int x = 0; x < 2; x++) {
+                        const bf16x8 vc = codes8(x ? vf[dt].z : vf[dt].x, x ? vf[dt].w : vf[dt].y, vs);
 #pragma unroll
-                    for (uint32_t e = 0; e < kParts; e++) o[dt] = mfma16(vc, w[x][e], o[dt]);
+                        for (uint32_t e = 0; e < kParts; e++) o[dt] = mfma16(vc, w[x][e], o[dt]);
+                    }
                 }
+                load_v();
             }
-            load_v();
         }
-    }
 
-    // The waves' results joined, a thread four d of a column at a time.
-    if (mine && !worked) {
-        nothing();
-        return;
-    }
-    {
-        float *at = joined + (wave * kCols + col) * kPart;
-        const float sum = rows4_sum(l);
-        if (grp == 0) {
-            at[0] = m;
-            at[1] = live ? sum : __builtin_nanf("");  // a refused column passed unmasked with the others
-        }
-#pragma unroll
-        for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[dt];
-    }
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < kCols * 32; e += 256) {
-        const uint32_t c = e / 32, d = e % 32 * 4;
-        if (!tile.column(p, c, r, h)) continue;
-        float M = -INFINITY;
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) M = fmaxf(M, joined[(w * kCols + c) * kPart]);
-        float L = 0.0f;
-        f32x4 O = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) {
-            const float *at = joined + (w * kCols + c) * kPart;
-            const float f = at[0] == -INFINITY ? (at[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(at[0] - M);
-            L += at[1] * f;
-            O += *(const f32x4 *)(at + 4 + d) * f;
-        }
-        if (mine) {
-            if (d == 0) {
-                mine[c * kPart] = M;
-                mine[c * kPart + 1] = L;
+        // The waves' results joined, a thread four d of a column at a time.
+        {
+            float *at = joined + (wave * kCols + col) * kPart;
+            const float sum = rows4_sum(l);
+            if (grp == 0) {
+                at[0] = m;
+                at[1] = live ? sum : __builtin_nanf("");  // a refused column passed unmasked with the others
             }
-            *(f32x4 *)(mine + c * kPart + 4 + d) = O;
-        } else {
-            store4(p, ((size_t)r * p.heads + h) * 128 + d, O / L);  // 0 / 0 of a refused row: NaN
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[dt];
         }
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < kCols * 32; e += 256) {
+            const uint32_t c = e / 32, d = e % 32 * 4;
+            if (!tile.column(p, c, r, h)) continue;
+            float M = -INFINITY;
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; w++) M = fmaxf(M, joined[(w * kCols + c) * kPart]);
+            float L = 0.0f;
+            f32x4 O = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; w++) {
+                const float *at = joined + (w * kCols + c) * kPart;
+                const float f = at[0] == -INFINITY ? (at[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(at[0] - M);
+                L += at[1] * f;
+                O += *(const f32x4 *)(at + 4 + d) * f;
+            }
+            if (part.partial) {
+                float *at = part.partial + c * kPart;
+                if (d == 0) {
+                    at[0] = M;
+                    at[1] = L;
+                }
+                *(f32x4 *)(at + 4 + d) = O;
+            } else {
+                store4(p, ((size_t)r * p.heads + h) * 128 + d, O / L);  // 0 / 0 of a refused row: NaN
+            }
+        }
+        share.unit += part.b - part.a;
+        share.tile++;
+        if (share.unit >= share.end) return;
+        __syncthreads();  // (the results joined are read, the next tile's may be written)
     }
 }
 
@@ -297,15 +290,20 @@ __global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_
     __shared__ f32x4 so[8][32];
     constexpr uint32_t kBatch = 4;
     const uint32_t gi = blockIdx.x / pieces, lg = threadIdx.x / 32, d = threadIdx.x % 32;
-    const Tile tile = tile_of(p, gi);
+    const Tile tile = {gi / p.kv_heads * p.tile_rows, gi % p.kv_heads};
+    const uint32_t parts = p.shares[gi / p.kv_heads * 2 + 1];
+    if (parts == 1) return;  // (its group has written the rows)
     const uint32_t c = blockIdx.x % pieces * (8 / S) + lg / S, j1 = lg % S;
     uint32_t r, h;
     const bool there = c < cols && tile.column(p, c, r, h);
-    const float *all = p.partials + ((size_t)gi * p.parts * cols + (there ? c : 0)) * kPart;
-    const size_t next = (size_t)cols * kPart;
+    // Part 0 is of a group that a later one goes on from, the others of groups that an earlier one began for.
+    const size_t next = (size_t)p.kv_heads * cols * kPart;  // from a group's results to the next's
+    const float *rest = p.partials + p.shares[gi / p.kv_heads * 2] * next +
+                        ((size_t)tile.kvh * cols + (there ? c : 0)) * kPart;
+    auto result = [&](uint32_t j) { return rest + (j ? j : p.groups) * next; };
     // The maximum: every lane of the lane group looks at parts of its own.
     float M = -INFINITY;
-    for (uint32_t j = j1 + S * d; j < p.parts; j += S * 32) M = fmaxf(M, all[j * next]);
+    for (uint32_t j = j1 + S * d; j < parts; j += S * 32) M = fmaxf(M, *result(j));
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
     if (S > 1) {
@@ -316,12 +314,12 @@ __global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_
     }
     float L = 0.0f;
     f32x4 O = f32x4{0, 0, 0, 0};
-    for (uint32_t j0 = j1; j0 < p.parts; j0 += S * kBatch) {
+    for (uint32_t j0 = j1; j0 < parts; j0 += S * kBatch) {
         float mq[kBatch], lq[kBatch];
         f32x4 oq[kBatch];
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {  // past the end: read, not used
-            const float *at = all + min(j0 + S * j, p.parts - 1) * next;
+            const float *at = result(min(j0 + S * j, parts - 1));
             mq[j] = at[0];
             lq[j] = at[1];
             oq[j] = *(const f32x4 *)(at + 4 + 4 * d);
@@ -329,7 +327,7 @@ __global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {
             // An empty part (max -inf, sum 0) has no O.
-            if (j0 + S * j >= p.parts || (mq[j] == -INFINITY && lq[j] == 0.0f)) continue;
+            if (j0 + S * j >= parts || (mq[j] == -INFINITY && lq[j] == 0.0f)) continue;
             const float f = mq[j] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mq[j] - M);
             L += lq[j] * f;
             O += oq[j] * f;
@@ -351,7 +349,7 @@ __global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_
 
 // How a call runs: `columns` (row, q head) pairs a tile; 16: the kernel above, more: kept8_rows.hip's.
 struct Plan {
-    uint32_t columns, tile_rows, groups, parts, chunk;  // groups: tiles times kv heads
+    uint32_t columns, tile_rows, tiles, groups, most;  // row tiles; groups a kv head; parts a tile at most
 };
 
 Plan plan(const ts_kept8_args *k) {
@@ -364,23 +362,30 @@ Plan plan(const ts_kept8_args *k) {
     // f32 q, in three parts, leaves a wave of the shared kernel 16 columns.
     s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 ? 128 : 256;
     s.tile_rows = std::min(run, s.columns / G);
-    const uint64_t groups = (uint64_t)((a->rows + s.tile_rows - 1) / s.tile_rows) * a->kv_heads;
-    s.groups = (uint32_t)std::min<uint64_t>(groups, 0xffffffffu);
-    // Keys are split into parts until the groups cover the chip about twice over (groups of four waves
-    // of two a SIMD: 512 at a time; of eight: 256), a part no less than a round of a group's waves.
-    const uint32_t least = s.columns == 16 ? kRound : 4 * kStep;
-    const uint64_t want = s.columns <= 64 ? 1024 : 512;
-    const uint64_t span = std::min<uint64_t>((uint64_t)a->max_position + 1, (uint64_t)a->back + s.tile_rows + kBlock);
-    const uint64_t rounds = (span + least - 1) / least;
-    s.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rounds, (want + groups - 1) / groups));
-    s.chunk = (uint32_t)((rounds + s.parts - 1) / s.parts) * least;
-    s.parts = (uint32_t)std::max<uint64_t>(1, (span + s.chunk - 1) / s.chunk);
+    s.tiles = (a->rows + s.tile_rows - 1) / s.tile_rows;
+    s.groups = s.tiles;
+    s.most = 1;
+    // Keys are shared out over as many groups as run at once (two of four waves a CU, one of eight): more would
+    // each cost 8 us before the first step is done, fewer leave CUs idle. Decode rows and drafts (32 sequences
+    // of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's longest span 78, a group a tile 106),
+    // beyond the groups at once too (128 of up to 4096: 128 us, a group a tile 137). Wide tiles, whose
+    // products bound them, only where there are fewer tiles than groups (3 chunks of up to 700 rows: 85 us, a
+    // group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile, the widest first, 112).
+    const uint32_t at_once = (s.columns <= 64 ? 512 : 256) / a->kv_heads, unit = s.columns == 16 ? kRound : kStep;
+    const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
+                                             (uint64_t)a->back + s.tile_rows + kBlock);
+    const uint64_t units = (span + unit - 1) / unit + 1;
+    if (at_once > 1 && s.tiles <= (s.columns <= 64 ? kMaxShared : std::min(kMaxShared, at_once - 1)) && span > unit) {
+        s.groups = (uint32_t)std::min<uint64_t>(at_once, s.tiles * units);
+        s.most = (uint32_t)std::min<uint64_t>(units, s.groups);
+    }
     return s;
 }
 
 size_t partial_bytes(const ts_kept8_args *k, const Plan &s) {
-    return s.parts <= 1 ? 0 : (size_t)s.groups * s.parts * s.columns * kPart * sizeof(float);
+    return s.most <= 1 ? 0 : (size_t)s.groups * 2 * k->rows.kv_heads * s.columns * kPart * sizeof(float);
 }
+size_t share_bytes(const Plan &s) { return s.most <= 1 ? 0 : (size_t)s.tiles * 2 * sizeof(uint32_t); }
 
 int check(const ts_kept8_args *k) {
     TS_REQUIRE(k, "attend_kept8: null args");
@@ -417,7 +422,8 @@ extern "C" size_t tessera_hip_attend_kept8_workspace(const ts_kept8_args *k) {
     if (!k || k->rows.kv_heads == 0 || k->rows.heads == 0 || k->rows.heads % k->rows.kv_heads ||
         k->rows.heads / k->rows.kv_heads > 64 || k->rows.rows == 0)
         return 0;
-    return partial_bytes(k, plan(k));
+    const Plan s = plan(k);
+    return partial_bytes(k, s) + share_bytes(s);
 }
 
 extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
@@ -426,31 +432,34 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
     const ts_rows_args *a = &k->rows;
     if (a->rows == 0) return TS_OK;
     const Plan s = plan(k);
-    TS_REQUIRE((uint64_t)s.groups * s.parts <= 0x7fffffffull / 128, "attend_kept8: %u rows in one launch", a->rows);
-    const size_t need = partial_bytes(k, s);
+    TS_REQUIRE((uint64_t)s.groups * a->kv_heads <= 0x7fffffffull / 128, "attend_kept8: %u rows in one launch", a->rows);
+    const size_t partials = partial_bytes(k, s), need = partials + share_bytes(s);
     if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
         return ts::fail(TS_ERR_WORKSPACE, "attend_kept8: workspace of %zu bytes, 16-byte aligned, needed", need);
     AttendParams p;
     p.q = a->q; p.k = (const uint8_t *)a->k; p.v = (const uint8_t *)a->v; p.scales = k->scales; p.out = a->out;
     p.partials = need ? (float *)a->workspace : nullptr;
+    p.shares = need ? (uint32_t *)((char *)a->workspace + partials) : nullptr;
     p.slots = a->slots; p.positions = a->positions; p.status = a->status;
     p.place.table = a->kept_table; p.place.keys = a->keys; p.place.slot_count = k->slot_count;
     p.place.kept_pages = a->kept_pages; p.place.page_shift = (uint32_t)__builtin_ctz(a->page); p.place.pages = k->pages;
     p.rows = a->rows; p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads;
     p.back = a->back; p.max_position = a->max_position;
-    p.tile_rows = s.tile_rows; p.chunk = s.chunk; p.parts = s.parts;
+    p.tile_rows = s.tile_rows; p.tiles = s.tiles; p.groups = s.groups;
     p.scale = a->scale; p.out_bf16 = a->out_dtype == TS_BF16;
-    const uint32_t groups = s.groups * s.parts;
+    const uint32_t groups = s.groups * a->kv_heads;
     const bool f32 = a->q_dtype == TS_F32;
     if (s.columns > 16)
         rc = ts::kept8_rows_launch(p, s.columns, f32, groups, stream);
     else
         rc = f32 ? launch<true>(p, groups, stream) : launch<false>(p, groups, stream);
-    if (rc || s.parts == 1) return rc;
-    const uint32_t used = s.tile_rows * p.group, S = s.parts <= 2 ? 1 : s.parts <= 8 ? 2 : 8;
+    if (rc || s.most == 1) return rc;
+    const uint32_t used = s.tile_rows * p.group, parts = std::min(s.most, s.groups / s.tiles + 2);
+    const uint32_t S = parts <= 2 ? 1 : parts <= 8 ? 2 : 8;
     const uint32_t pieces = (used * S + 7) / 8;
     const auto join = S == 1 ? join_kept8_kernel<1> : S == 2 ? join_kept8_kernel<2> : join_kept8_kernel<8>;
-    hipLaunchKernelGGL(join, dim3(s.groups * pieces), dim3(256), 0, (hipStream_t)stream, p, s.columns, pieces);
+    hipLaunchKernelGGL(join, dim3(s.tiles * a->kv_heads * pieces), dim3(256), 0, (hipStream_t)stream, p, s.columns,
+                       pieces);
     TS_CHECK_LAUNCH("attend_kept8 join launch");
     return TS_OK;
 }

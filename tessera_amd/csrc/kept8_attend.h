@@ -15,13 +15,16 @@ struct AttendParams {
     const uint8_t *k, *v;
     const float *scales;
     void *out;
-    float *partials;  // [tile][kv head][part][16 NT][kPart], or NULL: one part
+    // Where the keys are split: results of groups for a tile that an earlier group began, then for one that a
+    // later group goes on with, each [groups][kv_heads][columns][kPart]; and each row tile's groups (first,
+    // count). NULL: a group a tile.
+    float *partials;
+    uint32_t *shares;
     const uint32_t *slots, *positions;
     uint32_t *status;
     Place place;
     uint32_t rows, heads, kv_heads, group, back, max_position;
-    uint32_t tile_rows;     // rows a tile
-    uint32_t chunk, parts;  // keys of a part at a time; parts
+    uint32_t tile_rows, tiles, groups;  // rows a tile, row tiles, and groups a kv head
     float scale;
     int out_bf16;
 };
@@ -37,8 +40,6 @@ struct Tile {
         return ri < p.tile_rows && r < p.rows;
     }
 };
-TS_DEV Tile tile_of(const AttendParams &p, uint32_t gi) { return {gi / p.kv_heads * p.tile_rows, gi % p.kv_heads}; }
-
 TS_DEV float rows4_sum(float x) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -116,6 +117,94 @@ TS_DEV uint32_t block_of(const Place &p, uint32_t slot, uint32_t key, bool &lost
     lost = id >= p.pages;
     if (lost) id = 0;
     return (id << (p.page_shift - 4)) + (key & ((1u << p.page_shift) - 1)) / kBlock;
+}
+
+// Shared keys: a row tile is as many units of UNIT keys as its rows see, and the units of all tiles, one
+// behind the other, are dealt to a kv head's groups in equal runs, so that all groups end together however
+// the sequences differ in length. (A run's first and last tile are joined with other groups' by a second
+// kernel.)
+constexpr uint32_t kMaxShared = 256;  // tiles
+struct Share {
+    uint32_t unit, end, each;  // the group's units, and those of a group
+    uint32_t tile;             // the tile of the first
+};
+// Group u's share, false where nothing is left for it. starts[t], in LDS, becomes tile t's first unit. Every
+// wave works it out for itself, lane i for tiles i, i + 64 ..; a tile's units are told from its first and
+// last row (those of one sequence, consecutive, or of two).
+template <uint32_t UNIT>
+TS_DEV bool share_of(const AttendParams &p, uint32_t u, uint32_t lane, uint32_t *starts, Share &s) {
+    if (!p.partials) {
+        s = Share{0, 1, 1, u};
+        return true;
+    }
+    uint32_t end[4], all = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        end[k] = 0xffffffffu;
+        if (64 * k >= p.tiles) break;
+        const uint32_t t = 64 * k + lane;
+        uint32_t n = 0;
+        if (t < p.tiles) {
+            const uint32_t r0 = t * p.tile_rows, r1 = min(r0 + p.tile_rows, p.rows) - 1;
+            const uint32_t most = min(p.max_position, p.place.keys - 1);
+            const uint32_t p0 = min(p.positions[r0], most), p1 = min(p.positions[r1], most);
+            const uint32_t from0 = p0 > p.back ? p0 - p.back : 0, from1 = p1 > p.back ? p1 - p.back : 0;
+            auto units = [](uint32_t lo, uint32_t hi) { return (hi - (lo & ~(kBlock - 1))) / UNIT + 1; };
+            n = p.slots[r0] == p.slots[r1] ? units(min(from0, from1), max(p0, p1)) : units(from0, p0) + units(from1, p1);
+            n = min(n, 1u << 22);
+        }
+        uint32_t upto = n;  // and the lanes' before
+        upto += dpp_u<0x111>(upto);
+        upto += dpp_u<0x112>(upto);
+        upto += dpp_u<0x114>(upto);
+        upto += dpp_u<0x118>(upto);
+        const uint32_t a = __builtin_amdgcn_readlane(upto, 15), b = a + __builtin_amdgcn_readlane(upto, 31),
+                       c = b + __builtin_amdgcn_readlane(upto, 47);
+        upto += all + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
+        all = __builtin_amdgcn_readlane(upto, 63);
+        if (t < p.tiles) {
+            end[k] = upto;
+            starts[t + 1] = upto;
+        }
+    }
+    starts[0] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (each wave reads what it has written itself)
+    s.each = (all + p.groups - 1) / p.groups;
+    s.unit = u * s.each;
+    s.end = min(s.unit + s.each, all);
+    s.tile = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        if (64 * k >= p.tiles) break;
+        s.tile += __builtin_popcountll(__builtin_amdgcn_ballot_w64(end[k] <= s.unit));
+    }
+    return s.unit < all;
+}
+// A group's part of a tile: units [a, b) of its n.
+struct Part {
+    uint32_t a, b, n, row0;
+    float *partial;  // the columns' results, or NULL: out
+};
+TS_DEV Part part_of(const AttendParams &p, uint32_t u, uint32_t lane, uint32_t kvh, uint32_t columns,
+                    const uint32_t *starts, const Share &s) {
+    if (!p.partials) return Part{0, 1, 1, s.tile * p.tile_rows, nullptr};
+    const uint32_t t0 = __builtin_amdgcn_readfirstlane(starts[s.tile]);
+    const uint32_t t1 = __builtin_amdgcn_readfirstlane(starts[s.tile + 1]);
+    Part part = {s.unit - t0, min(s.end, t1) - t0, t1 - t0, s.tile * p.tile_rows, nullptr};
+    if (part.a || part.b < part.n)
+        part.partial = p.partials + ((size_t)((part.a ? 0 : p.groups) + u) * p.kv_heads + kvh) * columns * kPart;
+    if (part.a == 0 && lane == 0) {  // (by every wave and kv head alike)
+        p.shares[2 * s.tile] = u;
+        p.shares[2 * s.tile + 1] = (t1 - 1) / s.each - u + 1;
+    }
+    return part;
+}
+// Unit x of a tile's n, in a pass over np units of one slot: a tile of several slots is taken a slot at a time,
+// each in the same proportion.
+TS_DEV uint32_t pass_unit(uint32_t x, uint32_t n, uint32_t np) {
+    if (x >= n) return np;
+    if (n == np) return x;
+    return min(np, (uint32_t)((float)x * ((float)np * __builtin_amdgcn_rcpf((float)n))));
 }
 
 // Which of a lane's 16 keys key0 .. key0 + 15 lie in [from, pos], a bit each.

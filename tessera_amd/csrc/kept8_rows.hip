@@ -39,285 +39,280 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
     constexpr uint32_t kCols = 16 * QT * W, kParts = QF32 ? 3 : 1, kThreads = 64 * W;
     constexpr uint32_t kEach = 512 / kThreads;  // 16-byte pieces of K (and V) codes a thread and step
     extern __shared__ __attribute__((aligned(16))) char stage[];  // two of kStage
-    __shared__ uint32_t shared_words[W];
+    __shared__ uint32_t shared_words[W], starts[kMaxShared + 1];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = threadIdx.x;
     const uint32_t col = lane & 15, grp = lane >> 4;
 
-    // Widest tiles first.
-    const uint32_t part = blockIdx.x % p.parts, per = p.kv_heads;
-    uint32_t rank = blockIdx.x / p.parts / per;
-    const uint32_t in = blockIdx.x / p.parts % per, tiles = gridDim.x / p.parts / per;
-    if (tiles > 1 && tiles <= kMaxOrder) {
+    // Whole tiles: the widest first. Shared keys: all groups at once (share_of).
+    uint32_t u = blockIdx.x / p.kv_heads;
+    const uint32_t kvh = blockIdx.x % p.kv_heads;
+    if (!p.partials && p.tiles > 1 && p.tiles <= kMaxOrder) {
         uint32_t *cost = (uint32_t *)stage;
-        for (uint32_t i = t; i < tiles; i += kThreads) {
+        for (uint32_t i = t; i < p.tiles; i += kThreads) {
             const uint32_t pos = p.positions[min((i + 1) * p.tile_rows, p.rows) - 1];
             cost[i] = min(min(pos, p.max_position), p.back);
         }
         if (t == 0) shared_words[0] = 0;
         __syncthreads();
-        for (uint32_t i = t; i < tiles; i += kThreads) {
+        for (uint32_t i = t; i < p.tiles; i += kThreads) {
             const uint32_t c = cost[i];
             uint32_t before = 0;
-            for (uint32_t j = 0; j < tiles; j++) {
+            for (uint32_t j = 0; j < p.tiles; j++) {
                 const uint32_t d = cost[j];
                 before += (d > c) | ((d == c) & (j < i));
             }
-            if (before == rank) shared_words[0] = i;
+            if (before == u) shared_words[0] = i;
         }
         __syncthreads();
-        rank = __builtin_amdgcn_readfirstlane(shared_words[0]);
+        u = __builtin_amdgcn_readfirstlane(shared_words[0]);
     }
-    const uint32_t gi = rank * per + in;
-    const Tile tile = tile_of(p, gi);
-
-    uint32_t pos[QT], from[QT], slot[QT];
-    bool live[QT], wait[QT];
-    bf16x8 q[QT][4][kParts];
-    const float sl = base2_scale(p.scale);
-    float m[QT], l[QT];
-    f32x4 o[QT][8];  // O^T: lane's column, d 16 dt + 4 grp + i
-#pragma unroll
-    for (int qt = 0; qt < QT; qt++) {
-        uint32_t r, h;
-        const bool there = tile.column(p, 16 * (QT * wave + qt) + col, r, h);
-        pos[qt] = there ? p.positions[r] : 0;
-        slot[qt] = there ? p.slots[r] : 0;
-        live[qt] = there && pos[qt] <= p.max_position && holds(p.place, slot[qt], pos[qt]);
-        if (there && !live[qt] && p.status && part == 0 && grp == 0)
-            atomicOr(p.status, slot[qt] >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
-        from[qt] = pos[qt] > p.back ? pos[qt] - p.back : 0;
-        load_q<QF32, kParts>(p, live[qt], live[qt] ? ((size_t)r * p.heads + h) * 128 : 0, grp, q[qt]);
-        wait[qt] = live[qt];
-        m[qt] = -INFINITY;
-        l[qt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < 8; dt++) o[qt][dt] = f32x4{0, 0, 0, 0};
-    }
-
-    // LDS byte offsets of the lane's operands: K row (block col / 4, position 4 t + col % 4), chunk
-    // 8 (j / 2) + 2 grp + j % 2; V^T row 16 dt + col, chunk 2 grp + x.
-    uint32_t koff[4], voff[2];
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        koff[j] = (16 * (col >> 2) + (col & 3)) * 256 + (((8 * (j >> 1) + 2 * grp + (j & 1)) ^ col) << 4);
-#pragma unroll
-    for (int x = 0; x < 2; x++) voff[x] = kKBytes + col * 128 + (((2 * grp + x) ^ (col & 7)) << 4);
-
+    Share share;
+    if (!share_of<kStep>(p, u, lane, starts, share)) return;
     for (;;) {
-        // The slot of this pass: the first column's that still waits.
-        uint32_t first = 0xffffffffu;
-#pragma unroll
-        for (int qt = QT - 1; qt >= 0; qt--) {
-            const uint64_t b = __builtin_amdgcn_ballot_w64(wait[qt]);
-            if (b) first = __builtin_amdgcn_readlane(slot[qt], __builtin_ctzll(b));
-        }
-        const uint32_t now = over_waves<W>(shared_words, wave, first, [](uint32_t a, uint32_t b) { return min(a, b); });
-        if (now == 0xffffffffu) break;  // (a served slot is below slot_count)
-        bool act[QT];
-        uint32_t lo = 0xffffffffu, hi = 0, all_lo = 0, all_hi = 0xffffffffu;
+        const Part part = part_of(p, u, lane, kvh, kCols, starts, share);
+        const Tile tile = {part.row0, kvh};
+
+        uint32_t pos[QT], from[QT], slot[QT];
+        bool live[QT], wait[QT];
+        bf16x8 q[QT][4][kParts];
+        const float sl = base2_scale(p.scale);
+        float m[QT], l[QT];
+        f32x4 o[QT][8];  // O^T: lane's column, d 16 dt + 4 grp + i
 #pragma unroll
         for (int qt = 0; qt < QT; qt++) {
-            act[qt] = wait[qt] && slot[qt] == now;
-            wait[qt] = wait[qt] && !act[qt];
-            if (act[qt]) {
-                lo = min(lo, from[qt]);
-                hi = max(hi, pos[qt]);
-                all_lo = max(all_lo, from[qt]);
-                all_hi = min(all_hi, pos[qt]);
-            } else if (live[qt]) {
-                all_lo = 0xffffffffu;
-            }
+            uint32_t r, h;
+            const bool there = tile.column(p, 16 * (QT * wave + qt) + col, r, h);
+            pos[qt] = there ? p.positions[r] : 0;
+            slot[qt] = there ? p.slots[r] : 0;
+            live[qt] = there && pos[qt] <= p.max_position && holds(p.place, slot[qt], pos[qt]);
+            if (there && !live[qt] && p.status && part.a == 0 && grp == 0)
+                atomicOr(p.status, slot[qt] >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
+            from[qt] = pos[qt] > p.back ? pos[qt] - p.back : 0;
+            load_q<QF32, kParts>(p, live[qt], live[qt] ? ((size_t)r * p.heads + h) * 128 : 0, grp, q[qt]);
+            wait[qt] = live[qt];
+            m[qt] = -INFINITY;
+            l[qt] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++) o[qt][dt] = f32x4{0, 0, 0, 0};
         }
-        // The wave's own keys [wlo, whi] (none: wlo above whi), the group's [lo, hi].
-        const uint32_t wlo = row16_least(lo), whi = ~row16_least(~hi);
-        all_lo = ~row16_least(~all_lo);
-        all_hi = row16_least(all_hi);
-        lo = over_waves<W>(shared_words, wave, wlo, [](uint32_t a, uint32_t b) { return min(a, b); });
-        hi = over_waves<W>(shared_words, wave, whi, [](uint32_t a, uint32_t b) { return max(a, b); });
-        const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, span = hi - base0;
 
-        // A thread's pieces: number t + i kThreads of the step's 512, block (t + i kThreads) / 128 (the
-        // wave's own), 16 bytes of K and 16 of V.
-        u32x4 kraw[kEach], vraw[kEach];
-        float ks[kEach], vs[kEach];
-        auto fetch = [&](uint32_t base) {
+        // LDS byte offsets of the lane's operands: K row (block col / 4, position 4 t + col % 4), chunk
+        // 8 (j / 2) + 2 grp + j % 2; V^T row 16 dt + col, chunk 2 grp + x.
+        uint32_t koff[4], voff[2];
 #pragma unroll
-            for (uint32_t i = 0; i < kEach; i++) {
-                const uint32_t j = (wave + i * W) >> 1;
-                bool lost;
-                const uint32_t block = block_of(p.place, now, min(base / kBlock + j, last) * kBlock, lost);
-                const size_t at = ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + ((t + i * kThreads) & 127) * 16;
-                kraw[i] = *(const u32x4 *)(p.k + at);
-                vraw[i] = *(const u32x4 *)(p.v + at);
-                const_f32 *scale = in_constant<const_f32 *>(p.scales) + ((size_t)block * scale_heads(p.kv_heads) + tile.kvh) * 2;
-                ks[i] = scale[0];
-                vs[i] = scale[1];
-                if (lost) {  // a page that the buffers do not hold: NaN keys for the rows that see them
-                    kraw[i] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-                    vraw[i] = u32x4{0, 0, 0, 0};
-                    if (p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+        for (int j = 0; j < 4; j++)
+            koff[j] = (16 * (col >> 2) + (col & 3)) * 256 + (((8 * (j >> 1) + 2 * grp + (j & 1)) ^ col) << 4);
+#pragma unroll
+        for (int x = 0; x < 2; x++) voff[x] = kKBytes + col * 128 + (((2 * grp + x) ^ (col & 7)) << 4);
+
+        for (;;) {
+            // The slot of this pass: the first column's that still waits.
+            uint32_t first = 0xffffffffu;
+#pragma unroll
+            for (int qt = QT - 1; qt >= 0; qt--) {
+                const uint64_t b = __builtin_amdgcn_ballot_w64(wait[qt]);
+                if (b) first = __builtin_amdgcn_readlane(slot[qt], __builtin_ctzll(b));
+            }
+            const uint32_t now = over_waves<W>(shared_words, wave, first, [](uint32_t a, uint32_t b) { return min(a, b); });
+            if (now == 0xffffffffu) break;  // (a served slot is below slot_count)
+            bool act[QT];
+            uint32_t lo = 0xffffffffu, hi = 0, all_lo = 0, all_hi = 0xffffffffu;
+#pragma unroll
+            for (int qt = 0; qt < QT; qt++) {
+                act[qt] = wait[qt] && slot[qt] == now;
+                wait[qt] = wait[qt] && !act[qt];
+                if (act[qt]) {
+                    lo = min(lo, from[qt]);
+                    hi = max(hi, pos[qt]);
+                    all_lo = max(all_lo, from[qt]);
+                    all_hi = min(all_hi, pos[qt]);
+                } else if (live[qt]) {
+                    all_lo = 0xffffffffu;
                 }
             }
-        };
-        auto stash = [&](uint32_t buffer, uint32_t base) {
-            char *to = stage + buffer * kStage;
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; i++) {
-                const uint32_t j = (wave + i * W) >> 1, c = (t + i * kThreads) & 127;
-                const uint32_t key = c >> 3, chunk = 2 * (c & 7), swap = (key & 3) | (j << 2);
-                char *row = to + (16 * j + key) * 256;
-                *(bf16x8 *)(row + ((chunk ^ swap) << 4)) = codes8(kraw[i].x, kraw[i].y, ks[i]);
-                *(bf16x8 *)(row + (((chunk + 1) ^ swap) << 4)) = codes8(kraw[i].z, kraw[i].w, ks[i]);
-                u32x4 v = vraw[i];
-                if (base < lo || base + (kStep - 1) > hi) {  // codes outside [lo, hi] may be anything
-                    const uint32_t key0 = base + kBlock * j;
-                    v = u32x4{within4(v.x, key0, lo, hi), within4(v.y, key0 + 4, lo, hi), within4(v.z, key0 + 8, lo, hi),
-                              within4(v.w, key0 + 12, lo, hi)};
-                }
-                row = to + kKBytes + c * 128;
-                *(bf16x8 *)(row + (((2 * j) ^ (c & 7)) << 4)) = codes8(v.x, v.y, vs[i]);
-                *(bf16x8 *)(row + (((2 * j + 1) ^ (c & 7)) << 4)) = codes8(v.z, v.w, vs[i]);
-            }
-        };
+            // The wave's own keys [wlo, whi] (none: wlo above whi), the group's [lo, hi].
+            const uint32_t wlo = row16_least(lo), whi = ~row16_least(~hi);
+            all_lo = ~row16_least(~all_lo);
+            all_hi = row16_least(all_hi);
+            lo = over_waves<W>(shared_words, wave, wlo, [](uint32_t a, uint32_t b) { return min(a, b); });
+            hi = over_waves<W>(shared_words, wave, whi, [](uint32_t a, uint32_t b) { return max(a, b); });
+            const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, np = (hi - base0) / kStep + 1;
+            const uint32_t unit0 = pass_unit(part.a, part.n, np), unit1 = pass_unit(part.b, part.n, np);
+            if (unit0 >= unit1) continue;
 
-        // Keys from base0 + off on are the next step: a part takes chunks in turn.
-        uint64_t off = (uint64_t)part * p.chunk;
-        if (off > span) continue;
-        const uint32_t steps = p.chunk / kStep;
-        uint32_t left = steps;
-        auto after = [&](uint64_t at) {  // (moves `left` too)
-            at += kStep;
-            if (--left == 0) {
-                left = steps;
-                at += (uint64_t)(p.parts - 1) * p.chunk;
-            }
-            return at;
-        };
-        uint32_t base = base0 + (uint32_t)off;
-        fetch(base);
-        stash(0, base);
-        off = after(off);
-        bool more = off <= span;
-        uint32_t next = more ? base0 + (uint32_t)off : base;
-        fetch(next);
-        for (uint32_t buffer = 0;; buffer ^= 1) {
-            lds_barrier();  // this step's codes are in; the other buffer's readers are done
-            const bool go = more;
-            const uint32_t here = base;
-            if (go) {
-                stash(buffer ^ 1, next);
-                base = next;
-                off = after(off);
-                more = off <= span;
-                next = more ? base0 + (uint32_t)off : base;
-                fetch(next);
-            }
-            if (here <= whi && here + (kStep - 1) >= wlo) {
-                const char *kb = stage + buffer * kStage, *vb = kb;
-                f32x4 s[QT][4];
+            // A thread's pieces: number t + i kThreads of the step's 512, block (t + i kThreads) / 128 (the
+            // wave's own), 16 bytes of K and 16 of V.
+            u32x4 kraw[kEach], vraw[kEach];
+            float ks[kEach], vs[kEach];
+            auto fetch = [&](uint32_t base) {
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-#pragma unroll
-                    for (int qt = 0; qt < QT; qt++) s[qt][x] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const bf16x8 kc = *(const bf16x8 *)(kb + koff[j] + x * 1024);
-#pragma unroll
-                        for (int qt = 0; qt < QT; qt++)
-#pragma unroll
-                            for (uint32_t e = 0; e < kParts; e++) s[qt][x] = mfma16(kc, q[qt][j][e], s[qt][x]);
+                for (uint32_t i = 0; i < kEach; i++) {
+                    const uint32_t j = (wave + i * W) >> 1;
+                    bool lost;
+                    const uint32_t block = block_of(p.place, now, min(base / kBlock + j, last) * kBlock, lost);
+                    const size_t at =
+                        ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + ((t + i * kThreads) & 127) * 16;
+                    kraw[i] = *(const u32x4 *)(p.k + at);
+                    vraw[i] = *(const u32x4 *)(p.v + at);
+                    const_f32 *scale = in_constant<const_f32 *>(p.scales) +
+                                       ((size_t)block * scale_heads(p.kv_heads) + tile.kvh) * 2;
+                    ks[i] = scale[0];
+                    vs[i] = scale[1];
+                    if (lost) {  // a page that the buffers do not hold: NaN keys for the rows that see them
+                        kraw[i] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+                        vraw[i] = u32x4{0, 0, 0, 0};
+                        if (p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
                     }
                 }
-                const bool edge = here < all_lo || here + (kStep - 1) > all_hi;
-                uint32_t seen[QT];
-                if (edge) {
+            };
+            auto stash = [&](uint32_t buffer, uint32_t base) {
+                char *to = stage + buffer * kStage;
 #pragma unroll
-                    for (int qt = 0; qt < QT; qt++) {
-                        seen[qt] = act[qt] ? seen_keys(here + kBlock * grp, from[qt], pos[qt]) : 0u;
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                s[qt][x][e] = seen[qt] >> (4 * x + e) & 1 ? s[qt][x][e] : -INFINITY;
+                for (uint32_t i = 0; i < kEach; i++) {
+                    const uint32_t j = (wave + i * W) >> 1, c = (t + i * kThreads) & 127;
+                    const uint32_t key = c >> 3, chunk = 2 * (c & 7), swap = (key & 3) | (j << 2);
+                    char *row = to + (16 * j + key) * 256;
+                    *(bf16x8 *)(row + ((chunk ^ swap) << 4)) = codes8(kraw[i].x, kraw[i].y, ks[i]);
+                    *(bf16x8 *)(row + (((chunk + 1) ^ swap) << 4)) = codes8(kraw[i].z, kraw[i].w, ks[i]);
+                    u32x4 v = vraw[i];
+                    if (base < lo || base + (kStep - 1) > hi) {  // codes outside [lo, hi] may be anything
+                        const uint32_t key0 = base + kBlock * j;
+                        v = u32x4{within4(v.x, key0, lo, hi), within4(v.y, key0 + 4, lo, hi), within4(v.z, key0 + 8, lo, hi),
+                                  within4(v.w, key0 + 12, lo, hi)};
                     }
+                    row = to + kKBytes + c * 128;
+                    *(bf16x8 *)(row + (((2 * j) ^ (c & 7)) << 4)) = codes8(v.x, v.y, vs[i]);
+                    *(bf16x8 *)(row + (((2 * j + 1) ^ (c & 7)) << 4)) = codes8(v.z, v.w, vs[i]);
                 }
-                bf16x8 w[QT][2][kParts];
+            };
+
+            uint32_t base = base0 + unit0 * kStep;
+            const uint32_t end = base0 + (unit1 - 1) * kStep;  // the last step's
+            fetch(base);
+            stash(0, base);
+            uint32_t next = min(base + kStep, end);
+            fetch(next);
+            for (uint32_t buffer = 0;; buffer ^= 1) {
+                lds_barrier();  // this step's codes are in; the other buffer's readers are done
+                const bool go = base < end;
+                const uint32_t here = base;
+                if (go) {
+                    stash(buffer ^ 1, next);
+                    base = next;
+                    next = min(base + kStep, end);
+                    fetch(next);
+                }
+                if (here <= whi && here + (kStep - 1) >= wlo) {
+                    const char *kb = stage + buffer * kStage, *vb = kb;
+                    f32x4 s[QT][4];
 #pragma unroll
-                for (int qt = 0; qt < QT; qt++) weigh<kParts, 8>(s[qt], sl, m[qt], l[qt], o[qt], w[qt]);
+                    for (int x = 0; x < 4; x++) {
 #pragma unroll
-                for (int dt = 0; dt < 8; dt++) {
-                    bf16x8 vc[2];
+                        for (int qt = 0; qt < QT; qt++) s[qt][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int x = 0; x < 2; x++) vc[x] = *(const bf16x8 *)(vb + voff[x] + dt * 2048);
-                    if (edge) {
-                        // A NaN at a key that some columns see and some do not (kept8.hip): zero in the
-                        // product, marked where it is seen.
-                        uint32_t any = 0;
-                        u32x4 ones[2];
+                        for (int j = 0; j < 4; j++) {
+                            const bf16x8 kc = *(const bf16x8 *)(kb + koff[j] + x * 1024);
 #pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            u32x4 v = __builtin_bit_cast(u32x4, vc[x]);
+                            for (int qt = 0; qt < QT; qt++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const uint32_t low = (v[e] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u;
-                                const uint32_t high = (v[e] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
-                                ones[x][e] = (low | high) & 0x3f803f80u;
-                                v[e] &= ~(low | high);
-                                any |= low | high;
-                            }
-                            vc[x] = as_bf16x8(v);
+                                for (uint32_t e = 0; e < kParts; e++) s[qt][x] = mfma16(kc, q[qt][j][e], s[qt][x]);
                         }
-                        if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
+                    }
+                    const bool edge = here < all_lo || here + (kStep - 1) > all_hi;
+                    uint32_t seen[QT];
+                    if (edge) {
 #pragma unroll
-                            for (int qt = 0; qt < QT; qt++) {
-                                f32x4 hit = f32x4{0, 0, 0, 0};
+                        for (int qt = 0; qt < QT; qt++) {
+                            seen[qt] = act[qt] ? seen_keys(here + kBlock * grp, from[qt], pos[qt]) : 0u;
 #pragma unroll
-                                for (int x = 0; x < 2; x++) {
-                                    u32x4 sw;
-#pragma unroll
-                                    for (int e = 0; e < 4; e++) {
-                                        const uint32_t two = seen[qt] >> (8 * x + 2 * e);
-                                        sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
-                                    }
-                                    hit = mfma16(as_bf16x8(ones[x]), as_bf16x8(sw), hit);
-                                }
+                            for (int x = 0; x < 4; x++)
 #pragma unroll
                                 for (int e = 0; e < 4; e++)
-                                    if (hit[e] > 0.0f) o[qt][dt][e] = __builtin_nanf("");
-                            }
+                                    s[qt][x][e] = seen[qt] >> (4 * x + e) & 1 ? s[qt][x][e] : -INFINITY;
                         }
                     }
+                    bf16x8 w[QT][2][kParts];
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
+                    for (int qt = 0; qt < QT; qt++) weigh<kParts, 8>(s[qt], sl, m[qt], l[qt], o[qt], w[qt]);
 #pragma unroll
-                        for (int qt = 0; qt < QT; qt++)
+                    for (int dt = 0; dt < 8; dt++) {
+                        bf16x8 vc[2];
 #pragma unroll
-                            for (uint32_t e = 0; e < kParts; e++) o[qt][dt] = mfma16(vc[x], w[qt][x][e], o[qt][dt]);
+                        for (int x = 0; x < 2; x++) vc[x] = *(const bf16x8 *)(vb + voff[x] + dt * 2048);
+                        if (edge) {
+                            // A NaN at a key that some columns see and some do not (kept8.hip): zero in the
+                            // product, marked where it is seen.
+                            uint32_t any = 0;
+                            u32x4 ones[2];
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                u32x4 v = __builtin_bit_cast(u32x4, vc[x]);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t low = (v[e] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u;
+                                    const uint32_t high = (v[e] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
+                                    ones[x][e] = (low | high) & 0x3f803f80u;
+                                    v[e] &= ~(low | high);
+                                    any |= low | high;
+                                }
+                                vc[x] = as_bf16x8(v);
+                            }
+                            if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
+#pragma unroll
+                                for (int qt = 0; qt < QT; qt++) {
+                                    f32x4 hit = f32x4{0, 0, 0, 0};
+#pragma unroll
+                                    for (int x = 0; x < 2; x++) {
+                                        u32x4 sw;
+#pragma unroll
+                                        for (int e = 0; e < 4; e++) {
+                                            const uint32_t two = seen[qt] >> (8 * x + 2 * e);
+                                            sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
+                                        }
+                                        hit = mfma16(as_bf16x8(ones[x]), as_bf16x8(sw), hit);
+                                    }
+#pragma unroll
+                                    for (int e = 0; e < 4; e++)
+                                        if (hit[e] > 0.0f) o[qt][dt][e] = __builtin_nanf("");
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+#pragma unroll
+                            for (int qt = 0; qt < QT; qt++)
+#pragma unroll
+                                for (uint32_t e = 0; e < kParts; e++) o[qt][dt] = mfma16(vc[x], w[qt][x][e], o[qt][dt]);
+                    }
                 }
+                if (!go) break;
             }
-            if (!go) break;
         }
-    }
 
-    // A column is one wave's: O / l, or the part's result. Refused rows are NaN.
+        // A column is one wave's: O / l, or the part's result. Refused rows are NaN.
 #pragma unroll
-    for (int qt = 0; qt < QT; qt++) {
-        const uint32_t c = 16 * (QT * wave + qt) + col;
-        uint32_t r, h;
-        const float sum = live[qt] ? rows4_sum(l[qt]) : __builtin_nanf("");
-        if (!tile.column(p, c, r, h)) continue;
-        if (p.partials) {
-            float *at = p.partials + (((size_t)gi * p.parts + part) * kCols + c) * kPart;
-            if (grp == 0) {
-                at[0] = m[qt];
-                at[1] = sum;
+        for (int qt = 0; qt < QT; qt++) {
+            const uint32_t c = 16 * (QT * wave + qt) + col;
+            uint32_t r, h;
+            const float sum = live[qt] ? rows4_sum(l[qt]) : __builtin_nanf("");
+            if (!tile.column(p, c, r, h)) continue;
+            if (part.partial) {
+                float *at = part.partial + c * kPart;
+                if (grp == 0) {
+                    at[0] = m[qt];
+                    at[1] = sum;
+                }
+#pragma unroll
+                for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[qt][dt];
+            } else {
+#pragma unroll
+                for (int dt = 0; dt < 8; dt++)
+                    store4(p, ((size_t)r * p.heads + h) * 128 + 16 * dt + 4 * grp, o[qt][dt] / sum);
             }
-#pragma unroll
-            for (int dt = 0; dt < 8; dt++) *(f32x4 *)(at + 4 + 16 * dt + 4 * grp) = o[qt][dt];
-        } else {
-#pragma unroll
-            for (int dt = 0; dt < 8; dt++) store4(p, ((size_t)r * p.heads + h) * 128 + 16 * dt + 4 * grp, o[qt][dt] / sum);
         }
+        share.unit += part.b - part.a;
+        share.tile++;
+        if (share.unit >= share.end) return;
     }
 }
 
@@ -326,7 +321,8 @@ int launch(const AttendParams &p, uint32_t groups, void *stream) {
     static const hipError_t attr = hipFuncSetAttribute((const void *)attend_kept8_rows_kernel<QT, W, QF32>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kStage);
     if (attr != hipSuccess) return ts::hip_status(attr, "attend_kept8: shared memory attribute");
-    hipLaunchKernelGGL((attend_kept8_rows_kernel<QT, W, QF32>), dim3(groups), dim3(64 * W), 2 * kStage, (hipStream_t)stream, p);
+    hipLaunchKernelGGL((attend_kept8_rows_kernel<QT, W, QF32>), dim3(groups), dim3(64 * W), 2 * kStage,
+                       (hipStream_t)stream, p);
     TS_CHECK_LAUNCH("attend_kept8 rows launch");
     return TS_OK;
 }
