@@ -107,16 +107,18 @@ TS_DEV T in_constant(const void *p) { return (T)(uintptr_t)p; }
 // where the compiler would widen all of a step's and spill.
 TS_DEV void pin(u32x4 &v) { asm volatile("" : "+v"(v)); }
 
-// The pages of a step's blocks: block j's place in the kept blocks; one whose page is not held has its
-// bit in `lost` and stands at page 0's.
-TS_DEV uint32_t block_of(const Place &p, uint32_t slot, uint32_t key, bool &lost) {
+// The kept block of key `key` of a slot, whose page is `id`; a page that is not held is lost, and page 0
+// stands in its place.
+TS_DEV uint32_t block_in(const Place &p, uint32_t slot, uint32_t id, uint32_t key, bool &lost) {
     lost = false;
     if (!p.table) return slot * (p.keys / kBlock) + key / kBlock;
-    const_u32 *t = in_constant<const_u32 *>(p.table + (size_t)slot * p.kept_pages);
-    uint32_t id = t[key >> p.page_shift];
     lost = id >= p.pages;
     if (lost) id = 0;
     return (id << (p.page_shift - 4)) + (key & ((1u << p.page_shift) - 1)) / kBlock;
+}
+TS_DEV uint32_t block_of(const Place &p, uint32_t slot, uint32_t key, bool &lost) {
+    const_u32 *t = in_constant<const_u32 *>(p.table + (size_t)slot * p.kept_pages);
+    return block_in(p, slot, p.table ? t[key >> p.page_shift] : 0, key, lost);
 }
 
 // Shared keys: a row tile is as many units of UNIT keys as its rows see, and the units of all tiles, one

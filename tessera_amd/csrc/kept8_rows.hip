@@ -43,6 +43,11 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = threadIdx.x;
     const uint32_t col = lane & 15, grp = lane >> 4;
 
+    // What the steps read from uniform addresses goes through vector loads: a scalar load on its way would make
+    // every wait for LDS wait for it too.
+    uint32_t zero = 0;
+    asm volatile("" : "+v"(zero));
+
     // Whole tiles: the widest first. Shared keys: all groups at once (share_of).
     uint32_t u = blockIdx.x / p.kv_heads;
     const uint32_t kvh = blockIdx.x % p.kv_heads;
@@ -139,41 +144,61 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
             const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, np = (hi - base0) / kStep + 1;
             const uint32_t unit0 = pass_unit(part.a, part.n, np), unit1 = pass_unit(part.b, part.n, np);
             if (unit0 >= unit1) continue;
+            uint32_t base = base0 + unit0 * kStep;
+            const uint32_t end = base0 + (unit1 - 1) * kStep;  // the last step's
 
             // A thread's pieces: number t + i kThreads of the step's 512, block (t + i kThreads) / 128 (the
-            // wave's own), 16 bytes of K and 16 of V.
+            // wave's own), 16 bytes of K and 16 of V. The page's id is asked for a step before the codes.
             u32x4 kraw[kEach], vraw[kEach];
-            float ks[kEach], vs[kEach];
+            ts_f32x2 scale[kEach];
+            uint32_t id[kEach], gone;  // gone: bit i: piece i's page is not held
+            auto key_of = [&](uint32_t base, uint32_t i) {
+                return min(base / kBlock + ((wave + i * W) >> 1), last) * kBlock;
+            };
+            const uint32_t *pages = p.place.table + (size_t)now * p.place.kept_pages + zero;
+            auto look = [&](uint32_t base) {
+#pragma unroll
+                for (uint32_t i = 0; i < kEach; i++)
+                    id[i] = p.place.table ? pages[key_of(base, i) >> p.place.page_shift] : 0;
+            };
             auto fetch = [&](uint32_t base) {
+                uint32_t block[kEach];
+                gone = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < kEach; i++) {
-                    const uint32_t j = (wave + i * W) >> 1;
                     bool lost;
-                    const uint32_t block = block_of(p.place, now, min(base / kBlock + j, last) * kBlock, lost);
+                    block[i] = block_in(p.place, now, __builtin_amdgcn_readfirstlane(id[i]), key_of(base, i), lost);
+                    gone |= lost ? 1u << i : 0u;
+                }
+                look(min(base + kStep, end));
+#pragma unroll
+                for (uint32_t i = 0; i < kEach; i++) {
+                    const size_t at_scale = ((size_t)block[i] * scale_heads(p.kv_heads) + kvh) * 2;
+                    scale[i] = *(const ts_f32x2 *)(p.scales + at_scale + zero);
                     const size_t at =
-                        ((size_t)block * p.kv_heads + tile.kvh) * kBlockBytes + ((t + i * kThreads) & 127) * 16;
+                        ((size_t)block[i] * p.kv_heads + kvh) * kBlockBytes + ((t + i * kThreads) & 127) * 16;
                     kraw[i] = *(const u32x4 *)(p.k + at);
                     vraw[i] = *(const u32x4 *)(p.v + at);
-                    const_f32 *scale = in_constant<const_f32 *>(p.scales) +
-                                       ((size_t)block * scale_heads(p.kv_heads) + tile.kvh) * 2;
-                    ks[i] = scale[0];
-                    vs[i] = scale[1];
-                    if (lost) {  // a page that the buffers do not hold: NaN keys for the rows that see them
-                        kraw[i] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-                        vraw[i] = u32x4{0, 0, 0, 0};
-                        if (p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
-                    }
                 }
             };
             auto stash = [&](uint32_t buffer, uint32_t base) {
+                if (gone) {  // NaN keys for the rows that see them (put in here: at the loads it would wait for them)
+#pragma unroll
+                    for (uint32_t i = 0; i < kEach; i++)
+                        if (gone >> i & 1) {
+                            kraw[i] = u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+                            vraw[i] = u32x4{0, 0, 0, 0};
+                        }
+                    if (p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+                }
                 char *to = stage + buffer * kStage;
 #pragma unroll
                 for (uint32_t i = 0; i < kEach; i++) {
                     const uint32_t j = (wave + i * W) >> 1, c = (t + i * kThreads) & 127;
                     const uint32_t key = c >> 3, chunk = 2 * (c & 7), swap = (key & 3) | (j << 2);
                     char *row = to + (16 * j + key) * 256;
-                    *(bf16x8 *)(row + ((chunk ^ swap) << 4)) = codes8(kraw[i].x, kraw[i].y, ks[i]);
-                    *(bf16x8 *)(row + (((chunk + 1) ^ swap) << 4)) = codes8(kraw[i].z, kraw[i].w, ks[i]);
+                    *(bf16x8 *)(row + ((chunk ^ swap) << 4)) = codes8(kraw[i].x, kraw[i].y, scale[i].x);
+                    *(bf16x8 *)(row + (((chunk + 1) ^ swap) << 4)) = codes8(kraw[i].z, kraw[i].w, scale[i].x);
                     u32x4 v = vraw[i];
                     if (base < lo || base + (kStep - 1) > hi) {  // codes outside [lo, hi] may be anything
                         const uint32_t key0 = base + kBlock * j;
@@ -181,13 +206,12 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                                   within4(v.w, key0 + 12, lo, hi)};
                     }
                     row = to + kKBytes + c * 128;
-                    *(bf16x8 *)(row + (((2 * j) ^ (c & 7)) << 4)) = codes8(v.x, v.y, vs[i]);
-                    *(bf16x8 *)(row + (((2 * j + 1) ^ (c & 7)) << 4)) = codes8(v.z, v.w, vs[i]);
+                    *(bf16x8 *)(row + (((2 * j) ^ (c & 7)) << 4)) = codes8(v.x, v.y, scale[i].y);
+                    *(bf16x8 *)(row + (((2 * j + 1) ^ (c & 7)) << 4)) = codes8(v.z, v.w, scale[i].y);
                 }
             };
 
-            uint32_t base = base0 + unit0 * kStep;
-            const uint32_t end = base0 + (unit1 - 1) * kStep;  // the last step's
+            look(base);
             fetch(base);
             stash(0, base);
             uint32_t next = min(base + kStep, end);
