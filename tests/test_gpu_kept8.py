@@ -48,12 +48,13 @@ def call(q, k, v, scales, slots, positions, where, page, **kw):
 
 
 def bound(spread, size, f32):
-    """A score's error: f32 q enters as two bf16 parts, |q| 2^-17 off at most, and 128 products are summed
-    at 2^-21 each accumulating step (4 a part): spread (2^-17 + 8 2^-21). A weight is then off by twice
-    that (its own and the sum's), by 2^-22 of the exponential and by its rounding (two parts 2^-17, one
-    2^-9, half a step of bf16 2^-8); the output by that times the largest |v|, plus its own rounding."""
-    score = spread * ((2.0 ** -17 if f32 else 0) + 8 * 2.0 ** -21)
-    return (2 * score + 2.0 ** -20 + (2.0 ** -17 if f32 else 2.0 ** -8)) * size + (0 if f32 else 2.0 ** -8 * size)
+    """A score's error: f32 q enters as three bf16 parts, |q| 2^-24 off at most, and 128 products are summed
+    at 2^-21 each accumulating step (4 a part): spread (2^-24 + 12 2^-21), of bf16 q spread 4 2^-21. A weight
+    is then off by twice that (its own and the sum's), by 2^-20 of the exponential and the sums and by its
+    rounding (three parts 2^-24, one 2^-9, half a step of bf16 2^-8); the output by that times the largest
+    |v|, plus its own rounding."""
+    score = spread * (2.0 ** -24 + 12 * 2.0 ** -21 if f32 else 4 * 2.0 ** -21)
+    return (2 * score + 2.0 ** -20 + (2.0 ** -24 if f32 else 2.0 ** -8)) * size + (0 if f32 else 2.0 ** -8 * size)
 
 
 def check(out, want, spread, size, f32):
