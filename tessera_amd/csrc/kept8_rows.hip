@@ -34,6 +34,13 @@ TS_DEV uint32_t over_waves(uint32_t *mine, uint32_t wave, uint32_t v, F f) {
     return __builtin_amdgcn_readfirstlane(r);
 }
 
+// The XOR of a V^T row's eight chunks: distinct for the rows of one parity among 16, which share half the
+// banks, and so that lanes 0-3, 12-15 of one 16 and 4-11 of the next, which LDS serves together, meet no two either.
+TS_DEV uint32_t v_swap(uint32_t d) {
+    const uint32_t i = d >> 1;
+    return (i & 1) | (i >> 1 & 2) | ((i ^ i << 1) & 4);
+}
+
 template <int QT, int W, bool QF32>
 __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendParams p) {
     constexpr uint32_t kCols = 16 * QT * W, kParts = QF32 ? 3 : 1, kThreads = 64 * W;
@@ -108,7 +115,7 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
         for (int j = 0; j < 4; j++)
             koff[j] = (16 * (col >> 2) + (col & 3)) * 256 + (((8 * (j >> 1) + 2 * grp + (j & 1)) ^ col) << 4);
 #pragma unroll
-        for (int x = 0; x < 2; x++) voff[x] = kKBytes + col * 128 + (((2 * grp + x) ^ (col & 7)) << 4);
+        for (int x = 0; x < 2; x++) voff[x] = kKBytes + col * 128 + (((2 * grp + x) ^ v_swap(col)) << 4);
 
         for (;;) {
             // The slot of this pass: the first column's that still waits.
@@ -206,8 +213,8 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                                   within4(v.w, key0 + 12, lo, hi)};
                     }
                     row = to + kKBytes + c * 128;
-                    *(bf16x8 *)(row + (((2 * j) ^ (c & 7)) << 4)) = codes8(v.x, v.y, scale[i].y);
-                    *(bf16x8 *)(row + (((2 * j + 1) ^ (c & 7)) << 4)) = codes8(v.z, v.w, scale[i].y);
+                    *(bf16x8 *)(row + (((2 * j) ^ v_swap(c)) << 4)) = codes8(v.x, v.y, scale[i].y);
+                    *(bf16x8 *)(row + (((2 * j + 1) ^ v_swap(c)) << 4)) = codes8(v.z, v.w, scale[i].y);
                 }
             };
 
