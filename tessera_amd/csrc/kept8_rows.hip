@@ -47,6 +47,10 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
     constexpr uint32_t kEach = 512 / kThreads;  // 16-byte pieces of K (and V) codes a thread and step
     extern __shared__ __attribute__((aligned(16))) char stage[];  // two of kStage
     __shared__ uint32_t shared_words[W], starts[kMaxShared + 1];
+    // Per buffer and d: which of the step's 64 keys hold a NaN in V; and whether there has been any.
+    __shared__ uint64_t nan_keys[2][128];
+    __shared__ uint32_t nan_met;
+    if (threadIdx.x == 0) nan_met = 0;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = threadIdx.x;
     const uint32_t col = lane & 15, grp = lane >> 4;
 
@@ -212,6 +216,19 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                         v = u32x4{within4(v.x, key0, lo, hi), within4(v.y, key0 + 4, lo, hi), within4(v.z, key0 + 8, lo, hi),
                                   within4(v.w, key0 + 12, lo, hi)};
                     }
+                    // A NaN is 0 in the products, and reaches what sees it by itself (below): a weight of 0 times
+                    // NaN must not reach the columns that do not.
+                    const u32x4 nan = {nan_codes(v.x), nan_codes(v.y), nan_codes(v.z), nan_codes(v.w)};
+                    uint32_t keys = 0;
+                    if (__builtin_amdgcn_ballot_w64((nan.x | nan.y | nan.z | nan.w) != 0) != 0) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            v[e] &= ~((nan[e] >> 7) * 0xffu);
+                            keys |= ((nan[e] >> 7) * 0x10204080u >> 28 & 0xfu) << (4 * e);
+                        }
+                        if (lane == 0) nan_met = 1;
+                    }
+                    ((uint16_t *)nan_keys[buffer])[4 * c + j] = keys;
                     row = to + kKBytes + c * 128;
                     *(bf16x8 *)(row + (((2 * j) ^ v_swap(c)) << 4)) = codes8(v.x, v.y, scale[i].y);
                     *(bf16x8 *)(row + (((2 * j + 1) ^ v_swap(c)) << 4)) = codes8(v.z, v.w, scale[i].y);
@@ -235,6 +252,7 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                 }
                 if (here <= whi && here + (kStep - 1) >= wlo) {
                     const char *kb = stage + buffer * kStage, *vb = kb;
+                    const uint32_t nan = __builtin_amdgcn_readfirstlane(nan_met);
                     f32x4 s[QT][4];
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
@@ -249,17 +267,15 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                                 for (uint32_t e = 0; e < kParts; e++) s[qt][x] = mfma16(kc, q[qt][j][e], s[qt][x]);
                         }
                     }
-                    const bool edge = here < all_lo || here + (kStep - 1) > all_hi;
-                    uint32_t seen[QT];
-                    if (edge) {
+                    if (here < all_lo || here + (kStep - 1) > all_hi) {
 #pragma unroll
                         for (int qt = 0; qt < QT; qt++) {
-                            seen[qt] = act[qt] ? seen_keys(here + kBlock * grp, from[qt], pos[qt]) : 0u;
+                            const uint32_t seen = act[qt] ? seen_keys(here + kBlock * grp, from[qt], pos[qt]) : 0u;
 #pragma unroll
                             for (int x = 0; x < 4; x++)
 #pragma unroll
                                 for (int e = 0; e < 4; e++)
-                                    s[qt][x][e] = seen[qt] >> (4 * x + e) & 1 ? s[qt][x][e] : -INFINITY;
+                                    s[qt][x][e] = seen >> (4 * x + e) & 1 ? s[qt][x][e] : -INFINITY;
                         }
                     }
                     bf16x8 w[QT][2][kParts];
@@ -270,50 +286,26 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                         bf16x8 vc[2];
 #pragma unroll
                         for (int x = 0; x < 2; x++) vc[x] = *(const bf16x8 *)(vb + voff[x] + dt * 2048);
-                        if (edge) {
-                            // A NaN at a key that some columns see and some do not (kept8.hip): zero in the
-                            // product, marked where it is seen.
-                            uint32_t any = 0;
-                            u32x4 ones[2];
-#pragma unroll
-                            for (int x = 0; x < 2; x++) {
-                                u32x4 v = __builtin_bit_cast(u32x4, vc[x]);
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const uint32_t low = (v[e] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u;
-                                    const uint32_t high = (v[e] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
-                                    ones[x][e] = (low | high) & 0x3f803f80u;
-                                    v[e] &= ~(low | high);
-                                    any |= low | high;
-                                }
-                                vc[x] = as_bf16x8(v);
-                            }
-                            if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
-#pragma unroll
-                                for (int qt = 0; qt < QT; qt++) {
-                                    f32x4 hit = f32x4{0, 0, 0, 0};
-#pragma unroll
-                                    for (int x = 0; x < 2; x++) {
-                                        u32x4 sw;
-#pragma unroll
-                                        for (int e = 0; e < 4; e++) {
-                                            const uint32_t two = seen[qt] >> (8 * x + 2 * e);
-                                            sw[e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u);
-                                        }
-                                        hit = mfma16(as_bf16x8(ones[x]), as_bf16x8(sw), hit);
-                                    }
-#pragma unroll
-                                    for (int e = 0; e < 4; e++)
-                                        if (hit[e] > 0.0f) o[qt][dt][e] = __builtin_nanf("");
-                                }
-                            }
-                        }
 #pragma unroll
                         for (int x = 0; x < 2; x++)
 #pragma unroll
                             for (int qt = 0; qt < QT; qt++)
 #pragma unroll
                                 for (uint32_t e = 0; e < kParts; e++) o[qt][dt] = mfma16(vc[x], w[qt][x][e], o[qt][dt]);
+                    }
+                    if (nan) {
+#pragma unroll
+                        for (int qt = 0; qt < QT; qt++) {
+                            uint64_t seen = 0;
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                seen |= (uint64_t)(act[qt] ? seen_keys(here + kBlock * j, from[qt], pos[qt]) : 0) << (16 * j);
+#pragma unroll
+                            for (int dt = 0; dt < 8; dt++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    if (nan_keys[buffer][16 * dt + 4 * grp + e] & seen) o[qt][dt][e] = __builtin_nanf("");
+                        }
                     }
                 }
                 if (!go) break;
