@@ -365,13 +365,13 @@ Plan plan(const ts_kept8_args *k) {
     s.tiles = (a->rows + s.tile_rows - 1) / s.tile_rows;
     s.groups = s.tiles;
     s.most = 1;
-    // Keys are shared out over as many groups as run at once (two of four waves a CU, one of eight): more would
-    // each cost 8 us before the first step is done, fewer leave CUs idle. Decode rows and drafts (32 sequences
+    // Keys are shared out over as many groups as run at once (a CU's two of four waves, with 64 columns of bf16 q
+    // three, or one of eight): more would each cost 8 us before the first step is done, fewer leave CUs idle. Decode rows and drafts (32 sequences
     // of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's longest span 78, a group a tile 106),
     // beyond the groups at once too (128 of up to 4096: 128 us, a group a tile 137). Wide tiles, whose
     // products bound them, only where there are fewer tiles than groups (3 chunks of up to 700 rows: 85 us, a
     // group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile, the widest first, 112).
-    const uint32_t at_once = (s.columns <= 64 ? 512 : 256) / a->kv_heads, unit = s.columns == 16 ? kRound : kStep;
+    const uint32_t at_once = (s.columns == 64 && !f32 ? 768 : s.columns <= 64 ? 512 : 256) / a->kv_heads, unit = s.columns == 16 ? kRound : kStep;
     const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
                                              (uint64_t)a->back + s.tile_rows + kBlock);
     const uint64_t units = (span + unit - 1) / unit + 1;

@@ -41,14 +41,20 @@ TS_DEV uint32_t v_swap(uint32_t d) {
     return (i & 1) | (i >> 1 & 2) | ((i ^ i << 1) & 4);
 }
 
+// One buffer of codes, and two barriers a step, where the registers let three groups of four waves onto a CU, whose
+// LDS two buffers would fill with two (24 x 5 rows: 80 us, 88 with two buffers).
 template <int QT, int W, bool QF32>
-__global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendParams p) {
+constexpr uint32_t buffers() { return QT == 1 && W == 4 && !QF32 ? 1 : 2; }
+
+template <int QT, int W, bool QF32>
+__global__ __launch_bounds__(64 * W, (buffers<QT, W, QF32>() == 1 ? 3 : 2)) void attend_kept8_rows_kernel(AttendParams p) {
     constexpr uint32_t kCols = 16 * QT * W, kParts = QF32 ? 3 : 1, kThreads = 64 * W;
+    constexpr uint32_t kBuffers = buffers<QT, W, QF32>();
     constexpr uint32_t kEach = 512 / kThreads;  // 16-byte pieces of K (and V) codes a thread and step
-    extern __shared__ __attribute__((aligned(16))) char stage[];  // two of kStage
+    extern __shared__ __attribute__((aligned(16))) char stage[];  // kBuffers of kStage
     __shared__ uint32_t shared_words[W], starts[kMaxShared + 1];
     // Per buffer and d: which of the step's 64 keys hold a NaN in V; and whether there has been any.
-    __shared__ uint64_t nan_keys[2][128];
+    __shared__ uint64_t nan_keys[kBuffers][128];
     __shared__ uint32_t nan_met;
     if (threadIdx.x == 0) nan_met = 0;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = threadIdx.x;
@@ -237,19 +243,23 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
 
             look(base);
             fetch(base);
-            stash(0, base);
-            uint32_t next = min(base + kStep, end);
-            fetch(next);
-            for (uint32_t buffer = 0;; buffer ^= 1) {
-                lds_barrier();  // this step's codes are in; the other buffer's readers are done
+            uint32_t next = base;  // the step whose codes are in registers
+            if (kBuffers == 2) {
+                stash(0, base);
+                next = min(base + kStep, end);
+                fetch(next);
+            }
+            for (uint32_t buffer = 0;; buffer ^= kBuffers - 1) {
+                lds_barrier();  // two buffers: this step's codes are in; the readers of the other are done
                 const bool go = base < end;
                 const uint32_t here = base;
-                if (go) {
-                    stash(buffer ^ 1, next);
-                    base = next;
-                    next = min(base + kStep, end);
+                if (kBuffers == 1 || go) {
+                    stash(buffer ^ (kBuffers - 1), next);
+                    base = kBuffers == 1 ? min(base + kStep, end) : next;
+                    next = kBuffers == 1 ? base : min(base + kStep, end);
                     fetch(next);
                 }
+                if (kBuffers == 1) lds_barrier();
                 if (here <= whi && here + (kStep - 1) >= wlo) {
                     const char *kb = stage + buffer * kStage, *vb = kb;
                     const uint32_t nan = __builtin_amdgcn_readfirstlane(nan_met);
@@ -299,7 +309,7 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
                             uint64_t seen = 0;
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                seen |= (uint64_t)(act[qt] ? seen_keys(here + kBlock * j, from[qt], pos[qt]) : 0) << (16 * j);
+                                if (act[qt]) seen |= (uint64_t)seen_keys(here + kBlock * j, from[qt], pos[qt]) << (16 * j);
 #pragma unroll
                             for (int dt = 0; dt < 8; dt++)
 #pragma unroll
@@ -341,11 +351,11 @@ __global__ __launch_bounds__(64 * W, 2) void attend_kept8_rows_kernel(AttendPara
 
 template <int QT, int W, bool QF32>
 int launch(const AttendParams &p, uint32_t groups, void *stream) {
+    constexpr uint32_t kLds = buffers<QT, W, QF32>() * kStage;
     static const hipError_t attr = hipFuncSetAttribute((const void *)attend_kept8_rows_kernel<QT, W, QF32>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kStage);
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return ts::hip_status(attr, "attend_kept8: shared memory attribute");
-    hipLaunchKernelGGL((attend_kept8_rows_kernel<QT, W, QF32>), dim3(groups), dim3(64 * W), 2 * kStage,
-                       (hipStream_t)stream, p);
+    hipLaunchKernelGGL((attend_kept8_rows_kernel<QT, W, QF32>), dim3(groups), dim3(64 * W), kLds, (hipStream_t)stream, p);
     TS_CHECK_LAUNCH("attend_kept8 rows launch");
     return TS_OK;
 }
