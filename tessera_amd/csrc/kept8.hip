@@ -359,8 +359,11 @@ Plan plan(const ts_kept8_args *k) {
     Plan s;
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
     const uint64_t wanted = (uint64_t)run * G;
-    // f32 q, in three parts, leaves a wave of the shared kernel 16 columns.
-    s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 ? 128 : 256;
+    // f32 q, in three parts, leaves a wave of the shared kernel 16 columns. 256 columns widen the codes for fewer
+    // waves twice, but fill a CU with one group: only where there are two groups a CU in turn to even them out
+    // (4 prompts of 2048 rows, 8 kv heads: 111 us, 128 columns 122; 2 such prompts 86 us, 128 columns 83).
+    const uint64_t wide = (a->rows + 256 / G - 1) / (256 / G) * (uint64_t)a->kv_heads;
+    s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 || wide < 512 ? 128 : 256;
     s.tile_rows = std::min(run, s.columns / G);
     s.tiles = (a->rows + s.tile_rows - 1) / s.tile_rows;
     s.groups = s.tiles;
