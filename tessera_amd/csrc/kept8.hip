@@ -282,8 +282,9 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
     }
 }
 
-// The parts of a tile's columns joined: S lane groups of 32 (four d a lane) take a column's parts in turn,
-// 8 / S columns a group of 256. (One lane group walking 128 parts by itself waits 20 us.)
+// The parts of a tile's columns joined: S lane groups of 32 (four d a lane) take a column's parts in turn, four
+// at a time, 8 / S columns a group of 256. (One lane group walking 128 parts by itself waits 20 us; up to four
+// parts are one step of one.)
 template <uint32_t S>
 __global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_t cols, uint32_t pieces) {
     __shared__ float smax[8], ssum[8];
@@ -300,48 +301,54 @@ __global__ __launch_bounds__(256) void join_kept8_kernel(AttendParams p, uint32_
     const size_t next = (size_t)p.kv_heads * cols * kPart;  // from a group's results to the next's
     const float *rest = p.partials + p.shares[gi / p.kv_heads * 2] * next +
                         ((size_t)tile.kvh * cols + (there ? c : 0)) * kPart;
-    auto result = [&](uint32_t j) { return rest + (j ? j : p.groups) * next; };
-    // The maximum: every lane of the lane group looks at parts of its own.
-    float M = -INFINITY;
-    for (uint32_t j = j1 + S * d; j < parts; j += S * 32) M = fmaxf(M, *result(j));
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-    if (S > 1) {
-        if (d == 0) smax[lg] = M;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t s = 0; s < S; s++) M = fmaxf(M, smax[lg / S * S + s]);
-    }
-    float L = 0.0f;
+    float M = -INFINITY, L = 0.0f;
     f32x4 O = f32x4{0, 0, 0, 0};
+    // A maximum of -inf: an empty part, or a refused column's (whose sum is NaN): as it is.
+    auto factor = [](float m, float to) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to); };
     for (uint32_t j0 = j1; j0 < parts; j0 += S * kBatch) {
-        float mq[kBatch], lq[kBatch];
+        float mq[kBatch], lq[kBatch], top = M;
         f32x4 oq[kBatch];
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {  // past the end: read, not used
-            const float *at = result(min(j0 + S * j, parts - 1));
+            const uint32_t part = min(j0 + S * j, parts - 1);
+            const float *at = rest + (part ? part : p.groups) * next;
             mq[j] = at[0];
             lq[j] = at[1];
             oq[j] = *(const f32x4 *)(at + 4 + 4 * d);
         }
 #pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++)
+            if (j0 + S * j < parts) top = fmaxf(top, mq[j]);
+        const float f = factor(M, top);
+        M = top;
+        L *= f;
+        O *= f;
+#pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {
-            // An empty part (max -inf, sum 0) has no O.
-            if (j0 + S * j >= parts || (mq[j] == -INFINITY && lq[j] == 0.0f)) continue;
-            const float f = mq[j] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mq[j] - M);
-            L += lq[j] * f;
-            O += oq[j] * f;
+            if (j0 + S * j >= parts) continue;
+            const float g = factor(mq[j], M);
+            L += lq[j] * g;
+            O += oq[j] * g;
         }
     }
     if (S > 1) {
         so[lg][d] = O;
-        if (d == 0) ssum[lg] = L;
+        if (d == 0) {
+            smax[lg] = M;
+            ssum[lg] = L;
+        }
         __syncthreads();
         if (j1) return;
 #pragma unroll
+        for (uint32_t s = 1; s < S; s++) M = fmaxf(M, smax[lg + s]);
+        const float f = factor(smax[lg], M);
+        L *= f;
+        O *= f;
+#pragma unroll
         for (uint32_t s = 1; s < S; s++) {
-            L += ssum[lg + s];
-            O += so[lg + s][d];
+            const float g = factor(smax[lg + s], M);
+            L += ssum[lg + s] * g;
+            O += so[lg + s][d] * g;
         }
     }
     if (there) store4(p, ((size_t)r * p.heads + h) * 128 + 4 * d, O / L);
@@ -458,7 +465,7 @@ extern "C" int tessera_hip_attend_kept8(const ts_kept8_args *k, void *stream) {
         rc = f32 ? launch<true>(p, groups, stream) : launch<false>(p, groups, stream);
     if (rc || s.most == 1) return rc;
     const uint32_t used = s.tile_rows * p.group, parts = std::min(s.most, s.groups / s.tiles + 2);
-    const uint32_t S = parts <= 2 ? 1 : parts <= 8 ? 2 : 8;
+    const uint32_t S = parts <= 4 ? 1 : parts <= 8 ? 2 : 8;
     const uint32_t pieces = (used * S + 7) / 8;
     const auto join = S == 1 ? join_kept8_kernel<1> : S == 2 ? join_kept8_kernel<2> : join_kept8_kernel<8>;
     hipLaunchKernelGGL(join, dim3(s.tiles * a->kv_heads * pieces), dim3(256), 0, (hipStream_t)stream, p, s.columns,
