@@ -19,6 +19,10 @@
 // four positions of a d are one word of V's block. The rows of a call that meet in a block must
 // therefore stand together; a later segment of the same block is refused (TS_STATUS_TWICE), found by
 // looking through the rows before it.
+//
+// Many rows are bound by HBM: 6 ragged prompts of up to 2048 f32 rows, 16 + 2 x 8 heads, into blocks, 250 MB: 52 to
+// 61 us, 4.1 to 4.8 TB/s. Few by a chain of loads (position, page, row, scale, held codes) and by fetching code,
+// about 1 KiB a microsecond the first time: one row 4.5 us, 200 into bf16 rows 5.9, 48 x 5 into begun blocks 8.5.
 #include "kept8.h"
 
 namespace {

@@ -14,8 +14,11 @@
 //  * V: 16 bytes are the 16 positions of one d of block lane / 16, again two operands.
 //  Nothing passes through LDS: codes go from memory to registers, through the conversion that applies
 //  the block's scale, into the matrix unit; the next step's are asked for as soon as this step's are used.
-//  The four waves of a group, and the groups that share a tile's keys, are joined by their maxima and
-//  sums, the former in LDS, the latter by a second kernel.
+//  The four waves of a group, and the groups that share a tile's keys (share_of), are joined by their maxima
+//  and sums, the former in LDS, the latter by a second kernel.
+// HBM bounds it: 32 rows of 512 .. 8192 keys, 8 kv heads, 286 MB: 54 us and 5 for the join, 5.3 TB/s of codes;
+// 2 rows of 131000 keys, 4 kv heads: 42 and 5 us, 6 TB/s. A step costs a wave about 2.2 us with two waves a SIMD; a
+// group's first is done after some 8 us, which is what one row of 4000 keys takes (9.5 and 4 us).
 #include <algorithm>
 
 #include "kept8_attend.h"
@@ -376,12 +379,14 @@ Plan plan(const ts_kept8_args *k) {
     s.groups = s.tiles;
     s.most = 1;
     // Keys are shared out over as many groups as run at once (a CU's two of four waves, with 64 columns of bf16 q
-    // three, or one of eight): more would each cost 8 us before the first step is done, fewer leave CUs idle. Decode rows and drafts (32 sequences
-    // of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's longest span 78, a group a tile 106),
-    // beyond the groups at once too (128 of up to 4096: 128 us, a group a tile 137). Wide tiles, whose
-    // products bound them, only where there are fewer tiles than groups (3 chunks of up to 700 rows: 85 us, a
-    // group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile, the widest first, 112).
-    const uint32_t at_once = (s.columns == 64 && !f32 ? 768 : s.columns <= 64 ? 512 : 256) / a->kv_heads, unit = s.columns == 16 ? kRound : kStep;
+    // three, or one of eight): more would each cost 8 us before the first step is done, fewer leave CUs idle.
+    // Decode rows and drafts always (32 sequences of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's
+    // longest span 78, a group a tile 106), beyond the groups at once too (128 of up to 4096: 128 us, a group a
+    // tile 137). Wide tiles, whose partial results are large, only where there are fewer tiles than groups (3
+    // chunks of up to 700 rows: 85 us, a group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile, the
+    // widest first, 112).
+    const uint32_t at_once = (s.columns == 64 && !f32 ? 768 : s.columns <= 64 ? 512 : 256) / a->kv_heads;
+    const uint32_t unit = s.columns == 16 ? kRound : kStep;
     const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
                                              (uint64_t)a->back + s.tile_rows + kBlock);
     const uint64_t units = (span + unit - 1) / unit + 1;
