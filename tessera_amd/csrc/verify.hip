@@ -65,21 +65,19 @@ TS_DEV double scalar(double c) {
     return c;
 }
 
-// 2^t for -1200 < t <= 0: t = n + f, |f| <= 1/2, the series of 2^f = e^(f ln 2) up to the 10th power (the
-// 11th is 3e-13 at most, at |f| = 1/2).
+// 2^t for -1200 < t <= 0: t = n + f, |f| <= 1/2, n out of the low bits of t + 1.5 * 2^52, and 2^f = 1 + f g(f)
+// with g, of degree 6, through (2^f - 1) / f at the Chebyshev points: 1.1e-10 off at most, 2^0 exact. (f32
+// would be 6e-8 off. The series up to the 10th power, 3e-13, cost an eighth of both kernels.)
 TS_DEV double exp2_neg(double t) {
-    const double n = __builtin_rint(t), f = t - n;
-    double r = __builtin_fma(f, scalar(7.054911620801123e-09), scalar(1.01780860092397e-07));
-    r = __builtin_fma(r, f, scalar(1.321548679014431e-06));
-    r = __builtin_fma(r, f, scalar(1.5252733804059841e-05));
-    r = __builtin_fma(r, f, scalar(0.0001540353039338161));
-    r = __builtin_fma(r, f, scalar(0.0013333558146428443));
-    r = __builtin_fma(r, f, scalar(0.009618129107628477));
-    r = __builtin_fma(r, f, scalar(0.05550410866482158));
-    r = __builtin_fma(r, f, scalar(0.24022650695910072));
+    const double k = t + scalar(6755399441055744.0), f = t - (k - scalar(6755399441055744.0));
+    double r = __builtin_fma(f, scalar(1.5297324125640444e-05), scalar(0.00015461444699635));
+    r = __builtin_fma(r, f, scalar(0.0013333502384966778));
+    r = __builtin_fma(r, f, scalar(0.009618056678521874));
+    r = __builtin_fma(r, f, scalar(0.05550410883910522));
+    r = __builtin_fma(r, f, scalar(0.24022650922288763));
     r = __builtin_fma(r, f, scalar(0.6931471805599453));
     r = __builtin_fma(r, f, 1.0);
-    return __builtin_amdgcn_ldexp(r, (int)n);  // (0 below 2^-1074)
+    return __builtin_amdgcn_ldexp(r, (int)(uint32_t)__builtin_bit_cast(uint64_t, k));  // (0 below 2^-1074)
 }
 
 // e of logits side by side, `by` = log2(e) / temperature: 1 at the maximum (+inf too), 0 for NaN and -inf
