@@ -197,6 +197,31 @@ def test_refused_rows(run):
     spoilt(abi.TS_STATUS_PAGE, where=dict(where, table=table), lost=(slots == 1) & (positions >= 112))
 
 
+@pytest.mark.parametrize("name,dtype,f32", TYPES)
+@pytest.mark.parametrize("seqs,run,heads,kvh,back", [(70, 1, 2, 1, None), (200, 1, 6, 3, 150), (260, 1, 2, 1, None),
+                                                     (90, 3, 16, 1, None), (258, 3, 12, 1, 100), (20, 40, 4, 2, None)])
+def test_many_ragged_sequences(seqs, run, heads, kvh, back, name, dtype, f32):
+    """More sequences than one lane each of a wave, than the groups that share keys take, and tiles that begin
+    in one sequence and end in another: lengths of `run` to 640, shared out in runs that begin and end anywhere."""
+    r = rng(seqs + run)
+    page, each = 16, 40
+    blocks = seqs * each
+    table = r.permutation(blocks).astype(np.int32)
+    k, v = (r.integers(0, 256, s).astype(np.uint8) for s in ((blocks, kvh, 16, 128), (blocks, kvh, 128, 16)))
+    for x in (k, v):
+        x[(x & 0x7F) == 0x7F] = 0
+    scales = np.exp2(r.integers(-9, -6, (blocks, (kvh + 1) // 2 * 2, 2))).astype(np.float32)
+    where = dict(keys=each * page, table=table, kept_pages=each, page=page)
+    counts = r.integers(1, run + 1, seqs)  # rows of each sequence
+    lengths = np.maximum(r.integers(1, 641, seqs), counts)
+    slots = np.repeat(r.permutation(seqs), counts)
+    positions = np.concatenate([lengths[s] - n + np.arange(n) for s, n in zip(range(seqs), counts)])
+    q = dev((r.standard_normal((len(slots), heads, 128)) / 8).astype(np.float32), dtype)
+    kw = {} if back is None else {"back": back}
+    out = call(q, k, v, scales, slots, positions, where, page, out_dtype=dtype, run=run, **kw)
+    check(out, *K.attend(q.float().cpu().numpy(), k, v, scales, slots, positions, scale=SCALE, back=back, **where), f32)
+
+
 def test_many_parts_and_offsets_past_32_bits():
     """A cache of more than 4 GiB of codes, a long slot at its end: split over many groups."""
     kvh, page, n = 8, 64, 20000
