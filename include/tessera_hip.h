@@ -315,8 +315,9 @@ int tessera_hip_flash_rows(const ts_rows_args *a, void *stream);
  *  - Any other call lets a block's scales only grow, and moves the codes already there to the
  *    grown scale (exact, but for codes that turn subnormal). What a block holds thus depends on
  *    how its positions were divided among calls.
- *  - Codes are rounded to nearest even; infinities and NaN become NaN codes and take no part in
- *    the scale; values past 448 * 2^119 become the largest.
+ *  - Norm and rotation are in 64 bits where codes are kept, which are rounded from that to nearest
+ *    even; infinities and NaN become NaN codes and take no part in the scale; values past
+ *    448 * 2^119 become the largest.
  *  - Rows of one call that fall into one block (16 positions of a slot) stand together and in
  *    order; a later run of rows of the same block is kept nowhere and sets TS_STATUS_TWICE. Two
  *    slots of a call never share the page they append to (Pool::grow sees to it).

@@ -21,8 +21,8 @@
 // looking through the rows before it.
 //
 // Many rows are bound by HBM: 6 ragged prompts of up to 2048 f32 rows, 16 + 2 x 8 heads, into blocks, 250 MB: 52 to
-// 61 us, 4.1 to 4.8 TB/s. Few by a chain of loads (position, page, row, scale, held codes) and by fetching code,
-// about 1 KiB a microsecond the first time: one row 4.5 us, 200 into bf16 rows 5.9, 48 x 5 into begun blocks 8.5.
+// 65 us, 3.9 to 4.8 TB/s. Few by a chain of loads (position, page, row, scale, held codes) and by fetching code,
+// about 1 KiB a microsecond the first time: one row 4.8 us, 200 into bf16 rows 5.9, 48 x 5 into begun blocks 10.3.
 #include "kept8.h"
 
 namespace {
@@ -119,6 +119,51 @@ TS_DEV void turn8(float (&v)[8], const f32x4 (&cs)[2]) {
     }
 }
 
+// Rows that become codes are normed and rotated in f64 and come back as f32 rounded to odd (cut off, the last bit
+// set where anything was), so that the code is the nearest to the formula's value and the scale the least for it:
+// from f32 steps one code in a million or so is its neighbour, an eighth away. (6 prompts of up to 2048 rows: 63 us,
+// in f32 61.)
+TS_DEV float to_odd(double d) {
+    const float f = (float)d;
+    const uint64_t off = __builtin_bit_cast(uint64_t, d - (double)f);
+    const uint32_t high = (uint32_t)(off >> 32), u = __float_as_uint(f);
+    const uint32_t inexact = min((high & 0x7fffffffu) | (uint32_t)off, 1u), away = (high ^ u) >> 31;
+    const uint32_t odd = (u - (away & inexact)) | inexact;
+    return fabsf(f) < __builtin_inff() ? __uint_as_float(odd) : f;
+}
+template <bool HALVES>
+TS_DEV void norm_turn8(float (&v)[8], bool norm, const float (&gain)[8], float eps, bool turn, const f32x4 (&cs)[2]) {
+    double inv = 1.0;
+    if (norm) {
+        double sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum = __builtin_fma((double)v[k], (double)v[k], sum);
+        const double mean = row16_total(sum) * (1.0 / 128.0) + (double)eps;
+        inv = __builtin_amdgcn_rsq(mean);  // refined to 1e-15; 0 for infinity, as it is
+        const double e = __builtin_fma(-mean * inv, inv, 1.0);
+        inv = mean < __builtin_inf() ? __builtin_fma(inv * e, __builtin_fma(e, 0.375, 0.5), inv) : inv;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {  // (a pair at a time: all of them side by side in f64 would spill)
+        float &a = v[Lanes<HALVES>::pa(k)], &b = v[Lanes<HALVES>::pb(k)];
+        asm volatile("" : "+v"(a), "+v"(b));
+        double x = a, y = b;
+        if (norm) {
+            x *= inv * (double)gain[Lanes<HALVES>::pa(k)];
+            y *= inv * (double)gain[Lanes<HALVES>::pb(k)];
+        }
+        if (turn) {
+            const double c = cs[k / 2][2 * (k % 2)], sn = cs[k / 2][2 * (k % 2) + 1];
+            const double z = __builtin_fma(x, c, -(y * sn));
+            y = __builtin_fma(y, c, x * sn);
+            x = z;
+        }
+        a = to_odd(x);
+        b = to_odd(y);
+        asm volatile("" : "+v"(a), "+v"(b));
+    }
+}
+
 template <bool HALVES>
 TS_DEV void load_gain(const float *gain, uint32_t l, float (&g)[8]) {
 #pragma unroll
@@ -176,12 +221,19 @@ TS_DEV void append_one(const AppendParams &p, uint64_t row0, uint32_t pos, uint3
     load8<XBF16, HALVES>(is_v ? from : k, h * 128, l, v);
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = v[e];
-    if (p.k_gain) {
+    if (KEPT8 && (p.k_gain || p.turns)) {
+        float gain[8] = {};
+        f32x4 cs[2] = {};
+        if (p.k_gain) load_gain<HALVES>(p.k_gain, l, gain);
+        if (p.turns) load_turns(p.turns + (size_t)pos * 64, 0, l, cs);
+        norm_turn8<HALVES>(x, p.k_gain, gain, p.eps, p.turns, cs);
+    }
+    if (!KEPT8 && p.k_gain) {
         float gain[8];
         load_gain<HALVES>(p.k_gain, l, gain);
         norm8<HALVES>(x, gain, p.eps);
     }
-    if (p.turns) {
+    if (!KEPT8 && p.turns) {
         f32x4 cs[2];
         load_turns(p.turns + (size_t)pos * 64, 0, l, cs);
         turn8<HALVES>(x, cs);
@@ -238,7 +290,7 @@ TS_DEV void append_segment(const AppendParams &p, uint64_t row0, uint32_t pos, u
     const uint32_t g = lane >> 4, l = lane & 15, off = pos & (kBlock - 1);
     const uint32_t mine = (((1u << n) - 1) << off) >> (4 * g) & 15;
     const uint64_t first = row0 - off;  // kept row of the 16's position 0
-    if (!IS_V) {
+    if (!IS_V && !KEPT8) {
         if (p.k_gain) {
             float gain[8];
             load_gain<HALVES>(p.k_gain, l, gain);
@@ -253,6 +305,16 @@ TS_DEV void append_segment(const AppendParams &p, uint64_t row0, uint32_t pos, u
                 load_turns(row, segment_row(4 * g + i, off, n), l, cs);
                 turn8<HALVES>(x[i], cs);
             }
+        }
+    } else if (!IS_V && (p.k_gain || p.turns)) {
+        float gain[8] = {};
+        if (p.k_gain) load_gain<HALVES>(p.k_gain, l, gain);
+        const float2 *row = p.turns + (size_t)pos * 64;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            f32x4 cs[2] = {};
+            if (p.turns) load_turns(row, segment_row(4 * g + i, off, n), l, cs);
+            norm_turn8<HALVES>(x[i], p.k_gain, gain, p.eps, p.turns, cs);
         }
     }
     if (!KEPT8) {
@@ -312,7 +374,7 @@ TS_DEV void append_segment(const AppendParams &p, uint64_t row0, uint32_t pos, u
 constexpr uint32_t kWaves = 4;
 
 template <bool XBF16, bool KEPT8, bool HALVES>
-__global__ __launch_bounds__(64 * kWaves, 5) void append_kernel(AppendParams p) {
+__global__ __launch_bounds__(64 * kWaves, KEPT8 ? 4 : 5) void append_kernel(AppendParams p) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (blockIdx.x >= p.kv_groups) {  // four q heads of q_rows rows a wave
         const uint32_t u = (blockIdx.x - p.kv_groups) * kWaves + wave, r0 = u / p.head_quads * p.q_rows, l = lane & 15;

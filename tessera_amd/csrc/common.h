@@ -201,6 +201,22 @@ TS_DEV float row16_max(float v) {
     return v;
 }
 
+// The sum over a row of 16 lanes, in each of them, by DPP moves.
+template <int CTRL>
+TS_DEV double dpp_double(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+TS_DEV double row16_total(double v) {
+    v += dpp_double<0xB1>(v);   // lane ^ 1
+    v += dpp_double<0x4E>(v);   // lane ^ 2
+    v += dpp_double<0x141>(v);  // 7 - lane of each 8
+    v += dpp_double<0x140>(v);  // 15 - lane
+    return v;
+}
+
 // Whole-wave totals in every lane: rows by DPP, then two cross-row exchanges.
 TS_DEV float wave_sum(float v) {
     v = row16_sum(v);

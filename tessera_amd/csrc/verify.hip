@@ -138,22 +138,8 @@ TS_DEV Seq seq_of(const VerifyParams &p, uint32_t s) {
     return q;
 }
 
-// Sums over the wave, in every lane: DPP moves within rows of 16 lanes, then the permlane swaps across them
+// The sum over the wave, in every lane: within rows of 16 lanes, then by the permlane swaps across them
 // (through LDS, two exchanges a step of a double, the six steps take five times as long).
-template <int CTRL>
-TS_DEV double dpp_double(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-TS_DEV double row16_total(double v) {
-    v += dpp_double<0xB1>(v);   // lane ^ 1
-    v += dpp_double<0x4E>(v);   // lane ^ 2
-    v += dpp_double<0x141>(v);  // 7 - lane of each 8
-    v += dpp_double<0x140>(v);  // 15 - lane
-    return v;
-}
 TS_DEV double wave_total(double v) {
     v = row16_total(v);
     uint64_t b = __builtin_bit_cast(uint64_t, v);

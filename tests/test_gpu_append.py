@@ -113,6 +113,29 @@ def test_blocks(rows, past, heads, kvh, page, x, norm, turn, halves):
     assert np.array_equal(got_s[:, kvh:], held[:, kvh:]) and int(status) == 0
 
 
+@pytest.mark.parametrize("rows,norm,turn,halves", [(2050, True, True, True), (2050, True, True, False), (1500, True, False, True),
+                                                   (1500, False, True, True), (0, True, True, True)])
+def test_codes_are_the_nearest(rows, norm, turn, halves):
+    """Codes and scales equal the 64-bit form's: a value is 2^-52 or so off before it is rounded, which none of a
+    million comes that near a border of the codes to notice. rows 0: one row each of 900 slots."""
+    r = rng(rows + halves)
+    kvh, page = 4, 16
+    slots, keys = (np.zeros(rows, np.int32), 2064) if rows else (np.arange(900, dtype=np.int32), 32)
+    positions = np.arange(rows, dtype=np.int32) if rows else r.integers(0, 32, 900).astype(np.int32)
+    n = len(slots)
+    x = (r.standard_normal((n, kvh, 128)) * np.exp(2 * r.standard_normal((n, kvh, 1)))).astype(np.float32)
+    gain = (1 + 0.1 * r.standard_normal(128)).astype(np.float32) if norm else None
+    angles = angle_table(keys) if turn else None
+    pages = (int(slots.max()) + 1) * keys // page
+    k8, v8, s8 = rules.kept8(pages, kvh, page)
+    rules.append_rows(dev(x), dev(x), k8, v8, dev(slots), dev(positions), keys=keys, scales=s8, page=page, halves=halves,
+                      k_gain=None if not norm else dev(gain), angles=None if not turn else dev(angles), eps=EPS)
+    blocks, scales = np.zeros((pages, kvh, 16, 128), np.uint8), np.zeros((pages, kvh, 2))
+    K.append(blocks, scales, 0, K.turned(x, gain, angles, positions, halves, float(np.float32(EPS))), slots, positions, keys=keys)
+    assert np.array_equal(s8.cpu().numpy()[:, :, 0], scales[..., 0])
+    assert np.array_equal(k8.cpu().numpy(), blocks)
+
+
 @pytest.mark.parametrize("x", ["f32", "bf16"])
 @pytest.mark.parametrize("halves", [True, False])
 def test_bf16_rows_as_the_separate_stages_keep_them(x, halves):
