@@ -20,9 +20,9 @@
 // therefore stand together; a later segment of the same block is refused (TS_STATUS_TWICE), found by
 // looking through the rows before it.
 //
-// Many rows are bound by HBM: 6 ragged prompts of up to 2048 f32 rows, 16 + 2 x 8 heads, into blocks, 250 MB: 52 to
-// 65 us, 3.9 to 4.8 TB/s. Few by a chain of loads (position, page, row, scale, held codes) and by fetching code,
-// about 1 KiB a microsecond the first time: one row 4.8 us, 200 into bf16 rows 5.9, 48 x 5 into begun blocks 10.3.
+// Many rows are bound by HBM: 6 ragged prompts of up to 2048 f32 rows, 16 + 2 x 8 heads, into blocks, 250 MB: 51 to
+// 63 us, 4.0 to 4.9 TB/s. Few by a chain of loads (position, page, row, scale, held codes) and by fetching code,
+// about 1 KiB a microsecond the first time: one row 4.9 us, 200 into bf16 rows 5.9, 48 x 5 into begun blocks 10.4.
 #include "kept8.h"
 
 namespace {

@@ -18,7 +18,7 @@
 // Exponentials and sums are in f64 (the vector unit's f64 rate is f32's here): the draw compares u with
 // running sums whose borders lie 1 / 150,000 apart and closer, and f32 would move them by 1e-7 of the whole.
 // They bound the kernels (16 vector operations a logit), beside HBM: 32 sequences of up to 4 drafts with the
-// drafter's probabilities, 151936 f32 logits a row: rows 22 us, draw 17; one greedy sequence of 4 drafts: 4 and 3 us.
+// drafter's probabilities, 151936 f32 logits a row: rows 20 us, draw 16; one greedy sequence of 4 drafts: 4 and 3 us.
 #include <algorithm>
 
 #include "common.h"
