@@ -371,7 +371,7 @@ Plan plan(const ts_kept8_args *k) {
     const uint64_t wanted = (uint64_t)run * G;
     // f32 q, in three parts, leaves a wave of the shared kernel 16 columns. 256 columns widen the codes for fewer
     // waves twice, but fill a CU with one group: only where there are two groups a CU in turn to even them out
-    // (4 prompts of 2048 rows, 8 kv heads: 111 us, 128 columns 122; 2 such prompts 86 us, 128 columns 83).
+    // (4 prompts of 2048 rows, 8 kv heads: 106 us, 128 columns 124; 2 such prompts 79 us, 128 columns 73).
     const uint64_t wide = (a->rows + 256 / G - 1) / (256 / G) * (uint64_t)a->kv_heads;
     s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 || wide < 512 ? 128 : 256;
     s.tile_rows = std::min(run, s.columns / G);
@@ -383,7 +383,7 @@ Plan plan(const ts_kept8_args *k) {
     // Decode rows and drafts always (32 sequences of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's
     // longest span 78, a group a tile 106), beyond the groups at once too (128 of up to 4096: 128 us, a group a
     // tile 137). Wide tiles, whose partial results are large, only where there are fewer tiles than groups (3
-    // chunks of up to 700 rows: 85 us, a group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile, the
+    // chunks of up to 700 rows: 85 us when a group a tile took 137; but 4 prompts of 2048 rows 168 us, a group a tile, the
     // widest first, 112).
     const uint32_t at_once = (s.columns == 64 && !f32 ? 768 : s.columns <= 64 ? 512 : 256) / a->kv_heads;
     const uint32_t unit = s.columns == 16 ? kRound : kStep;

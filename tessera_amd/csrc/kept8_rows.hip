@@ -13,9 +13,9 @@
 //    first (by their last row's position), heads fastest, so that consecutive groups, which go to
 //    different XCDs, leave each XCD one kv head's keys. Fewer tiles than groups share their keys (share_of).
 // A wave's step is a chain (K from LDS, scores, softmax, V from LDS, product) that two or three waves a SIMD overlap
-// in part: vector work takes half of the cycles, the matrix unit 28%. 4 prompts of 2048 rows, 16 heads over 8:
-// 107 us, 640 TFLOP/s; 24 x 5 drafted rows, 64 heads over 8, 1000 .. 9001 keys: 63 us and 6 for the join, 4 TB/s of
-// codes; f32 chunks of up to 700 rows with a window of 1000, 16 heads over 8: 59 and 8 us.
+// in part: vector work takes half of the cycles, the matrix unit 30%. 4 prompts of 2048 rows, 16 heads over 8:
+// 101 us, 680 TFLOP/s; 24 x 5 drafted rows, 64 heads over 8, 1000 .. 9001 keys: 60 us and 6 for the join, 4.2 TB/s of
+// codes; f32 chunks of up to 700 rows with a window of 1000, 16 heads over 8: 54 and 8 us.
 #include <algorithm>
 
 #include "kept8_attend.h"
@@ -47,7 +47,7 @@ TS_DEV uint32_t v_swap(uint32_t d) {
 }
 
 // One buffer of codes, and two barriers a step, where the registers let three groups of four waves onto a CU, whose
-// LDS two buffers would fill with two (24 x 5 rows: 80 us, 88 with two buffers).
+// LDS two buffers would fill with two (24 x 5 rows: 79 us, 87 with two buffers).
 template <int QT, int W, bool QF32>
 constexpr uint32_t buffers() { return QT == 1 && W == 4 && !QF32 ? 1 : 2; }
 
