@@ -494,6 +494,8 @@ def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=
         q_type = _DT[q_out.dtype]
     if rows == 1:  # any distance will do
         q_stride, k_stride, v_stride = heads * width, kv_heads * width, kv_heads * width
+    elif (q_stride | k_stride | v_stride) >> 32:
+        raise ValueError("append_rows: rows more than 2^32 elements apart")
     if scales is not None:
         held = _kept8_blocks(what, k_kept, v_kept, scales, kv_heads) * KEPT_BLOCK
         kept, kv = _CODES, abi.TS_E4M3
@@ -523,8 +525,8 @@ def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=
                        k_kept.data_ptr(), v_kept.data_ptr(), None if scales is None else scales.data_ptr(),
                        slots.data_ptr(), positions.data_ptr(), None if table is None else table.data_ptr(),
                        None if status is None else status.data_ptr(), rows, heads, kv_heads, width, q_stride,
-                       k_stride, v_stride, keys, _slots(what, table, kept_pages, held, keys), kept_pages, page, held // page,
-                       0 if angles is None else angles.numel() // width, halves, _DT[x], q_type, kv, eps)
+                       k_stride, v_stride, keys, _slots(what, table, kept_pages, held, keys), kept_pages, page,
+                       held // max(page, 1), 0 if angles is None else angles.numel() // width, halves, _DT[x], q_type, kv, eps)
     _call_on(on, abi.load().tessera_hip_append_rows, a)
     return q_out
 
@@ -561,7 +563,7 @@ def attend_kept8(q, k, v, scales, slots, positions, *, keys, scale, table=None, 
                                    keys, heads, kv_heads, width, back, kept_pages, page, scale, _DT[q.dtype],
                                    abi.TS_E4M3, _DT[out.dtype], max_position,
                                    None if status is None else status.data_ptr()),
-                      scales.data_ptr(), _slots(what, table, kept_pages, held, keys), held // page, run)
+                      scales.data_ptr(), _slots(what, table, kept_pages, held, keys), held // max(page, 1), run)
     lib = abi.load()
     need = lib.tessera_hip_attend_kept8_workspace(a)
     if need:
@@ -588,7 +590,7 @@ def verify(logits, drafts, uniforms=None, *, counts=None, first=None, draft_prob
     stride, inner = logits.stride()
     if rows <= 1:
         stride = width
-    if (inner != 1 and width > 1) or stride < width or logits.dtype not in _ROWS:
+    if (inner != 1 and width > 1) or stride < width or stride >> 32 or logits.dtype not in _ROWS:
         raise ValueError("verify: logits are f32 or bf16, a row's back to back, rows apart")
     if tokens is None:
         tokens = drafts.new_empty(seqs, most + 1)

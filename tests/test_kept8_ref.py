@@ -208,3 +208,17 @@ def test_rules_refuse_what_is_not_on_a_gpu_or_misshapen():
         rules.verify(torch.zeros(3, 50), torch.zeros(1, 2, dtype=torch.int32))
     with pytest.raises(ValueError, match="rows apart"):
         rules.verify(torch.zeros(1, 50).expand(3, 50), torch.zeros(1, 2, dtype=torch.int32))
+
+
+def test_rules_refuse_rows_further_apart_than_the_arguments_say():
+    """A distance past 32 bits would be taken modulo 2^32 by the C structs."""
+    far = torch.empty(3, (1 << 32) // 128 + 8, 128, device="meta")
+    i = torch.zeros(3, dtype=torch.int32)
+    kk, kv, sc = rules.kept8(4, 8, device="cpu")
+    with pytest.raises(ValueError, match="apart"):
+        rules.append_rows(far[:, :8], far[:, 8:16], kk, kv, i, i, keys=32, scales=sc)
+    near = torch.zeros(3, 8, 128)
+    with pytest.raises(ValueError, match="apart"):
+        rules.append_rows(near, near, kk, kv, i, i, keys=32, scales=sc, q=far[:, :8])
+    with pytest.raises(ValueError, match="apart"):
+        rules.verify(far.view(3, -1)[:, :50], torch.zeros(1, 2, dtype=torch.int32))
