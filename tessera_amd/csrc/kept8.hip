@@ -383,8 +383,8 @@ Plan plan(const ts_kept8_args *k) {
     // Decode rows and drafts always (32 sequences of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's
     // longest span 78, a group a tile 106), beyond the groups at once too (128 of up to 4096: 128 us, a group a
     // tile 137). Wide tiles, whose partial results are large, only where there are fewer tiles than groups (3
-    // chunks of up to 700 rows: 85 us when a group a tile took 137; but 4 prompts of 2048 rows 168 us, a group a tile, the
-    // widest first, 112).
+    // chunks of up to 700 f32 rows: 85 us, a group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile,
+    // the widest first, 112; before LDS was read ahead).
     const uint32_t at_once = (s.columns == 64 && !f32 ? 768 : s.columns <= 64 ? 512 : 256) / a->kv_heads;
     const uint32_t unit = s.columns == 16 ? kRound : kStep;
     const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
