@@ -18,7 +18,7 @@
 // Exponentials and sums are in f64 (the vector unit's f64 rate is f32's here): the draw compares u with
 // running sums whose borders lie 1 / 150,000 apart and closer, and f32 would move them by 1e-7 of the whole.
 // They bound the kernels (16 vector operations a logit), beside HBM: 32 sequences of up to 4 drafts with the
-// drafter's probabilities, 151936 f32 logits a row: rows 20 us, draw 16; one greedy sequence of 4 drafts: 4 and 3 us.
+// drafter's probabilities, 151936 f32 logits a row: rows 19 us, draw 16; one greedy sequence of 4 drafts: 4 and 3 us.
 #include <algorithm>
 
 #include "common.h"
@@ -56,7 +56,6 @@ struct VerifyParams {
     uint32_t pieces, parts;  // of the rows' kernel: pieces a chunk, chunks a row
     uint32_t runs, groups;   // of the draw's: runs a row, groups a sequence
     float temperature;
-    int whole_x, whole_q;  // four consecutive logits, or probabilities, are one aligned load
 };
 
 // A constant in scalar registers: as an addend it would otherwise be copied to vector ones each time.
@@ -100,26 +99,44 @@ TS_DEV float logit(const VerifyParams &p, uint32_t row, uint32_t i) {
     return BF16 ? bf16_float(((const uint16_t *)p.logits)[at]) : ((const float *)p.logits)[at];
 }
 
-// Four consecutive logits of a row, NaN and indices past the row as -inf.
-template <bool BF16>
-TS_DEV void load4(const VerifyParams &p, uint32_t row, uint32_t i, float *x) {
-    if (p.whole_x && i + 3 < p.width) {
-        const size_t at = (size_t)row * p.stride + i;
+// Four consecutive logits of a row (or probabilities); past the row, its last. VEC: they are one load, and the width
+// a multiple of four. No branch and no use of a value here: either would make a loop that asks for the next ones
+// before it uses these wait for both (32 x 4 drafts 36 us, 35 so).
+template <bool BF16, bool VEC>
+TS_DEV void load4(const void *row, uint32_t i, uint32_t width, uint32_t (&x)[4]) {
+    if (VEC) {
+        const uint32_t at = min(i, width - 4);
         if (BF16) {
-            const u32x2 w = *(const u32x2 *)((const uint16_t *)p.logits + at);
-            x[0] = lo_bf16(w.x);
-            x[1] = hi_bf16(w.x);
-            x[2] = lo_bf16(w.y);
-            x[3] = hi_bf16(w.y);
+            const u32x2 w = *(const u32x2 *)((const uint16_t *)row + at);
+            x[0] = w.x;
+            x[1] = w.y;
         } else {
-            const f32x4 w = *(const f32x4 *)((const float *)p.logits + at);
+            const u32x4 w = *(const u32x4 *)((const uint32_t *)row + at);
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] = w[e];
         }
     } else {
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) x[e] = i + e < p.width ? logit<BF16>(p, row, i + e) : -__builtin_inff();
+        for (uint32_t e = 0; e < 4; e++) {
+            const uint32_t at = min(i + e, width - 1);
+            x[e] = BF16 ? ((const uint16_t *)row)[at] : ((const uint32_t *)row)[at];
+        }
     }
+}
+// What load4 has brought, as f32: indices past the width as `past`, where the wave has any (`edge`).
+template <bool BF16, bool VEC>
+TS_DEV void values4(const uint32_t (&x)[4], uint32_t i, uint32_t width, bool edge, float past, float *v) {
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++)
+        v[e] = !BF16 ? __uint_as_float(x[e]) : !VEC ? lo_bf16(x[e]) : e % 2 ? hi_bf16(x[e / 2]) : lo_bf16(x[e / 2]);
+    if (edge) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) v[e] = i + e < width ? v[e] : past;
+    }
+}
+template <bool BF16>
+TS_DEV const void *row_of(const VerifyParams &p, uint32_t row) {
+    return (const char *)p.logits + (size_t)row * p.stride * (BF16 ? 2 : 4);
 }
 
 // A sequence's drafts, first row of logits and temperature (<= 0: greedy); false where it is out of range.
@@ -155,7 +172,7 @@ TS_DEV double wave_total(double v) {
 // A chunk's pieces, the next one's logits asked for before this one's are weighed. Each lane keeps a
 // maximum and a sum of its own; they meet once, at the end. A lane has two fours of consecutive indices
 // of a piece, 256 apart.
-template <bool BF16>
+template <bool BF16, bool VEC>
 __global__ __launch_bounds__(64 * kWaves) void verify_rows_kernel(VerifyParams p) {
     __shared__ Chunk waves[kWaves];
     const uint32_t part = blockIdx.x % p.parts, sr = blockIdx.x / p.parts;
@@ -166,17 +183,23 @@ __global__ __launch_bounds__(64 * kWaves) void verify_rows_kernel(VerifyParams p
     const double by = per_unit(q.temperature);
     const uint32_t first = part * p.pieces, end = min(first + p.pieces, (p.width + kPiece - 1) / kPiece);
     const uint32_t mine = wave * (kPiece / kWaves) + lane * 4;
-    float x[kEach], most = -__builtin_inff();
-    uint32_t at = p.width;
+    const void *row = row_of<BF16>(p, q.first + t);
+    float most = -__builtin_inff();
+    uint32_t at = p.width, raw[2][4];
     double sum = 0.0;
-    auto load = [&](uint32_t piece, float (&to)[kEach]) {
-        load4<BF16>(p, q.first + t, piece * kPiece + mine, to);
-        load4<BF16>(p, q.first + t, piece * kPiece + mine + 256, to + 4);
+    auto load = [&](uint32_t piece, uint32_t (&to)[2][4]) {
+        load4<BF16, VEC>(row, piece * kPiece + mine, p.width, to[0]);
+        load4<BF16, VEC>(row, piece * kPiece + mine + 256, p.width, to[1]);
     };
-    load(first, x);
+    load(first, raw);
     for (uint32_t piece = first; piece < end; piece++) {
-        float next[kEach];
+        uint32_t next[2][4];
         load(min(piece + 1, end - 1), next);  // (the last piece's again, not used)
+        float x[kEach];
+        const bool edge = (piece + 1) * kPiece > p.width;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; h++)
+            values4<BF16, VEC>(raw[h], piece * kPiece + mine + 256 * h, p.width, edge, -__builtin_inff(), x + 4 * h);
         float top = x[0];
 #pragma unroll
         for (uint32_t j = 1; j < kEach; j++) top = fmaxf(top, x[j]);  // (NaN: the other operand)
@@ -201,7 +224,7 @@ __global__ __launch_bounds__(64 * kWaves) void verify_rows_kernel(VerifyParams p
             for (uint32_t j = 0; j < kEach; j++) sum += w[j];
         }
 #pragma unroll
-        for (uint32_t j = 0; j < kEach; j++) x[j] = next[j];
+        for (uint32_t j = 0; j < kEach; j++) raw[j / 4][j % 4] = next[j / 4][j % 4];
     }
     float own[1] = {most};
     double scale[1];
@@ -328,7 +351,7 @@ __global__ __launch_bounds__(256) void verify_greedy_kernel(VerifyParams p) {
 }
 
 // The draw. Runs of 256 indices, four consecutive ones a lane.
-template <bool BF16>
+template <bool BF16, bool VEC>
 __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyParams p) {
     __shared__ uint32_t before, found[2];
     __shared__ double ends[kDrawWaves], starts[2];
@@ -355,30 +378,34 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyPara
     uint32_t r0 = part * kDrawWaves + wave, apart = p.groups * kDrawWaves, run = 0xffffffffu;
     double w[4], target = 0.0, start = 0.0;
     bool alone = false, searching = false;
-    auto load = [&](uint32_t r, float (&x)[4], float (&c)[4]) {
-        const uint32_t i = r * kRun + lane * 4;
-        load4<BF16>(p, v.row, i, x);
-#pragma unroll
-        for (uint32_t e = 0; e < 4; e++) c[e] = 0.0f;
-        if (residual && probs) {
-            if (p.whole_q && i + 3 < p.width) {
-                const f32x4 y = *(const f32x4 *)(probs + i);
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++) c[e] = y[e];
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++) c[e] = i + e < p.width ? probs[i + e] : 0.0f;
-            }
-        }
+    const void *row = row_of<BF16>(p, v.row);
+    // (Without probabilities the logits are read in their place, from the caches, and not used.)
+    const bool rest = v.refused && probs;
+    const void *beside = rest ? (const void *)probs : row;
+    auto load = [&](uint32_t r, uint32_t (&x)[4], uint32_t (&c)[4]) {
+        load4<BF16, VEC>(row, r * kRun + lane * 4, p.width, x);
+        if (BF16 && !rest)
+            load4<true, VEC>(beside, r * kRun + lane * 4, p.width, c);
+        else
+            load4<false, VEC>(beside, r * kRun + lane * 4, p.width, c);
     };
     for (;;) {
-        float x[4], c[4];
+        uint32_t raw[4], rawc[4];
         uint32_t r = r0;
-        if (r < p.runs) load(r, x, c);
+        if (r < p.runs) load(r, raw, rawc);
         while (r < p.runs) {
             const uint32_t next = searching ? p.runs : r + apart;
-            float nx[4], nc[4];
-            if (next < p.runs) load(next, nx, nc);
+            uint32_t nx[4], nc[4];
+            load(min(next, p.runs - 1), nx, nc);  // (past the last: not used)
+            float x[4], c[4];
+            const uint32_t i = r * kRun + lane * 4;
+            const bool edge = (r + 1) * kRun > p.width;
+            values4<BF16, VEC>(raw, i, p.width, edge, -__builtin_inff(), x);
+            values4<false, VEC>(rawc, i, p.width, edge, 0.0f, c);
+            if (!rest || !residual) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) c[e] = 0.0f;
+            }
             weights(x, v.most, by, w);
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
@@ -396,8 +423,8 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyPara
             r = next;
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
-                x[e] = nx[e];
-                c[e] = nc[e];
+                raw[e] = nx[e];
+                rawc[e] = nc[e];
             }
         }
         if (searching) break;  // wave 0 has the weights of the run found
@@ -546,11 +573,13 @@ int check(const ts_verify_args *a) {
 }
 
 template <bool BF16>
-int launch(const VerifyParams &p, hipStream_t stream) {
-    hipLaunchKernelGGL(verify_rows_kernel<BF16>, dim3(p.seqs * (p.most + 1) * p.parts), dim3(64 * kWaves), 0, stream, p);
+int launch(const VerifyParams &p, bool vec_x, bool vec_q, hipStream_t stream) {
+    const auto rows = vec_x ? verify_rows_kernel<BF16, true> : verify_rows_kernel<BF16, false>;
+    const auto draw = vec_x && vec_q ? verify_draw_kernel<BF16, true> : verify_draw_kernel<BF16, false>;
+    hipLaunchKernelGGL(rows, dim3(p.seqs * (p.most + 1) * p.parts), dim3(64 * kWaves), 0, stream, p);
     TS_CHECK_LAUNCH("verify rows launch");
     if (p.uniforms)
-        hipLaunchKernelGGL(verify_draw_kernel<BF16>, dim3(p.seqs * p.groups), dim3(64 * kDrawWaves), 0, stream, p);
+        hipLaunchKernelGGL(draw, dim3(p.seqs * p.groups), dim3(64 * kDrawWaves), 0, stream, p);
     else
         hipLaunchKernelGGL(verify_greedy_kernel<BF16>, dim3(p.seqs), dim3(256), 0, stream, p);
     TS_CHECK_LAUNCH("verify draw launch");
@@ -580,7 +609,9 @@ extern "C" int tessera_hip_verify(const ts_verify_args *a, void *stream) {
     const Cut c = cut(a);
     p.pieces = c.pieces; p.parts = c.parts; p.runs = c.runs; p.groups = c.groups;
     p.temperature = a->temperature;
-    p.whole_x = a->stride % 4 == 0 && ts::aligned(a->logits, a->logits_dtype == TS_BF16 ? 8 : 16);
-    p.whole_q = a->width % 4 == 0 && ts::aligned(a->draft_probs, 16);
-    return a->logits_dtype == TS_BF16 ? launch<true>(p, (hipStream_t)stream) : launch<false>(p, (hipStream_t)stream);
+    // Four consecutive logits, and probabilities, are one aligned load.
+    const bool bf16 = a->logits_dtype == TS_BF16;
+    const bool vec_x = a->width % 4 == 0 && a->stride % 4 == 0 && ts::aligned(a->logits, bf16 ? 8 : 16);
+    const bool vec_q = ts::aligned(a->draft_probs, 16);
+    return bf16 ? launch<true>(p, vec_x, vec_q, (hipStream_t)stream) : launch<false>(p, vec_x, vec_q, (hipStream_t)stream);
 }

@@ -134,6 +134,21 @@ def test_sequences_out_of_range_are_refused():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width,off_x,off_q", [(4096, 0, 1), (4096, 1, 0), (1028, 4, 4), (4, 0, 0), (2052, 2, 3)])
+def test_any_alignment(width, off_x, off_q, dtype):
+    """Logits and probabilities that begin anywhere; rows of whole fours and a last run that is not full."""
+    r = rng(width + off_x)
+    logits, drafts, u, counts, first, probs = problem(r, 6, 4, width, "probs")
+    x = torch.empty(logits.size + 8, dtype=dtype, device="cuda")[2 * off_x:][:logits.size].view(logits.shape)
+    q = torch.empty(probs.size + 4, device="cuda")[off_q:][:probs.size].view(probs.shape)
+    x.copy_(dev(logits))
+    q.copy_(dev(probs))
+    tokens, accepted = rules.verify(x, dev(drafts), dev(u), counts=dev(counts), first=dev(first), draft_probs=q)
+    want_t, want_a = K.verify(x.float().cpu().numpy(), drafts, u, counts=counts, first=first, probs=probs)
+    assert np.array_equal(accepted.cpu().numpy(), want_a) and np.array_equal(tokens.cpu().numpy(), want_t)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_apart(dtype):
     """Rows of a padded product (odd distance), and given outputs."""
     r = rng(7)
