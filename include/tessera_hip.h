@@ -340,7 +340,8 @@ typedef struct {
     uint32_t q_stride, k_stride, v_stride; /* elements from a row to the next, whole 16-byte pieces */
     uint32_t keys;                 /* positions a slot may hold */
     uint32_t slot_count, kept_pages;
-    uint32_t page, pages;          /* rows a page (power of two >= 16), pages the kept rows hold */
+    uint32_t page, pages;          /* rows a page (power of two >= 16), pages the kept rows hold (dense: a
+                                    * begun last one counted) */
     uint32_t rope_rows;            /* >= keys */
     int32_t halves;
     int32_t x_dtype, q_out_dtype;  /* f32 or bf16 */

@@ -464,6 +464,12 @@ def _slots(what, table, kept_pages, held, keys):
     return slots
 
 
+def _pages(table, held, page):
+    """Pages that `held` kept rows are; of dense ones, which no page divides, a begun last one too."""
+    page = max(page, 1)
+    return held // page if table is not None else -(-held // page)
+
+
 def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=None, k_gain=None, angles=None,
                 halves=True, eps=1e-6, scales=None, table=None, kept_pages=0, page=16, q_out=None, status=None):
     """New rows k, v [rows, kv_heads, 128] (views of a product's rows serve: only the rows' distance is
@@ -526,7 +532,8 @@ def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=
                        slots.data_ptr(), positions.data_ptr(), None if table is None else table.data_ptr(),
                        None if status is None else status.data_ptr(), rows, heads, kv_heads, width, q_stride,
                        k_stride, v_stride, keys, _slots(what, table, kept_pages, held, keys), kept_pages, page,
-                       held // max(page, 1), 0 if angles is None else angles.numel() // width, halves, _DT[x], q_type, kv, eps)
+                       _pages(table, held, page), 0 if angles is None else angles.numel() // width, halves, _DT[x],
+                       q_type, kv, eps)
     _call_on(on, abi.load().tessera_hip_append_rows, a)
     return q_out
 
@@ -563,7 +570,7 @@ def attend_kept8(q, k, v, scales, slots, positions, *, keys, scale, table=None, 
                                    keys, heads, kv_heads, width, back, kept_pages, page, scale, _DT[q.dtype],
                                    abi.TS_E4M3, _DT[out.dtype], max_position,
                                    None if status is None else status.data_ptr()),
-                      scales.data_ptr(), _slots(what, table, kept_pages, held, keys), held // max(page, 1), run)
+                      scales.data_ptr(), _slots(what, table, kept_pages, held, keys), _pages(table, held, page), run)
     lib = abi.load()
     need = lib.tessera_hip_attend_kept8_workspace(a)
     if need:
