@@ -501,7 +501,9 @@ int ts::kept_check(const char *rule, const uint32_t *table, uint32_t page, uint3
 }
 
 extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
-    TS_REQUIRE(a && a->k && a->v && a->k_kept && a->v_kept && a->slots && a->positions, "append_rows: null pointer");
+    TS_REQUIRE(a, "append_rows: null args");
+    const bool some = a->rows != 0;  // (what has an element a row may be NULL without rows)
+    TS_REQUIRE(a->k_kept && a->v_kept && (!some || (a->k && a->v && a->slots && a->positions)), "append_rows: null pointer");
     TS_REQUIRE(a->width == 128, "append_rows: head width %u (128 supported)", a->width);
     TS_REQUIRE(a->kv_heads >= 1 && a->kv_heads <= 1024, "append_rows: %u kv heads", a->kv_heads);
     TS_REQUIRE(a->x_dtype == TS_F32 || a->x_dtype == TS_BF16, "append_rows: rows f32 or bf16 supported");
@@ -524,7 +526,7 @@ extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
                "append_rows: k, v, kept rows and scales must be 16-byte aligned, the angle table 8");
     const bool q = a->q != nullptr;
     if (q) {
-        TS_REQUIRE(a->q_out, "append_rows: q without q_out");
+        TS_REQUIRE(a->q_out || !some, "append_rows: q without q_out");
         TS_REQUIRE(a->heads >= 1 && a->heads <= 16384, "append_rows: %u heads", a->heads);
         TS_REQUIRE(a->q_stride >= a->heads * 128 && a->q_stride % unit == 0,
                    "append_rows: q rows %u apart must hold %u heads and be whole 16-byte pieces", a->q_stride, a->heads);
@@ -533,7 +535,7 @@ extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
         TS_REQUIRE(a->q_out != a->q || (a->q_out_dtype == a->x_dtype && a->q_stride == a->heads * 128),
                    "append_rows: q in place needs rows back to back of the same type");
     }
-    if (a->rows == 0) return TS_OK;
+    if (!some) return TS_OK;
     AppendParams p;
     p.q = a->q; p.k = a->k; p.v = a->v; p.q_gain = a->q_gain; p.k_gain = a->k_gain;
     p.turns = (const float2 *)a->rope_table;

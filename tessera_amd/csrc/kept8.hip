@@ -405,7 +405,8 @@ size_t share_bytes(const Plan &s) { return s.most <= 1 ? 0 : (size_t)s.tiles * 2
 int check(const ts_kept8_args *k) {
     TS_REQUIRE(k, "attend_kept8: null args");
     const ts_rows_args *a = &k->rows;
-    TS_REQUIRE(a->q && a->k && a->v && a->out && a->slots && a->positions && k->scales, "attend_kept8: null pointer");
+    TS_REQUIRE(a->k && a->v && k->scales && (a->rows == 0 || (a->q && a->out && a->slots && a->positions)),
+               "attend_kept8: null pointer");
     TS_REQUIRE(a->width == 128, "attend_kept8: head width %u (128 supported)", a->width);
     TS_REQUIRE(a->kv_heads >= 1 && a->kv_heads <= 1024 && a->heads >= 1 && a->heads % a->kv_heads == 0 &&
                    a->heads / a->kv_heads <= 64,

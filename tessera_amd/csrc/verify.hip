@@ -558,8 +558,9 @@ Sizes sizes(const ts_verify_args *a) {
 }
 
 int check(const ts_verify_args *a) {
-    TS_REQUIRE(a && a->logits && a->tokens && a->accepted, "verify: null pointer");
-    TS_REQUIRE(a->drafts || a->most == 0, "verify: null pointer");
+    TS_REQUIRE(a, "verify: null args");
+    TS_REQUIRE(a->seqs == 0 || ((a->logits || a->rows == 0) && a->tokens && a->accepted && (a->drafts || a->most == 0)),
+               "verify: null pointer");
     TS_REQUIRE(a->most <= kMostDrafts, "verify: %u drafts a sequence (at most %u)", a->most, kMostDrafts);
     TS_REQUIRE(a->logits_dtype == TS_F32 || a->logits_dtype == TS_BF16, "verify: logits f32 or bf16 supported");
     TS_REQUIRE(a->width >= 1 && a->width <= 1u << 28 && a->stride >= a->width, "verify: rows of %u logits, %u apart",

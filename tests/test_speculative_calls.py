@@ -1,0 +1,39 @@
+"""CPU checks of calls of the 8-bit cache's operators: what is empty, what is refused, where a call goes."""
+import ctypes as C
+
+import pytest
+
+from tessera_amd import abi
+from test_kept8_ref import FAKE, _append, _attend, _no_gpu, _verify
+
+torch = pytest.importorskip("torch")
+
+
+def test_no_rows_and_no_sequences_need_no_pointers():
+    """Tensors without elements have no address."""
+    _no_gpu()
+    lib = abi.load()
+    none = dict.fromkeys(("q", "k", "v", "q_out", "slots", "positions"))
+    assert lib.tessera_hip_append_rows(C.byref(_append(rows=0, **none)), None) == abi.TS_OK
+    assert lib.tessera_hip_append_rows(C.byref(_append(rows=0, **dict(none, q=FAKE))), None) == abi.TS_OK
+    a = _attend(rows=0, q=None, out=None, slots=None, positions=None)
+    assert lib.tessera_hip_attend_kept8_workspace(C.byref(a)) == 0
+    assert lib.tessera_hip_attend_kept8(C.byref(a), None) == abi.TS_OK
+    for uniforms in (None, FAKE):
+        a = _verify(seqs=0, drafts=None, tokens=None, accepted=None, uniforms=uniforms, workspace=None)
+        assert lib.tessera_hip_verify_workspace(C.byref(a)) == 0
+        assert lib.tessera_hip_verify(C.byref(a), None) == abi.TS_OK
+        a.rows, a.logits = 0, None
+        assert lib.tessera_hip_verify(C.byref(a), None) == abi.TS_OK
+
+
+def test_arguments_of_no_rows_are_still_checked():
+    _no_gpu()
+    lib = abi.load()
+    assert lib.tessera_hip_append_rows(C.byref(_append(rows=0, width=64)), None) == abi.TS_ERR_ARG
+    assert lib.tessera_hip_append_rows(C.byref(_append(rows=0, k_kept=None)), None) == abi.TS_ERR_ARG
+    assert lib.tessera_hip_attend_kept8(C.byref(_attend(rows=0, page=20)), None) == abi.TS_ERR_ARG
+    assert lib.tessera_hip_verify(C.byref(_verify(seqs=0, width=0)), None) == abi.TS_ERR_ARG
+    assert lib.tessera_hip_verify(C.byref(_verify(logits=None)), None) == abi.TS_ERR_ARG
+    for fn in (lib.tessera_hip_append_rows, lib.tessera_hip_attend_kept8, lib.tessera_hip_verify):
+        assert fn(None, None) == abi.TS_ERR_ARG
