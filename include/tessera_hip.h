@@ -321,8 +321,9 @@ int tessera_hip_flash_rows(const ts_rows_args *a, void *stream);
  *  - Rows of one call that fall into one block (16 positions of a slot) stand together and in
  *    order; a later run of rows of the same block is kept nowhere and sets TS_STATUS_TWICE. Two
  *    slots of a call never share the page they append to (Pool::grow sees to it).
- *  - A row past its slot's positions is kept nowhere (its q is NaN) and sets
- *    TS_STATUS_POSITION, one whose page the buffers do not hold TS_STATUS_PAGE.
+ *  - A row past its slot's positions (or its table's pages) is kept nowhere and sets TS_STATUS_POSITION,
+ *    one of a slot or page that the buffers do not hold TS_STATUS_PAGE. The q of both is NaN. That of a
+ *    row refused as TS_STATUS_TWICE is as ever: only `status` tells of it.
  * No counterpart in the reference (its append follows separate norm and rotation stages,
  * engine/models/src/shared.rs:109-145, engine/ir/interp/src/run.rs:122-198). */
 typedef struct {

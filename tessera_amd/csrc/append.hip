@@ -388,9 +388,10 @@ __global__ __launch_bounds__(64 * kWaves, KEPT8 ? 4 : 5) void append_kernel(Appe
         for (uint32_t i = 0; i < kQRows; i++) {
             if (i >= n) continue;
             load8<XBF16, HALVES>(row_base<XBF16>(p.q, r0 + i, p.q_stride), h * 128, l, v[i]);
-            const uint32_t pos = p.positions[r0 + i];
-            held[i] = pos < p.place.keys;
-            if (p.turns) load_turns(p.turns + (held[i] ? (size_t)pos * 64 : 0), 0, l, cs[i]);
+            const uint32_t slot = p.slots[r0 + i], pos = p.positions[r0 + i];
+            if (p.turns) load_turns(p.turns + (pos < p.place.keys ? (size_t)pos * 64 : 0), 0, l, cs[i]);
+            uint64_t row;  // (its page is asked for beside the angles)
+            held[i] = holds(p.place, slot, pos) && row_of(p.place, slot, pos, row);
         }
         if (p.q_gain) load_gain<HALVES>(p.q_gain, l, gain);
 #pragma unroll

@@ -476,8 +476,10 @@ def append_rows(k, v, k_kept, v_kept, slots, positions, *, keys, q=None, q_gain=
     free) into the kept rows, q [rows, heads, 128] rotated to q_out (of q's type unless given). With
     gains q / k pass through RmsNorm, with `angles` (rope_table's, at least `keys` positions) through the
     rotation. `scales` given: k_kept, v_kept are kept8() blocks; else bf16 rows [*, kv_heads, 128].
-    Rows of one call that fall into one block of 16 positions stand together, in order. status: int32
-    device word, TS_STATUS_* bits of rows that were not kept. Returns q_out."""
+    Rows of one call that fall into one block of 16 positions stand together, in order; later ones that do
+    not are kept nowhere, which only status tells. Rows without a place (position, slot or page) are kept
+    nowhere and their q is NaN. status: int32 device word, TS_STATUS_* bits of rows that were not kept.
+    Returns q_out."""
     what = "append_rows"
     rows, kv_heads, width = shape = k.shape
     on, x = k.get_device(), k.dtype

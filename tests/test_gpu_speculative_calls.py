@@ -39,3 +39,42 @@ def test_sequences_without_a_row_of_logits_are_refused():
         tokens, accepted = rules.verify(torch.empty(0, 50, device="cuda"), torch.zeros(2, 1, dtype=torch.int32, device="cuda"),
                                         uniforms, counts=one, first=one, status=status)
         assert tokens.tolist() == [[50, 50]] * 2 and accepted.tolist() == [0, 0] and int(status) == abi.TS_STATUS_POSITION
+
+
+@pytest.mark.parametrize("many", [0, 1200])
+@pytest.mark.parametrize("kept", ["e4m3", "bf16"])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_q_of_rows_without_a_place_is_nan(out, kept, many):
+    """Positions past the slot or past its table's pages, slots and pages that are not there: kept nowhere, q NaN;
+    the rows beside them, and one refused for meeting a block twice, have theirs."""
+    r = rng(3 + many)
+    page, each, kvh, heads = 16, 3, 2, 5
+    table = np.array([0, 1, 2, 3, 99, 5], np.int32)  # slot 1's second page does not exist
+    slots = np.array([0, 0, 1, 2, 0, 0, 1, 0, 0xFFFFFFFF], np.uint32).astype(np.int32)
+    # 60 and 47 + 1 are within `keys` but not within the table's three pages.
+    positions = np.array([46, 47, 17, 3, 48, 60, 40, 45, 3], np.int32)
+    bad = np.array([0, 0, 1, 1, 1, 1, 0, 0, 1], bool)
+    bits = abi.TS_STATUS_POSITION | abi.TS_STATUS_PAGE | abi.TS_STATUS_TWICE
+    # Beyond 1024 rows a wave takes four of them: others, of a slot that is not there, before these.
+    slots, positions = np.append(np.full(many, 7, np.int32), slots), np.append(np.zeros(many, np.int32), positions)
+    bad = np.append(np.ones(many, bool), bad)
+    n = len(slots)
+    x = dev(r.standard_normal((n, heads + 2 * kvh, 128)).astype(np.float32))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    if kept == "e4m3":
+        k, v, scales = rules.kept8(6, kvh)
+    else:
+        k, v, scales = *(torch.zeros(96, kvh, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)), None
+    angles = rules.rope_table(64, 1e4)
+    q_out = torch.empty(n, heads, 128, dtype=out, device="cuda")
+    q = rules.append_rows(x[:, heads:heads + kvh], x[:, heads + kvh:], k, v, dev(slots), dev(positions), q=x[:, :heads],
+                          keys=64, scales=scales, table=dev(table), kept_pages=each, page=page, status=status,
+                          angles=angles, q_out=q_out)
+    assert int(status) == bits
+    got = q.double().cpu().numpy()
+    assert np.isnan(got[bad]).all()
+    want = K.turned(x[:, :heads].cpu().numpy(), None, angles.cpu().numpy(), np.where(bad, 0, positions), True, 0)
+    size = np.abs(want).max(-1, keepdims=True)
+    # Three f32 steps of the rotation (2^-24 each of the pair's size), and the rounding of bf16.
+    slack = size * 2.0 ** -21 + np.abs(want) * (2.0 ** -8 if out == torch.bfloat16 else 0)
+    assert np.all((np.abs(got - want) <= slack)[~bad])
