@@ -569,7 +569,8 @@ int check(const ts_verify_args *a) {
                a->seqs, a->most + 1, a->rows);
     TS_REQUIRE((uint64_t)a->seqs * (a->most + 1) * ((a->width + kPiece - 1) / kPiece) <= 0x7fffffffull,
                "verify: %u sequences in one launch", a->seqs);
-    TS_REQUIRE(ts::aligned(a->logits, 4), "verify: logits must be 4-byte aligned");
+    const uint32_t one = a->logits_dtype == TS_BF16 ? 2 : 4;
+    TS_REQUIRE(ts::aligned(a->logits, one), "verify: logits must be %u-byte aligned", one);
     return TS_OK;
 }
 

@@ -78,3 +78,23 @@ def test_q_of_rows_without_a_place_is_nan(out, kept, many):
     # Three f32 steps of the rotation (2^-24 each of the pair's size), and the rounding of bf16.
     slack = size * 2.0 ** -21 + np.abs(want) * (2.0 ** -8 if out == torch.bfloat16 else 0)
     assert np.all((np.abs(got - want) <= slack)[~bad])
+
+
+@pytest.mark.parametrize("width,off,apart", [(4096, 1, 4097), (777, 3, 777), (1028, 5, 1031), (1, 1, 1)])
+@pytest.mark.parametrize("greedy", [False, True])
+def test_bf16_logits_at_odd_elements(width, off, apart, greedy):
+    """Rows of bf16 logits that begin at an odd element, whole fours wide or not."""
+    r = rng(width + off)
+    seqs, most = 4, 3
+    rows = seqs * (most + 1)
+    held = torch.full((off + rows * apart,), 60.0, dtype=torch.bfloat16, device="cuda")
+    x = held[off:].view(rows, apart)[:, :width]
+    x.copy_(dev((3 * r.standard_normal((rows, width))).astype(np.float32)))
+    assert x.data_ptr() % 4 == 2
+    at = x.float().cpu().numpy()
+    drafts = at.argmax(-1).reshape(seqs, most + 1)[:, :most].astype(np.int32)
+    drafts[1, 1] = (drafts[1, 1] + 1) % width
+    u = None if greedy else r.random((seqs, most + 1)).astype(np.float32)
+    tokens, accepted = rules.verify(x, dev(drafts), None if greedy else dev(u))
+    want_t, want_a = K.verify(at, drafts, u)
+    assert np.array_equal(accepted.cpu().numpy(), want_a) and np.array_equal(tokens.cpu().numpy(), want_t)

@@ -37,3 +37,13 @@ def test_arguments_of_no_rows_are_still_checked():
     assert lib.tessera_hip_verify(C.byref(_verify(logits=None)), None) == abi.TS_ERR_ARG
     for fn in (lib.tessera_hip_append_rows, lib.tessera_hip_attend_kept8, lib.tessera_hip_verify):
         assert fn(None, None) == abi.TS_ERR_ARG
+
+
+def test_bf16_logits_may_begin_at_any_element():
+    """f32 logits at any f32, bf16 ones at any bf16: past the alignment, the workspace is what is asked for."""
+    _no_gpu()
+    lib = abi.load()
+    for dtype, at, want in ((abi.TS_BF16, 2, abi.TS_ERR_WORKSPACE), (abi.TS_BF16, 1, abi.TS_ERR_ARG),
+                            (abi.TS_F32, 4, abi.TS_ERR_WORKSPACE), (abi.TS_F32, 2, abi.TS_ERR_ARG)):
+        a = _verify(logits=FAKE + at, logits_dtype=dtype, workspace=None)
+        assert lib.tessera_hip_verify(C.byref(a), None) == want
