@@ -566,7 +566,8 @@ def attend_kept8(q, k, v, scales, slots, positions, *, keys, scale, table=None, 
                  ("scales", scales, _F32, -1), ("slots", slots, _INTS, rows), ("positions", positions, _INTS, rows),
                  ("table", table, _INTS, -1), ("out", out, _ROWS, -1), ("status", status, _INTS, -1))
     if max_position is None:
-        max_position = int(positions.max().item()) if rows else 0
+        # (as int32, which has a maximum; a position from 2^31 on is past any slot's)
+        max_position = int(positions.view(torch.int32).max().item()) if rows else 0
     a = abi.Kept8Args(abi.RowsArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), slots.data_ptr(),
                                    positions.data_ptr(), None if table is None else table.data_ptr(), None, 0, rows,
                                    keys, heads, kv_heads, width, back, kept_pages, page, scale, _DT[q.dtype],

@@ -98,3 +98,21 @@ def test_bf16_logits_at_odd_elements(width, off, apart, greedy):
     tokens, accepted = rules.verify(x, dev(drafts), None if greedy else dev(u))
     want_t, want_a = K.verify(at, drafts, u)
     assert np.array_equal(accepted.cpu().numpy(), want_a) and np.array_equal(tokens.cpu().numpy(), want_t)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.uint32])
+def test_positions_of_either_type_without_a_stated_bound(dtype):
+    """Their maximum is found of int32 and uint32 positions, beside rows that are refused (2^32 - 1)."""
+    r = rng(31)
+    k8, v8, s8 = rules.kept8(4, 1)
+    x = dev(r.standard_normal((64, 1, 128)).astype(np.float32))
+    i = torch.arange(64, dtype=torch.int32, device="cuda")
+    rules.append_rows(x, x, k8, v8, torch.zeros_like(i), i, keys=64, scales=s8)
+    q = dev(r.standard_normal((3, 2, 128)).astype(np.float32))
+    slots = torch.zeros(3, dtype=torch.int32, device="cuda")
+    positions = torch.tensor([63, -1, 5], dtype=torch.int32, device="cuda")
+    want = rules.attend_kept8(q, k8, v8, s8, slots, positions, keys=64, scale=0.1, max_position=63)
+    got = rules.attend_kept8(q, k8, v8, s8, slots.view(dtype), positions.view(dtype), keys=64, scale=0.1)
+    assert torch.isnan(got[1]).all() and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    got = rules.attend_kept8(q[1:2], k8, v8, s8, slots[:1].view(dtype), positions[1:2].view(dtype), keys=64, scale=0.1)
+    assert torch.isnan(got).all()
