@@ -199,7 +199,8 @@ def copy_pages(buffers, copies, *, page, pages, status=None, check=True):
     a.buffer_count, a.copy_count, a.page, a.pages = len(buffers), len(copies), page, pages
     a.row_bytes = buffers[0][0].numel() * buffers[0].element_size()
     a.status = status.data_ptr() if status is not None else None
-    rc = lib().tessera_hip_kv_copy(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    with torch.cuda.device(dev):  # its stream, whichever device is current
+        rc = lib().tessera_hip_kv_copy(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream))
     abi.check(rc, "tessera_hip_kv_copy")
 
 

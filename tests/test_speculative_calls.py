@@ -47,3 +47,36 @@ def test_bf16_logits_may_begin_at_any_element():
                             (abi.TS_F32, 4, abi.TS_ERR_WORKSPACE), (abi.TS_F32, 2, abi.TS_ERR_ARG)):
         a = _verify(logits=FAKE + at, logits_dtype=dtype, workspace=None)
         assert lib.tessera_hip_verify(C.byref(a), None) == want
+
+
+def test_page_copies_go_to_the_buffers_device(monkeypatch):
+    """The copies of kept blocks (and kept rows) run on the stream of the device that holds them, whichever device is
+    current: the launch is made under that device."""
+    from tessera_amd import kv, rules
+    under, launched = [], []
+
+    class Device:
+        def __init__(self, on):
+            self.on = on
+
+        def __enter__(self):
+            under.append(self.on)
+
+        def __exit__(self, *_):
+            under.pop()
+
+    class Stream:
+        cuda_stream = 64
+
+    class Library:
+        def tessera_hip_kv_copy(self, args, stream):
+            launched.append((list(under), stream.value))
+            return abi.TS_OK
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: Stream)
+    monkeypatch.setattr(kv, "lib", Library)
+    k8, v8, s8 = rules.kept8(4, 2, device="cpu")
+    kv.copy_kept8(k8, v8, s8, [(0, 3, 5)], page=16)
+    kv.copy_pages([torch.zeros(64, 2, 128)], [(1, 2, 16)], page=16, pages=4)
+    assert launched == [([torch.device("cpu")], 64)] * 3 and not under
