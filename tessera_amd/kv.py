@@ -207,7 +207,11 @@ def copy_pages(buffers, copies, *, page, pages, status=None, check=True):
 def copy_kept8(k, v, scales, copies, *, page, status=None):
     """Pool.grow's copies over kept8() blocks, in stream order: whole pages (a block's positions share
     their scales, so a page copies with all of them). copies: [(from, to, rows), ...]."""
-    pages = k.shape[0] * 16 // page
+    each = page // 16  # blocks a page; those past the last whole page are nobody's
+    if each < 1 or page % 16:
+        raise ValueError(f"copy_kept8: pages of {page} rows are not whole blocks of 16")
+    pages = k.shape[0] // each
+    k, v, scales = (t[:pages * each].view(pages, -1) for t in (k, v, scales))
     whole = [(f, t, 1) for f, t, _ in copies]
-    copy_pages([k.view(pages, -1), v.view(pages, -1)], whole, page=1, pages=pages, status=status)
-    copy_pages([scales.view(pages, -1)], whole, page=1, pages=pages, status=status)
+    copy_pages([k, v], whole, page=1, pages=pages, status=status)
+    copy_pages([scales], whole, page=1, pages=pages, status=status)

@@ -80,3 +80,17 @@ def test_page_copies_go_to_the_buffers_device(monkeypatch):
     kv.copy_kept8(k8, v8, s8, [(0, 3, 5)], page=16)
     kv.copy_pages([torch.zeros(64, 2, 128)], [(1, 2, 16)], page=16, pages=4)
     assert launched == [([torch.device("cpu")], 64)] * 3 and not under
+
+
+@pytest.mark.parametrize("blocks,page,want", [(5, 32, (2, 8192)), (8, 64, (2, 16384)), (3, 16, (3, 4096))])
+def test_copied_pages_are_whole_blocks(monkeypatch, blocks, page, want):
+    """A page is page / 16 blocks, however many blocks are left over; pages that are not blocks are refused."""
+    from tessera_amd import kv, rules
+    copied = []
+    monkeypatch.setattr(kv, "copy_pages", lambda buffers, copies, **kw: copied.extend((tuple(b.shape), kw["pages"]) for b in buffers))
+    k8, v8, s8 = rules.kept8(blocks, 2, device="cpu")
+    kv.copy_kept8(k8, v8, s8, [(0, 1, 7)], page=page)
+    assert copied == [(want, want[0])] * 2 + [((want[0], page // 16 * 4), want[0])]
+    for bad in (24, 8, 0):
+        with pytest.raises(ValueError, match="whole blocks"):
+            kv.copy_kept8(k8, v8, s8, [(0, 1, 7)], page=bad)
