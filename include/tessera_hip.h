@@ -580,8 +580,10 @@ int tessera_hip_top_k(const ts_top_k_args *a, void *stream);
  * NaN and -inf logits have probability 0; a row of nothing else refuses its draft and picks
  * `width`. +inf logits share the whole. Probabilities of the drafter that are NaN or negative
  * count as 0. A sequence with counts[s] > most or rows past `rows` gets accepted 0 and `width`
- * throughout, and sets TS_STATUS_POSITION. Exponentials and sums are in f64: over a vocabulary
- * of 150,000 the running sum's borders in f32 would move by more than they are apart.
+ * throughout, and sets TS_STATUS_POSITION.
+ * Sums are in f64, exponentials within 1.1e-10 of their value. A border of the running sum is thus off
+ * by at most 2.2e-10 of Z (over 150,000 logits by 6e-12, which decides about one draw in two million),
+ * and a draft is judged as by the exact form unless u q / p is within 2.2e-10 of 1.
  * No counterpart in the reference (its engine decodes greedily, one token a step,
  * engine/engine/src/lib.rs:401-470). */
 typedef struct {

@@ -15,8 +15,10 @@
 //      whole, and one wave the index in it.
 // Code that runs once costs its fetch (about 1 KiB a microsecond), so nothing here is unrolled or inlined
 // twice that need not be.
-// Exponentials and sums are in f64 (the vector unit's f64 rate is f32's here): the draw compares u with
-// running sums whose borders lie 1 / 150,000 apart and closer, and f32 would move them by 1e-7 of the whole.
+// Sums are in f64 and exponentials good to 33 bits (the vector unit's f64 rate is f32's here): the draw compares u
+// with running sums. Over rows of 151936 logits the exponentials' error moves their borders by up to 6e-12 of the
+// whole and, all borders together, decides about one draw in two million; f32 exponentials would move them by up to
+// 2e-8 and decide one draw in a thousand.
 // They bound the kernels (16 vector operations a logit), beside HBM: 32 sequences of up to 4 drafts with the
 // drafter's probabilities, 151936 f32 logits a row: rows 19 us, draw 16; one greedy sequence of 4 drafts: 4 and 3 us.
 #include <algorithm>

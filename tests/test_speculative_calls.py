@@ -94,3 +94,36 @@ def test_copied_pages_are_whole_blocks(monkeypatch, blocks, page, want):
     for bad in (24, 8, 0):
         with pytest.raises(ValueError, match="whole blocks"):
             kv.copy_kept8(k8, v8, s8, [(0, 1, 7)], page=bad)
+
+
+def test_the_stated_error_of_the_verifications_exponentials():
+    """verify.hip's series for 2^f, its coefficients read from the source, against longdouble exponentials: at most
+    1.1e-10 off, 2^0 exact; and what that does to the borders of a wide row's running sum."""
+    import os
+    import re
+
+    import numpy as np
+    with open(os.path.join(os.path.dirname(abi.__file__), "csrc", "verify.hip")) as f:
+        source = f.read()
+    body = source[source.index("TS_DEV double exp2_neg"):source.index("TS_DEV void weights")]
+    magic, same, *series = (float(c) for c in re.findall(r"scalar\(([\d.e+-]+)\)", body))
+    assert magic == same == 1.5 * 2 ** 52 and len(series) == 7
+
+    def exp2(t):
+        n = (t + magic) - magic
+        f, r = t - n, np.float64(series[0])
+        for c in series[1:]:
+            r = r * f + c
+        return np.ldexp(r * f + 1.0, n.astype(int))
+
+    t = np.linspace(-3, 0, 3000001)
+    exact = np.exp2(t.astype(np.longdouble))
+    assert np.max(np.abs(exp2(t) / exact - 1)) < 1.101e-10 and exp2(np.zeros(1))[0] == 1.0
+    r = np.random.default_rng(1)
+    for temperature in (0.75, 1.0, 1.25):
+        x = 2 * r.standard_normal(151936)
+        x[r.integers(0, len(x), 24)] = 9 + 3 * r.standard_normal(24)
+        y = (x - x.max()) * (np.log2(np.e) / temperature)
+        a, b = exp2(y).astype(np.longdouble), np.exp2(y.astype(np.longdouble))
+        moved = np.abs(np.cumsum(a) / a.sum() - np.cumsum(b) / b.sum())
+        assert moved.max() < 6e-12 and moved.sum() < 6e-7
