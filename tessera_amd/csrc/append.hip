@@ -129,7 +129,7 @@ TS_DEV float to_odd(double d) {
     const uint32_t high = (uint32_t)(off >> 32), u = __float_as_uint(f);
     const uint32_t inexact = min((high & 0x7fffffffu) | (uint32_t)off, 1u), away = (high ^ u) >> 31;
     const uint32_t odd = (u - (away & inexact)) | inexact;
-    return fabsf(f) < __builtin_inff() ? __uint_as_float(odd) : f;
+    return fabs(d) < __builtin_inf() ? __uint_as_float(odd) : f;  // (past f32's range its largest, cut off)
 }
 template <bool HALVES>
 TS_DEV void norm_turn8(float (&v)[8], bool norm, const float (&gain)[8], float eps, bool turn, const f32x4 (&cs)[2]) {

@@ -116,3 +116,30 @@ def test_positions_of_either_type_without_a_stated_bound(dtype):
     assert torch.isnan(got[1]).all() and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
     got = rules.attend_kept8(q[1:2], k8, v8, s8, slots[:1].view(dtype), positions[1:2].view(dtype), keys=64, scale=0.1)
     assert torch.isnan(got).all()
+
+
+@pytest.mark.parametrize("one", [True, False])
+@pytest.mark.parametrize("halves", [True, False])
+def test_values_that_pass_f32_on_the_way_to_their_codes(one, halves):
+    """A rotation (or a gain) that takes finite values past f32's range: as the formula has it, the largest code of
+    the largest scale, of their sign, and no NaN; what was infinite or NaN before is a NaN code."""
+    r = rng(41)
+    n = 1 if one else 16
+    x = (r.standard_normal((n, 1, 128)) * 1e30).astype(np.float32)
+    pairs = ([3, 67], [5, 69]) if halves else ([6, 7], [10, 11])
+    x[:, 0, pairs[0]] = 3.3e38, -3.3e38
+    x[:, 0, pairs[1]] = -3.3e38, 3.3e38
+    x[0, 0, 20], x[-1, 0, 31] = np.inf, np.nan
+    turn = np.zeros((16, 64, 2), np.float32)
+    turn[...] = np.sqrt(0.5)
+    i = np.arange(n, dtype=np.int32)
+    k8, v8, s8 = rules.kept8(1, 1)
+    rules.append_rows(dev(x), dev(x), k8, v8, dev(np.zeros(n, np.int32)), dev(i), keys=16, scales=s8, angles=dev(turn),
+                      halves=halves)
+    blocks, scales = np.zeros((1, 1, 16, 128), np.uint8), np.zeros((1, 2, 2))
+    want = K.turned(x, None, turn, i, halves, 0)
+    assert np.abs(want[np.isfinite(want)]).max() > np.finfo(np.float32).max
+    K.append(blocks, scales, 0, want, np.zeros(n), i, keys=16)
+    got = k8.cpu().numpy()
+    assert s8[0, 0, 0].item() == scales[0, 0, 0] == 2.0 ** 119
+    assert np.array_equal(K.CODES[got], K.CODES[blocks], equal_nan=True) and np.isnan(K.CODES[got[0, 0, :n]]).sum() == 4
