@@ -354,11 +354,12 @@ int tessera_hip_append_rows(const ts_append_args *a, void *stream);
 /* Ragged-row attention over kept blocks: attend_rows' and flash_rows' semantics (row r sees keys
  * [max(0, p - back), p] of its slot), q f32 or bf16, out f32 or bf16. rows.k, rows.v: the
  * blocks; rows.kv_dtype TS_E4M3. Codes enter the products exactly, times their scale; sums and
- * softmax in f32; f32 q and, with f32 q, the softmax weights enter as three bf16 parts (24 bits),
- * with bf16 q the weights as one.
+ * softmax in f32; f32 q and, with f32 q, the softmax weights enter as three bf16 parts (24 bits).
+ * With bf16 q the weights enter as two (16 bits) where `run` rows have up to 16 q heads of a kv head
+ * between them (decode rows, a few drafts), else as one.
  *  - `run`: how many rows of a slot stand together (1: a decode step; the drafted rows of a
  *    sequence; a prompt chunk's rows; an average serves for ragged ones). It decides how rows are
- *    grouped and which kernel runs, never what is computed. How the keys are divided follows from the
+ *    grouped and which kernel runs, never which keys a row sees. How the keys are divided follows from the
  *    rows of the call and their positions, so a row's last bits may depend on the rows beside it;
  *    the same call gives the same bits.
  *  - Refused rows (a position as for attend_rows; a slot >= slot_count; a page >= pages among the

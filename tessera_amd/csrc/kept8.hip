@@ -32,7 +32,10 @@ constexpr uint32_t kRound = kStep * kWaves;  // keys of a group's waves at a tim
 
 template <bool QF32>
 __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
-    constexpr uint32_t kCols = 16, kParts = QF32 ? 3 : 1;
+    // The weights of bf16 q in two parts (16 bits): in one the outputs' error against 64 bits is 2.3e-3 of them, in two
+    // 1.6e-3, what rounding them to bf16 makes; the keys' bytes hide most of it (2 rows of 131000 keys 58.1 -> 58.4 us,
+    // 32 of 8192 65.2 -> 65.9, 8 of 4096 17.9 -> 18.5).
+    constexpr uint32_t kCols = 16, kParts = QF32 ? 3 : 1, kWeights = QF32 ? 3 : 2;
     extern __shared__ __attribute__((aligned(16))) float joined[];  // [kWaves][kCols][kPart]
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4;
@@ -224,8 +227,8 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
                         }
                     }
                 }
-                bf16x8 w[2][kParts];
-                weigh<kParts, 8>(sc, sl, m, l, o, w);
+                bf16x8 w[2][kWeights];
+                weigh<kWeights, 8>(sc, sl, m, l, o, w);
 #pragma unroll
                 for (int dt = 0; dt < 8; dt++) {
                     pin(vf[dt]);
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(256, 2) void attend_kept8_kernel(AttendParams p) {
                     for (int x = 0; x < 2; x++) {
                         const bf16x8 vc = codes8(x ? vf[dt].z : vf[dt].x, x ? vf[dt].w : vf[dt].y, vs);
 #pragma unroll
-                        for (uint32_t e = 0; e < kParts; e++) o[dt] = mfma16(vc, w[x][e], o[dt]);
+                        for (uint32_t e = 0; e < kWeights; e++) o[dt] = mfma16(vc, w[x][e], o[dt]);
                     }
                 }
                 load_v();

@@ -83,7 +83,7 @@ TS_DEV uint32_t within4(uint32_t w, uint32_t pos, uint32_t lo, uint32_t hi) {
 TS_DEV uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(ts_f32x2{a, b}, ts_bf16x2));
 }
-// P parts of two f32 values: bf16 values that add up to them (24 bits in three parts, 8 in one).
+// P parts of two f32 values: bf16 values that add up to them (24 bits in three parts, 16 in two, 8 in one).
 template <uint32_t P>
 TS_DEV void split_pair(float a, float b, uint32_t (&w)[P]) {
 #pragma unroll
@@ -217,7 +217,7 @@ TS_DEV uint32_t seen_keys(uint32_t key0, uint32_t from, uint32_t pos) {
 }
 
 // The softmax of one column over a step's 64 keys: the lane's 16 raw scores (scaled by sl > 0 to base 2,
-// -inf where masked) to weights 2^(score - m) in kParts bf16 parts, as the second product takes them
+// -inf where masked) to weights 2^(score - m) in P bf16 parts, as the second product takes them
 // (operand x: positions 8 x .. 8 x + 7 of the lane's block). m moves only when a score passes it by
 // 2^kSlack, so most steps leave the sum and O as they are and no weight passes 2^kSlack; l adds up the
 // lane's own keys. O (NO tiles) is rescaled when some column of the wave moved.

@@ -199,3 +199,18 @@ def test_calls_on_two_streams(form, name, dtype):
                 got.append(kept.attend(q, slots, positions, run=run))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(alone, got))
+
+
+@pytest.mark.parametrize("heads,kvh,run", [(1, 1, 1), (16, 8, 1), (32, 2, 1), (8, 2, 4), (6, 2, 5)])
+def test_weights_of_bf16_decode_rows_hold_16_bits(heads, kvh, run):
+    """Tiles of up to 16 columns, f32 out: bf16 q's weights are off by half a step of two bf16 parts (2^-8 2^-8) where
+    one would be off by 2^-8."""
+    r = rng(heads + run)
+    kept = Kept(r, [5, 40, 700, 3000], kvh)
+    slots = np.repeat(np.arange(4), run)
+    positions = np.concatenate([n - run + np.arange(run) for n in (5, 40, 700, 3000)])
+    q = dev(r.standard_normal((len(slots), heads, 128)).astype(np.float32), torch.bfloat16)
+    out = kept.attend(q, slots, positions, run=run, out_dtype=torch.float32)
+    want, spread, size = kept.exact(q, slots, positions)
+    bound = (2 * spread * 4 * 2.0 ** -21 + 2.0 ** -20 + 2.0 ** -16) * size
+    assert bool(((out.double() - want).abs() <= bound[..., None]).all())
