@@ -373,21 +373,23 @@ Plan plan(const ts_kept8_args *k) {
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
     const uint64_t wanted = (uint64_t)run * G;
     // f32 q, in three parts, leaves a wave of the shared kernel 16 columns. 256 columns widen the codes for fewer
-    // waves twice, but fill a CU with one group: only where there are two groups a CU in turn to even them out
-    // (4 prompts of 2048 rows, 8 kv heads: 106 us, 128 columns 124; 2 such prompts 79 us, 128 columns 73).
+    // waves twice, but fill a CU with one group: only where there are one and a half groups a CU to even them out
+    // (prompts of 2048 rows, 16 heads over 8: 4 of them 105 us, 128 columns 119; 3, the border, 81 and 92; 2 81 and
+    // 75. Between one and one and a half groups either may win: 3 of 1600 86 and 64, 9 of 512 36 and 41.)
     const uint64_t wide = (a->rows + 256 / G - 1) / (256 / G) * (uint64_t)a->kv_heads;
-    s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 || wide < 512 ? 128 : 256;
+    s.columns = wanted <= 16 ? 16 : wanted <= 64 ? 64 : wanted <= 128 || f32 || wide < 384 ? 128 : 256;
     s.tile_rows = std::min(run, s.columns / G);
     s.tiles = (a->rows + s.tile_rows - 1) / s.tile_rows;
     s.groups = s.tiles;
     s.most = 1;
     // Keys are shared out over as many groups as run at once (a CU's two of four waves, with 64 columns of bf16 q
     // three, or one of eight): more would each cost 8 us before the first step is done, fewer leave CUs idle.
-    // Decode rows and drafts always (32 sequences of 512 .. 8192, 8 kv heads: 68 us; equal parts of every tile's
-    // longest span 78, a group a tile 106), beyond the groups at once too (128 of up to 4096: 128 us, a group a
-    // tile 137). Wide tiles, whose partial results are large, only where there are fewer tiles than groups (3
-    // chunks of up to 700 f32 rows: 85 us, a group a tile 137; but 4 prompts of 2048 rows 168 us, a group a tile,
-    // the widest first, 112; before LDS was read ahead).
+    // Up to 64 columns always: 32 sequences of 512 .. 8192, 8 kv heads, 68 us, a group a tile 116; 24 x 5 drafted rows
+    // 73 and 197; 128 sequences of up to 4096, beyond the groups at once, 127 and 138 (but 250 of up to 2000 143 and
+    // 135, 100 x 5 drafted rows 141 and 125). Wide tiles, whose partial results are large, only where there are fewer
+    // tiles than groups: 2 chunks of 700 f32 rows behind 4300 145 us, a group a tile 313; 1 of 1024 bf16 rows behind
+    // 7168 130 and 229. From as many on, a group a tile, the widest first: 1 of 2048 bf16 rows 68, shared 89; 2 of
+    // them behind 2048 142 and 213 (but 4 chunks of 700 f32 rows behind 4300, 44 tiles for 32 groups, 484 and 277).
     const uint32_t at_once = (s.columns == 64 && !f32 ? 768 : s.columns <= 64 ? 512 : 256) / a->kv_heads;
     const uint32_t unit = s.columns == 16 ? kRound : kStep;
     const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),

@@ -97,6 +97,7 @@ FORMS = {
     "256 ordered": (16, 8, [2300, 1000, 2048, 2900], [0, 37, 500, 3], 2048),  # 256 columns (bf16; f32: 128)
     "256 of three": (24, 8, [3000, 2500], [0, 1], 3000),          # 255 of 256 columns used
     "256 many": (128, 2, [1100], [30], 1100),                     # 275 tiles of four rows: in the order they come
+    "256 border": (16, 8, [3100, 3044], [0, 9], 3000),             # as few rows as take 256 columns
     "256 heads": (128, 128, [700, 300, 24], [0, 100, 1000], 512), # one head a kv head, 256 rows a tile
 }
 
