@@ -319,8 +319,10 @@ int tessera_hip_flash_rows(const ts_rows_args *a, void *stream);
  *    even; infinities and NaN become NaN codes and take no part in the scale; values past
  *    448 * 2^119 become the largest.
  *  - Rows of one call that fall into one block (16 positions of a slot) stand together and in
- *    order; a later run of rows of the same block is kept nowhere and sets TS_STATUS_TWICE. Two
- *    slots of a call never share the page they append to (Pool::grow sees to it).
+ *    order; a later run of rows of the same block is kept nowhere and sets TS_STATUS_TWICE (into
+ *    bf16 rows too). Two slots of a call never share the page they append to (Pool::grow sees to it).
+ *    Such runs are looked for among all rows before them: beyond some 32,000 rows of a call that is
+ *    felt (131072 rows take 1.7 times what their bytes would).
  *  - A row past its slot's positions (or its table's pages) is kept nowhere and sets TS_STATUS_POSITION,
  *    one of a slot or page that the buffers do not hold TS_STATUS_PAGE. The q of both is NaN. That of a
  *    row refused as TS_STATUS_TWICE is as ever: only `status` tells of it.

@@ -20,9 +20,11 @@
 // therefore stand together; a later segment of the same block is refused (TS_STATUS_TWICE), found by
 // looking through the rows before it.
 //
-// Many rows are bound by HBM: 6 ragged prompts of up to 2048 f32 rows, 16 + 2 x 8 heads, into blocks, 250 MB: 51 to
-// 63 us, 4.0 to 4.9 TB/s. Few by a chain of loads (position, page, row, scale, held codes) and by fetching code,
-// about 1 KiB a microsecond the first time: one row 4.9 us, 200 into bf16 rows 5.9, 48 x 5 into begun blocks 10.4.
+// Many rows are bound by HBM: 6 ragged prompts of up to 2048 f32 rows, 16 + 2 x 8 heads, into blocks, 250 MB: 52 to
+// 64 us, 3.9 to 4.8 TB/s. Few by a chain of loads (position, page, row, scale, held codes): one row 4.6 us, 200 into
+// bf16 rows 5.9, 48 x 5 into begun blocks 10.4.
+// The look through the rows before grows with the square of the rows: a prompt of 32768 rows takes 221 us (186 at the
+// rate of a large copy), of 65536 508 (372), of 131072 1290 (744). Longer ones are best appended in parts.
 #include "kept8.h"
 
 namespace {
@@ -551,7 +553,10 @@ extern "C" int tessera_hip_append_rows(const ts_append_args *a, void *stream) {
     p.fours = ts::aligned(a->slots, 16) && ts::aligned(a->positions, 16);
     // Few rows are taken for a decode step, a segment each: a group looks at one row. Of many, most
     // go on from the row before them, and a group looks at 16; and a wave of q heads takes four rows,
-    // whose loads are in flight together.
+    // whose loads are in flight together. (A group looking at one row, or at 16, into blocks: 256 decode rows 12 and
+    // 53 us, 1024 36 and 57, 2048 68 and 82, 4096 150 and 143; 128 x 9 drafted rows 21 and 29, 200 x 9 32 and 33, 512 x
+    // 9 87 and 70. A prompt by itself, which the count does not tell from them, takes 12 and 8 at 256 rows, 26 and 12
+    // at 1024, 46 and 16 at 2048.)
     const bool few = a->rows <= 1024;
     p.window = few ? 1 : 16;
     p.q_rows = few ? 1 : kQRows;

@@ -16,8 +16,8 @@
 //  the block's scale, into the matrix unit; the next step's are asked for as soon as this step's are used.
 //  The four waves of a group, and the groups that share a tile's keys (share_of), are joined by their maxima
 //  and sums, the former in LDS, the latter by a second kernel.
-// HBM bounds it: 32 rows of 512 .. 8192 keys, 8 kv heads, 286 MB: 54 us and 5 for the join, 5.3 TB/s of codes;
-// 2 rows of 131000 keys, 4 kv heads: 42 and 5 us, 6 TB/s. A step costs a wave about 2.2 us with two waves a SIMD; a
+// HBM bounds it: 32 rows of 512 .. 8192 keys, 8 kv heads, 286 MB: 56 us and 5 for the join, 5.1 TB/s of codes;
+// 2 rows of 131000 keys, 4 kv heads: 43 and 5 us, 6 TB/s. A step costs a wave about 2.2 us with two waves a SIMD; a
 // group's first is done after some 8 us, which is what one row of 4000 keys takes (9.5 and 4 us).
 #include <algorithm>
 

@@ -15,9 +15,10 @@
 //    first (by their last row's position), heads fastest, so that consecutive groups, which go to
 //    different XCDs, leave each XCD one kv head's keys. Fewer tiles than groups share their keys (share_of).
 // A wave's step is a chain (K from LDS, scores, softmax, V from LDS, product) that two or three waves a SIMD overlap
-// in part: vector work takes half of the cycles, the matrix unit 30%. 4 prompts of 2048 rows, 16 heads over 8:
-// 101 us, 680 TFLOP/s; 24 x 5 drafted rows, 64 heads over 8, 1000 .. 9001 keys: 60 us and 6 for the join, 4.2 TB/s of
-// codes; f32 chunks of up to 700 rows with a window of 1000, 16 heads over 8: 54 and 8 us.
+// in part. 4 prompts of 2048 rows, 16 heads over 8: 95 us one pass after the other, 720 TFLOP/s (104 us each by
+// itself); vector work takes 54% of the cycles, the matrix unit 31%. 24 x 5 drafted rows, 64 heads over 8, 1000 .. 9001
+// keys: 58 us and 6 for the join, 4.3 TB/s of codes; vector 43%, matrix 20%, LDS conflicts 14%. f32 chunks of up to 700
+// rows with a window of 1000, 16 heads over 8: 54 and 8 us; vector 43%, matrix 38%.
 #include <algorithm>
 
 #include "kept8_attend.h"

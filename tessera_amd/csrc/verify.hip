@@ -13,14 +13,15 @@
 //      then weighs its share of the row to draw from, a wave a run of 256 indices at a time. The
 //      group that is last of a sequence to do so finds the run where the running sum passes u times the
 //      whole, and one wave the index in it.
-// Code that runs once costs its fetch (about 1 KiB a microsecond), so nothing here is unrolled or inlined
-// twice that need not be.
+// Code that runs once costs its fetch, so nothing here is unrolled or inlined twice that need not be.
 // Sums are in f64 and exponentials good to 33 bits (the vector unit's f64 rate is f32's here): the draw compares u
 // with running sums. Over rows of 151936 logits the exponentials' error moves their borders by up to 6e-12 of the
 // whole and, all borders together, decides about one draw in two million; f32 exponentials would move them by up to
 // 2e-8 and decide one draw in a thousand.
-// They bound the kernels (16 vector operations a logit), beside HBM: 32 sequences of up to 4 drafts with the
-// drafter's probabilities, 151936 f32 logits a row: rows 19 us, draw 16; one greedy sequence of 4 drafts: 4 and 3 us.
+// 32 sequences of up to 4 drafts with the drafter's probabilities, 81 rows of 151936 f32 logits: rows 19 us, draw 16.
+// The rows' 49 MB are 10 us at a large copy's rate; their 29 vector instructions a logit keep the vector unit busy for
+// 79% of the cycles in which a CU has waves, and a CU has them for some 60% of the kernel's time. The draw reads the drawn row again and the drafter's (39 MB, 8 us), after the verdict (3 us) and before
+// the last group's search; the vector unit is busy for half of it. One greedy sequence of 4 drafts: 4 and 3 us.
 #include <algorithm>
 
 #include "common.h"
@@ -419,7 +420,9 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(VerifyPara
             }
             if (!searching) {
                 const double sum = wave_total((w[0] + w[1]) + (w[2] + w[3]));
-                // Past the XCD's own L2, where the sequence's last group reads it.
+                // Past the XCD's own L2, where the sequence's last group reads it. (Its loads pass their L2 too. So
+                // stores that have arrived, the wait below, before the group's add to `done`, are what whoever sees
+                // that add reads: no release of the whole L2, which would cost microseconds, is needed.)
                 if (lane == 0) __hip_atomic_store(sums + r, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             r = next;
