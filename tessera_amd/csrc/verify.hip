@@ -20,8 +20,9 @@
 // 2e-8 and decide one draw in a thousand.
 // 32 sequences of up to 4 drafts with the drafter's probabilities, 81 rows of 151936 f32 logits: rows 19 us, draw 16.
 // The rows' 49 MB are 10 us at a large copy's rate; their 29 vector instructions a logit keep the vector unit busy for
-// 79% of the cycles in which a CU has waves, and a CU has them for some 60% of the kernel's time. The draw reads the drawn row again and the drafter's (39 MB, 8 us), after the verdict (3 us) and before
-// the last group's search; the vector unit is busy for half of it. One greedy sequence of 4 drafts: 4 and 3 us.
+// 79% of the cycles in which a CU has waves, and a CU has them for some 60% of the kernel's time. The draw reads the
+// drawn row again and the drafter's (39 MB, 8 us), after the verdict (3 us) and before the last group's search; the
+// vector unit is busy for half of it. One greedy sequence of 4 drafts: 4 and 3 us.
 #include <algorithm>
 
 #include "common.h"
