@@ -378,6 +378,116 @@ int tessera_hip_attend_kept8(const ts_kept8_args *a, void *stream);
 size_t tessera_hip_attend_kept8_workspace(const ts_kept8_args *a);
 
 /* ----------------------------------------------------------------------------
+ * Latent attention: the keys and values of all heads come from one kept row a position, a
+ * normed latent of `rank` values and a rotated key part of `rope`:
+ *   kept    [pages * page][rank + rope] bf16
+ * The row of position j of slot s is table[s * kept_pages + (j >> log2 page)] * page +
+ * (j & (page - 1)), or s * keys + j when kept_table is NULL. Pages copy as any kept row's
+ * (tessera_hip_kv_copy, row_bytes 2 (rank + rope)).
+ * Two forms of the attention: absorbed (tessera_hip_attend_latent), where q has been taken into
+ * the latent space and its sums are taken out of it (tessera_hip_linear_heads twice), over the
+ * kept rows; and expanded (tessera_hip_flash_latent), where a product has made every head's own
+ * keys and values of the latents, for prompts.
+ * The reference describes such a model (engine/models) but has no kernel for it; it composes the
+ * expanded form of separate stages.
+ * ------------------------------------------------------------------------- */
+
+/* New rows into the kept rows: c's first `rank` values through RmsNorm (gain, or not where it is
+ * NULL), its last `rope` through the rotation of their position (pairs (j, j + rope / 2), or (2j,
+ * 2j + 1) without `halves`; not where rope_table is NULL), kept at (slot, position); and the
+ * rotated part of q, to q_out. Any scaling of the angles is in the table's.
+ *  - c_out, r_out: the kept rows' values again, back to back, for the expanded form's product.
+ *  - A row past its slot's positions (or its table's pages) is kept nowhere and sets
+ *    TS_STATUS_POSITION, one of a slot or page that the buffers do not hold TS_STATUS_PAGE; its
+ *    q_out, c_out and r_out are NaN.
+ *  - Two rows of one call are not for one place: which row's values are then kept there is not
+ *    defined, piece by piece. Two slots of a call never share the page they append to.
+ * Norm and rotation are in f32, each value rounded once. */
+typedef struct {
+    const void *c;                 /* [rows, rank + rope], c_stride elements apart */
+    const void *q;                 /* [rows, heads, rope]: rows q_stride, heads q_head apart; or NULL */
+    const float *gain;             /* [rank] or NULL */
+    const float *rope_table;       /* [rope_rows][rope / 2][2] (cos, sin), or NULL */
+    void *q_out;                   /* [rows, heads, rope]: rows q_out_stride, heads q_out_head apart; may be q
+                                      where both are laid out alike and of one type */
+    void *kept;
+    void *c_out, *r_out;           /* bf16 [rows, rank], [rows, rope], either or both NULL */
+    const uint32_t *slots, *positions; /* [rows] */
+    const uint32_t *kept_table;    /* [slot_count * kept_pages], or NULL for dense */
+    uint32_t *status;              /* device word or NULL: TS_STATUS_* bits are OR-ed in */
+    uint32_t rows, heads;
+    uint32_t rank;                 /* a multiple of 8, at most 1024 */
+    uint32_t rope;                 /* 16, 32, 64 or 128 */
+    uint32_t c_stride, q_stride, q_head, q_out_stride, q_out_head; /* whole 16-byte pieces */
+    uint32_t keys;                 /* positions a slot may hold */
+    uint32_t slot_count, kept_pages;
+    uint32_t page, pages;          /* as ts_append_args' */
+    uint32_t rope_rows;            /* >= keys */
+    int32_t halves;
+    int32_t x_dtype, q_out_dtype;  /* c and q; q_out: f32 or bf16 */
+    float eps;
+} ts_append_latent_args;
+int tessera_hip_append_latent(const ts_append_latent_args *a, void *stream);
+
+/* A product a head: out[r, h, :] = sum_k x[r, h, k] * w[h, :, k]. x f32 or bf16 (f32 enters as three
+ * bf16 parts, 24 bits), w bf16, out f32 or bf16; sums in f32. x and out may be parts of wider rows.
+ * No counterpart in the reference (a product a head is a batch of products there). */
+typedef struct {
+    const void *x;      /* [rows, heads, k]: rows x_stride, heads x_head elements apart, whole 16-byte pieces */
+    const void *w;      /* [heads, n, k] bf16: heads w_head apart (a multiple of 8), a head's rows back to back */
+    void *out;          /* [rows, heads, n]: rows out_stride, heads out_head elements apart */
+    uint32_t rows, heads, n;
+    uint32_t k;         /* a multiple of 8 */
+    uint32_t x_stride, x_head, out_stride, out_head;
+    uint64_t w_head;
+    int32_t x_dtype, out_dtype;
+} ts_heads_args;
+int tessera_hip_linear_heads(const ts_heads_args *a, void *stream);
+
+/* The absorbed form, ragged rows over kept rows: row r (slot s, position p) sees the keys at
+ * [max(0, p - back), p] of its slot, w = softmax(q . row * scale) over rank + rope values, out = the
+ * sum of w times the rows' first `rank` values. rows.q [rows, heads, rank + rope] bf16, rows.k the
+ * kept rows (rows.v is not read), rows.out [rows, heads, rank] bf16, rows.kv_heads 1, rows.width
+ * rank + rope. rank 512 with rope 64, or 256 with 32. Scores, softmax and sums in f32; weights enter
+ * their product in bf16, in two parts (16 bits) where `run` rows have up to 32 heads between them.
+ *  - `run`: how many rows of a slot stand together (1: a decode step; drafted rows; a prompt chunk's).
+ *    It groups rows and picks the kernel, never which keys a row sees. A row's last bits may depend on
+ *    the rows beside it; the same call gives the same bits.
+ *  - Refused rows (a position as for attend_rows; a slot >= slot_count; a page >= pages among the
+ *    row's keys) write NaN and set their status bit.
+ *  - Infinities and NaN reach the rows that see them alone; kept rows past a sequence's last position
+ *    may hold anything. Dense kept rows: keys a multiple of 16. */
+typedef struct {
+    ts_rows_args rows;
+    uint32_t rank, slot_count, pages, run;
+} ts_latent_args;
+int tessera_hip_attend_latent(const ts_latent_args *a, void *stream);
+size_t tessera_hip_attend_latent_workspace(const ts_latent_args *a);
+
+/* The expanded form over whole sequences, packed back to back: row i of a sequence of n rows and m keys
+ * stands at position m - n + i (its keys end where its rows do) and sees the keys [position - back,
+ * position] of its sequence: w = softmax((q . k + q' . r) * scale), q the first `nope` values of a q
+ * row's head and q' its last `rope`, k the head's keys and r the keys' shared part; out = sum of w v.
+ * Sequence s's rows are first[s] .. first[s + 1], its keys key_first[s] .. key_first[s + 1]. nope and
+ * value 128 with rope 64, or 64 with 32. Scores, softmax and sums in f32, weights in bf16.
+ *  - A row that sees no key (more rows than keys) is zero. Rows behind the last sequence, and of
+ *    a sequence whose bounds do not ascend or pass `rows` or `key_rows`, are left as they were.
+ *  - Infinities and NaN reach the rows that see them alone. */
+typedef struct {
+    const void *q;             /* [rows, heads, nope + rope] bf16: rows q_stride apart, a row's heads back to back */
+    const void *k, *v;         /* [key_rows, heads, nope], [key_rows, heads, value] bf16: rows *_stride, heads *_head apart */
+    const void *r;             /* [key_rows, rope] bf16, r_stride apart */
+    void *out;                 /* [rows, heads, value] bf16 */
+    const uint32_t *first;     /* [seqs + 1] ascending, or NULL: one sequence of all rows (seqs 1) */
+    const uint32_t *key_first; /* [seqs + 1] ascending, or NULL: first's (one sequence: all keys) */
+    uint32_t rows, key_rows, seqs, heads, nope, rope, value;
+    uint32_t q_stride, k_stride, k_head, v_stride, v_head, r_stride; /* elements, multiples of 8 */
+    uint32_t back;             /* keys a row sees before its own; UINT32_MAX: all */
+    float scale;
+} ts_flash_latent_args;
+int tessera_hip_flash_latent(const ts_flash_latent_args *a, void *stream);
+
+/* ----------------------------------------------------------------------------
  * Elementwise chains not fused into a product.
  * out[i] = chain(x[i], operands at i) for i < len, with `after` as above (read
  * `after.sum` is x; operands with spans repeat). out may alias x or an operand.

@@ -153,6 +153,23 @@ VerifyArgs = _args("VerifyArgs", "ts_verify_args", [
     ("status", _v), ("seqs", _u), ("most", _u), ("rows", _u), ("width", _u), ("stride", _u),
     ("logits_dtype", C.c_int32), ("temperature", _f)])
 
+AppendLatentArgs = _args("AppendLatentArgs", "ts_append_latent_args", [
+    ("c", _v), ("q", _v), ("gain", _v), ("rope_table", _v), ("q_out", _v), ("kept", _v), ("c_out", _v), ("r_out", _v),
+    ("slots", _v), ("positions", _v), ("kept_table", _v), ("status", _v), ("rows", _u), ("heads", _u), ("rank", _u),
+    ("rope", _u), ("c_stride", _u), ("q_stride", _u), ("q_head", _u), ("q_out_stride", _u), ("q_out_head", _u),
+    ("keys", _u), ("slot_count", _u), ("kept_pages", _u), ("page", _u), ("pages", _u), ("rope_rows", _u),
+    ("halves", C.c_int32), ("x_dtype", C.c_int32), ("q_out_dtype", C.c_int32), ("eps", _f)])
+HeadsArgs = _args("HeadsArgs", "ts_heads_args", [
+    ("x", _v), ("w", _v), ("out", _v), ("rows", _u), ("heads", _u), ("n", _u), ("k", _u), ("x_stride", _u),
+    ("x_head", _u), ("out_stride", _u), ("out_head", _u), ("w_head", C.c_uint64), ("x_dtype", C.c_int32),
+    ("out_dtype", C.c_int32)])
+LatentArgs = _args("LatentArgs", "ts_latent_args", [
+    ("rows", RowsArgs), ("rank", _u), ("slot_count", _u), ("pages", _u), ("run", _u)])
+FlashLatentArgs = _args("FlashLatentArgs", "ts_flash_latent_args", [
+    ("q", _v), ("k", _v), ("v", _v), ("r", _v), ("out", _v), ("first", _v), ("key_first", _v), ("rows", _u),
+    ("key_rows", _u), ("seqs", _u), ("heads", _u), ("nope", _u), ("rope", _u), ("value", _u), ("q_stride", _u),
+    ("k_stride", _u), ("k_head", _u), ("v_stride", _u), ("v_head", _u), ("r_stride", _u), ("back", _u), ("scale", _f)])
+
 
 _P = C.c_void_p
 _U = C.c_uint32
@@ -197,6 +214,11 @@ SIGNATURES = {
     "tessera_hip_attend_kept8_workspace": (C.c_size_t, [C.POINTER(Kept8Args)]),
     "tessera_hip_verify": (C.c_int, [C.POINTER(VerifyArgs), _P]),
     "tessera_hip_verify_workspace": (C.c_size_t, [C.POINTER(VerifyArgs)]),
+    "tessera_hip_append_latent": (C.c_int, [C.POINTER(AppendLatentArgs), _P]),
+    "tessera_hip_linear_heads": (C.c_int, [C.POINTER(HeadsArgs), _P]),
+    "tessera_hip_attend_latent": (C.c_int, [C.POINTER(LatentArgs), _P]),
+    "tessera_hip_attend_latent_workspace": (C.c_size_t, [C.POINTER(LatentArgs)]),
+    "tessera_hip_flash_latent": (C.c_int, [C.POINTER(FlashLatentArgs), _P]),
 }
 
 

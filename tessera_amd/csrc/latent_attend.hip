@@ -1,0 +1,719 @@
+// The absorbed form of latent attention: every head of row r (slot s, position p) sees the kept rows of its slot at
+// [max(0, p - back), p], w = softmax(q . row * scale), out = sum of w row[: RANK].
+//
+// A tile is the heads of R rows that stand together, its (row, head) pairs the columns of 16-wide matrix products
+// S^T = K q^T and O^T = V^T P^T, so a column's scores stay in its lanes and P^T is the second product's operand as
+// it stands. Keys and values are one row, which goes from memory to LDS once, 32 keys a step, without passing
+// registers; K's operand is 16 bytes of a row, V^T's comes through the transposing LDS read. A wave holds 16
+// columns: 128 (RANK 512) registers of O and 72 of q.
+//  * WC waves share a step's keys, 16 columns each; the teams of a group take steps in turn, and are joined in LDS at
+//    the end. With WC = 1 each wave streams keys of its own and waits for no other.
+//  * Keys are dealt to the groups in equal runs over all tiles, so that groups end together however the sequences
+//    differ in length; a tile that several groups have is joined by a second kernel.
+#include <algorithm>
+
+#include "kept8_attend.h"
+
+namespace {
+
+using namespace kept8;
+
+constexpr uint32_t kKeys = 32;         // keys of a step
+constexpr uint32_t kMaxTiles = 1024;   // row tiles whose keys are shared
+constexpr uint32_t kJoinThreads = 256;
+constexpr uint32_t kAhead = 2;         // operands read ahead of their products
+
+struct LatentParams {
+    const uint16_t *q, *kept;
+    uint16_t *out;
+    // Where keys are shared: results of groups for a tile that an earlier group began, then for one that a later
+    // group goes on with, each [groups][blocks] of a tile's columns; and each row tile's groups (first, count).
+    float *partials;
+    uint32_t *shares;
+    const uint32_t *slots, *positions;
+    uint32_t *status;
+    Place place;
+    uint32_t rows, heads, back, max_position;
+    uint32_t tile_rows, tiles, groups;  // rows a tile, row tiles, and groups a block of heads
+    uint32_t block_heads, blocks;       // a row's heads in a tile, and the blocks they make
+    float scale;
+};
+
+// Column c's row and head of a tile; false where it has none.
+TS_DEV bool column_of(const LatentParams &p, uint32_t row0, uint32_t block, uint32_t c, uint32_t &r, uint32_t &h) {
+    const uint32_t ri = c / p.block_heads;
+    r = row0 + ri;
+    h = block * p.block_heads + c % p.block_heads;
+    return ri < p.tile_rows && r < p.rows && h < p.heads;
+}
+
+// A column's partial result: RANK / 4 times [columns] of four sums, then [columns] maxima and sums.
+template <uint32_t RANK>
+constexpr uint32_t part_floats(uint32_t columns) { return columns * (RANK + 2); }
+
+// The XOR of a row's 16-byte pieces in LDS: among eight where rows begin 128 bytes apart (modulo the 256 that LDS
+// serves at a time), among four where 64. It keeps the lanes that are served together in 16 places: of K's read
+// lanes 0-3 and 12-15 of one 16 and 4-11 of the next, of V^T's the two pieces of eight rows.
+template <uint32_t CH>
+TS_DEV uint32_t swap_of(uint32_t row) {
+    const uint32_t i = CH % 16 == 8 ? row >> 1 & 7 : row >> 2 & 3;
+    if (CH % 16 == 8) return (i & 1) << 2 | ((i ^ i >> 1) & 2) | i >> 2;
+    return ((i ^ i >> 1) & 1) << 1 | i >> 1;
+}
+
+typedef short ts_v4i16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) ts_v4i16 lds_v4i16;
+// Four keys of one d, from the 8-byte pieces of four rows (lane 4 e + c of 16: row e, d 4 c ..).
+TS_DEV u32x2 read_vt4(const char *a) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *)a));
+}
+
+// The bits of the bf16 values of a pair that are not finite. (All ones are a NaN.)
+TS_DEV uint32_t odd_mask(uint32_t x) {
+    return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+// A lane's number that what follows is computed from where it is used: rare steps' addresses would otherwise be
+// computed ahead of the loops, and push what the common ones use out of the registers.
+TS_DEV uint32_t again(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// 2^(a - b) of maxima, 0 where a has seen nothing.
+TS_DEV float weight_of(float a, float b) { return a == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(a - b); }
+
+template <uint32_t RANK, uint32_t ROPE, uint32_t WC>
+struct Shape {
+    static constexpr uint32_t kWidth = RANK + ROPE, kRow = 2 * kWidth, kPieces = kWidth / 8;
+    static constexpr uint32_t kWaves = WC < 4 ? 4 : WC, kTeams = kWaves / WC;
+    static constexpr uint32_t kRing = 4 / kTeams;                // rounds of kTeams steps in LDS
+    static constexpr uint32_t kTile = kKeys * kRow, kLds = 4 * kTile;
+    static constexpr uint32_t kUnit = kKeys * kTeams;            // keys of a round
+    static constexpr uint32_t kParts = kTile / 1024;             // loads of a step, dealt to the team's waves
+    static constexpr uint32_t kLoads = (kParts + WC - 1) / WC, kLeast = kParts / WC;
+    static constexpr uint32_t kOwn = kLoads < 9 ? kLoads : 9;    // those of different places within a block
+    static constexpr uint32_t kCols = 16 * WC, kWeights = WC == 8 ? 1 : 2;
+    static constexpr uint32_t kQ = kWidth / 32, kD = RANK / 16;  // operands of q, tiles of O
+    static constexpr uint32_t kIds = WC == 1 ? 2 : 2 * kTeams;   // blocks whose pages a wave looks up
+    static constexpr uint32_t kXor = kPieces % 16 == 8 ? 8 : 4;  // pieces that the XOR permutes
+    static constexpr bool kAside = RANK == 512;                  // the loads' places are kept in LDS: registers are few
+};
+
+template <uint32_t RANK, uint32_t ROPE, uint32_t WC>
+__global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void attend_latent_kernel(LatentParams p) {
+    using S = Shape<RANK, ROPE, WC>;
+    constexpr uint32_t kThreads = 64 * S::kWaves;
+    extern __shared__ __attribute__((aligned(16))) char stage[];
+    __shared__ uint32_t starts[kMaxTiles + 1], words[S::kWaves], odd_keys[S::kWaves], found;
+    __shared__ uint32_t from_aside[S::kAside ? S::kOwn : 1][S::kAside ? kThreads : 1];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t col = lane & 15, grp = lane >> 4, team = wave / WC, mine = wave % WC;
+    const uint32_t u = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
+
+    // The group's units of keys: a row tile is as many as its rows see, all tiles' one behind the other are dealt to
+    // the groups in equal runs. (A tile's units are told from its first and last row.)
+    uint32_t unit = 0, end = 1, each = 1, tile = u;
+    if (p.partials) {
+        constexpr uint32_t kEach = kMaxTiles / kThreads;
+        uint32_t n[kEach], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            const uint32_t t = threadIdx.x * kEach + i;
+            n[i] = 0;
+            if (t < p.tiles) {
+                const uint32_t r0 = t * p.tile_rows, r1 = min(r0 + p.tile_rows, p.rows) - 1;
+                const uint32_t most = min(p.max_position, p.place.keys - 1);
+                const uint32_t p0 = min(p.positions[r0], most), p1 = min(p.positions[r1], most);
+                const uint32_t from0 = p0 > p.back ? p0 - p.back : 0, from1 = p1 > p.back ? p1 - p.back : 0;
+                auto units = [](uint32_t lo, uint32_t hi) { return (hi - (lo & ~(kBlock - 1))) / S::kUnit + 1; };
+                n[i] = p.slots[r0] == p.slots[r1] ? units(min(from0, from1), max(p0, p1))
+                                                  : units(from0, p0) + units(from1, p1);
+                n[i] = min(n[i], 1u << 21);
+            }
+            sum += n[i];
+        }
+        uint32_t upto = sum;
+        for (uint32_t d = 1; d < 64; d <<= 1) {
+            const uint32_t x = __shfl_up((int)upto, d, 64);
+            if (lane >= d) upto += x;
+        }
+        if (lane == 63) words[wave] = upto;
+        __syncthreads();
+        uint32_t all = 0, before = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < S::kWaves; w++) {
+            if (w < wave) before += words[w];
+            all += words[w];
+        }
+        all = __builtin_amdgcn_readfirstlane(all);
+        each = (all + p.groups - 1) / p.groups;
+        unit = u * each;
+        end = min(unit + each, all);
+        if (unit >= all) return;
+        uint32_t at = before + upto - sum;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            const uint32_t t = threadIdx.x * kEach + i;
+            if (t >= p.tiles) break;
+            starts[t] = at;
+            if (unit >= at && unit < at + n[i]) found = t;
+            at += n[i];
+        }
+        if (threadIdx.x == 0) starts[p.tiles] = all;
+        __syncthreads();
+        tile = __builtin_amdgcn_readfirstlane(found);
+    }
+
+    // Where the lane's 16 bytes of the wave's loads of a step come from, in their block of 16 rows (LDS holds rows back
+    // to back). They repeat after nine loads: in the other block, or (WC = 1) eight rows on, where the XOR differs by 3.
+    uint32_t from_at[S::kOwn];
+#pragma unroll
+    for (uint32_t i = 0; i < S::kOwn; i++) {
+        const uint32_t g = 64 * ((mine + i * WC) % (S::kParts / 2)) + lane, row = g / S::kPieces;
+        from_at[i] = row * S::kRow + ((g % S::kPieces) ^ swap_of<S::kPieces>(row)) * 16;
+        if (S::kAside) from_aside[i][threadIdx.x] = from_at[i];
+    }
+    // LDS offsets of the lane's operands: K piece grp of row `col`, and V^T d 8 (lane / 2 % 2) + 4 (lane % 2) .. of keys
+    // 4 grp + lane / 4 % 4; others by the XOR of their piece.
+    const uint32_t koff = col * S::kRow + (grp ^ swap_of<S::kPieces>(col)) * 16;
+    const uint32_t vrow = 4 * grp + (lane >> 2 & 3);
+    const uint32_t voff = vrow * S::kRow + ((lane >> 1 & 1) ^ swap_of<S::kPieces>(vrow)) * 16 + (lane & 1) * 8;
+    const float sl = base2_scale(p.scale);
+    const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;
+
+    for (;;) {
+        const uint32_t row0 = tile * p.tile_rows;
+        uint32_t a = 0, b = 1, units = 1;
+        float *partial = nullptr;
+        if (p.partials) {
+            const uint32_t t0 = __builtin_amdgcn_readfirstlane(starts[tile]);
+            const uint32_t t1 = __builtin_amdgcn_readfirstlane(starts[tile + 1]);
+            a = unit - t0;
+            b = min(end, t1) - t0;
+            units = t1 - t0;
+            if (a || b < units)
+                partial = p.partials + ((size_t)((a ? 0 : p.groups) + u) * p.blocks + block) * part_floats<RANK>(S::kCols);
+            if (a == 0 && block == 0 && threadIdx.x == 0) {
+                p.shares[2 * tile] = u;
+                p.shares[2 * tile + 1] = (t1 - 1) / each - u + 1;
+            }
+        }
+        uint32_t pos, slot;
+        bool live;
+        bf16x8 q[S::kQ];
+        {
+            uint32_t r, h;
+            const uint32_t l0 = again(lane);
+            const bool there = column_of(p, row0, block, 16 * mine + (l0 & 15), r, h);
+            pos = there ? p.positions[r] : 0;
+            slot = there ? p.slots[r] : 0;
+            live = there && pos <= p.max_position && holds(p.place, slot, pos);
+            if (there && !live && p.status && a == 0 && team == 0 && l0 < 16)
+                atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
+            const uint16_t *at = p.q + (live ? ((size_t)r * p.heads + h) * S::kWidth : 0) + 8 * (l0 >> 4);
+#pragma unroll
+            for (uint32_t j = 0; j < S::kQ; j++) {
+                const u32x4 w = *(const u32x4 *)(at + 32 * j);
+                q[j] = as_bf16x8((w ^ qsign) & (live ? 0xffffffffu : 0u));
+            }
+        }
+        const uint32_t from = pos > p.back ? pos - p.back : 0;
+        bool wait = live;
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o[S::kD];
+#pragma unroll
+        for (uint32_t d = 0; d < S::kD; d++) o[d] = f32x4{0, 0, 0, 0};
+
+        // A pass over the keys for each slot among the columns (one, where rows of a slot stand together).
+        for (;;) {
+            const uint64_t waiting = __builtin_amdgcn_ballot_w64(wait);
+            const uint32_t first = waiting ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(waiting)) : 0xffffffffu;
+            auto over = [&](uint32_t v, bool least) {  // over the group's waves
+                __syncthreads();
+                words[wave] = v;
+                __syncthreads();
+                uint32_t x = words[0];
+#pragma unroll
+                for (uint32_t w = 1; w < S::kWaves; w++) x = least ? min(x, words[w]) : max(x, words[w]);
+                return (uint32_t)__builtin_amdgcn_readfirstlane(x);
+            };
+            const uint32_t now = over(first, true);
+            if (now == 0xffffffffu) break;  // (a served slot is below slot_count)
+            const bool act = wait && slot == now;
+            wait = wait && !act;
+            // Keys that some column of the wave sees, [wlo, whi], and of the group; and those that all of the wave's do.
+            const uint32_t wlo = row16_least(act ? from : 0xffffffffu), whi = ~row16_least(act ? ~pos : 0xffffffffu);
+            const uint32_t all_lo = ~row16_least(act ? ~from : live ? 0u : 0xffffffffu);
+            const uint32_t all_hi = row16_least(act ? pos : live ? 0u : 0xffffffffu);
+            const uint32_t lo = over(wlo, true), hi = over(whi, false);
+            // (Keys [same_lo, same_hi] are seen by all columns alike.)
+            const uint32_t same_lo = WC == 1 ? all_lo : over(all_lo, false), same_hi = WC == 1 ? all_hi : over(all_hi, true);
+            auto differ = [&](uint32_t here, uint32_t n) { return max(here, lo) < same_lo || min(here + n - 1, hi) > same_hi; };
+            const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, np = (hi - base0) / S::kUnit + 1;
+            const uint32_t unit0 = pass_unit(a, units, np), unit1 = pass_unit(b, units, np);
+            if (unit0 >= unit1) continue;
+
+            // Pages of a round's blocks (the wave's own step's where teams do not meet), asked for a round ahead.
+            uint32_t id[S::kIds];
+            auto key_of = [&](uint32_t round, uint32_t i) {
+                const uint32_t at = base0 + round * S::kUnit + (WC == 1 ? kKeys * wave : 0);
+                return min(at / kBlock + i, last) * kBlock;
+            };
+            const_u32 *pages = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
+            auto look = [&](uint32_t round) {
+#pragma unroll
+                for (uint32_t i = 0; i < S::kIds; i++)
+                    id[i] = p.place.table ? pages[key_of(round, i) >> p.place.page_shift] : 0;
+            };
+            // The blocks of a round that are not held, a bit each.
+            auto gone_of = [&]() {
+                uint32_t gone = 0;
+                if (p.place.table)
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kIds; i++) gone |= id[i] >= p.place.pages ? 1u << i : 0u;
+                return gone;
+            };
+            auto issue = [&](uint32_t round, uint32_t slot_of_ring) {
+                char *to = stage + (slot_of_ring * S::kTeams + team) * S::kTile;
+                __amdgpu_buffer_rsrc_t buf[2];
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) {
+                    uint32_t page = id[0], key = key_of(round, 0);
+#pragma unroll
+                    for (uint32_t e = 1; e < S::kIds; e++)
+                        if (e == (WC == 1 ? i : 2 * team + i)) {
+                            page = id[e];
+                            key = key_of(round, e);
+                        }
+                    bool lost;
+                    const uint32_t kept_block = block_in(p.place, now, page, key, lost);
+                    buf[i] = raw_buffer((const char *)p.kept + (size_t)kept_block * (kBlock * S::kRow));
+                }
+                uint32_t from[S::kOwn];
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOwn; i++) from[i] = S::kAside ? from_aside[i][threadIdx.x] : from_at[i];
+#pragma unroll
+                for (uint32_t i = 0; i < S::kLoads; i++) {
+                    const uint32_t part = mine + i * WC;
+                    if (S::kLoads != S::kLeast && part >= S::kParts) break;
+                    const bool on = WC == 1 && S::kParts == 36 && (i / 9 & 1);
+                    buffer_to_lds16(part < S::kParts / 2 ? buf[0] : buf[1], to + part * 1024,
+                                    on ? from[i % S::kOwn] ^ 48 : from[i % S::kOwn], on ? 8 * S::kRow : 0);
+                }
+            };
+
+            // One step: the wave's columns against the keys here .. here + 31 at `at`.
+            auto step = [&](uint32_t here, char *at, uint32_t gone, bool apart) {
+                // Register i of s[t]: key 16 t + 4 grp + i.
+                f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                const uint32_t k0 = again(koff), v0 = again(voff);
+                // Operands are read kAhead products ahead: left to itself, the compiler reads all it has registers for, or
+                // one at a time and waits for each.
+                bf16x8 ahead[2][kAhead];
+                auto read_k = [&](uint32_t x) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; i++) {
+                        const uint32_t j = (x * kAhead + i) / 2, t = (x * kAhead + i) % 2;
+                        ahead[x & 1][i] = *(const bf16x8 *)(at + (k0 ^ j % (S::kXor / 4) * 64) +
+                                                            j / (S::kXor / 4) * (S::kXor * 16) + t * kBlock * S::kRow);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                constexpr uint32_t kReads = 2 * S::kQ / kAhead;
+                static_assert(2 * S::kQ % kAhead == 0 && S::kD % kAhead == 0, "whole batches");
+                read_k(0);
+#pragma unroll
+                for (uint32_t x = 0; x < kReads; x++) {
+                    if (x + 1 < kReads) read_k(x + 1);
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; i++) {
+                        const uint32_t j = (x * kAhead + i) / 2, t = (x * kAhead + i) % 2;
+                        s[t] = mfma16(ahead[x & 1][i], q[j], s[t]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (here < all_lo || here + (kKeys - 1) > all_hi || gone) {
+                    const int upto = act ? (int)(pos - here) - 4 * (int)grp : -1, since = (int)(from - here) - 4 * (int)grp;
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const bool seen = 16 * t + i <= upto && 16 * t + i >= since;
+                            s[t][i] = seen ? (gone >> t & 1 ? __builtin_nanf("") : s[t][i]) : -INFINITY;
+                        }
+                }
+                float mx = s[0][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i / 4][i % 4]);
+                mx = rows4_max(mx) * sl;
+                const bool raise = mx > m + kSlack;
+                const float mn = raise ? mx : m, mo = mn == -INFINITY ? 0.0f : mn;
+                uint32_t pw[4][S::kWeights];
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sl, -mo));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4 + 1], sl, -mo));
+                    sum += x + y;
+                    split_pair<S::kWeights>(x, y, pw[i / 2]);
+                }
+                if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+                    const float alpha = raise ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                    l *= alpha;
+                    m = mn;
+#pragma unroll
+                    for (uint32_t d = 0; d < S::kD; d++) o[d] *= alpha;
+                }
+                l += sum;
+                u32x4 w[S::kWeights];
+#pragma unroll
+                for (uint32_t e = 0; e < S::kWeights; e++) w[e] = u32x4{pw[0][e], pw[1][e], pw[2][e], pw[3][e]};
+                // V^T: d 16 dt + col of keys 4 grp .. and 16 + 4 grp .. (eight of them).
+                auto read_v = [&](uint32_t d) {
+                    const char *v = at + d / (S::kXor / 2) * (S::kXor * 16) + (v0 ^ d % (S::kXor / 2) * 32);
+                    const u32x2 lo4 = read_vt4(v), hi4 = read_vt4(v + kBlock * S::kRow);
+                    return u32x4{lo4.x, lo4.y, hi4.x, hi4.y};
+                };
+                if (apart) {
+                    // Some key here is one column's and not another's. A value that is not finite must reach the former
+                    // alone, and the product's 0 times it would be NaN: such values are looked for, become NaN where they
+                    // are seen (their key's score is infinite or NaN as well, so the column's sum can be nothing else), and
+                    // are cleared. (By all waves of the group together, but where each has keys of its own.)
+                    uint32_t bad = 0;  // keys that hold one
+#pragma unroll 1
+                    for (uint32_t k = mine; k < kKeys; k += WC) {
+                        const uint32_t *x = (const uint32_t *)(at + k * S::kRow) + again(lane) * (RANK / 128);
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (uint32_t e = 0; e < RANK / 128; e++)
+                            odd |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+                        bad |= __builtin_amdgcn_ballot_w64(odd) != 0 ? 1u << k : 0u;
+                    }
+                    uint32_t any = bad;
+                    if (WC > 1) {
+                        odd_keys[wave] = bad;
+                        lds_barrier();
+                        any = bad = 0;
+#pragma unroll
+                        for (uint32_t i = 0; i < S::kWaves; i++) {
+                            const uint32_t x = __builtin_amdgcn_readfirstlane(odd_keys[i]);
+                            any |= x;
+                            bad |= i / WC == team ? x : 0u;
+                        }
+                    }
+                    for (uint32_t left = bad; left;) {
+                        const uint32_t k = __builtin_ctz(left), swap = swap_of<S::kPieces>(k), g = again(grp);
+                        left &= left - 1;
+                        const uint32_t keep = act && here + k <= pos && here + k >= from ? 0xffffffffu : 0u;
+                        const char *row = at + k * S::kRow + 8 * (g & 1);
+#pragma unroll
+                        for (uint32_t d = 0; d < S::kD; d++) {
+                            u32x2 x = *(const u32x2 *)(row + ((2 * d + (g >> 1)) ^ swap) * 16);
+                            x = u32x2{odd_mask(x[0]), odd_mask(x[1])} & keep;
+                            o[d] += f32x4{lo_bf16(x[0]), hi_bf16(x[0]), lo_bf16(x[1]), hi_bf16(x[1])};
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    if (any) {
+                        if (WC > 1) lds_barrier();
+#pragma unroll 1
+                        for (uint32_t k = mine; k < kKeys; k += WC) {
+                            uint32_t *x = (uint32_t *)(at + k * S::kRow) + again(lane) * (RANK / 128);
+                            if (bad >> k & 1)
+#pragma unroll
+                                for (uint32_t e = 0; e < RANK / 128; e++) x[e] &= ~odd_mask(x[e]);
+                        }
+                        if (WC > 1) lds_barrier();
+                    }
+                }
+                auto read_batch = [&](uint32_t x) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; i++) ahead[x & 1][i] = as_bf16x8(read_v(x * kAhead + i));
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                read_batch(0);
+#pragma unroll
+                for (uint32_t x = 0; x < S::kD / kAhead; x++) {
+                    if (x + 1 < S::kD / kAhead) read_batch(x + 1);
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; i++)
+#pragma unroll
+                        for (uint32_t e = 0; e < S::kWeights; e++)
+                            o[x * kAhead + i] = mfma16(ahead[x & 1][i], as_bf16x8(w[e]), o[x * kAhead + i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            // Rows of a step that no column of the pass sees, or of no page, are zero in the products.
+            auto clear = [&](uint32_t here, char *at, uint32_t gone) {
+                for (uint32_t g = mine * 64 + again(lane); g < kKeys * S::kPieces; g += 64 * WC) {
+                    const uint32_t row = g / S::kPieces, key = here + row;
+                    if (key < lo || key > hi || gone >> (row / kBlock) & 1) *(u32x4 *)(at + g * 16) = u32x4{0, 0, 0, 0};
+                }
+                if (gone && p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+            };
+
+            if (WC == 1) {
+                char *at = stage + team * S::kTile;
+                uint32_t round = unit0;
+                look(round);
+                for (; round < unit1; round++) {
+                    const uint32_t here = base0 + round * S::kUnit + kKeys * wave;
+                    if (here > hi) break;
+                    const uint32_t gone = gone_of();
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads
+                    issue(round, 0);
+                    look(min(round + 1, unit1 - 1));
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    if (here < lo || here + (kKeys - 1) > hi || gone) clear(here, at, gone);
+                    step(here, at, gone, differ(here, kKeys));
+                }
+            } else {
+                // kRing - 1 rounds on their way.
+                constexpr uint32_t kLater = S::kRing > 1 ? (S::kRing - 2) * S::kLeast : 0;
+                uint32_t gone[S::kRing], n = 0;
+                look(unit0);
+#pragma unroll
+                for (uint32_t i = 0; i + 1 < S::kRing; i++) {
+                    gone[i] = gone_of();
+                    if (unit0 + i < unit1) issue(unit0 + i, i);
+                    look(min(unit0 + i + 1, unit1 - 1));
+                }
+                for (uint32_t round = unit0; round < unit1; round++) {
+                    if (unit1 - round >= S::kRing - 1)
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
+                    else
+                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    gone[S::kRing - 1] = gone_of();
+                    if (round + S::kRing - 1 < unit1) {
+                        issue(round + S::kRing - 1, (n + S::kRing - 1) % S::kRing);
+                        look(min(round + S::kRing, unit1 - 1));
+                    }
+                    const uint32_t here = base0 + round * S::kUnit;
+                    const uint32_t at_here = here + team * kKeys, lost = gone[0] >> (2 * team) & 3;
+                    char *at = stage + (n * S::kTeams + team) * S::kTile;
+                    if (here < lo || here + (S::kUnit - 1) > hi || gone[0]) {
+                        clear(at_here, at, lost);
+                        lds_barrier();
+                    }
+                    const bool apart = differ(here, S::kUnit);
+                    if (apart || (at_here <= whi && at_here + (kKeys - 1) >= wlo)) step(at_here, at, lost, apart);
+                    n = n + 1 == S::kRing ? 0 : n + 1;
+#pragma unroll
+                    for (uint32_t i = 0; i + 1 < S::kRing; i++) gone[i] = gone[i + 1];
+                }
+                lds_barrier();  // the last reads, before the next pass's loads
+            }
+        }
+
+        // The teams' results into the first's, by halves.
+        if (S::kTeams > 1) {
+#pragma unroll
+            for (uint32_t n = S::kTeams / 2; n; n /= 2) {
+                __syncthreads();
+                const uint32_t l0 = again(lane);
+                char *at = stage + (team % n * WC + mine) * (RANK * 64 + 512) + l0 * 16;
+                float *ml = (float *)(stage + (team % n * WC + mine) * (RANK * 64 + 512) + RANK * 64) + l0;
+                if (team >= n && team < 2 * n) {
+#pragma unroll
+                    for (uint32_t d = 0; d < S::kD; d++) *(f32x4 *)(at + d * 1024) = o[d];
+                    ml[0] = m;
+                    ml[64] = l;
+                }
+                __syncthreads();
+                if (team < n) {
+                    const float most = fmaxf(m, ml[0]), f = weight_of(m, most), g = weight_of(ml[0], most);
+                    m = most;
+                    l = l * f + ml[64] * g;
+#pragma unroll
+                    for (uint32_t d = 0; d < S::kD; d++) o[d] = o[d] * f + *(const f32x4 *)(at + d * 1024) * g;
+                }
+            }
+        }
+        const float sum = live ? rows4_sum(l) : __builtin_nanf("");
+        const uint32_t l0 = again(lane), c = 16 * mine + (l0 & 15), g = l0 >> 4;
+        uint32_t r, h;
+        if (column_of(p, row0, block, c, r, h) && team == 0) {
+            if (partial) {
+#pragma unroll
+                for (uint32_t d = 0; d < S::kD; d++) *(f32x4 *)(partial + ((4 * d + g) * S::kCols + c) * 4) = o[d];
+                if (g == 0) {
+                    partial[RANK * S::kCols + c] = m;
+                    partial[RANK * S::kCols + S::kCols + c] = sum;
+                }
+            } else {
+                uint16_t *to = p.out + ((size_t)r * p.heads + h) * RANK + 4 * g;
+                const float by = 1.0f / sum;
+#pragma unroll
+                for (uint32_t d = 0; d < S::kD; d++)
+                    *(u32x2 *)(to + 16 * d) = u32x2{pack_bf16x2(o[d][0] * by, o[d][1] * by),
+                                                    pack_bf16x2(o[d][2] * by, o[d][3] * by)};
+            }
+        }
+        unit += b - a;
+        tile++;
+        if (unit >= end) return;
+        __syncthreads();
+    }
+}
+
+// The parts of tiles that several groups have: a group takes 16 columns and 64 values of O, a thread four of one
+// column. Tiles that one group had alone are out already.
+template <uint32_t RANK>
+__global__ __launch_bounds__(kJoinThreads) void join_latent_kernel(LatentParams p, uint32_t columns) {
+    uint32_t u = blockIdx.x;
+    const uint32_t piece = u % (RANK / 64), c0 = u / (RANK / 64) % (columns / 16) * 16;
+    u /= RANK / 64 * (columns / 16);
+    const uint32_t block = u % p.blocks, tile = u / p.blocks;
+    const uint32_t first = p.shares[2 * tile], parts = p.shares[2 * tile + 1];
+    if (parts < 2) return;
+    const uint32_t c = c0 + (threadIdx.x & 15), quad = piece * 16 + (threadIdx.x >> 4);
+    uint32_t r, h;
+    if (!column_of(p, tile * p.tile_rows, block, c, r, h)) return;
+    auto part_at = [&](uint32_t j) {
+        return p.partials + ((size_t)((j ? 0 : p.groups) + first + j) * p.blocks + block) * part_floats<RANK>(columns);
+    };
+    float most = -INFINITY, sum = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    constexpr uint32_t kBatch = 8;
+    for (uint32_t j0 = 0; j0 < parts; j0 += kBatch) {
+        float mq[kBatch], lq[kBatch];
+        f32x4 oq[kBatch];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) {
+            const float *at = part_at(min(j0 + j, parts - 1));
+            mq[j] = at[RANK * columns + c];
+            lq[j] = at[RANK * columns + columns + c];
+            oq[j] = *(const f32x4 *)(at + (quad * columns + c) * 4);
+        }
+        float top = most;
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) top = fmaxf(top, mq[j]);
+        const float f = weight_of(most, top);
+        most = top;
+        sum *= f;
+        o *= f;
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; j++) {
+            if (j0 + j >= parts) continue;
+            const float g = weight_of(mq[j], top);
+            // (A part that has seen nothing of the column holds no sums, but one that met a NaN has no maximum either.)
+            sum += mq[j] == -INFINITY ? lq[j] : lq[j] * g;
+            o += mq[j] == -INFINITY ? oq[j] : oq[j] * g;
+        }
+    }
+    o /= sum;
+    *(u32x2 *)(p.out + ((size_t)r * p.heads + h) * RANK + 4 * quad) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+}
+
+struct Plan {
+    uint32_t columns, block_heads, blocks, tile_rows, tiles, groups;
+    bool shared;
+};
+
+Plan plan(const ts_latent_args *k) {
+    const ts_rows_args *a = &k->rows;
+    Plan s;
+    const uint32_t run = std::max(1u, std::min(k->run, a->rows));
+    const uint64_t wanted = (uint64_t)run * a->heads;
+    s.columns = wanted <= 16 ? 16 : wanted <= 32 ? 32 : wanted <= 64 ? 64 : 128;
+    s.block_heads = std::min(a->heads, s.columns);
+    s.blocks = (a->heads - 1) / s.block_heads + 1;
+    s.tile_rows = std::max(1u, std::min(run, s.columns / s.block_heads));
+    s.tiles = (a->rows - 1) / s.tile_rows + 1;
+    s.groups = s.tiles;
+    s.shared = false;
+    const uint32_t at_once = std::max(1u, (k->rank == 512 || s.columns == 128 ? 256u : 512u) / s.blocks);  // a CU's one or two
+    const uint32_t unit = kKeys * (s.columns < 64 ? 64 / s.columns : 1);
+    const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
+                                             (uint64_t)a->back + s.tile_rows + kBlock);
+    const uint64_t units = (span + unit - 1) / unit + 1;
+    if (at_once > 1 && s.tiles <= std::min(kMaxTiles, 4 * at_once) && span > unit) {
+        s.groups = (uint32_t)std::min<uint64_t>(at_once, s.tiles * units);
+        s.shared = true;
+    }
+    return s;
+}
+
+size_t partial_bytes(const ts_latent_args *k, const Plan &s) {
+    return s.shared ? (size_t)s.groups * 2 * s.blocks * s.columns * (k->rank + 2) * sizeof(float) : 0;
+}
+size_t share_bytes(const Plan &s) { return s.shared ? (size_t)s.tiles * 2 * sizeof(uint32_t) : 0; }
+
+bool wide(const ts_latent_args *k) { return k->rank == 512 && k->rows.width == 576; }
+bool narrow(const ts_latent_args *k) { return k->rank == 256 && k->rows.width == 288; }
+
+int check(const ts_latent_args *k) {
+    TS_REQUIRE(k, "attend_latent: null args");
+    const ts_rows_args *a = &k->rows;
+    TS_REQUIRE(a->k && (a->rows == 0 || (a->q && a->out && a->slots && a->positions)), "attend_latent: null pointer");
+    TS_REQUIRE(wide(k) || narrow(k), "attend_latent: rows of %u values, %u of them latent (576 and 512, or 288 and 256)",
+               a->width, k->rank);
+    TS_REQUIRE(a->kv_heads == 1 && a->heads >= 1 && a->heads <= 1024, "attend_latent: %u heads over %u rows a position",
+               a->heads, a->kv_heads);
+    TS_REQUIRE(a->q_dtype == TS_BF16 && a->kv_dtype == TS_BF16 && a->out_dtype == TS_BF16,
+               "attend_latent: q, kept rows and out bf16 supported");
+    int rc = ts::kept_check("attend_latent", a->kept_table, a->page, a->keys, k->slot_count, a->kept_pages, k->pages, true);
+    if (rc) return rc;
+    TS_REQUIRE(a->keys <= 1u << 30, "attend_latent: %u positions a slot", a->keys);
+    TS_REQUIRE((uint64_t)k->pages * a->page <= 1ull << 36, "attend_latent: %u pages of %u rows", k->pages, a->page);
+    TS_REQUIRE(ts::aligned(a->k, 16) && ts::aligned(a->q, 16) && ts::aligned(a->out, 16),
+               "attend_latent: q, kept rows and out must be 16-byte aligned");
+    return TS_OK;
+}
+
+template <uint32_t RANK, uint32_t ROPE, uint32_t WC>
+int launch(const LatentParams &p, uint32_t groups, void *stream) {
+    using S = Shape<RANK, ROPE, WC>;
+    static const hipError_t attr = hipFuncSetAttribute((const void *)attend_latent_kernel<RANK, ROPE, WC>,
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+    if (attr != hipSuccess) return ts::hip_status(attr, "attend_latent: shared memory attribute");
+    hipLaunchKernelGGL((attend_latent_kernel<RANK, ROPE, WC>), dim3(groups), dim3(64 * S::kWaves), S::kLds, (hipStream_t)stream, p);
+    TS_CHECK_LAUNCH("attend_latent launch");
+    return TS_OK;
+}
+template <uint32_t RANK, uint32_t ROPE>
+int launch(const LatentParams &p, const Plan &s, void *stream) {
+    const uint32_t groups = s.groups * s.blocks;
+    const int rc = s.columns == 16 ? launch<RANK, ROPE, 1>(p, groups, stream)
+                   : s.columns == 32 ? launch<RANK, ROPE, 2>(p, groups, stream)
+                   : s.columns == 64 ? launch<RANK, ROPE, 4>(p, groups, stream)
+                                     : launch<RANK, ROPE, 8>(p, groups, stream);
+    if (rc || !s.shared) return rc;
+    hipLaunchKernelGGL(join_latent_kernel<RANK>, dim3(s.tiles * s.blocks * (s.columns / 16) * (RANK / 64)), dim3(kJoinThreads), 0,
+                       (hipStream_t)stream, p, s.columns);
+    TS_CHECK_LAUNCH("attend_latent join launch");
+    return TS_OK;
+}
+
+}  // namespace
+
+extern "C" size_t tessera_hip_attend_latent_workspace(const ts_latent_args *k) {
+    if (!k || k->rows.heads == 0 || k->rows.rows == 0 || !(wide(k) || narrow(k))) return 0;
+    const Plan s = plan(k);
+    return partial_bytes(k, s) + share_bytes(s);
+}
+
+extern "C" int tessera_hip_attend_latent(const ts_latent_args *k, void *stream) {
+    const int rc = check(k);
+    if (rc) return rc;
+    const ts_rows_args *a = &k->rows;
+    if (a->rows == 0) return TS_OK;
+    const Plan s = plan(k);
+    TS_REQUIRE((uint64_t)s.tiles * s.blocks <= 0x7fffffffull / 64, "attend_latent: %u rows in one launch", a->rows);
+    const size_t partials = partial_bytes(k, s), need = partials + share_bytes(s);
+    if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
+        return ts::fail(TS_ERR_WORKSPACE, "attend_latent: workspace of %zu bytes, 16-byte aligned, needed", need);
+    LatentParams p;
+    p.q = (const uint16_t *)a->q; p.kept = (const uint16_t *)a->k; p.out = (uint16_t *)a->out;
+    p.partials = need ? (float *)a->workspace : nullptr;
+    p.shares = need ? (uint32_t *)((char *)a->workspace + partials) : nullptr;
+    p.slots = a->slots; p.positions = a->positions; p.status = a->status;
+    p.place.table = a->kept_table; p.place.keys = a->keys; p.place.slot_count = k->slot_count;
+    p.place.kept_pages = a->kept_pages; p.place.page_shift = (uint32_t)__builtin_ctz(a->page); p.place.pages = k->pages;
+    p.rows = a->rows; p.heads = a->heads; p.back = a->back; p.max_position = a->max_position;
+    p.tile_rows = s.tile_rows; p.tiles = s.tiles; p.groups = s.groups;
+    p.block_heads = s.block_heads; p.blocks = s.blocks;
+    p.scale = a->scale;
+    return k->rank == 512 ? launch<512, 64>(p, s, stream) : launch<256, 32>(p, s, stream);
+}

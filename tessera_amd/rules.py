@@ -2,7 +2,7 @@
 
 Each function is named for the reference rule whose kernel it launches
 (``tiled``, ``lanes``, ``linear``, ``attend_rows``, ``flash_rows``, ``rms_norm``,
-``rope``, ``argmax``, ``top_k``, ``gather``; ``append_rows``, ``attend_kept8`` and ``verify``
+``rope``, ``argmax``, ``top_k``, ``gather``; ``append_rows``, ``attend_kept8``, ``verify`` and the latent ones
 have no rule of the reference beside them) and takes the same operands in the
 same order as that rule's Launch (reads, epilogue operands, output, counts:
 engine/plan/lower/src/abi.rs:148-153, product.rs:70-76, rule.rs:92-110).
@@ -640,3 +640,191 @@ def verify(logits, drafts, uniforms=None, *, counts=None, first=None, draft_prob
         a.workspace, a.workspace_bytes = scratch.data_ptr(), need
     _call_on(on, lib.tessera_hip_verify, a)
     return tokens, accepted
+
+
+# ---------------------------------------------------------------------------------------------
+# Latent attention: one kept row a position for all heads, absorbed and expanded forms.
+# ---------------------------------------------------------------------------------------------
+
+_BF16 = (torch.bfloat16,)
+
+
+def _rows_of(what, name, t, on, dtype, heads=None):
+    """The distances (of rows, of heads) of t [rows, heads, width], any of them where there is one row or head."""
+    rows, n, width = t.shape
+    if t.get_device() != on or t.dtype is not dtype or (t.stride(2) != 1 and width > 1) or (heads is not None and n != heads):
+        raise ValueError(f"{what}: {name} must be [rows, heads, width] of {str(dtype).replace('torch.', '')} on GPU {on}, a "
+                         "head's values back to back")
+    head = t.stride(1) if n > 1 else 0
+    row = t.stride(0) if rows > 1 else 0
+    if row >> 32 or head >> 32:
+        raise ValueError(f"{what}: {name} rows or heads more than 2^32 elements apart")
+    return row, head
+
+
+def append_latent(c, kept, slots, positions, *, keys, rank, gain=None, angles=None, halves=True, eps=1e-6, q=None,
+                  q_out=None, c_out=None, r_out=None, table=None, kept_pages=0, page=16, status=None):
+    """New rows of latent attention: c [rows, rank + rope] (f32 or bf16; rows any distance apart), its latent through
+    RmsNorm (with `gain` [rank]) and its last `rope` values through the rotation (with `angles`, rope_table's of width
+    `rope`, at least `keys` positions, or any scaled ones of its shape) into kept [*, rank + rope] bf16. q [rows, heads,
+    rope] (a view of wider heads serves) is rotated to q_out (a view too, f32 or bf16; made in q's type if not given).
+    c_out [rows, rank], r_out [rows, rope] bf16: the kept rows' values back to back. Rows without a place (position,
+    slot or page) are kept nowhere, their outputs are NaN, and status (int32 device word) tells of them. No two rows of
+    a call are for one place. Returns q_out."""
+    what = "append_latent"
+    rows, width = c.shape
+    on, x = c.get_device(), c.dtype
+    rope = width - rank
+    stride = c.stride(0) if rows > 1 else width
+    if x not in _ROWS or (c.stride(1) != 1 and width > 1) or stride >> 32:
+        raise ValueError("append_latent: c must be rows of f32 or bf16, a row's values back to back")
+    if kept.shape[-1] != width:
+        raise ValueError(f"append_latent: kept rows of {kept.shape[-1]} values for rows of {width}")
+    held = kept.numel() // width if width else 0
+    heads = q_row = q_head = o_row = o_head = q_type = 0
+    if q is not None:
+        heads = q.shape[1]
+        q_row, q_head = _rows_of(what, "q", q, on, x)
+        if q_out is None:
+            q_out = q.new_empty(rows, heads, rope)
+        elif q_out.dtype not in _ROWS:
+            raise ValueError("append_latent: q_out must be f32 or bf16")
+        o_row, o_head = _rows_of(what, "q_out", q_out, on, q_out.dtype, heads)
+        if q.shape != (rows, heads, rope) or q_out.shape != (rows, heads, rope):
+            raise ValueError(f"append_latent: q and q_out must be {[rows, heads, rope]}")
+        q_type = _DT[q_out.dtype]
+    if not (on >= 0 and kept.get_device() == slots.get_device() == positions.get_device() == on
+            and kept.dtype is torch.bfloat16 and kept.is_contiguous() and slots.dtype in _INTS and positions.dtype in _INTS
+            and slots.numel() == positions.numel() == rows and slots.is_contiguous() and positions.is_contiguous()
+            and (table is None or table.get_device() == on and table.dtype in _INTS and table.is_contiguous())
+            and (gain is None or gain.get_device() == on and gain.dtype is torch.float32 and gain.numel() == rank
+                 and gain.is_contiguous())
+            and (angles is None or angles.get_device() == on and angles.dtype is torch.float32 and angles.is_contiguous())
+            and (c_out is None or c_out.get_device() == on and c_out.dtype is torch.bfloat16
+                 and c_out.numel() == rows * rank and c_out.is_contiguous())
+            and (r_out is None or r_out.get_device() == on and r_out.dtype is torch.bfloat16
+                 and r_out.numel() == rows * rope and r_out.is_contiguous())
+            and (status is None or status.get_device() == on and status.dtype in _INTS)):
+        _checked(what, on, ("kept", kept, _BF16, -1), ("slots", slots, _INTS, rows), ("positions", positions, _INTS, rows),
+                 ("table", table, _INTS, -1), ("gain", gain, _F32, rank), ("angles", angles, _F32, -1),
+                 ("c_out", c_out, _BF16, rows * rank), ("r_out", r_out, _BF16, rows * rope), ("status", status, _INTS, -1))
+    a = abi.AppendLatentArgs(c.data_ptr(), None if q is None else q.data_ptr(), None if gain is None else gain.data_ptr(),
+                             None if angles is None else angles.data_ptr(), None if q is None else q_out.data_ptr(),
+                             kept.data_ptr(), None if c_out is None else c_out.data_ptr(),
+                             None if r_out is None else r_out.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+                             None if table is None else table.data_ptr(), None if status is None else status.data_ptr(),
+                             rows, heads, rank, rope, stride, q_row, q_head, o_row, o_head, keys,
+                             _slots(what, table, kept_pages, held, keys), kept_pages, page, _pages(table, held, page),
+                             0 if angles is None or not rope else angles.numel() // rope, halves, _DT[x], q_type, eps)
+    _call_on(on, abi.load().tessera_hip_append_latent, a)
+    return q_out
+
+
+def linear_heads(x, w, *, out=None, out_dtype=torch.float32):
+    """A product a head: out[r, h] = w[h] x[r, h]. x [rows, heads, k] f32 or bf16 and out [rows, heads, n] f32 or bf16
+    may be views of wider rows and heads; w [heads, n, k] bf16, heads any distance apart. (q into the latent space with
+    w [heads, rank, nope], latent sums out of it with w [heads, value, rank].)"""
+    what = "linear_heads"
+    on, dtype = x.get_device(), x.dtype
+    rows, heads, k = x.shape
+    n = w.shape[1]
+    x_row, x_head = _rows_of(what, "x", x, on, dtype)
+    w_head = w.stride(0) if heads > 1 else 0
+    if out is None:
+        out = x.new_empty(rows, heads, n, dtype=out_dtype)
+    o_row, o_head = _rows_of(what, "out", out, on, out.dtype, heads)
+    if on < 0 or dtype not in _ROWS or out.dtype not in _ROWS or out.shape != (rows, heads, n):
+        raise ValueError(f"linear_heads: x and out [rows, heads, *] must be f32 or bf16 on a GPU, out {[rows, heads, n]}")
+    if w.shape != (heads, n, k) or w.get_device() != on or w.dtype is not torch.bfloat16 or \
+            (w.stride(2) != 1 and k > 1) or (w.stride(1) != k and n > 1):
+        raise ValueError(f"linear_heads: w must be bf16 {[heads, n, k]} on GPU {on}, a head's rows back to back")
+    a = abi.HeadsArgs(x.data_ptr(), w.data_ptr(), out.data_ptr(), rows, heads, n, k, x_row, x_head, o_row, o_head, w_head,
+                      _DT[dtype], _DT[out.dtype])
+    _call_on(on, abi.load().tessera_hip_linear_heads, a)
+    return out
+
+
+def attend_latent(q, kept, slots, positions, *, keys, rank, scale, table=None, kept_pages=0, page=16, back=abi.U32_MAX,
+                  run=1, max_position=None, out=None, status=None):
+    """The absorbed form of latent attention: q [rows, heads, rank + rope] bf16 (the absorbed part, then the rotated one)
+    over kept [*, rank + rope] bf16; out [rows, heads, rank] bf16, each row's weighted sum of latents. run: how many rows
+    of a slot stand together (a hint: it groups rows and picks the kernel). max_position (an upper bound on positions)
+    defaults to their maximum (a host read: pass it when capturing a graph)."""
+    what = "attend_latent"
+    rows, heads, width = q.shape
+    on = q.get_device()
+    if kept.shape[-1] != width:
+        raise ValueError(f"attend_latent: kept rows of {kept.shape[-1]} values for q of {width}")
+    held = kept.numel() // width if width else 0
+    if out is None:
+        out = q.new_empty(rows, heads, rank)
+    elif out.shape != (rows, heads, rank):
+        raise ValueError(f"attend_latent: out must be {[rows, heads, rank]}")
+    bf16 = torch.bfloat16
+    if not (on >= 0 and kept.get_device() == slots.get_device() == positions.get_device() == out.get_device() == on
+            and q.dtype is bf16 and kept.dtype is bf16 and out.dtype is bf16 and slots.dtype in _INTS
+            and positions.dtype in _INTS and slots.numel() == positions.numel() == rows and q.is_contiguous()
+            and kept.is_contiguous() and slots.is_contiguous() and positions.is_contiguous() and out.is_contiguous()
+            and (table is None or table.get_device() == on and table.dtype in _INTS and table.is_contiguous())
+            and (status is None or status.get_device() == on and status.dtype in _INTS)):
+        _checked(what, on, ("q", q, _BF16, -1), ("kept", kept, _BF16, -1), ("slots", slots, _INTS, rows),
+                 ("positions", positions, _INTS, rows), ("table", table, _INTS, -1), ("out", out, _BF16, -1),
+                 ("status", status, _INTS, -1))
+    if max_position is None:
+        # (as int32, which has a maximum; a position from 2^31 on is past any slot's)
+        max_position = int(positions.view(torch.int32).max().item()) if rows else 0
+    a = abi.LatentArgs(abi.RowsArgs(q.data_ptr(), kept.data_ptr(), None, out.data_ptr(), slots.data_ptr(),
+                                    positions.data_ptr(), None if table is None else table.data_ptr(), None, 0, rows, keys,
+                                    heads, 1, width, back, kept_pages, page, scale, abi.TS_BF16, abi.TS_BF16, abi.TS_BF16,
+                                    max_position, None if status is None else status.data_ptr()),
+                       rank, _slots(what, table, kept_pages, held, keys), _pages(table, held, page), run)
+    lib = abi.load()
+    need = lib.tessera_hip_attend_latent_workspace(a)
+    if need:
+        scratch = slots.new_empty((need + 3) // 4)
+        a.rows.workspace, a.rows.workspace_bytes = scratch.data_ptr(), need
+    _call_on(on, lib.tessera_hip_attend_latent, a)
+    return out
+
+
+def flash_latent(q, k, v, r, *, scale, first=None, key_first=None, back=abi.U32_MAX, out=None):
+    """The expanded form of latent attention over whole sequences packed back to back, causal, ends aligned (a row of a
+    sequence of n rows and m keys stands at m - n + its number) and with a window of `back` keys before its own: q [rows,
+    heads, nope + rope] bf16 (rows any distance apart), k [keys, heads, nope] and v [keys, heads, value] bf16 (views of
+    one product's rows serve), r [keys, rope] bf16: the keys' rotated part, all heads'. first [seqs + 1]: each sequence's
+    first row, then the end (None: one sequence); key_first: the same of the keys (None: first's). Returns out [rows,
+    heads, value] bf16; rows outside the sequences are left as they were, rows that see no key are zero."""
+    what = "flash_latent"
+    rows, heads, width = q.shape
+    on, bf16 = q.get_device(), torch.bfloat16
+    key_rows, _, nope = k.shape
+    value, rope = v.shape[-1], r.shape[-1]
+    q_row, q_head = _rows_of(what, "q", q, on, bf16)
+    k_row, k_head = _rows_of(what, "k", k, on, bf16, heads)
+    v_row, v_head = _rows_of(what, "v", v, on, bf16, heads)
+    if (heads > 1 and q_head != width) or width != nope + rope or v.shape[0] != key_rows:
+        raise ValueError("flash_latent: q [rows, heads, nope + rope] with a row's heads back to back, k [keys, heads, nope], "
+                         "v [keys, heads, value] and r [keys, rope]")
+    if r.shape != (key_rows, rope) or r.get_device() != on or r.dtype is not bf16 or (r.stride(1) != 1 and rope > 1):
+        raise ValueError(f"flash_latent: r must be bf16 {[key_rows, rope]} on GPU {on}, a row's values back to back")
+    r_row = r.stride(0) if key_rows > 1 else 0
+    if out is None:
+        out = q.new_empty(rows, heads, value)
+    elif out.shape != (rows, heads, value):
+        raise ValueError(f"flash_latent: out must be {[rows, heads, value]}")
+    if first is None and key_first is not None:
+        raise ValueError("flash_latent: key_first without first")
+    seqs = 1 if first is None else first.numel() - 1
+    if seqs < 0:
+        raise ValueError("flash_latent: first must hold each sequence's first row and the end")
+    if not (on >= 0 and out.get_device() == on and out.dtype is bf16 and out.is_contiguous()
+            and (first is None or first.get_device() == on and first.dtype in _INTS and first.is_contiguous())
+            and (key_first is None or key_first.get_device() == on and key_first.dtype in _INTS
+                 and key_first.numel() == seqs + 1 and key_first.is_contiguous())):
+        _checked(what, on, ("out", out, _BF16, -1), ("first", first, _INTS, -1), ("key_first", key_first, _INTS, seqs + 1))
+    a = abi.FlashLatentArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.data_ptr(), out.data_ptr(),
+                            None if first is None else first.data_ptr(), None if key_first is None else key_first.data_ptr(),
+                            rows, key_rows, seqs, heads, nope, rope, value, q_row or heads * width, k_row, k_head, v_row,
+                            v_head, r_row, back, scale)
+    _call_on(on, abi.load().tessera_hip_flash_latent, a)
+    return out
