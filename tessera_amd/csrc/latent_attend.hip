@@ -11,17 +11,23 @@
 //  * Keys are dealt to the groups in equal runs over all tiles, so that groups end together however the sequences
 //    differ in length; a tile that several groups have is joined by a second kernel.
 #include <algorithm>
+#include <stdlib.h>
 
 #include "kept8_attend.h"
+#include "latent.h"
 
 namespace {
 
 using namespace kept8;
+using namespace latent;
 
 constexpr uint32_t kKeys = 32;         // keys of a step
 constexpr uint32_t kMaxTiles = 1024;   // row tiles whose keys are shared
 constexpr uint32_t kJoinThreads = 256;
-constexpr uint32_t kAhead = 2;         // operands read ahead of their products
+#ifndef KAH
+#define KAH 3
+#endif
+constexpr uint32_t kAhead = KAH;         // operands read ahead of their products
 
 struct LatentParams {
     const uint16_t *q, *kept;
@@ -61,25 +67,6 @@ TS_DEV uint32_t swap_of(uint32_t row) {
     return ((i ^ i >> 1) & 1) << 1 | i >> 1;
 }
 
-typedef short ts_v4i16 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) ts_v4i16 lds_v4i16;
-// Four keys of one d, from the 8-byte pieces of four rows (lane 4 e + c of 16: row e, d 4 c ..).
-TS_DEV u32x2 read_vt4(const char *a) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *)a));
-}
-
-// The bits of the bf16 values of a pair that are not finite. (All ones are a NaN.)
-TS_DEV uint32_t odd_mask(uint32_t x) {
-    return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-}
-
-// A lane's number that what follows is computed from where it is used: rare steps' addresses would otherwise be
-// computed ahead of the loops, and push what the common ones use out of the registers.
-TS_DEV uint32_t again(uint32_t v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
 // 2^(a - b) of maxima, 0 where a has seen nothing.
 TS_DEV float weight_of(float a, float b) { return a == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(a - b); }
 
@@ -105,11 +92,13 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     using S = Shape<RANK, ROPE, WC>;
     constexpr uint32_t kThreads = 64 * S::kWaves;
     extern __shared__ __attribute__((aligned(16))) char stage[];
-    __shared__ uint32_t starts[kMaxTiles + 1], words[S::kWaves], odd_keys[S::kWaves], found;
+    __shared__ uint32_t starts[kMaxTiles + 1], words[S::kWaves], odd_met[S::kWaves], found;
     __shared__ uint32_t from_aside[S::kAside ? S::kOwn : 1][S::kAside ? kThreads : 1];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4, team = wave / WC, mine = wave % WC;
-    const uint32_t u = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
+    // Groups go to the eight XCDs in turn: those of a tile's blocks of heads, which read the same keys, to one.
+    const uint32_t block = (blockIdx.x >> 3) % p.blocks, u = (blockIdx.x >> 3) / p.blocks * 8 + (blockIdx.x & 7);
+    if (u >= p.groups) return;
 
     // The group's units of keys: a row tile is as many as its rows see, all tiles' one behind the other are dealt to
     // the groups in equal runs. (A tile's units are told from its first and last row.)
@@ -275,8 +264,8 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 return gone;
             };
             auto issue = [&](uint32_t round, uint32_t slot_of_ring) {
-                char *to = stage + (slot_of_ring * S::kTeams + team) * S::kTile;
-                __amdgpu_buffer_rsrc_t buf[2];
+                const uint32_t to = lds_address(stage) + (slot_of_ring * S::kTeams + team) * S::kTile;
+                u32x4 buf[2];
 #pragma unroll
                 for (uint32_t i = 0; i < 2; i++) {
                     uint32_t page = id[0], key = key_of(round, 0);
@@ -288,7 +277,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                         }
                     bool lost;
                     const uint32_t kept_block = block_in(p.place, now, page, key, lost);
-                    buf[i] = raw_buffer((const char *)p.kept + (size_t)kept_block * (kBlock * S::kRow));
+                    buf[i] = rows_buffer((const char *)p.kept + (size_t)kept_block * (kBlock * S::kRow));
                 }
                 uint32_t from[S::kOwn];
 #pragma unroll
@@ -298,68 +287,81 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     const uint32_t part = mine + i * WC;
                     if (S::kLoads != S::kLeast && part >= S::kParts) break;
                     const bool on = WC == 1 && S::kParts == 36 && (i / 9 & 1);
-                    buffer_to_lds16(part < S::kParts / 2 ? buf[0] : buf[1], to + part * 1024,
-                                    on ? from[i % S::kOwn] ^ 48 : from[i % S::kOwn], on ? 8 * S::kRow : 0);
+                    rows_to_lds16(part < S::kParts / 2 ? buf[0] : buf[1], to + part * 1024,
+                                  on ? (from[i % S::kOwn] ^ 48) + 8 * S::kRow : from[i % S::kOwn]);
                 }
             };
 
-            // One step: the wave's columns against the keys here .. here + 31 at `at`.
-            auto step = [&](uint32_t here, char *at, uint32_t gone, bool apart) {
-                // Register i of s[t]: key 16 t + 4 grp + i.
-                f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                const uint32_t k0 = again(koff), v0 = again(voff);
-                // Operands are read kAhead products ahead: left to itself, the compiler reads all it has registers for, or
-                // one at a time and waits for each.
-                bf16x8 ahead[2][kAhead];
-                auto read_k = [&](uint32_t x) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kAhead; i++) {
-                        const uint32_t j = (x * kAhead + i) / 2, t = (x * kAhead + i) % 2;
-                        ahead[x & 1][i] = *(const bf16x8 *)(at + (k0 ^ j % (S::kXor / 4) * 64) +
-                                                            j / (S::kXor / 4) * (S::kXor * 16) + t * kBlock * S::kRow);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+            // A step is the wave's columns against the keys here .. here + 31 at `at`. Its scores: register i of s[t] is key
+            // 16 t + 4 grp + i. Operands are read kAhead products ahead: left to itself, the compiler reads all it has
+            // registers for, or one at a time and waits for each. `beside(i)` is done after the i-th product.
+            auto scores = [&](const char *at, f32x4 (&s)[2], auto beside) {
+                const uint32_t k0 = again(koff);
+                bf16x8 ring[kAhead + 1];
+                auto read_k = [&](uint32_t i) {
+                    const uint32_t j = i / 2, t = i % 2;
+                    ring[i % (kAhead + 1)] = *(const bf16x8 *)(at + (k0 ^ j % (S::kXor / 4) * 64) +
+                                                               j / (S::kXor / 4) * (S::kXor * 16) + t * kBlock * S::kRow);
                 };
-                constexpr uint32_t kReads = 2 * S::kQ / kAhead;
-                static_assert(2 * S::kQ % kAhead == 0 && S::kD % kAhead == 0, "whole batches");
-                read_k(0);
+                s[0] = s[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (uint32_t x = 0; x < kReads; x++) {
-                    if (x + 1 < kReads) read_k(x + 1);
+                for (uint32_t i = 0; i < kAhead; i++) read_k(i);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (uint32_t i = 0; i < kAhead; i++) {
-                        const uint32_t j = (x * kAhead + i) / 2, t = (x * kAhead + i) % 2;
-                        s[t] = mfma16(ahead[x & 1][i], q[j], s[t]);
-                    }
+                for (uint32_t i = 0; i < 2 * S::kQ; i++) {
+                    if (i + kAhead < 2 * S::kQ) read_k(i + kAhead);
+                    s[i % 2] = mfma16(ring[i % (kAhead + 1)], q[i / 2], s[i % 2]);
+                    beside(i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (here < all_lo || here + (kKeys - 1) > all_hi || gone) {
-                    const int upto = act ? (int)(pos - here) - 4 * (int)grp : -1, since = (int)(from - here) - 4 * (int)grp;
+            };
+            auto masked = [&](uint32_t here, uint32_t gone, f32x4 (&s)[2]) {
+                if (here >= all_lo && here + (kKeys - 1) <= all_hi && !gone) return;
+                const int upto = act ? (int)(pos - here) - 4 * (int)grp : -1, since = (int)(from - here) - 4 * (int)grp;
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const bool seen = 16 * t + i <= upto && 16 * t + i >= since;
-                            s[t][i] = seen ? (gone >> t & 1 ? __builtin_nanf("") : s[t][i]) : -INFINITY;
-                        }
-                }
-                float mx = s[0][0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i / 4][i % 4]);
-                mx = rows4_max(mx) * sl;
-                const bool raise = mx > m + kSlack;
-                const float mn = raise ? mx : m, mo = mn == -INFINITY ? 0.0f : mn;
-                uint32_t pw[4][S::kWeights];
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sl, -mo));
-                    const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4 + 1], sl, -mo));
+                    for (int i = 0; i < 4; i++) {
+                        const bool seen = 16 * t + i <= upto && 16 * t + i >= since;
+                        s[t][i] = seen ? (gone >> t & 1 ? __builtin_nanf("") : s[t][i]) : -INFINITY;
+                    }
+            };
+            // The softmax of a step in kSoft pieces: weights 2^(score - m) in bf16 parts. m moves only when a score passes it
+            // by 2^kSlack, so most steps leave the sum and O as they are and no weight passes 2^kSlack.
+            constexpr uint32_t kSoft = 8;
+            float mx, mn, mo, sum;
+            uint32_t pw[4][S::kWeights];
+            auto soft = [&](uint32_t i, const f32x4 (&s)[2]) {
+                if (i == 0) {
+                    mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                               fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+                } else if (i == 1) {
+                    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                    mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+                } else if (i == 2) {
+                    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                    mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) * sl;
+                } else if (i == 3) {
+                    mn = mx > m + kSlack ? mx : m;
+                    mo = mn == -INFINITY ? 0.0f : mn;
+                    pinned(mn);
+                    pinned(mo);
+                    sum = 0.0f;
+                } else if (i < kSoft) {
+                    const uint32_t t = (i - 4) / 2, e = (i - 4) % 2 * 2;
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][e], sl, -mo));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], sl, -mo));
                     sum += x + y;
-                    split_pair<S::kWeights>(x, y, pw[i / 2]);
+                    split_pair<S::kWeights>(x, y, pw[i - 4]);
+#pragma unroll
+                    for (uint32_t f = 0; f < S::kWeights; f++) pinned(pw[i - 4][f]);
+                    pinned(sum);
                 }
-                if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-                    const float alpha = raise ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+            };
+            // The step's weights times its values, onto O.
+            auto product = [&](uint32_t here, char *at, bool apart) {
+                if (__builtin_amdgcn_ballot_w64(mn > m) != 0) {
+                    const float alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
                     l *= alpha;
                     m = mn;
 #pragma unroll
@@ -369,80 +371,76 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 u32x4 w[S::kWeights];
 #pragma unroll
                 for (uint32_t e = 0; e < S::kWeights; e++) w[e] = u32x4{pw[0][e], pw[1][e], pw[2][e], pw[3][e]};
-                // V^T: d 16 dt + col of keys 4 grp .. and 16 + 4 grp .. (eight of them).
-                auto read_v = [&](uint32_t d) {
-                    const char *v = at + d / (S::kXor / 2) * (S::kXor * 16) + (v0 ^ d % (S::kXor / 2) * 32);
-                    const u32x2 lo4 = read_vt4(v), hi4 = read_vt4(v + kBlock * S::kRow);
-                    return u32x4{lo4.x, lo4.y, hi4.x, hi4.y};
-                };
                 if (apart) {
                     // Some key here is one column's and not another's. A value that is not finite must reach the former
                     // alone, and the product's 0 times it would be NaN: such values are looked for, become NaN where they
                     // are seen (their key's score is infinite or NaN as well, so the column's sum can be nothing else), and
                     // are cleared. (By all waves of the group together, but where each has keys of its own.)
-                    uint32_t bad = 0;  // keys that hold one
-#pragma unroll 1
-                    for (uint32_t k = mine; k < kKeys; k += WC) {
-                        const uint32_t *x = (const uint32_t *)(at + k * S::kRow) + again(lane) * (RANK / 128);
-                        uint32_t odd = 0;
+                    uint32_t odd = 0;
+#pragma unroll 2
+                    for (uint32_t g = mine * 64 + again(lane); g < kKeys * RANK / 8; g += 64 * WC) {
+                        const u32x4 x = *(const u32x4 *)(at + g / (RANK / 8) * S::kRow + g % (RANK / 8) * 16);
 #pragma unroll
-                        for (uint32_t e = 0; e < RANK / 128; e++)
-                            odd |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
-                        bad |= __builtin_amdgcn_ballot_w64(odd) != 0 ? 1u << k : 0u;
+                        for (uint32_t e = 0; e < 4; e++) odd |= odd_mask(x[e]);
                     }
-                    uint32_t any = bad;
+                    uint32_t any = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
                     if (WC > 1) {
-                        odd_keys[wave] = bad;
+                        odd_met[wave] = any;
                         lds_barrier();
-                        any = bad = 0;
 #pragma unroll
-                        for (uint32_t i = 0; i < S::kWaves; i++) {
-                            const uint32_t x = __builtin_amdgcn_readfirstlane(odd_keys[i]);
-                            any |= x;
-                            bad |= i / WC == team ? x : 0u;
-                        }
-                    }
-                    for (uint32_t left = bad; left;) {
-                        const uint32_t k = __builtin_ctz(left), swap = swap_of<S::kPieces>(k), g = again(grp);
-                        left &= left - 1;
-                        const uint32_t keep = act && here + k <= pos && here + k >= from ? 0xffffffffu : 0u;
-                        const char *row = at + k * S::kRow + 8 * (g & 1);
-#pragma unroll
-                        for (uint32_t d = 0; d < S::kD; d++) {
-                            u32x2 x = *(const u32x2 *)(row + ((2 * d + (g >> 1)) ^ swap) * 16);
-                            x = u32x2{odd_mask(x[0]), odd_mask(x[1])} & keep;
-                            o[d] += f32x4{lo_bf16(x[0]), hi_bf16(x[0]), lo_bf16(x[1]), hi_bf16(x[1])};
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
+                        for (uint32_t i = 0; i < S::kWaves; i++) any |= __builtin_amdgcn_readfirstlane(odd_met[i]);
                     }
                     if (any) {
+#pragma unroll 1
+                        for (uint32_t k = 0; k < kKeys; k++) {
+                            const uint32_t swap = swap_of<S::kPieces>(k), g = again(grp);
+                            const uint32_t keep = act && here + k <= pos && here + k >= from ? 0xffffffffu : 0u;
+                            const char *row = at + k * S::kRow + 8 * (g & 1);
+#pragma unroll
+                            for (uint32_t d = 0; d < S::kD; d++) {
+                                u32x2 x = *(const u32x2 *)(row + ((2 * d + (g >> 1)) ^ swap) * 16);
+                                x = u32x2{odd_mask(x[0]), odd_mask(x[1])} & keep;
+                                o[d] += f32x4{lo_bf16(x[0]), hi_bf16(x[0]), lo_bf16(x[1]), hi_bf16(x[1])};
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
                         if (WC > 1) lds_barrier();
 #pragma unroll 1
                         for (uint32_t k = mine; k < kKeys; k += WC) {
                             uint32_t *x = (uint32_t *)(at + k * S::kRow) + again(lane) * (RANK / 128);
-                            if (bad >> k & 1)
 #pragma unroll
-                                for (uint32_t e = 0; e < RANK / 128; e++) x[e] &= ~odd_mask(x[e]);
+                            for (uint32_t e = 0; e < RANK / 128; e++) x[e] &= ~odd_mask(x[e]);
                         }
                         if (WC > 1) lds_barrier();
                     }
                 }
-                auto read_batch = [&](uint32_t x) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kAhead; i++) ahead[x & 1][i] = as_bf16x8(read_v(x * kAhead + i));
-                    __builtin_amdgcn_sched_barrier(0);
+                // V^T: d 16 dt + col of keys 4 grp .. and 16 + 4 grp .. (eight of them).
+                const uint32_t v0 = again(voff);
+                u32x4 ring[kAhead + 1];
+                auto read_v = [&](uint32_t d) {
+                    const char *v = at + d / (S::kXor / 2) * (S::kXor * 16) + (v0 ^ d % (S::kXor / 2) * 32);
+                    const u32x2 lo4 = read_vt4(v), hi4 = read_vt4(v + kBlock * S::kRow);
+                    ring[d % (kAhead + 1)] = u32x4{lo4.x, lo4.y, hi4.x, hi4.y};
                 };
-                read_batch(0);
 #pragma unroll
-                for (uint32_t x = 0; x < S::kD / kAhead; x++) {
-                    if (x + 1 < S::kD / kAhead) read_batch(x + 1);
+                for (uint32_t i = 0; i < kAhead; i++) read_v(i);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (uint32_t i = 0; i < kAhead; i++)
+                for (uint32_t i = 0; i < S::kD; i++) {
+                    if (i + kAhead < S::kD) read_v(i + kAhead);
 #pragma unroll
-                        for (uint32_t e = 0; e < S::kWeights; e++)
-                            o[x * kAhead + i] = mfma16(ahead[x & 1][i], as_bf16x8(w[e]), o[x * kAhead + i]);
+                    for (uint32_t e = 0; e < S::kWeights; e++)
+                        o[i] = mfma16(as_bf16x8(ring[i % (kAhead + 1)]), as_bf16x8(w[e]), o[i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+            };
+            auto step = [&](uint32_t here, char *at, uint32_t gone, bool apart) {
+                f32x4 s[2];
+                scores(at, s, [](uint32_t) {});
+                masked(here, gone, s);
+#pragma unroll
+                for (uint32_t i = 0; i < kSoft; i++) soft(i, s);
+                product(here, at, apart);
             };
             // Rows of a step that no column of the pass sees, or of no page, are zero in the products.
             auto clear = [&](uint32_t here, char *at, uint32_t gone) {
@@ -469,8 +467,10 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     step(here, at, gone, differ(here, kKeys));
                 }
             } else {
-                // kRing - 1 rounds on their way.
-                constexpr uint32_t kLater = S::kRing > 1 ? (S::kRing - 2) * S::kLeast : 0;
+                // kRing - 1 rounds on their way. With four the next round's scores are worked out beside this one's softmax
+                // (the matrix unit would wait for it), so the next round must have come.
+                constexpr bool kPipe = false && S::kRing == 4;
+                constexpr uint32_t kLater = (S::kRing - 2 - kPipe) * S::kLeast;
                 uint32_t gone[S::kRing], n = 0;
                 look(unit0);
 #pragma unroll
@@ -478,6 +478,15 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     gone[i] = gone_of();
                     if (unit0 + i < unit1) issue(unit0 + i, i);
                     look(min(unit0 + i + 1, unit1 - 1));
+                }
+                auto useful = [&](uint32_t here) { return here <= whi && here + (kKeys - 1) >= wlo; };
+                f32x4 s[2];
+                if (kPipe) {
+                    if (unit1 - unit0 >= 3)
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * S::kLeast) : "memory");
+                    else
+                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    scores(stage, s, [](uint32_t) {});
                 }
                 for (uint32_t round = unit0; round < unit1; round++) {
                     if (unit1 - round >= S::kRing - 1)
@@ -497,8 +506,25 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                         lds_barrier();
                     }
                     const bool apart = differ(here, S::kUnit);
-                    if (apart || (at_here <= whi && at_here + (kKeys - 1) >= wlo)) step(at_here, at, lost, apart);
                     n = n + 1 == S::kRing ? 0 : n + 1;
+                    if (kPipe) {
+                        const char *then = stage + n * S::kTile;  // (of the last round whatever is there: not used)
+                        if (apart || useful(at_here)) {
+                            masked(at_here, lost, s);
+                            f32x4 t[2];
+                            constexpr uint32_t kEvery = 2 * S::kQ / kSoft;
+                            scores(then, t, [&](uint32_t i) {
+                                if (i % kEvery == 0) soft(i / kEvery, s);
+                            });
+                            product(at_here, at, apart);
+                            s[0] = t[0];
+                            s[1] = t[1];
+                        } else if (useful(at_here + kKeys)) {
+                            scores(then, s, [](uint32_t) {});
+                        }
+                    } else if (apart || useful(at_here)) {
+                        step(at_here, at, lost, apart);
+                    }
 #pragma unroll
                     for (uint32_t i = 0; i + 1 < S::kRing; i++) gone[i] = gone[i + 1];
                 }
@@ -617,6 +643,7 @@ Plan plan(const ts_latent_args *k) {
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
     const uint64_t wanted = (uint64_t)run * a->heads;
     s.columns = wanted <= 16 ? 16 : wanted <= 32 ? 32 : wanted <= 64 ? 64 : 128;
+    if (getenv("TSC")) s.columns = atoi(getenv("TSC"));
     s.block_heads = std::min(a->heads, s.columns);
     s.blocks = (a->heads - 1) / s.block_heads + 1;
     s.tile_rows = std::max(1u, std::min(run, s.columns / s.block_heads));
@@ -674,7 +701,7 @@ int launch(const LatentParams &p, uint32_t groups, void *stream) {
 }
 template <uint32_t RANK, uint32_t ROPE>
 int launch(const LatentParams &p, const Plan &s, void *stream) {
-    const uint32_t groups = s.groups * s.blocks;
+    const uint32_t groups = (s.groups + 7) / 8 * 8 * s.blocks;
     const int rc = s.columns == 16 ? launch<RANK, ROPE, 1>(p, groups, stream)
                    : s.columns == 32 ? launch<RANK, ROPE, 2>(p, groups, stream)
                    : s.columns == 64 ? launch<RANK, ROPE, 4>(p, groups, stream)

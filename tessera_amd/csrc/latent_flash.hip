@@ -4,15 +4,18 @@
 //
 // A wave has 32 rows of one head, the columns of S^T = K q^T and O^T = V^T P^T on the 32-wide matrix products, so a
 // row's scores stay in two lanes and P^T is the second product's operand as it stands. The four waves of a group have
-// 128 neighbouring rows and share the keys, 32 a step: k, r and v rows go from memory straight to LDS, two steps ahead
-// of their use; V^T comes through the transposing LDS read. Two groups share a CU, so that one's softmax runs under the
-// other's products.
-#include "common.h"
+// 128 neighbouring rows and share the keys, 64 a step: k, r and v rows go from memory straight to LDS, a step ahead of
+// their use; V^T comes through the transposing LDS read. Two groups share a CU (all of its LDS: there is none besides
+// the steps'), so that one's softmax runs under the other's products.
+#include "latent.h"
 
 namespace {
 
-constexpr uint32_t kWaves = 4, kThreads = 64 * kWaves, kRows = 32 * kWaves, kKeys = 32, kRing = 3;
-constexpr uint32_t kMaxOrder = 256;  // row tiles that are ordered by cost
+using namespace latent;
+
+constexpr uint32_t kWaves = 4, kThreads = 64 * kWaves, kRows = 32 * kWaves, kKeys = 64, kRing = 2;
+constexpr uint32_t kAhead = 4;       // operands read ahead of their products
+constexpr int kCostBits = 12;  // of the steps that tiles are ordered by
 constexpr float kSlack = 8.0f;       // base-2 headroom of the softmax reference point
 
 struct FlashParams {
@@ -57,17 +60,11 @@ TS_DEV uint32_t tiles_upto(const FlashParams &p, uint32_t s, Sequence &q, uint32
     }
     return upto;
 }
-// How many keys the rows of a sequence's tile t see (of its last row, at most `back` and its own).
-TS_DEV uint32_t span_of(const FlashParams &p, const Sequence &q, uint32_t t) {
+// The steps that a sequence's tile t takes (as far as kCostBits tell), and one.
+TS_DEV uint32_t cost_of(const FlashParams &p, const Sequence &q, uint32_t t) {
     const int64_t last = (int64_t)q.m - q.n + min((t + 1) * kRows, q.n);
-    return last <= 0 ? 0 : (uint32_t)min(last, (int64_t)p.back + kRows);
-}
-
-typedef short ts_v4i16 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) ts_v4i16 lds_v4i16;
-// Four keys of one d, from the 8-byte pieces of four rows (lane 4 e + c of 16: row e, d 4 c ..).
-TS_DEV u32x2 read_vt4(const char *a) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *)a));
+    const uint32_t keys = last <= 0 ? 0 : (uint32_t)min(last, (int64_t)p.back + kRows);
+    return min(keys / kKeys, (1u << kCostBits) - 2) + 1;
 }
 TS_DEV float halves_max(float x) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -80,15 +77,6 @@ TS_DEV float halves_sum(float x) {
 TS_DEV uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(ts_f32x2{a, b}, ts_bf16x2));
 }
-// The bits of the bf16 values of a pair that are not finite.
-TS_DEV uint32_t odd_mask(uint32_t x) {
-    return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-}
-TS_DEV uint32_t again(uint32_t v) {  // (keeps rare steps' addresses from being computed ahead of the loop)
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
 // The XOR of a row's 16-byte pieces in LDS, of P pieces: the 16 rows that an operand's read serves at once meet 16
 // places (LDS serves 256 bytes at a time); the four rows by four pieces of a transposing read likewise.
 template <uint32_t P>
@@ -106,44 +94,63 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
     constexpr uint32_t kK = kKeys * NOPE * 2, kR = kKeys * ROPE * 2, kV = kKeys * VALUE * 2, kStage = kK + kR + kV;
     constexpr uint32_t kD = VALUE / 32;
     extern __shared__ __attribute__((aligned(16))) char stage[];  // kRing of kStage: k, r, v rows
-    __shared__ uint32_t cost[kMaxOrder], chosen, odd_keys[kWaves];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 31, half = lane >> 5;
-    const uint32_t h = blockIdx.x % p.heads;
+    // Groups go to the eight XCDs in turn: where heads are whole eights, a head's tiles go to one, one head after the other,
+    // so that the tiles that run at once share their keys in its L2.
+    const uint32_t x = blockIdx.x & 7, y = blockIdx.x >> 3;
+    const bool eights = p.heads % 8 == 0;
+    const uint32_t h = eights ? y / p.tiles * 8 + x : blockIdx.x % p.heads;
+    uint32_t t = eights ? y % p.tiles : blockIdx.x / p.heads;
 
-    // The group's row tile: those of all sequences, one behind the other, the widest first.
-    uint32_t t = blockIdx.x / p.heads;
-    if (p.tiles > 1 && p.tiles <= kMaxOrder) {
-        for (uint32_t i = threadIdx.x; i < kMaxOrder; i += kThreads) cost[i] = 0;
-        if (threadIdx.x == 0) chosen = 0;
-        __syncthreads();
-        uint32_t before = 0;
-        for (uint32_t s0 = 0; s0 < p.seqs; s0 += 64) {
-            Sequence q;
-            uint32_t n;
-            const uint32_t upto = before + tiles_upto(p, s0 + lane, q, n);
-            if (wave == 0)
-                for (uint32_t t = 0; t < n && upto - n + t < kMaxOrder; t++) cost[upto - n + t] = span_of(p, q, t) + 1;
-            before = __builtin_amdgcn_readlane(upto, 63);
-        }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < p.tiles; i += kThreads) {
-            const uint32_t c = cost[i];
-            uint32_t ahead = 0;
-            for (uint32_t j = 0; j < p.tiles; j++) {
-                const uint32_t d = cost[j];
-                ahead += (d > c) | ((d == c) & (j < i));
-            }
-            if (ahead == t) chosen = i;
-        }
-        __syncthreads();
-        t = __builtin_amdgcn_readfirstlane(chosen);
-    }
+    // The group's row tile: those of all sequences, one behind the other, 64 at a time the widest first. Every wave works
+    // it out for itself.
+    uint32_t n;
     Sequence q;
-    for (uint32_t s0 = 0;; s0 += 64) {
-        if (s0 >= p.seqs) return;
-        uint32_t n;
-        const uint32_t upto = tiles_upto(p, s0 + lane, q, n);
+    uint32_t upto = tiles_upto(p, lane, q, n);
+    if (p.tiles > 1) {
+        // The costs of the 64 into LDS (the same by every wave, at any time), one a lane; 0: no tile.
+        uint32_t *cost = (uint32_t *)stage, before = 0;
+        const uint32_t base = t & ~63u;
+        t &= 63;
+        for (uint32_t s0 = 0;;) {
+            if (p.seqs <= 16) {  // a sequence after the other, a tile a lane
+                for (uint32_t s = 0; s < p.seqs; s++) {
+                    const Sequence x = {0, (uint32_t)__builtin_amdgcn_readlane(q.n, s), 0, (uint32_t)__builtin_amdgcn_readlane(q.m, s)};
+                    const uint32_t all = tiles_of(x), first = __builtin_amdgcn_readlane(upto, s) - all, y = base + lane - first;
+                    if (base + lane >= first && y < all) cost[lane] = cost_of(p, x, y);
+                }
+            } else {
+                const uint32_t first = before + upto - n;
+                for (uint32_t y = first < base ? base - first : 0; y < n && first + y < base + 64; y++)
+                    cost[first + y - base] = cost_of(p, q, y);
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+            s0 += 64;
+            if (s0 >= p.seqs || before >= base + 64) break;
+            upto = tiles_upto(p, s0 + lane, q, n);
+        }
+        if (base + lane >= before) cost[lane] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // The cost of rank t, bit by bit from the highest; then the t-th of those that cost as much, in order.
+        const uint32_t c = cost[lane];
+        uint32_t want = 0;
+#pragma unroll
+        for (int bit = kCostBits - 1; bit >= 0; bit--) {
+            const uint32_t with = want | 1u << bit;
+            const uint32_t more = __builtin_popcountll(__builtin_amdgcn_ballot_w64(c >> bit == with >> bit));
+            if (t < more)
+                want = with;
+            else
+                t -= more;
+        }
+        const uint64_t same = __builtin_amdgcn_ballot_w64(c == want);
+        const uint32_t rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+        t = base + __builtin_ctzll(__builtin_amdgcn_ballot_w64(c == want && rank == t));
+        __syncthreads();  // (before the first step's rows)
+        if (p.seqs > 64) upto = tiles_upto(p, lane, q, n);
+    }
+    for (uint32_t s0 = 64;; s0 += 64) {
         const uint64_t here = __builtin_amdgcn_ballot_w64(t < upto);
         if (here) {
             const uint32_t at = __builtin_ctzll(here);
@@ -152,8 +159,13 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
                          (uint32_t)__builtin_amdgcn_readlane(q.key0, at), (uint32_t)__builtin_amdgcn_readlane(q.m, at)};
             break;
         }
+        if (s0 >= p.seqs) return;
         t -= __builtin_amdgcn_readlane(upto, 63);
+        upto = tiles_upto(p, s0 + lane, q, n);
     }
+    t = __builtin_amdgcn_readfirstlane(t);
+    q = Sequence{(uint32_t)__builtin_amdgcn_readfirstlane(q.row0), (uint32_t)__builtin_amdgcn_readfirstlane(q.n),
+                 (uint32_t)__builtin_amdgcn_readfirstlane(q.key0), (uint32_t)__builtin_amdgcn_readfirstlane(q.m)};
     const uint32_t i0 = t * kRows;
     // Position of the group's row i: shift + i, negative where it sees nothing.
     const int32_t shift = (int32_t)((int64_t)q.m - q.n);
@@ -194,42 +206,59 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
     const uint32_t voff = kK + kR + vrow * (2 * VALUE) + (((lane >> 4 & 1) * 2 + (lane >> 1 & 1)) ^ value_swap<kPv>(vrow)) * 16 +
                           (lane & 1) * 8;
 
-    const uint32_t steps = hi < 0 ? 0 : (uint32_t)(hi - (lo & ~31)) / kKeys + 1;
     const int32_t base = lo & ~31;
+    const uint32_t steps = hi < 0 ? 0 : (uint32_t)(hi - base) / kKeys + 1;
+    // Where the lane's 16 bytes of each of the wave's loads of a step come from.
+    constexpr uint32_t kPartsK = kK / 1024 / kWaves, kPartsR = kR / 1024 / kWaves, kPartsV = kV / 1024 / kWaves;
+    uint32_t kplace[kPartsK], rplace[kPartsR], vplace[kPartsV];
+#pragma unroll
+    for (uint32_t x = 0; x < kPartsK; x++) {
+        const uint32_t g = 64 * (x * kWaves + wave) + lane, r = g / kPk;
+        kplace[x] = r * p.k_stride * 2 + (g % kPk ^ key_swap<kPk>(r)) * 16;
+    }
+#pragma unroll
+    for (uint32_t x = 0; x < kPartsR; x++) {
+        const uint32_t g = 64 * (x * kWaves + wave) + lane, r = g / kPr;
+        rplace[x] = r * p.r_stride * 2 + (g % kPr ^ key_swap<kPr>(r)) * 16;
+    }
+#pragma unroll
+    for (uint32_t x = 0; x < kPartsV; x++) {
+        const uint32_t g = 64 * (x * kWaves + wave) + lane, r = g / kPv;
+        vplace[x] = r * p.v_stride * 2 + (g % kPv ^ value_swap<kPv>(r)) * 16;
+    }
     // One step's rows, a KiB a load; keys past the last are the last again.
     auto issue = [&](uint32_t n, uint32_t slot) {
-        char *to = stage + slot * kStage;
+        const uint32_t to = lds_address(stage) + slot * kStage;
         const uint32_t key0 = base + n * kKeys, most = (uint32_t)hi - key0;
-        const auto kbuf = raw_buffer(p.k + (size_t)(q.key0 + key0) * p.k_stride + (size_t)h * p.k_head);
-        const auto vbuf = raw_buffer(p.v + (size_t)(q.key0 + key0) * p.v_stride + (size_t)h * p.v_head);
-        const auto rbuf = raw_buffer(p.r + (size_t)(q.key0 + key0) * p.r_stride);
-        auto load = [&](auto buf, char *at, uint32_t part, uint32_t pieces, uint32_t stride, uint32_t swap_kind) {
-            const uint32_t g = 64 * part + lane, r = g / pieces, pc = g % pieces;
-            const uint32_t swap = swap_kind == 0 ? (pieces == 16 ? key_swap<16>(r) : pieces == 8 ? key_swap<8>(r) : key_swap<4>(r))
-                                                 : (pieces == 16 ? value_swap<16>(r) : value_swap<8>(r));
-            buffer_to_lds16(buf, at + part * 1024, min(r, most) * stride * 2 + (pc ^ swap) * 16, 0);
+        const auto kbuf = rows_buffer(p.k + (size_t)(q.key0 + key0) * p.k_stride + (size_t)h * p.k_head);
+        const auto vbuf = rows_buffer(p.v + (size_t)(q.key0 + key0) * p.v_stride + (size_t)h * p.v_head);
+        const auto rbuf = rows_buffer(p.r + (size_t)(q.key0 + key0) * p.r_stride);
+        auto loads = [&](auto place) {  // (place(where a row lies, its number, its distance))
+#pragma unroll
+            for (uint32_t x = 0; x < kPartsK; x++)
+                rows_to_lds16(kbuf, to + (x * kWaves + wave) * 1024, place(kplace[x], (x * kWaves + wave) * (64 / kPk), kPk, p.k_stride));
+#pragma unroll
+            for (uint32_t x = 0; x < kPartsR; x++)
+                rows_to_lds16(rbuf, to + kK + (x * kWaves + wave) * 1024, place(rplace[x], (x * kWaves + wave) * (64 / kPr), kPr, p.r_stride));
+#pragma unroll
+            for (uint32_t x = 0; x < kPartsV; x++)
+                rows_to_lds16(vbuf, to + kK + kR + (x * kWaves + wave) * 1024,
+                              place(vplace[x], (x * kWaves + wave) * (64 / kPv), kPv, p.v_stride));
         };
-#pragma unroll
-        for (uint32_t x = 0; x < kK / 1024; x += kWaves)
-            if (x + kWaves <= kK / 1024 || wave + x < kK / 1024) load(kbuf, to, x + wave, kPk, p.k_stride, 0);
-#pragma unroll
-        for (uint32_t x = 0; x < kR / 1024; x += kWaves)
-            if (x + kWaves <= kR / 1024 || wave + x < kR / 1024) load(rbuf, to + kK, x + wave, kPr, p.r_stride, 0);
-#pragma unroll
-        for (uint32_t x = 0; x < kV / 1024; x += kWaves)
-            if (x + kWaves <= kV / 1024 || wave + x < kV / 1024) load(vbuf, to + kK + kR, x + wave, kPv, p.v_stride, 1);
+        if (most >= kKeys - 1)
+            loads([](uint32_t at, uint32_t, uint32_t, uint32_t) { return at; });
+        else
+            loads([&](uint32_t at, uint32_t row0, uint32_t pieces, uint32_t stride) {
+                const uint32_t row = row0 + again(lane) / pieces;
+                return at - (row > most ? (row - most) * stride * 2 : 0);
+            });
     };
-    // Loads of a step by the wave with the fewest.
-    constexpr uint32_t kLeast = kK / 1024 / kWaves + kR / 1024 / kWaves + kV / 1024 / kWaves;
 
 #pragma unroll
     for (uint32_t n = 0; n + 1 < kRing; n++)
         if (n < steps) issue(n, n);
     for (uint32_t n = 0, slot = 0; n < steps; n++) {
-        if (steps - n >= kRing - 1)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kRing - 2) * kLeast) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (n + kRing - 1 < steps) issue(n + kRing - 1, (slot + kRing - 1) % kRing);
         char *at = stage + slot * kStage;
         slot = slot + 1 == kRing ? 0 : slot + 1;
@@ -238,102 +267,151 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         const bool work = here <= whi && end >= wlo;
         if (!apart && !work) continue;
 
-        f32x16 s;
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = 0.0f;
+        // Half t of the step, 32 keys: its scores, register e key 32 t + 8 (e / 4) + 4 half + e % 4; its softmax; its
+        // values. The first half's softmax runs beside the second's scores, the second's beside the first's values, in
+        // pieces between the products (a wave's instructions issue in order). Operands are read kAhead products ahead.
+        f32x16 s[2];
+        bf16x8 ring[kAhead + 1];
         const uint32_t k0 = again(koff), r0 = again(roff), v0 = again(voff);
+        auto scores = [&](uint32_t t, auto beside) {
+            auto read_k = [&](uint32_t j) {
+                ring[j % (kAhead + 1)] = j < NOPE / 16 ? *(const bf16x8 *)(at + (k0 ^ 32 * j) + t * 32 * (2 * NOPE))
+                                                       : *(const bf16x8 *)(at + (r0 ^ 32 * (j - NOPE / 16)) + t * 32 * (2 * ROPE));
+            };
 #pragma unroll
-        for (uint32_t j = 0; j < kQ; j++) {
-            const bf16x8 a = j < NOPE / 16 ? *(const bf16x8 *)(at + (k0 ^ 32 * j))
-                                           : *(const bf16x8 *)(at + (r0 ^ 32 * (j - NOPE / 16)));
-            s = mfma32(a, qv[j], s);
-        }
-        // Register e of a lane: key 8 (e / 4) + 4 half + e % 4.
-        if (here < wsame_lo || end > wsame_hi) {
+            for (int e = 0; e < 16; e++) s[t][e] = 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; j++) read_k(j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (uint32_t j = 0; j < kQ; j++) {
+                if (j + kAhead < kQ) read_k(j + kAhead);
+                s[t] = mfma32(ring[j % (kAhead + 1)], qv[j], s[t]);
+                beside(j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto masked = [&](uint32_t t) {
+            if (here >= wsame_lo && end <= wsame_hi) return;
             const int32_t upto = pos - here - 4 * (int32_t)half, since = from - here - 4 * (int32_t)half;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const int32_t x = 8 * (e / 4) + e % 4;
-                s[e] = x <= upto && x >= since ? s[e] : -INFINITY;
+                const int32_t x = 32 * t + 8 * (e / 4) + e % 4;
+                s[t][e] = x <= upto && x >= since ? s[t][e] : -INFINITY;
             }
-        }
-        float mx = s[0];
+        };
+        // The softmax in kSoft pieces. m moves only when a score passes it by 2^kSlack, so most steps leave the sum and O as
+        // they are and no weight passes 2^kSlack.
+        constexpr uint32_t kSoft = 11;
+        float mx, mn, mo, sum;
+        uint32_t w[2][8];
+        auto soft = [&](uint32_t t, uint32_t i) {
+            if (i < 2) {
+                float x = fmaxf(s[t][8 * i], s[t][8 * i + 1]);
 #pragma unroll
-        for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[e]);
-        mx = halves_max(mx) * sl;
-        const bool raise = mx > m + kSlack;
-        const float mn = raise ? mx : m, mo = mn == -INFINITY ? 0.0f : mn;
-        uint32_t w[8];
-        float sum = 0.0f;
+                for (int e = 2; e < 8; e++) x = fmaxf(x, s[t][8 * i + e]);
+                mx = i ? fmaxf(mx, x) : x;
+                pinned(mx);
+            } else if (i == 2) {
+                mx = halves_max(mx) * sl;
+                mn = mx > m + kSlack ? mx : m;
+                mo = mn == -INFINITY ? 0.0f : mn;
+                sum = 0.0f;
+                pinned(mn);
+                pinned(mo);
+            } else {
+                const uint32_t e = 2 * (i - 3);
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][e], sl, -mo)), y = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], sl, -mo));
+                sum += x + y;
+                w[t][i - 3] = bf16_pair(x, y);
+                pinned(sum);
+                pinned(w[t][i - 3]);
+            }
+        };
+        // The pieces that belong to product i of n.
+        auto pieces = [&](uint32_t t, uint32_t i, uint32_t n) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[e], sl, -mo)), y = __builtin_amdgcn_exp2f(fmaf(s[e + 1], sl, -mo));
-            sum += x + y;
-            w[e / 2] = bf16_pair(x, y);
-        }
-        if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-            const float alpha = raise ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-            l *= alpha;
-            m = mn;
+            for (uint32_t x = 0; x < kSoft; x++)
+                if (x * n / kSoft == i) soft(t, x);
+        };
+        auto raised = [&]() {
+            if (__builtin_amdgcn_ballot_w64(mn > m) != 0) {
+                // (Not 0, which would make a NaN of an infinite sum.)
+                const float alpha = mn > m ? fmaxf(__builtin_amdgcn_exp2f(m - mn), 0x1p-126f) : 1.0f;
+                l *= alpha;
+                m = mn;
 #pragma unroll
-            for (uint32_t d = 0; d < kD; d++) o[d] *= alpha;
-        }
-        l += sum;
+                for (uint32_t d = 0; d < kD; d++) o[d] *= alpha;
+            }
+            l += sum;
+        };
+        auto values = [&](uint32_t t, auto beside) {
+            // Product i: keys 32 t + 16 (i / kD) .., d 32 (i % kD) .. . (Eight rows on the XOR is the same.)
+            auto read_v = [&](uint32_t i) {
+                const char *v = at + (v0 ^ i % kD * 64) + (32 * t + i / kD * 16) * (2 * VALUE);
+                const u32x2 lo4 = read_vt4(v), hi4 = read_vt4(v + 8 * (2 * VALUE));
+                ring[i % (kAhead + 1)] = as_bf16x8(u32x4{lo4.x, lo4.y, hi4.x, hi4.y});
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead && i < 2 * kD; i++) read_v(i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * kD; i++) {
+                if (i + kAhead < 2 * kD) read_v(i + kAhead);
+                const uint32_t x = 4 * (i / kD);
+                o[i % kD] = mfma32(ring[i % (kAhead + 1)], as_bf16x8(u32x4{w[t][x], w[t][x + 1], w[t][x + 2], w[t][x + 3]}),
+                                   o[i % kD]);
+                beside(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        scores(0, [](uint32_t) {});
+        masked(0);
+        scores(1, [&](uint32_t i) { pieces(0, i, kQ); });
+        masked(1);
+        raised();
         if (apart) {
             // A value that is not finite must reach the rows that see it alone, and the product's 0 times it would be
-            // NaN: such values are looked for, added by themselves, and cleared, by all waves of the group together.
-            uint32_t bad = 0;  // keys that hold one
+            // NaN: such values are looked for, added by themselves, and cleared, by all waves of the group alike.
+            float odd = 0.0f;
+#pragma unroll 4
+            for (uint32_t g = again(lane); g < kV / 16; g += 64) {
+                const u32x4 x = *(const u32x4 *)(at + kK + kR + g * 16);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) odd = odd_sum(x[e], odd);
+            }
+            if (__builtin_amdgcn_ballot_w64(odd != odd) != 0) {
 #pragma unroll 1
-            for (uint32_t k = wave; k < kKeys; k += kWaves) {
-                const uint32_t l0 = again(lane);
-                const uint32_t x = *(const uint32_t *)(at + kK + kR + k * (2 * VALUE) + (l0 % (VALUE / 2)) * 4);
-                bad |= __builtin_amdgcn_ballot_w64(odd_mask(x) != 0) != 0 ? 1u << k : 0u;
-            }
-            odd_keys[wave] = bad;
-            lds_barrier();
-            bad = 0;
+                for (uint32_t k = 0; k < kKeys; k++) {
+                    const uint32_t swap = value_swap<kPv>(k), g = again(half);
+                    const uint32_t keep = here + (int32_t)k <= pos && here + (int32_t)k >= from ? 0xffffffffu : 0u;
+                    const char *vk = at + kK + kR + k * (2 * VALUE) + 8 * g;
 #pragma unroll
-            for (uint32_t x = 0; x < kWaves; x++) bad |= __builtin_amdgcn_readfirstlane(odd_keys[x]);
-            for (uint32_t left = bad; left;) {
-                const uint32_t k = __builtin_ctz(left), swap = value_swap<kPv>(k), g = again(half);
-                left &= left - 1;
-                const uint32_t keep = here + (int32_t)k <= pos && here + (int32_t)k >= from ? 0xffffffffu : 0u;
-                const char *vk = at + kK + kR + k * (2 * VALUE) + 8 * g;
+                    for (uint32_t d = 0; d < kD; d++)
 #pragma unroll
-                for (uint32_t d = 0; d < kD; d++)
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; e++) {
-                        u32x2 x = *(const u32x2 *)(vk + ((4 * d + e) ^ swap) * 16);
-                        x = u32x2{x[0] & odd_mask(x[0]), x[1] & odd_mask(x[1])} & keep;
-                        o[d][4 * e] += lo_bf16(x[0]);
-                        o[d][4 * e + 1] += hi_bf16(x[0]);
-                        o[d][4 * e + 2] += lo_bf16(x[1]);
-                        o[d][4 * e + 3] += hi_bf16(x[1]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            }
-            if (bad) {
+                        for (uint32_t e = 0; e < 4; e++) {
+                            u32x2 x = *(const u32x2 *)(vk + ((4 * d + e) ^ swap) * 16);
+                            x = u32x2{x[0] & odd_mask(x[0]), x[1] & odd_mask(x[1])} & keep;
+                            o[d][4 * e] += lo_bf16(x[0]);
+                            o[d][4 * e + 1] += hi_bf16(x[0]);
+                            o[d][4 * e + 2] += lo_bf16(x[1]);
+                            o[d][4 * e + 3] += hi_bf16(x[1]);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                }
                 lds_barrier();
-#pragma unroll 1
-                for (uint32_t k = wave; k < kKeys; k += kWaves) {
-                    const uint32_t l0 = again(lane);
-                    uint32_t *x = (uint32_t *)(at + kK + kR + k * (2 * VALUE)) + l0;
-                    if (l0 < VALUE / 2) *x &= ~odd_mask(*x);
+                for (uint32_t g = wave * 64 + again(lane); g < kV / 16; g += kThreads) {
+                    u32x4 x = *(const u32x4 *)(at + kK + kR + g * 16);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) x[e] &= ~odd_mask(x[e]);
+                    *(u32x4 *)(at + kK + kR + g * 16) = x;
                 }
                 lds_barrier();
             }
         }
-#pragma unroll
-        for (uint32_t x = 0; x < kKeys / 16; x++)
-#pragma unroll
-            for (uint32_t d = 0; d < kD; d++) {
-                const char *v = at + (v0 ^ d * 64) + x * 16 * (2 * VALUE);
-                const u32x2 lo4 = read_vt4(v);
-                // (Eight rows on the XOR is the same.)
-                const u32x2 hi4 = read_vt4(v + 8 * (2 * VALUE));
-                o[d] = mfma32(as_bf16x8(u32x4{lo4.x, lo4.y, hi4.x, hi4.y}),
-                              as_bf16x8(u32x4{w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]}), o[d]);
-            }
+        values(0, [&](uint32_t i) { pieces(1, i, 2 * kD); });
+        raised();
+        values(1, [](uint32_t) {});
     }
     if (!there) return;
     // A row that sees no key is zero.
@@ -343,8 +421,8 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
     for (uint32_t d = 0; d < kD; d++)
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++)
-            *(u32x2 *)(to + 32 * d + 8 * e) = u32x2{pack_bf16x2(o[d][4 * e] * by, o[d][4 * e + 1] * by),
-                                                    pack_bf16x2(o[d][4 * e + 2] * by, o[d][4 * e + 3] * by)};
+            *(u32x2 *)(to + 32 * d + 8 * e) = u32x2{bf16_pair(o[d][4 * e] * by, o[d][4 * e + 1] * by),
+                                                    bf16_pair(o[d][4 * e + 2] * by, o[d][4 * e + 3] * by)};
 }
 
 template <uint32_t NOPE, uint32_t ROPE, uint32_t VALUE>
@@ -378,7 +456,7 @@ extern "C" int tessera_hip_flash_latent(const ts_flash_latent_args *a, void *str
     TS_REQUIRE(ts::aligned(a->q, 16) && ts::aligned(a->k, 16) && ts::aligned(a->v, 16) && ts::aligned(a->r, 16) &&
                    ts::aligned(a->out, 16),
                "flash_latent: q, k, v, r and out must be 16-byte aligned");
-    // (32 keys within a 32-bit offset.)
+    // (64 keys within a 32-bit offset.)
     TS_REQUIRE(a->k_stride <= 1u << 25 && a->v_stride <= 1u << 25 && a->r_stride <= 1u << 25,
                "flash_latent: keys %u, %u and %u elements apart", a->k_stride, a->v_stride, a->r_stride);
     FlashParams p;
