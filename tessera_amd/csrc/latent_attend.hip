@@ -23,11 +23,8 @@ using namespace latent;
 
 constexpr uint32_t kKeys = 32;         // keys of a step
 constexpr uint32_t kMaxTiles = 1024;   // row tiles whose keys are shared
+constexpr uint32_t kWholeTiles = 128;  // and those of which each group has one
 constexpr uint32_t kJoinThreads = 256;
-#ifndef KAH
-#define KAH 3
-#endif
-constexpr uint32_t kAhead = KAH;         // operands read ahead of their products
 
 struct LatentParams {
     const uint16_t *q, *kept;
@@ -41,6 +38,7 @@ struct LatentParams {
     Place place;
     uint32_t rows, heads, back, max_position;
     uint32_t tile_rows, tiles, groups;  // rows a tile, row tiles, and groups a block of heads
+    int whole;                          // where keys are shared: a group has keys of one tile only
     uint32_t block_heads, blocks;       // a row's heads in a tile, and the blocks they make
     float scale;
 };
@@ -67,13 +65,37 @@ TS_DEV uint32_t swap_of(uint32_t row) {
     return ((i ^ i >> 1) & 1) << 1 | i >> 1;
 }
 
+// The least over a wave, uniform; the total; and the lanes' sums up to each.
+TS_DEV uint32_t wave_least(uint32_t v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t x = min((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return row16_least(min((uint32_t)b[0], (uint32_t)b[1]));
+}
+TS_DEV uint32_t wave_upto(uint32_t v, uint32_t lane) {
+    v += dpp_u<0x111>(v);
+    v += dpp_u<0x112>(v);
+    v += dpp_u<0x114>(v);
+    v += dpp_u<0x118>(v);
+    const uint32_t a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31),
+                   c = b + __builtin_amdgcn_readlane(v, 47);
+    return v + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
+}
+TS_DEV uint32_t rows4_total(uint32_t v) {  // over the four lanes of a column
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t x = (uint32_t)a[0] + (uint32_t)a[1];
+    const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return (uint32_t)b[0] + (uint32_t)b[1];
+}
+TS_DEV uint32_t wave_total(uint32_t v) { return __builtin_amdgcn_readlane(wave_upto(v, threadIdx.x & 63), 63); }
+
 // 2^(a - b) of maxima, 0 where a has seen nothing.
 TS_DEV float weight_of(float a, float b) { return a == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(a - b); }
 
 template <uint32_t RANK, uint32_t ROPE, uint32_t WC>
 struct Shape {
     static constexpr uint32_t kWidth = RANK + ROPE, kRow = 2 * kWidth, kPieces = kWidth / 8;
-    static constexpr uint32_t kWaves = WC < 4 ? 4 : WC, kTeams = kWaves / WC;
+    static constexpr uint32_t kWaves = WC < 4 ? 4 : 8, kTeams = kWaves / WC;
     static constexpr uint32_t kRing = 4 / kTeams;                // rounds of kTeams steps in LDS
     static constexpr uint32_t kTile = kKeys * kRow, kLds = 4 * kTile;
     static constexpr uint32_t kUnit = kKeys * kTeams;            // keys of a round
@@ -81,6 +103,7 @@ struct Shape {
     static constexpr uint32_t kLoads = (kParts + WC - 1) / WC, kLeast = kParts / WC;
     static constexpr uint32_t kOwn = kLoads < 9 ? kLoads : 9;    // those of different places within a block
     static constexpr uint32_t kCols = 16 * WC, kWeights = WC == 8 ? 1 : 2;
+    static constexpr uint32_t kAhead = WC == 8 ? 3 : 2;          // operands read ahead of their products
     static constexpr uint32_t kQ = kWidth / 32, kD = RANK / 16;  // operands of q, tiles of O
     static constexpr uint32_t kIds = WC == 1 ? 2 : 2 * kTeams;   // blocks whose pages a wave looks up
     static constexpr uint32_t kXor = kPieces % 16 == 8 ? 8 : 4;  // pieces that the XOR permutes
@@ -92,17 +115,29 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     using S = Shape<RANK, ROPE, WC>;
     constexpr uint32_t kThreads = 64 * S::kWaves;
     extern __shared__ __attribute__((aligned(16))) char stage[];
+    __shared__ uint32_t rows_at[2][128];  // the tile's rows' positions and slots (each wave writes all, the same)
     __shared__ uint32_t starts[kMaxTiles + 1], words[S::kWaves], odd_met[S::kWaves], found;
-    __shared__ uint32_t from_aside[S::kAside ? S::kOwn : 1][S::kAside ? kThreads : 1];
+    __shared__ uint16_t from_aside[S::kAside ? S::kOwn : 1][S::kAside ? kThreads : 1];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4, team = wave / WC, mine = wave % WC;
-    // Groups go to the eight XCDs in turn: those of a tile's blocks of heads, which read the same keys, to one.
-    const uint32_t block = (blockIdx.x >> 3) % p.blocks, u = (blockIdx.x >> 3) / p.blocks * 8 + (blockIdx.x & 7);
+    // Groups go to the eight XCDs in turn. Those of a tile's parts, which read the same q, and of its blocks of heads,
+    // which read the same keys, belong to one.
+    const uint32_t block = (blockIdx.x >> 3) % p.blocks, u = (blockIdx.x & 7) * ((p.groups + 7) / 8) + (blockIdx.x >> 3) / p.blocks;
     if (u >= p.groups) return;
 
-    // The group's units of keys: a row tile is as many as its rows see, all tiles' one behind the other are dealt to
-    // the groups in equal runs. (A tile's units are told from its first and last row.)
-    uint32_t unit = 0, end = 1, each = 1, tile = u;
+    // The group's part of the keys: units [a, b) of a row tile's. A tile has as many as its rows see, told from its first
+    // and last row. All groups work the division out alike, every wave for itself but for the tiles' units.
+    uint32_t tile = u, a = 0, b = 1, units = 1, unit = 0, end = 1, each = 1;
+    float *partial = nullptr;
+    auto part = [&](bool some) {
+        partial = !some ? nullptr : p.partials + ((size_t)((a ? 0 : p.groups) + u) * p.blocks + block) * part_floats<RANK>(S::kCols);
+    };
+    auto share = [&](uint32_t first, uint32_t count) {
+        if (a == 0 && block == 0 && threadIdx.x == 0) {
+            p.shares[2 * tile] = first;
+            p.shares[2 * tile + 1] = count;
+        }
+    };
     if (p.partials) {
         constexpr uint32_t kEach = kMaxTiles / kThreads;
         uint32_t n[kEach], sum = 0;
@@ -122,46 +157,114 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             }
             sum += n[i];
         }
-        uint32_t upto = sum;
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint32_t x = __shfl_up((int)upto, d, 64);
-            if (lane >= d) upto += x;
-        }
-        if (lane == 63) words[wave] = upto;
-        __syncthreads();
-        uint32_t all = 0, before = 0;
+        if (p.whole) {
+            // Each tile's keys in as many equal parts as leave none longer than `each`: the shortest `each` (of 16 tried,
+            // one a column's lanes) whose parts are no more than the groups.
 #pragma unroll
-        for (uint32_t w = 0; w < S::kWaves; w++) {
-            if (w < wave) before += words[w];
-            all += words[w];
-        }
-        all = __builtin_amdgcn_readfirstlane(all);
-        each = (all + p.groups - 1) / p.groups;
-        unit = u * each;
-        end = min(unit + each, all);
-        if (unit >= all) return;
-        uint32_t at = before + upto - sum;
+            for (uint32_t i = 0; i < kEach; i++) {
+                const uint32_t t = threadIdx.x * kEach + i;
+                if (t < kWholeTiles) starts[t] = n[i];
+            }
+            __syncthreads();
+            uint32_t m[kWholeTiles / 64], all = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; i++) {
-            const uint32_t t = threadIdx.x * kEach + i;
-            if (t >= p.tiles) break;
-            starts[t] = at;
-            if (unit >= at && unit < at + n[i]) found = t;
-            at += n[i];
+            for (uint32_t i = 0; i < kWholeTiles / 64; i++) all += m[i] = starts[64 * i + lane];
+            all = wave_total(all);
+            const float least = (float)all / (float)p.groups, most = (float)all / (float)(p.groups - p.tiles) + 1.0f;
+            const float by = __builtin_amdgcn_rcpf(least + (most - least) * (float)col * (1.0f / 15.0f));
+            auto parts_of = [](uint32_t n, float by) { return min(max((uint32_t)ceilf((float)n * by), 1u), n); };
+            uint32_t parts = 0;
+#pragma unroll 4
+            for (uint32_t t = grp; t < p.tiles; t += 4) parts += parts_of(starts[t], by);
+            parts = rows4_total(parts);
+            const uint64_t fit = __builtin_amdgcn_ballot_w64(parts <= p.groups);
+            const float chosen = fit ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), __builtin_ctzll(fit))) : 0.0f;
+            uint32_t before = 0;
+            bool mine_found = false;
+#pragma unroll
+            for (uint32_t i = 0; i < kWholeTiles / 64; i++) {
+                const uint32_t own = 64 * i + lane < p.tiles ? parts_of(m[i], chosen) : 0, upto = before + wave_upto(own, lane);
+                const uint64_t here = __builtin_amdgcn_ballot_w64(u < upto && u >= upto - own);
+                before = __builtin_amdgcn_readlane(upto, 63);
+                if (!here) continue;
+                const uint32_t at = __builtin_ctzll(here), count = __builtin_amdgcn_readlane(own, at);
+                const uint32_t first = __builtin_amdgcn_readlane(upto, at) - count;
+                mine_found = true;
+                tile = 64 * i + at;
+                units = __builtin_amdgcn_readlane(m[i], at);
+                a = units * (u - first) / count;
+                b = units * (u - first + 1) / count;
+                part(count > 1);
+                share(first, count);
+            }
+            if (!mine_found) return;
+        } else {
+            // All tiles' units, one behind the other, in equal runs.
+            const uint32_t upto = wave_upto(sum, lane);
+            if (lane == 63) words[wave] = upto;
+            __syncthreads();
+            uint32_t all = 0, before = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < S::kWaves; w++) {
+                if (w < wave) before += words[w];
+                all += words[w];
+            }
+            all = __builtin_amdgcn_readfirstlane(all);
+            each = (all + p.groups - 1) / p.groups;
+            unit = u * each;
+            end = min(unit + each, all);
+            if (unit >= all) return;
+            uint32_t at = before + upto - sum;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; i++) {
+                const uint32_t t = threadIdx.x * kEach + i;
+                if (t >= p.tiles) break;
+                starts[t] = at;
+                if (unit >= at && unit < at + n[i]) found = t;
+                at += n[i];
+            }
+            if (threadIdx.x == 0) starts[p.tiles] = all;
+            __syncthreads();
+            tile = __builtin_amdgcn_readfirstlane(found);
         }
-        if (threadIdx.x == 0) starts[p.tiles] = all;
-        __syncthreads();
-        tile = __builtin_amdgcn_readfirstlane(found);
     }
+
+    // A tile's rows, two a lane, for what all waves agree on, and the lane's column. (Columns that are not there, or are
+    // refused, go along with what is loaded for them.)
+    uint32_t row_pos[2], row_slot[2], pos, slot;
+    bool there;
+    bf16x8 q[S::kQ];
+    const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;
+    auto fetch = [&]() {
+        const uint32_t row0 = tile * p.tile_rows, l0 = again(lane);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++) {
+            const uint32_t r = min(row0 + min(l0 + 64 * i, p.tile_rows - 1), p.rows - 1);
+            row_pos[i] = p.positions[r];
+            row_slot[i] = p.slots[r];
+        }
+        uint32_t r, h;
+        there = column_of(p, row0, block, 16 * mine + (l0 & 15), r, h);
+        if (!there) r = row0, h = 0;
+        pos = p.positions[r];
+        slot = p.slots[r];
+        const uint16_t *at = p.q + ((size_t)r * p.heads + h) * S::kWidth + 8 * (l0 >> 4);
+#pragma unroll
+        for (uint32_t j = 0; j < S::kQ; j++) q[j] = *(const bf16x8 *)(at + 32 * j);
+    };
+    fetch();
 
     // Where the lane's 16 bytes of the wave's loads of a step come from, in their block of 16 rows (LDS holds rows back
     // to back). They repeat after nine loads: in the other block, or (WC = 1) eight rows on, where the XOR differs by 3.
-    uint32_t from_at[S::kOwn];
-#pragma unroll
+    uint32_t from_at[S::kAside ? 1 : S::kOwn];
+#pragma unroll(S::kAside ? 1 : S::kOwn)
     for (uint32_t i = 0; i < S::kOwn; i++) {
         const uint32_t g = 64 * ((mine + i * WC) % (S::kParts / 2)) + lane, row = g / S::kPieces;
-        from_at[i] = row * S::kRow + ((g % S::kPieces) ^ swap_of<S::kPieces>(row)) * 16;
-        if (S::kAside) from_aside[i][threadIdx.x] = from_at[i];
+        const uint32_t at = row * S::kRow + ((g % S::kPieces) ^ swap_of<S::kPieces>(row)) * 16;
+        if (S::kAside)
+            from_aside[i][threadIdx.x] = (uint16_t)at;
+        else
+            from_at[S::kAside ? 0 : i] = at;
     }
     // LDS offsets of the lane's operands: K piece grp of row `col`, and V^T d 8 (lane / 2 % 2) + 4 (lane % 2) .. of keys
     // 4 grp + lane / 4 % 4; others by the XOR of their piece.
@@ -169,44 +272,36 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     const uint32_t vrow = 4 * grp + (lane >> 2 & 3);
     const uint32_t voff = vrow * S::kRow + ((lane >> 1 & 1) ^ swap_of<S::kPieces>(vrow)) * 16 + (lane & 1) * 8;
     const float sl = base2_scale(p.scale);
-    const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;
 
     for (;;) {
-        const uint32_t row0 = tile * p.tile_rows;
-        uint32_t a = 0, b = 1, units = 1;
-        float *partial = nullptr;
-        if (p.partials) {
+        if (p.partials && !p.whole) {
             const uint32_t t0 = __builtin_amdgcn_readfirstlane(starts[tile]);
             const uint32_t t1 = __builtin_amdgcn_readfirstlane(starts[tile + 1]);
             a = unit - t0;
             b = min(end, t1) - t0;
             units = t1 - t0;
-            if (a || b < units)
-                partial = p.partials + ((size_t)((a ? 0 : p.groups) + u) * p.blocks + block) * part_floats<RANK>(S::kCols);
-            if (a == 0 && block == 0 && threadIdx.x == 0) {
-                p.shares[2 * tile] = u;
-                p.shares[2 * tile + 1] = (t1 - 1) / each - u + 1;
-            }
+            part(a || b < units);
+            share(u, (t1 - 1) / each - u + 1);
         }
-        uint32_t pos, slot;
-        bool live;
-        bf16x8 q[S::kQ];
+        const uint32_t row0 = tile * p.tile_rows;
+        auto lives = [&](uint32_t pos, uint32_t slot) { return pos <= p.max_position && holds(p.place, slot, pos); };
+        uint64_t row_waits[2], row_live[2];
         {
-            uint32_t r, h;
             const uint32_t l0 = again(lane);
-            const bool there = column_of(p, row0, block, 16 * mine + (l0 & 15), r, h);
-            pos = there ? p.positions[r] : 0;
-            slot = there ? p.slots[r] : 0;
-            live = there && pos <= p.max_position && holds(p.place, slot, pos);
-            if (there && !live && p.status && a == 0 && team == 0 && l0 < 16)
-                atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
-            const uint16_t *at = p.q + (live ? ((size_t)r * p.heads + h) * S::kWidth : 0) + 8 * (l0 >> 4);
 #pragma unroll
-            for (uint32_t j = 0; j < S::kQ; j++) {
-                const u32x4 w = *(const u32x4 *)(at + 32 * j);
-                q[j] = as_bf16x8((w ^ qsign) & (live ? 0xffffffffu : 0u));
+            for (uint32_t i = 0; i < 2; i++) {
+                rows_at[0][64 * i + l0] = row_pos[i];
+                rows_at[1][64 * i + l0] = row_slot[i];
+                const bool here = 64 * i + l0 < p.tile_rows && row0 + 64 * i + l0 < p.rows;
+                row_waits[i] = row_live[i] = __builtin_amdgcn_ballot_w64(here && lives(row_pos[i], row_slot[i]));
             }
+            if (there && !lives(pos, slot) && p.status && a == 0 && team == 0 && l0 < 16)
+                atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
         }
+        const bool live = there && lives(pos, slot);
+        if (qsign)
+#pragma unroll
+            for (uint32_t j = 0; j < S::kQ; j++) q[j] = as_bf16x8(__builtin_bit_cast(u32x4, q[j]) ^ qsign);
         const uint32_t from = pos > p.back ? pos - p.back : 0;
         bool wait = live;
         float m = -INFINITY, l = 0.0f;
@@ -216,28 +311,34 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
 
         // A pass over the keys for each slot among the columns (one, where rows of a slot stand together).
         for (;;) {
-            const uint64_t waiting = __builtin_amdgcn_ballot_w64(wait);
-            const uint32_t first = waiting ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(waiting)) : 0xffffffffu;
-            auto over = [&](uint32_t v, bool least) {  // over the group's waves
-                __syncthreads();
-                words[wave] = v;
-                __syncthreads();
-                uint32_t x = words[0];
+            if (!(row_waits[0] | row_waits[1])) break;
+            const uint32_t l0 = again(lane);
+            const uint32_t now = __builtin_amdgcn_readfirstlane(
+                rows_at[1][row_waits[0] ? __builtin_ctzll(row_waits[0]) : 64 + __builtin_ctzll(row_waits[1])]);
+            // Keys that some row sees, [lo, hi], and those that all rows see alike, [same_lo, same_hi].
+            uint32_t least[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
 #pragma unroll
-                for (uint32_t w = 1; w < S::kWaves; w++) x = least ? min(x, words[w]) : max(x, words[w]);
-                return (uint32_t)__builtin_amdgcn_readfirstlane(x);
-            };
-            const uint32_t now = over(first, true);
-            if (now == 0xffffffffu) break;  // (a served slot is below slot_count)
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t row_pos = rows_at[0][64 * i + l0], since = row_pos > p.back ? row_pos - p.back : 0;
+                const bool here = (row_waits[i] >> l0 & 1) && rows_at[1][64 * i + l0] == now;
+                row_waits[i] &= ~__builtin_amdgcn_ballot_w64(here);
+                if (here) {
+                    least[0] = min(least[0], since);
+                    least[1] = min(least[1], ~row_pos);
+                    least[2] = min(least[2], ~since);
+                    least[3] = min(least[3], row_pos);
+                } else if (row_live[i] >> l0 & 1) {
+                    least[2] = least[3] = 0;
+                }
+            }
+            const uint32_t lo = wave_least(least[0]), hi = ~wave_least(least[1]);
+            const uint32_t same_lo = ~wave_least(least[2]), same_hi = wave_least(least[3]);
+            // Those of the wave's columns: [wlo, whi] and [all_lo, all_hi].
             const bool act = wait && slot == now;
             wait = wait && !act;
-            // Keys that some column of the wave sees, [wlo, whi], and of the group; and those that all of the wave's do.
             const uint32_t wlo = row16_least(act ? from : 0xffffffffu), whi = ~row16_least(act ? ~pos : 0xffffffffu);
             const uint32_t all_lo = ~row16_least(act ? ~from : live ? 0u : 0xffffffffu);
             const uint32_t all_hi = row16_least(act ? pos : live ? 0u : 0xffffffffu);
-            const uint32_t lo = over(wlo, true), hi = over(whi, false);
-            // (Keys [same_lo, same_hi] are seen by all columns alike.)
-            const uint32_t same_lo = WC == 1 ? all_lo : over(all_lo, false), same_hi = WC == 1 ? all_hi : over(all_hi, true);
             auto differ = [&](uint32_t here, uint32_t n) { return max(here, lo) < same_lo || min(here + n - 1, hi) > same_hi; };
             const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, np = (hi - base0) / S::kUnit + 1;
             const uint32_t unit0 = pass_unit(a, units, np), unit1 = pass_unit(b, units, np);
@@ -250,10 +351,10 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 return min(at / kBlock + i, last) * kBlock;
             };
             const_u32 *pages = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
+            auto page_of = [&](uint32_t round, uint32_t i) { return p.place.table ? pages[key_of(round, i) >> p.place.page_shift] : 0; };
             auto look = [&](uint32_t round) {
 #pragma unroll
-                for (uint32_t i = 0; i < S::kIds; i++)
-                    id[i] = p.place.table ? pages[key_of(round, i) >> p.place.page_shift] : 0;
+                for (uint32_t i = 0; i < S::kIds; i++) id[i] = page_of(round, i);
             };
             // The blocks of a round that are not held, a bit each.
             auto gone_of = [&]() {
@@ -281,7 +382,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 }
                 uint32_t from[S::kOwn];
 #pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; i++) from[i] = S::kAside ? from_aside[i][threadIdx.x] : from_at[i];
+                for (uint32_t i = 0; i < S::kOwn; i++) from[i] = S::kAside ? from_aside[i][threadIdx.x] : from_at[S::kAside ? 0 : i];
 #pragma unroll
                 for (uint32_t i = 0; i < S::kLoads; i++) {
                     const uint32_t part = mine + i * WC;
@@ -294,24 +395,23 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
 
             // A step is the wave's columns against the keys here .. here + 31 at `at`. Its scores: register i of s[t] is key
             // 16 t + 4 grp + i. Operands are read kAhead products ahead: left to itself, the compiler reads all it has
-            // registers for, or one at a time and waits for each. `beside(i)` is done after the i-th product.
-            auto scores = [&](const char *at, f32x4 (&s)[2], auto beside) {
+            // registers for, or one at a time and waits for each.
+            auto scores = [&](const char *at, f32x4 (&s)[2]) {
                 const uint32_t k0 = again(koff);
-                bf16x8 ring[kAhead + 1];
+                bf16x8 ring[S::kAhead + 1];
                 auto read_k = [&](uint32_t i) {
                     const uint32_t j = i / 2, t = i % 2;
-                    ring[i % (kAhead + 1)] = *(const bf16x8 *)(at + (k0 ^ j % (S::kXor / 4) * 64) +
+                    ring[i % (S::kAhead + 1)] = *(const bf16x8 *)(at + (k0 ^ j % (S::kXor / 4) * 64) +
                                                                j / (S::kXor / 4) * (S::kXor * 16) + t * kBlock * S::kRow);
                 };
                 s[0] = s[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (uint32_t i = 0; i < kAhead; i++) read_k(i);
+                for (uint32_t i = 0; i < S::kAhead; i++) read_k(i);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (uint32_t i = 0; i < 2 * S::kQ; i++) {
-                    if (i + kAhead < 2 * S::kQ) read_k(i + kAhead);
-                    s[i % 2] = mfma16(ring[i % (kAhead + 1)], q[i / 2], s[i % 2]);
-                    beside(i);
+                    if (i + S::kAhead < 2 * S::kQ) read_k(i + S::kAhead);
+                    s[i % 2] = mfma16(ring[i % (S::kAhead + 1)], q[i / 2], s[i % 2]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
@@ -326,36 +426,22 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                         s[t][i] = seen ? (gone >> t & 1 ? __builtin_nanf("") : s[t][i]) : -INFINITY;
                     }
             };
-            // The softmax of a step in kSoft pieces: weights 2^(score - m) in bf16 parts. m moves only when a score passes it
-            // by 2^kSlack, so most steps leave the sum and O as they are and no weight passes 2^kSlack.
-            constexpr uint32_t kSoft = 8;
-            float mx, mn, mo, sum;
+            // The softmax of a step: weights 2^(score - m) in bf16 parts. m moves only when a score passes it by 2^kSlack, so
+            // most steps leave the sum and O as they are and no weight passes 2^kSlack.
+            float mn, sum;
             uint32_t pw[4][S::kWeights];
-            auto soft = [&](uint32_t i, const f32x4 (&s)[2]) {
-                if (i == 0) {
-                    mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                               fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-                } else if (i == 1) {
-                    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                    mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-                } else if (i == 2) {
-                    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                    mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])) * sl;
-                } else if (i == 3) {
-                    mn = mx > m + kSlack ? mx : m;
-                    mo = mn == -INFINITY ? 0.0f : mn;
-                    pinned(mn);
-                    pinned(mo);
-                    sum = 0.0f;
-                } else if (i < kSoft) {
-                    const uint32_t t = (i - 4) / 2, e = (i - 4) % 2 * 2;
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][e], sl, -mo));
-                    const float y = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], sl, -mo));
-                    sum += x + y;
-                    split_pair<S::kWeights>(x, y, pw[i - 4]);
+            auto soft = [&](const f32x4 (&s)[2]) {
+                const float mx = rows4_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                                 fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])))) * sl;
+                mn = mx > m + kSlack ? mx : m;
+                const float mo = mn == -INFINITY ? 0.0f : mn;
+                sum = 0.0f;
 #pragma unroll
-                    for (uint32_t f = 0; f < S::kWeights; f++) pinned(pw[i - 4][f]);
-                    pinned(sum);
+                for (uint32_t i = 0; i < 4; i++) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 2][i % 2 * 2], sl, -mo));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[i / 2][i % 2 * 2 + 1], sl, -mo));
+                    sum += x + y;
+                    split_pair<S::kWeights>(x, y, pw[i]);
                 }
             };
             // The step's weights times its values, onto O.
@@ -416,30 +502,29 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 }
                 // V^T: d 16 dt + col of keys 4 grp .. and 16 + 4 grp .. (eight of them).
                 const uint32_t v0 = again(voff);
-                u32x4 ring[kAhead + 1];
+                u32x4 ring[S::kAhead + 1];
                 auto read_v = [&](uint32_t d) {
                     const char *v = at + d / (S::kXor / 2) * (S::kXor * 16) + (v0 ^ d % (S::kXor / 2) * 32);
                     const u32x2 lo4 = read_vt4(v), hi4 = read_vt4(v + kBlock * S::kRow);
-                    ring[d % (kAhead + 1)] = u32x4{lo4.x, lo4.y, hi4.x, hi4.y};
+                    ring[d % (S::kAhead + 1)] = u32x4{lo4.x, lo4.y, hi4.x, hi4.y};
                 };
 #pragma unroll
-                for (uint32_t i = 0; i < kAhead; i++) read_v(i);
+                for (uint32_t i = 0; i < S::kAhead; i++) read_v(i);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (uint32_t i = 0; i < S::kD; i++) {
-                    if (i + kAhead < S::kD) read_v(i + kAhead);
+                    if (i + S::kAhead < S::kD) read_v(i + S::kAhead);
 #pragma unroll
                     for (uint32_t e = 0; e < S::kWeights; e++)
-                        o[i] = mfma16(as_bf16x8(ring[i % (kAhead + 1)]), as_bf16x8(w[e]), o[i]);
+                        o[i] = mfma16(as_bf16x8(ring[i % (S::kAhead + 1)]), as_bf16x8(w[e]), o[i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
             auto step = [&](uint32_t here, char *at, uint32_t gone, bool apart) {
                 f32x4 s[2];
-                scores(at, s, [](uint32_t) {});
+                scores(at, s);
                 masked(here, gone, s);
-#pragma unroll
-                for (uint32_t i = 0; i < kSoft; i++) soft(i, s);
+                soft(s);
                 product(here, at, apart);
             };
             // Rows of a step that no column of the pass sees, or of no page, are zero in the products.
@@ -467,26 +552,21 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     step(here, at, gone, differ(here, kKeys));
                 }
             } else {
-                // kRing - 1 rounds on their way. With four the next round's scores are worked out beside this one's softmax
-                // (the matrix unit would wait for it), so the next round must have come.
-                constexpr bool kPipe = false && S::kRing == 4;
-                constexpr uint32_t kLater = (S::kRing - 2 - kPipe) * S::kLeast;
+                // kRing - 1 rounds on their way.
+                constexpr uint32_t kLater = (S::kRing - 2) * S::kLeast;
                 uint32_t gone[S::kRing], n = 0;
-                look(unit0);
+                uint32_t first_id[S::kRing][S::kIds];
 #pragma unroll
-                for (uint32_t i = 0; i + 1 < S::kRing; i++) {
-                    gone[i] = gone_of();
-                    if (unit0 + i < unit1) issue(unit0 + i, i);
-                    look(min(unit0 + i + 1, unit1 - 1));
-                }
-                auto useful = [&](uint32_t here) { return here <= whi && here + (kKeys - 1) >= wlo; };
-                f32x4 s[2];
-                if (kPipe) {
-                    if (unit1 - unit0 >= 3)
-                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * S::kLeast) : "memory");
-                    else
-                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    scores(stage, s, [](uint32_t) {});
+                for (uint32_t r = 0; r < S::kRing; r++)
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kIds; i++) first_id[r][i] = page_of(min(unit0 + r, unit1 - 1), i);
+#pragma unroll
+                for (uint32_t r = 0; r < S::kRing; r++) {
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kIds; i++) id[i] = first_id[r][i];
+                    if (r + 1 == S::kRing) break;
+                    gone[r] = gone_of();
+                    if (unit0 + r < unit1) issue(unit0 + r, r);
                 }
                 for (uint32_t round = unit0; round < unit1; round++) {
                     if (unit1 - round >= S::kRing - 1)
@@ -507,24 +587,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     }
                     const bool apart = differ(here, S::kUnit);
                     n = n + 1 == S::kRing ? 0 : n + 1;
-                    if (kPipe) {
-                        const char *then = stage + n * S::kTile;  // (of the last round whatever is there: not used)
-                        if (apart || useful(at_here)) {
-                            masked(at_here, lost, s);
-                            f32x4 t[2];
-                            constexpr uint32_t kEvery = 2 * S::kQ / kSoft;
-                            scores(then, t, [&](uint32_t i) {
-                                if (i % kEvery == 0) soft(i / kEvery, s);
-                            });
-                            product(at_here, at, apart);
-                            s[0] = t[0];
-                            s[1] = t[1];
-                        } else if (useful(at_here + kKeys)) {
-                            scores(then, s, [](uint32_t) {});
-                        }
-                    } else if (apart || useful(at_here)) {
-                        step(at_here, at, lost, apart);
-                    }
+                    if (apart || (at_here <= whi && at_here + (kKeys - 1) >= wlo)) step(at_here, at, lost, apart);
 #pragma unroll
                     for (uint32_t i = 0; i + 1 < S::kRing; i++) gone[i] = gone[i + 1];
                 }
@@ -532,53 +595,77 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             }
         }
 
-        // The teams' results into the first's, by halves.
+        // The teams' results joined: each team sums its share of O's tiles, which the others give it in LDS.
+        constexpr uint32_t kShare = S::kD / S::kTeams;
+        const uint32_t l0 = again(lane), c = 16 * mine + (l0 & 15), g = l0 >> 4;
+        float most = m, sum = rows4_sum(l), weight[S::kTeams];
+        weight[0] = 1.0f;
+        char *given = stage + mine * ((S::kTeams - 1) * S::kD * 1024) + l0 * 16;
         if (S::kTeams > 1) {
+            float *ml = (float *)(stage + WC * (S::kTeams - 1) * S::kD * 1024) + mine * S::kTeams * 32 + (l0 & 15);
+            __syncthreads();
 #pragma unroll
-            for (uint32_t n = S::kTeams / 2; n; n /= 2) {
-                __syncthreads();
-                const uint32_t l0 = again(lane);
-                char *at = stage + (team % n * WC + mine) * (RANK * 64 + 512) + l0 * 16;
-                float *ml = (float *)(stage + (team % n * WC + mine) * (RANK * 64 + 512) + RANK * 64) + l0;
-                if (team >= n && team < 2 * n) {
+            for (uint32_t t = 0; t < S::kTeams; t++)
+                if (t != team)
 #pragma unroll
-                    for (uint32_t d = 0; d < S::kD; d++) *(f32x4 *)(at + d * 1024) = o[d];
-                    ml[0] = m;
-                    ml[64] = l;
-                }
-                __syncthreads();
-                if (team < n) {
-                    const float most = fmaxf(m, ml[0]), f = weight_of(m, most), g = weight_of(ml[0], most);
-                    m = most;
-                    l = l * f + ml[64] * g;
+                    for (uint32_t d = 0; d < kShare; d++)
+                        *(f32x4 *)(given + ((t * (S::kTeams - 1) + (team < t ? team : team - 1)) * kShare + d) * 1024) = o[t * kShare + d];
+            if (g == 0) {
+                ml[team * 32] = m;
+                ml[team * 32 + 16] = sum;
+            }
+            __syncthreads();
 #pragma unroll
-                    for (uint32_t d = 0; d < S::kD; d++) o[d] = o[d] * f + *(const f32x4 *)(at + d * 1024) * g;
-                }
+            for (uint32_t t = 0; t < S::kTeams; t++) most = fmaxf(most, ml[t * 32]);
+            sum = 0.0f;
+#pragma unroll
+            for (uint32_t t = 0; t < S::kTeams; t++) {
+                weight[t] = weight_of(ml[t * 32], most);
+                // (A part that has met nothing but NaN has no maximum either.)
+                const float x = ml[t * 32 + 16];
+                sum += x != x ? x : x * weight[t];
             }
         }
-        const float sum = live ? rows4_sum(l) : __builtin_nanf("");
-        const uint32_t l0 = again(lane), c = 16 * mine + (l0 & 15), g = l0 >> 4;
-        uint32_t r, h;
-        if (column_of(p, row0, block, c, r, h) && team == 0) {
-            if (partial) {
+        if (!live) sum = __builtin_nanf("");
+        // The wave's share of O, one team's code after the other (registers have no index): four sums of a column a lane.
+        auto each_of = [&](auto put) {
 #pragma unroll
-                for (uint32_t d = 0; d < S::kD; d++) *(f32x4 *)(partial + ((4 * d + g) * S::kCols + c) * 4) = o[d];
-                if (g == 0) {
-                    partial[RANK * S::kCols + c] = m;
+            for (uint32_t t = 0; t < S::kTeams; t++) {
+                if (t != team) continue;
+#pragma unroll
+                for (uint32_t d = t * kShare; d < (t + 1) * kShare; d++) {
+                    f32x4 x = o[d] * weight[t];
+#pragma unroll
+                    for (uint32_t e = 0; e < S::kTeams; e++)
+                        if (e != t)
+                            x += weight[e] * *(const f32x4 *)(given + ((t * (S::kTeams - 1) + (e < t ? e : e - 1)) * kShare +
+                                                                       d - t * kShare) * 1024);
+                    put(d, x);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        };
+        uint32_t r, h;
+        if (column_of(p, row0, block, c, r, h)) {
+            if (partial) {
+                float *to = partial + (g * S::kCols + c) * 4;
+                each_of([&](uint32_t d, f32x4 x) { *(f32x4 *)(to + 4 * d * S::kCols * 4) = x; });
+                if (team == 0 && g == 0) {
+                    partial[RANK * S::kCols + c] = most;
                     partial[RANK * S::kCols + S::kCols + c] = sum;
                 }
             } else {
                 uint16_t *to = p.out + ((size_t)r * p.heads + h) * RANK + 4 * g;
                 const float by = 1.0f / sum;
-#pragma unroll
-                for (uint32_t d = 0; d < S::kD; d++)
-                    *(u32x2 *)(to + 16 * d) = u32x2{pack_bf16x2(o[d][0] * by, o[d][1] * by),
-                                                    pack_bf16x2(o[d][2] * by, o[d][3] * by)};
+                each_of([&](uint32_t d, f32x4 x) {
+                    *(u32x2 *)(to + 16 * d) = u32x2{bf16_pair(x[0] * by, x[1] * by), bf16_pair(x[2] * by, x[3] * by)};
+                });
             }
         }
         unit += b - a;
         tile++;
-        if (unit >= end) return;
+        if (p.whole || unit >= end) return;
+        fetch();
         __syncthreads();
     }
 }
@@ -591,7 +678,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_latent_kernel(LatentParams 
     const uint32_t piece = u % (RANK / 64), c0 = u / (RANK / 64) % (columns / 16) * 16;
     u /= RANK / 64 * (columns / 16);
     const uint32_t block = u % p.blocks, tile = u / p.blocks;
-    const uint32_t first = p.shares[2 * tile], parts = p.shares[2 * tile + 1];
+    const uint32_t first = __builtin_amdgcn_readfirstlane(p.shares[2 * tile]);
+    const uint32_t parts = __builtin_amdgcn_readfirstlane(p.shares[2 * tile + 1]);
     if (parts < 2) return;
     const uint32_t c = c0 + (threadIdx.x & 15), quad = piece * 16 + (threadIdx.x >> 4);
     uint32_t r, h;
@@ -601,13 +689,15 @@ __global__ __launch_bounds__(kJoinThreads) void join_latent_kernel(LatentParams 
     };
     float most = -INFINITY, sum = 0.0f;
     f32x4 o = {0, 0, 0, 0};
-    constexpr uint32_t kBatch = 8;
+    constexpr uint32_t kBatch = 16;
     for (uint32_t j0 = 0; j0 < parts; j0 += kBatch) {
         float mq[kBatch], lq[kBatch];
         f32x4 oq[kBatch];
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; j++) {
-            const float *at = part_at(min(j0 + j, parts - 1));
+            mq[j] = -INFINITY;
+            if (j0 + j >= parts) continue;  // (all lanes alike)
+            const float *at = part_at(j0 + j);
             mq[j] = at[RANK * columns + c];
             lq[j] = at[RANK * columns + columns + c];
             oq[j] = *(const f32x4 *)(at + (quad * columns + c) * 4);
@@ -634,7 +724,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_latent_kernel(LatentParams 
 
 struct Plan {
     uint32_t columns, block_heads, blocks, tile_rows, tiles, groups;
-    bool shared;
+    bool shared, whole;
 };
 
 Plan plan(const ts_latent_args *k) {
@@ -649,15 +739,16 @@ Plan plan(const ts_latent_args *k) {
     s.tile_rows = std::max(1u, std::min(run, s.columns / s.block_heads));
     s.tiles = (a->rows - 1) / s.tile_rows + 1;
     s.groups = s.tiles;
-    s.shared = false;
-    const uint32_t at_once = std::max(1u, (k->rank == 512 || s.columns == 128 ? 256u : 512u) / s.blocks);  // a CU's one or two
-    const uint32_t unit = kKeys * (s.columns < 64 ? 64 / s.columns : 1);
+    s.shared = s.whole = false;
+    const uint32_t at_once = std::max(1u, (k->rank == 512 || s.columns >= 64 ? 256u : 512u) / s.blocks);  // a CU's one or two
+    const uint32_t unit = kKeys * (s.columns == 16 ? 4 : s.columns == 128 ? 1 : 2);
     const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
                                              (uint64_t)a->back + s.tile_rows + kBlock);
     const uint64_t units = (span + unit - 1) / unit + 1;
     if (at_once > 1 && s.tiles <= std::min(kMaxTiles, 4 * at_once) && span > unit) {
         s.groups = (uint32_t)std::min<uint64_t>(at_once, s.tiles * units);
         s.shared = true;
+        s.whole = s.tiles <= kWholeTiles && 3 * s.tiles <= s.groups;
     }
     return s;
 }
@@ -741,6 +832,7 @@ extern "C" int tessera_hip_attend_latent(const ts_latent_args *k, void *stream) 
     p.rows = a->rows; p.heads = a->heads; p.back = a->back; p.max_position = a->max_position;
     p.tile_rows = s.tile_rows; p.tiles = s.tiles; p.groups = s.groups;
     p.block_heads = s.block_heads; p.blocks = s.blocks;
+    p.whole = s.shared && s.whole;
     p.scale = a->scale;
     return k->rank == 512 ? launch<512, 64>(p, s, stream) : launch<256, 32>(p, s, stream);
 }
