@@ -1,24 +1,27 @@
 // A product a head: out[r, h, n] = sum_k x[r, h, k] w[h, n, k] (q into a latent space, latent sums out of it).
 //
 // 2 n k flops against 2 (n + k) bytes of x and out: at k or n of 128 at most 128 flops a byte, a fifth of what the
-// matrix unit needs for each byte from HBM, so bytes bound it (few rows: the weights') and operands go from memory
-// to registers as they lie: a lane's 16 bytes are eight neighbouring k of one row of w (the left operand, 32
-// columns of out) or of x (the right one, 32 rows of out). A wave has 32 columns and MT times 32 rows; the four
-// waves of a group have neighbouring columns and the same rows, whose second to fourth reads the vector cache
-// serves. Loads run a chunk of 64 k ahead of the matrix unit.
+// matrix unit needs for each byte from HBM, so bytes bound it (few rows: the weights'). A chunk of 64 k of a group's rows
+// of x and w, 128 or 256 bytes of each, goes straight to LDS, two chunks ahead of the products: reads of whole lines, where
+// operands taken from memory as they lie (32 rows, 32 bytes of each) were bound by the vector cache's tags.
+// 1024 rows of 32 heads, 512 -> 128 to f32: 13.5 us, 4.0 TB/s (from memory to registers 27.5 us); 32 rows of 128 heads,
+// 128 -> 512: 5.5 us, 4.0 TB/s (7.6 us); 8192 rows of 16 heads, 512 -> 128: 39 us, 5.2 TB/s. What is left is the start
+// of each group, before its first chunk has come, and its end; f32 rows are bound by vector work (25 us, 3.5 TB/s).
 #include "common.h"
+
+#include <algorithm>
 
 namespace {
 
-constexpr uint32_t kWaves = 4, kSteps = 4;  // steps of 16 k a chunk
+constexpr uint32_t kChunk = 64;
 
 struct HeadsParams {
     const void *x;
     const uint16_t *w;
     void *out;
-    uint32_t rows, heads, n, k, x_stride, x_head, out_stride, out_head;
+    uint32_t rows, n, k, x_stride, x_head, out_stride, out_head;
     uint64_t w_head;
-    uint32_t row_tiles, col_groups;
+    uint32_t row_tiles, col_tiles, groups;
     int out_bf16, fours;  // fours: four columns of out are one aligned store
 };
 
@@ -42,100 +45,179 @@ TS_DEV void split8(const f32x4 &a, const f32x4 &b, bf16x8 (&to)[3]) {
     for (int e = 0; e < 3; e++) to[e] = as_bf16x8(w[e]);
 }
 
-template <bool XBF16, int MT>
-__global__ __launch_bounds__(64 * kWaves) void linear_heads_kernel(HeadsParams p) {
+// 16 bytes a lane from `from` straight to LDS, where the lane lands at `lds` + 16 lane. Nothing but LDS (and m0) is
+// written, and only the caller's own waits (vmcnt) and barrier tell when. (Beside the builtin's loads the compiler waits
+// for all of them before any read of LDS.)
+TS_DEV void row_to_lds16(const char *from, uint32_t lds) {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+#endif
+}
+
+// NW waves along the columns, 32 MN each, and RW along the rows, 32 MT each.
+template <bool XBF16, uint32_t NW, uint32_t RW, uint32_t MT, uint32_t MN>
+struct Tile {
+    static constexpr uint32_t kWaves = NW * RW, kThreads = 64 * kWaves, kRows = 32 * MT * RW, kCols = 32 * MN * NW;
+    static constexpr uint32_t kXRow = kChunk * (XBF16 ? 2 : 4), kWRow = kChunk * 2;
+    static constexpr uint32_t kX = kRows * kXRow, kStage = kX + kCols * kWRow;
+    static constexpr uint32_t kXLoads = kX / 1024 / kWaves, kWLoads = kCols * kWRow / 1024 / kWaves;  // a wave's
+    static constexpr uint32_t kOutRow = kCols * 4 + 16, kOut = kRows * kOutRow;
+    static_assert(kX % (1024 * kWaves) == 0 && kCols * kWRow % (1024 * kWaves) == 0, "equal loads for all waves");
+};
+
+template <bool XBF16, uint32_t NW, uint32_t RW, uint32_t MT, uint32_t MN>
+__global__ __launch_bounds__(64 * NW * RW, 2) void linear_heads_kernel(HeadsParams p) {
+    using T = Tile<XBF16, NW, RW, MT, MN>;
+    constexpr uint32_t kWaves = T::kWaves;
+    extern __shared__ __attribute__((aligned(16))) char stage[];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 31, half = lane >> 5;
-    uint32_t u = blockIdx.x;
-    const uint32_t cg = u % p.col_groups;
-    u /= p.col_groups;
-    const uint32_t h = u % p.heads, r0 = u / p.heads * (32 * MT);
-    const uint32_t n0 = (cg * kWaves + wave) * 32;
-    if (n0 >= p.n) return;
-    // Rows and columns past the last are the last again, and are not stored.
-    const uint16_t *w = p.w + h * p.w_head + (uint64_t)min(n0 + col, p.n - 1) * p.k + 8 * half;
-    const char *x[MT];
+    // Groups go to the eight XCDs in turn: those of a head, which read the same x or w, belong to one.
+    uint32_t u = (blockIdx.x & 7) * ((p.groups + 7) / 8) + (blockIdx.x >> 3);
+    if (u >= p.groups) return;
+    const uint32_t n0 = u % p.col_tiles * T::kCols;
+    u /= p.col_tiles;
+    const uint32_t r0 = u % p.row_tiles * T::kRows, h = u / p.row_tiles;
+
+    // LDS holds a chunk's rows back to back, their pieces of 16 bytes permuted by an XOR that has the 16 lanes of a read,
+    // one piece of 16 rows, meet all banks. Rows and columns past the last are the last again, and are not stored.
+    auto swap_w = [](uint32_t row) { return row >> 1 & 7; };
+    auto swap_x = [](uint32_t row) { return XBF16 ? row >> 1 & 7 : row & 15; };
+    const char *x[T::kXLoads], *w[T::kWLoads];
+    uint32_t x_k[T::kXLoads], w_k[T::kWLoads];  // the first k of the lane's piece
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-        x[m] = (const char *)p.x + ((uint64_t)min(r0 + 32 * m + col, p.rows - 1) * p.x_stride +
-                                    (uint64_t)h * p.x_head + 8 * half) * (XBF16 ? 2 : 4);
-    struct Chunk {
-        u32x4 w[kSteps];
-        u32x4 x[MT][kSteps][XBF16 ? 1 : 2];
-    };
-    // Step j's k: 16 j + 8 half .. + 7, zero past the last.
-    auto load = [&](uint32_t j0, Chunk &c) {
-#pragma unroll
-        for (uint32_t s = 0; s < kSteps; s++) {
-            const uint32_t at = 16 * (j0 + s);
-            const bool in = at + 8 * half < p.k;
-            const uint32_t d = in ? at : 0;
-            const uint32_t keep = in ? 0xffffffffu : 0u;
-            c.w[s] = *(const u32x4 *)(w + (in ? d : 0)) & keep;
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                c.x[m][s][0] = *(const u32x4 *)(x[m] + d * (XBF16 ? 2 : 4)) & keep;
-                if (!XBF16) c.x[m][s][XBF16 ? 0 : 1] = *(const u32x4 *)(x[m] + d * 4 + 16) & keep;
-            }
-        }
-    };
-    f32x16 acc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) acc[m][i] = 0.0f;
-    const uint32_t steps = (p.k + 15) / 16;
-    Chunk c, next;
-    load(0, c);
-    for (uint32_t j = 0;;) {
-        const bool more = j + kSteps < steps;
-        if (more) load(j + kSteps, next);
-#pragma unroll
-        for (uint32_t s = 0; s < kSteps; s++) {
-            const bf16x8 a = as_bf16x8(c.w[s]);
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                if (XBF16) {
-                    acc[m] = mfma32(a, as_bf16x8(c.x[m][s][0]), acc[m]);
-                } else {
-                    bf16x8 part[3];
-                    split8(__builtin_bit_cast(f32x4, c.x[m][s][0]), __builtin_bit_cast(f32x4, c.x[m][s][XBF16 ? 0 : 1]), part);
-#pragma unroll
-                    for (int e = 0; e < 3; e++) acc[m] = mfma32(a, part[e], acc[m]);
-                }
-            }
-        }
-        if (!more) break;
-        c = next;
-        j += kSteps;
+    for (uint32_t i = 0; i < T::kXLoads; i++) {
+        const uint32_t at = (wave + i * kWaves) * 64 + lane, row = at / (T::kXRow / 16);
+        x_k[i] = (at % (T::kXRow / 16) ^ swap_x(row)) * (XBF16 ? 8 : 4);
+        x[i] = (const char *)p.x + ((uint64_t)min(r0 + row, p.rows - 1) * p.x_stride + (uint64_t)h * p.x_head) * (XBF16 ? 2 : 4);
     }
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const uint32_t r = r0 + 32 * m + col;
-        if (r >= p.rows) continue;
-        const uint64_t at = (uint64_t)r * p.out_stride + (uint64_t)h * p.out_head;
+    for (uint32_t i = 0; i < T::kWLoads; i++) {
+        const uint32_t at = (wave + i * kWaves) * 64 + lane, row = at / 8;
+        w_k[i] = (at % 8 ^ swap_w(row)) * 8;
+        w[i] = (const char *)(p.w + h * p.w_head + (uint64_t)min(n0 + row, p.n - 1) * p.k);
+    }
+    // (Pieces past the last k are the row's first, and zero in the products.)
+    auto issue = [&](uint32_t k0, uint32_t to) {
+        const uint32_t lds = (uint32_t)(uintptr_t)(ts_lds *)stage + to * T::kStage + wave * 1024;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t n = n0 + 8 * q + 4 * half;
-            const f32x4 v = {acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
-            if (p.fours) {
-                if (n >= p.n) continue;
-                if (p.out_bf16)
-                    *(u32x2 *)((uint16_t *)p.out + at + n) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        for (uint32_t i = 0; i < T::kXLoads; i++)
+            row_to_lds16(x[i] + (k0 + x_k[i] < p.k ? (k0 + x_k[i]) * (XBF16 ? 2 : 4) : 0), lds + i * (kWaves * 1024));
+#pragma unroll
+        for (uint32_t i = 0; i < T::kWLoads; i++)
+            row_to_lds16(w[i] + (k0 + w_k[i] < p.k ? (k0 + w_k[i]) * 2 : 0), lds + T::kX + i * (kWaves * 1024));
+    };
+
+    f32x16 acc[MT][MN];
+#pragma unroll
+    for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+        for (uint32_t j = 0; j < MN; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[m][j][i] = 0.0f;
+    const uint32_t n1 = wave % NW * (32 * MN), r1 = wave / NW * (32 * MT);
+    // Four steps of 16 k: the lane has the eight of its half of column `col` of w (the left operand) and of row `col` of x.
+    auto products = [&](const char *at, uint32_t left) {
+        const uint32_t row_w = n1 + col, row_x = r1 + col;  // (32 more rows have the same XOR)
+#pragma unroll
+        for (uint32_t s = 0; s < kChunk / 16; s++) {
+            if (16 * s >= left) break;
+            const uint32_t keep = 16 * s + 8 * half < left ? 0xffffffffu : 0u, piece = 2 * s + half;
+            bf16x8 a[MN];
+#pragma unroll
+            for (uint32_t j = 0; j < MN; j++)
+                a[j] = as_bf16x8(*(const u32x4 *)(at + T::kX + (row_w + 32 * j) * T::kWRow + (piece ^ swap_w(row_w)) * 16) & keep);
+#pragma unroll
+            for (uint32_t m = 0; m < MT; m++) {
+                const char *row = at + (row_x + 32 * m) * T::kXRow;
+                bf16x8 part[XBF16 ? 1 : 3];
+                if constexpr (XBF16)
+                    part[0] = as_bf16x8(*(const u32x4 *)(row + (piece ^ swap_x(row_x)) * 16) & keep);
                 else
-                    *(f32x4 *)((float *)p.out + at + n) = v;
-            } else {
+                    split8(__builtin_bit_cast(f32x4, *(const u32x4 *)(row + (2 * piece ^ swap_x(row_x)) * 16) & keep),
+                           __builtin_bit_cast(f32x4, *(const u32x4 *)(row + ((2 * piece + 1) ^ swap_x(row_x)) * 16) & keep), part);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (n + i >= p.n) continue;
-                    if (p.out_bf16)
-                        ((uint16_t *)p.out)[at + n + i] = bf16_bits(v[i]);
-                    else
-                        ((float *)p.out)[at + n + i] = v[i];
-                }
+                for (uint32_t e = 0; e < (XBF16 ? 1 : 3); e++)
+#pragma unroll
+                    for (uint32_t j = 0; j < MN; j++) acc[m][j] = mfma32(a[j], part[e], acc[m][j]);
             }
         }
+    };
+    constexpr uint32_t kLoads = T::kXLoads + T::kWLoads;
+    issue(0, 0);
+    if (kChunk < p.k) issue(kChunk, 1);
+    uint32_t now = 0;
+    for (uint32_t k0 = 0; k0 < p.k; k0 += kChunk) {
+        if (k0 + kChunk < p.k)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (k0 + 2 * kChunk < p.k) issue(k0 + 2 * kChunk, now ? now - 1 : 2);
+        if (n0 + n1 < p.n) {
+            if (k0 + kChunk <= p.k)
+                products(stage + now * T::kStage, kChunk);
+            else
+                products(stage + now * T::kStage, p.k - k0);
+        }
+        now = now == 2 ? 0 : now + 1;
     }
+    // Sums change places in LDS, so that a store has whole rows' columns: register 4 q + i of a lane is column
+    // 8 q + 4 half + i of row `col`.
+    lds_barrier();
+#pragma unroll
+    for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+        for (uint32_t q = 0; q < 4 * MN; q++) {
+            const f32x16 &v = acc[m][q / 4];
+            *(f32x4 *)(stage + (r1 + 32 * m + col) * T::kOutRow + (n1 + 8 * q + 4 * half) * 4) =
+                f32x4{v[q % 4 * 4], v[q % 4 * 4 + 1], v[q % 4 * 4 + 2], v[q % 4 * 4 + 3]};
+        }
+    lds_barrier();
+    const uint64_t out = (uint64_t)h * p.out_head + n0;
+    if (p.fours) {
+#pragma unroll 4
+        for (uint32_t e = threadIdx.x; e < T::kRows * T::kCols / 4; e += T::kThreads) {
+            const uint32_t row = e / (T::kCols / 4), n = e % (T::kCols / 4) * 4;
+            if (r0 + row >= p.rows || n0 + n >= p.n) continue;
+            const f32x4 v = *(const f32x4 *)(stage + row * T::kOutRow + n * 4);
+            const uint64_t at = out + (uint64_t)(r0 + row) * p.out_stride + n;
+            if (p.out_bf16)
+                *(u32x2 *)((uint16_t *)p.out + at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            else
+                *(f32x4 *)((float *)p.out + at) = v;
+        }
+    } else {
+        for (uint32_t e = threadIdx.x; e < T::kRows * T::kCols; e += T::kThreads) {
+            const uint32_t row = e / T::kCols, n = e % T::kCols;
+            if (r0 + row >= p.rows || n0 + n >= p.n) continue;
+            const float v = *(const float *)(stage + row * T::kOutRow + n * 4);
+            const uint64_t at = out + (uint64_t)(r0 + row) * p.out_stride + n;
+            if (p.out_bf16)
+                ((uint16_t *)p.out)[at] = bf16_bits(v);
+            else
+                ((float *)p.out)[at] = v;
+        }
+    }
+}
+
+template <bool XBF16, uint32_t NW, uint32_t RW, uint32_t MT, uint32_t MN>
+int launch(HeadsParams &p, uint32_t heads, void *stream) {
+    using T = Tile<XBF16, NW, RW, MT, MN>;
+    const auto kernel = linear_heads_kernel<XBF16, NW, RW, MT, MN>;
+    constexpr uint32_t kMost = std::max(3 * T::kStage, T::kOut);
+    static const hipError_t attr =
+        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (attr != hipSuccess) return ts::hip_status(attr, "linear_heads: shared memory attribute");
+    p.row_tiles = (p.rows - 1) / T::kRows + 1;
+    p.col_tiles = (p.n - 1) / T::kCols + 1;
+    const uint64_t all = (uint64_t)p.row_tiles * p.col_tiles * heads;
+    TS_REQUIRE(all <= 0x7ffffff0ull, "linear_heads: %u rows in one launch", p.rows);
+    p.groups = (uint32_t)all;
+    const uint32_t stages = std::min(3u, (p.k - 1) / kChunk + 1);  // (fewer: more groups a CU)
+    hipLaunchKernelGGL(kernel, dim3((p.groups + 7) / 8 * 8), dim3(T::kThreads), std::max(stages * T::kStage, T::kOut),
+                       (hipStream_t)stream, p);
+    TS_CHECK_LAUNCH("linear_heads launch");
+    return TS_OK;
 }
 
 }  // namespace
@@ -161,20 +243,23 @@ extern "C" int tessera_hip_linear_heads(const ts_heads_args *a, void *stream) {
     if (a->rows == 0) return TS_OK;
     HeadsParams p;
     p.x = a->x; p.w = (const uint16_t *)a->w; p.out = a->out;
-    p.rows = a->rows; p.heads = a->heads; p.n = a->n; p.k = a->k;
+    p.rows = a->rows; p.n = a->n; p.k = a->k;
     p.x_stride = a->x_stride; p.x_head = a->x_head; p.out_stride = a->out_stride; p.out_head = a->out_head;
     p.w_head = a->w_head;
     p.out_bf16 = a->out_dtype == TS_BF16;
     p.fours = a->n % 4 == 0 && a->out_stride % 4 == 0 && a->out_head % 4 == 0 && ts::aligned(a->out, 4 * size);
-    const int mt = a->rows <= 32 ? 1 : 2;
-    p.row_tiles = (a->rows - 1) / (32 * mt) + 1;
-    p.col_groups = (a->n - 1) / (32 * kWaves) + 1;
-    const uint64_t all = (uint64_t)p.row_tiles * p.col_groups * a->heads;
-    TS_REQUIRE(all <= 0x7fffffffull, "linear_heads: %u rows in one launch", a->rows);
     const bool bf16 = a->x_dtype == TS_BF16;
-    const auto kernel = mt == 1 ? bf16 ? linear_heads_kernel<true, 1> : linear_heads_kernel<false, 1>
-                                : bf16 ? linear_heads_kernel<true, 2> : linear_heads_kernel<false, 2>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)all), dim3(64 * kWaves), 0, (hipStream_t)stream, p);
-    TS_CHECK_LAUNCH("linear_heads launch");
-    return TS_OK;
+    // Up to 64 rows a tile has 32 of them and more groups share the chip (33 rows, 128 heads, 512 -> 128: 6.7 us against 7.8
+    // with 64 rows; 64 rows of f32 14.0 against 19.4; but 1024 rows of 32 heads 16.0 against 13.5), and 64 columns where
+    // 128 would leave CUs without a group (1 row, 16 heads, 128 -> 512: 3.9 us against 4.6).
+    if (a->rows <= 64) {
+        if ((uint64_t)a->heads * ((a->n - 1) / 128 + 1) * ((a->rows - 1) / 32 + 1) < 256)
+            return bf16 ? launch<true, 2, 1, 1, 1>(p, a->heads, stream) : launch<false, 2, 1, 1, 1>(p, a->heads, stream);
+        return bf16 ? launch<true, 4, 1, 1, 1>(p, a->heads, stream) : launch<false, 4, 1, 1, 1>(p, a->heads, stream);
+    }
+    // 64 columns have a tile of their own (1000 rows of 16 heads, 256 -> 64: 5.3 us against 6.2). A wave of f32 rows has all
+    // of the group's columns: taking them apart is vector work, which waves along the columns would repeat (1024 rows of
+    // 32 heads, 512 -> 128: 25 us against 40).
+    if (a->n <= 64) return bf16 ? launch<true, 2, 2, 1, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 2>(p, a->heads, stream);
+    return bf16 ? launch<true, 4, 1, 2, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 4>(p, a->heads, stream);
 }

@@ -257,7 +257,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     // Where the lane's 16 bytes of the wave's loads of a step come from, in their block of 16 rows (LDS holds rows back
     // to back). They repeat after nine loads: in the other block, or (WC = 1) eight rows on, where the XOR differs by 3.
     uint32_t from_at[S::kAside ? 1 : S::kOwn];
-#pragma unroll(S::kAside ? 1 : S::kOwn)
+#pragma unroll S::kAside ? 1 : S::kOwn
     for (uint32_t i = 0; i < S::kOwn; i++) {
         const uint32_t g = 64 * ((mine + i * WC) % (S::kParts / 2)) + lane, row = g / S::kPieces;
         const uint32_t at = row * S::kRow + ((g % S::kPieces) ^ swap_of<S::kPieces>(row)) * 16;
