@@ -11,7 +11,6 @@
 //  * Keys are dealt to the groups in equal runs over all tiles, so that groups end together however the sequences
 //    differ in length; a tile that several groups have is joined by a second kernel.
 #include <algorithm>
-#include <stdlib.h>
 
 #include "kept8_attend.h"
 #include "latent.h"
@@ -727,30 +726,45 @@ struct Plan {
     bool shared, whole;
 };
 
+// How many columns a group has, and how the keys are divided. A group takes some time for its q, its partial sums and
+// their share of the join, and some for each key it reads; both grow with its columns, a key's less than they do. Of 16, 32,
+// 64 and 128 columns those are taken whose groups are done first. (us, sequences x heads x keys; 16, 32, 64, 128 columns:
+// 1 x 16 x 4000 18, 22, 23, 29; 1 x 128 x 4000 22, 29, 32, 43; 4 x 128 x 4000 30, 30, 34, 41; 32 x 64 x 4000 66, 55, 47, 46;
+// 32 x 128 x 4000 99, 86, 68, 63; 2 x 400 rows of 16 heads x 2500 183, 158, 117, 103.)
+//
+// Rows of a tile that belong to two slots take two passes over keys, one after the other. So a tile has no more rows than
+// a fourth of those that stand together (24 sequences of up to 5 rows, 16 heads, 4000 keys: 48 us with one row a
+// tile, 82 with two to five).
 Plan plan(const ts_latent_args *k) {
     const ts_rows_args *a = &k->rows;
-    Plan s;
+    constexpr double kStart[4] = {19, 22, 30, 40}, kKey[4] = {0.020, 0.032, 0.039, 0.050};  // us (512 + 64 values)
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
-    const uint64_t wanted = (uint64_t)run * a->heads;
-    s.columns = wanted <= 16 ? 16 : wanted <= 32 ? 32 : wanted <= 64 ? 64 : 128;
-    if (getenv("TSC")) s.columns = atoi(getenv("TSC"));
-    s.block_heads = std::min(a->heads, s.columns);
-    s.blocks = (a->heads - 1) / s.block_heads + 1;
-    s.tile_rows = std::max(1u, std::min(run, s.columns / s.block_heads));
-    s.tiles = (a->rows - 1) / s.tile_rows + 1;
-    s.groups = s.tiles;
-    s.shared = s.whole = false;
-    const uint32_t at_once = std::max(1u, (k->rank == 512 || s.columns >= 64 ? 256u : 512u) / s.blocks);  // a CU's one or two
-    const uint32_t unit = kKeys * (s.columns == 16 ? 4 : s.columns == 128 ? 1 : 2);
-    const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
-                                             (uint64_t)a->back + s.tile_rows + kBlock);
-    const uint64_t units = (span + unit - 1) / unit + 1;
-    if (at_once > 1 && s.tiles <= std::min(kMaxTiles, 4 * at_once) && span > unit) {
-        s.groups = (uint32_t)std::min<uint64_t>(at_once, s.tiles * units);
-        s.shared = true;
-        s.whole = s.tiles <= kWholeTiles && 3 * s.tiles <= s.groups;
+    Plan best = {};
+    double least = INFINITY;
+    for (uint32_t i = 0; i < 4; i++) {
+        Plan s;
+        s.columns = 16u << i;
+        s.block_heads = std::min(a->heads, s.columns);
+        s.blocks = (a->heads - 1) / s.block_heads + 1;
+        s.tile_rows = std::max(1u, std::min(run / 4, s.columns / s.block_heads));
+        s.tiles = (a->rows - 1) / s.tile_rows + 1;
+        s.groups = s.tiles;
+        s.shared = s.whole = false;
+        const uint32_t at_once = std::max(1u, (k->rank == 512 || s.columns >= 64 ? 256u : 512u) / s.blocks);  // a CU's one or two
+        const uint32_t unit = kKeys * (s.columns == 16 ? 4 : s.columns == 128 ? 1 : 2);
+        const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
+                                                 (uint64_t)a->back + s.tile_rows + kBlock);
+        const uint64_t units = (span + unit - 1) / unit + 1;
+        if (at_once > 1 && s.tiles <= std::min(kMaxTiles, 4 * at_once) && span > unit) {
+            s.groups = (uint32_t)std::min<uint64_t>(at_once, s.tiles * units);
+            s.shared = true;
+            s.whole = s.tiles <= kWholeTiles && 3 * s.tiles <= s.groups;
+        }
+        const double keys = (double)span * s.tiles * s.blocks / 256.0;  // a CU's
+        const double takes = kStart[i] + keys * kKey[i] * a->width / 576.0;
+        if (takes < least) least = takes, best = s;
     }
-    return s;
+    return best;
 }
 
 size_t partial_bytes(const ts_latent_args *k, const Plan &s) {
