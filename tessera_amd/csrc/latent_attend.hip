@@ -8,8 +8,17 @@
 // columns: 128 (RANK 512) registers of O and 72 of q.
 //  * WC waves share a step's keys, 16 columns each; the teams of a group take steps in turn, and are joined in LDS at
 //    the end. With WC = 1 each wave streams keys of its own and waits for no other.
-//  * Keys are dealt to the groups in equal runs over all tiles, so that groups end together however the sequences
-//    differ in length; a tile that several groups have is joined by a second kernel.
+//  * Keys are dealt to the groups, the tiles' one behind the other, so that groups end together however the sequences
+//    differ in length; a tile that several groups have is joined by a second kernel. Few tiles: each in equal parts of
+//    its own, a group one of them, which spares groups a second start (24 sequences of up to 5 rows, 32 heads, 1000 ..
+//    9001 keys: 84 us against 97).
+//  * A weight enters the product in two bf16 parts where up to 32 columns leave the matrix unit time for it, in one else
+//    (64 columns, 32 sequences of 128 heads, 512 .. 8192 keys: 70 us against 78).
+//
+// 32 sequences of 16 heads, 32000 keys each: 5.3 TB/s, what a copy reaches. 8 prompts' chunks of 512 rows behind 8000 keys,
+// 16 heads: 1020 TFLOP/s; there the LDS reads bound it (a wave's 16 columns read a step's whole rows, 68 KB, for 68 products of
+// 16x16x32; 32 columns a wave do not fit the registers). Short calls are bound by a group's start (positions, pages, q and the
+// first keys come one after the other, 7 us) and by the join (5 us, 13 for 128 columns a group).
 #include <algorithm>
 
 #include "kept8_attend.h"
@@ -101,7 +110,7 @@ struct Shape {
     static constexpr uint32_t kParts = kTile / 1024;             // loads of a step, dealt to the team's waves
     static constexpr uint32_t kLoads = (kParts + WC - 1) / WC, kLeast = kParts / WC;
     static constexpr uint32_t kOwn = kLoads < 9 ? kLoads : 9;    // those of different places within a block
-    static constexpr uint32_t kCols = 16 * WC, kWeights = WC == 8 ? 1 : 2;
+    static constexpr uint32_t kCols = 16 * WC, kWeights = WC >= 4 ? 1 : 2;
     static constexpr uint32_t kAhead = WC == 8 ? 3 : 2;          // operands read ahead of their products
     static constexpr uint32_t kQ = kWidth / 32, kD = RANK / 16;  // operands of q, tiles of O
     static constexpr uint32_t kIds = WC == 1 ? 2 : 2 * kTeams;   // blocks whose pages a wave looks up
@@ -729,15 +738,15 @@ struct Plan {
 // How many columns a group has, and how the keys are divided. A group takes some time for its q, its partial sums and
 // their share of the join, and some for each key it reads; both grow with its columns, a key's less than they do. Of 16, 32,
 // 64 and 128 columns those are taken whose groups are done first. (us, sequences x heads x keys; 16, 32, 64, 128 columns:
-// 1 x 16 x 4000 18, 22, 23, 29; 1 x 128 x 4000 22, 29, 32, 43; 4 x 128 x 4000 30, 30, 34, 41; 32 x 64 x 4000 66, 55, 47, 46;
-// 32 x 128 x 4000 99, 86, 68, 63; 2 x 400 rows of 16 heads x 2500 183, 158, 117, 103.)
+// 1 x 16 x 4000 18, 22, 23, 29; 1 x 128 x 4000 22, 29, 31, 43; 4 x 128 x 4000 30, 30, 33, 41; 32 x 64 x 4000 65, 55, 45, 46;
+// 32 x 128 x 512 .. 8192 118, 109, 70, 72; 2 x 512 rows of 16 heads x 2500 .. 4600 318, 277, 168, 155.)
 //
 // Rows of a tile that belong to two slots take two passes over keys, one after the other. So a tile has no more rows than
 // a fourth of those that stand together (24 sequences of up to 5 rows, 16 heads, 4000 keys: 48 us with one row a
 // tile, 82 with two to five).
 Plan plan(const ts_latent_args *k) {
     const ts_rows_args *a = &k->rows;
-    constexpr double kStart[4] = {19, 22, 30, 40}, kKey[4] = {0.020, 0.032, 0.039, 0.050};  // us (512 + 64 values)
+    constexpr double kStart[4] = {19, 22, 29, 40}, kKey[4] = {0.020, 0.032, 0.033, 0.0565};  // us (512 + 64 values)
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
     Plan best = {};
     double least = INFINITY;
