@@ -280,6 +280,9 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     const uint32_t vrow = 4 * grp + (lane >> 2 & 3);
     const uint32_t voff = vrow * S::kRow + ((lane >> 1 & 1) ^ swap_of<S::kPieces>(vrow)) * 16 + (lane & 1) * 8;
     const float sl = base2_scale(p.scale);
+    const uint32_t page_blocks = p.place.table ? p.place.page_shift - 4 : 0;  // (the logarithm)
+    const uint32_t page_mask = p.place.table ? (1u << page_blocks) - 1 : 0xffffffffu;
+    const uint32_t page_count = p.place.table ? p.place.pages : 0xffffffffu;
 
     for (;;) {
         if (p.partials && !p.whole) {
@@ -352,24 +355,26 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             const uint32_t unit0 = pass_unit(a, units, np), unit1 = pass_unit(b, units, np);
             if (unit0 >= unit1) continue;
 
-            // Pages of a round's blocks (the wave's own step's where teams do not meet), asked for a round ahead.
+            // Pages of a round's blocks (the wave's own step's where teams do not meet), asked for a round ahead. (Without
+            // a table a slot is one page.)
             uint32_t id[S::kIds];
-            auto key_of = [&](uint32_t round, uint32_t i) {
-                const uint32_t at = base0 + round * S::kUnit + (WC == 1 ? kKeys * wave : 0);
-                return min(at / kBlock + i, last) * kBlock;
-            };
+            const uint32_t first_block = base0 / kBlock + (WC == 1 ? 2 * wave : 0);
+            auto block_at = [&](uint32_t round, uint32_t i) { return min(first_block + round * (S::kUnit / kBlock) + i, last); };
             const_u32 *pages = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
-            auto page_of = [&](uint32_t round, uint32_t i) { return p.place.table ? pages[key_of(round, i) >> p.place.page_shift] : 0; };
-            auto look = [&](uint32_t round) {
+            auto look = [&](uint32_t round, uint32_t (&id)[S::kIds]) {
+                if (p.place.table) {
 #pragma unroll
-                for (uint32_t i = 0; i < S::kIds; i++) id[i] = page_of(round, i);
+                    for (uint32_t i = 0; i < S::kIds; i++) id[i] = pages[block_at(round, i) >> page_blocks];
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < S::kIds; i++) id[i] = now * (p.place.keys / kBlock);
+                }
             };
             // The blocks of a round that are not held, a bit each.
             auto gone_of = [&]() {
                 uint32_t gone = 0;
-                if (p.place.table)
 #pragma unroll
-                    for (uint32_t i = 0; i < S::kIds; i++) gone |= id[i] >= p.place.pages ? 1u << i : 0u;
+                for (uint32_t i = 0; i < S::kIds; i++) gone |= id[i] >= page_count ? 1u << i : 0u;
                 return gone;
             };
             auto issue = [&](uint32_t round, uint32_t slot_of_ring) {
@@ -377,15 +382,15 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 u32x4 buf[2];
 #pragma unroll
                 for (uint32_t i = 0; i < 2; i++) {
-                    uint32_t page = id[0], key = key_of(round, 0);
+                    uint32_t page = id[0], block = block_at(round, 0);
 #pragma unroll
                     for (uint32_t e = 1; e < S::kIds; e++)
                         if (e == (WC == 1 ? i : 2 * team + i)) {
                             page = id[e];
-                            key = key_of(round, e);
+                            block = block_at(round, e);
                         }
-                    bool lost;
-                    const uint32_t kept_block = block_in(p.place, now, page, key, lost);
+                    page = page < page_count ? page : 0;  // (one that is not held: page 0, whose rows are cleared)
+                    const uint32_t kept_block = (page << page_blocks) + (block & page_mask);
                     buf[i] = rows_buffer((const char *)p.kept + (size_t)kept_block * (kBlock * S::kRow));
                 }
                 uint32_t from[S::kOwn];
@@ -547,14 +552,14 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             if (WC == 1) {
                 char *at = stage + team * S::kTile;
                 uint32_t round = unit0;
-                look(round);
+                look(round, id);
                 for (; round < unit1; round++) {
                     const uint32_t here = base0 + round * S::kUnit + kKeys * wave;
                     if (here > hi) break;
                     const uint32_t gone = gone_of();
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads
                     issue(round, 0);
-                    look(min(round + 1, unit1 - 1));
+                    look(min(round + 1, unit1 - 1), id);
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     if (here < lo || here + (kKeys - 1) > hi || gone) clear(here, at, gone);
                     step(here, at, gone, differ(here, kKeys));
@@ -565,9 +570,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 uint32_t gone[S::kRing], n = 0;
                 uint32_t first_id[S::kRing][S::kIds];
 #pragma unroll
-                for (uint32_t r = 0; r < S::kRing; r++)
-#pragma unroll
-                    for (uint32_t i = 0; i < S::kIds; i++) first_id[r][i] = page_of(min(unit0 + r, unit1 - 1), i);
+                for (uint32_t r = 0; r < S::kRing; r++) look(min(unit0 + r, unit1 - 1), first_id[r]);
 #pragma unroll
                 for (uint32_t r = 0; r < S::kRing; r++) {
 #pragma unroll
@@ -584,7 +587,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     gone[S::kRing - 1] = gone_of();
                     if (round + S::kRing - 1 < unit1) {
                         issue(round + S::kRing - 1, (n + S::kRing - 1) % S::kRing);
-                        look(min(round + S::kRing, unit1 - 1));
+                        look(min(round + S::kRing, unit1 - 1), id);
                     }
                     const uint32_t here = base0 + round * S::kUnit;
                     const uint32_t at_here = here + team * kKeys, lost = gone[0] >> (2 * team) & 3;
