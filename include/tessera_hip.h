@@ -449,8 +449,7 @@ int tessera_hip_linear_heads(const ts_heads_args *a, void *stream);
  * sum of w times the rows' first `rank` values. rows.q [rows, heads, rank + rope] bf16, rows.k the
  * kept rows (rows.v is not read), rows.out [rows, heads, rank] bf16, rows.kv_heads 1, rows.width
  * rank + rope. rank 512 with rope 64, or 256 with 32. Scores, softmax and sums in f32; weights enter
- * their product in bf16, in one part or two (16 bits; always two where `run` rows have up to 32
- * heads between them).
+ * their product in bf16, in one part or two (16 bits; two for decode rows of up to 16 heads).
  *  - `run`: how many rows of a slot stand together (1: a decode step; drafted rows; a prompt chunk's).
  *    It groups rows and picks the kernel, never which keys a row sees. A row's last bits may depend on
  *    the rows beside it; the same call gives the same bits.

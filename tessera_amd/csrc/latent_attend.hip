@@ -12,11 +12,12 @@
 //    differ in length; a tile that several groups have is joined by a second kernel. Few tiles: each in equal parts of
 //    its own, a group one of them, which spares groups a second start (24 sequences of up to 5 rows, 32 heads, 1000 ..
 //    9001 keys: 84 us against 97).
-//  * A weight enters the product in two bf16 parts where up to 32 columns leave the matrix unit time for it, in one else
-//    (64 columns, 32 sequences of 128 heads, 512 .. 8192 keys: 70 us against 78).
+//  * A weight enters the product in two bf16 parts with 16 columns, which leave the matrix unit time for it, in one else
+//    (24 sequences of up to 5 rows, 32 heads, 1000 .. 9001 keys, 32 columns: 75 us against 82; 32 sequences of 128 heads,
+//    512 .. 8192 keys, 64 columns: 70 against 78).
 //
 // 32 sequences of 16 heads, 32000 keys each: 5.3 TB/s, what a copy reaches. 8 prompts' chunks of 512 rows behind 8000 keys,
-// 16 heads: 1020 TFLOP/s; there the LDS reads bound it (a wave's 16 columns read a step's whole rows, 68 KB, for 68 products of
+// 16 heads: 1050 TFLOP/s; there the LDS reads bound it (a wave's 16 columns read a step's whole rows, 68 KB, for 68 products of
 // 16x16x32; 32 columns a wave do not fit the registers). Short calls are bound by a group's start (positions, pages, q and the
 // first keys come one after the other, 7 us) and by the join (5 us, 13 for 128 columns a group).
 #include <algorithm>
@@ -110,7 +111,7 @@ struct Shape {
     static constexpr uint32_t kParts = kTile / 1024;             // loads of a step, dealt to the team's waves
     static constexpr uint32_t kLoads = (kParts + WC - 1) / WC, kLeast = kParts / WC;
     static constexpr uint32_t kOwn = kLoads < 9 ? kLoads : 9;    // those of different places within a block
-    static constexpr uint32_t kCols = 16 * WC, kWeights = WC >= 4 ? 1 : 2;
+    static constexpr uint32_t kCols = 16 * WC, kWeights = WC == 1 ? 2 : 1;
     static constexpr uint32_t kAhead = WC == 8 ? 3 : 2;          // operands read ahead of their products
     static constexpr uint32_t kQ = kWidth / 32, kD = RANK / 16;  // operands of q, tiles of O
     static constexpr uint32_t kIds = WC == 1 ? 2 : 2 * kTeams;   // blocks whose pages a wave looks up

@@ -417,6 +417,93 @@ def test_offsets_past_32_bits():
     assert torch.equal(kept[-each * page + n - 1], c[0].to(BF16))
 
 
+# Slots that could hold more keys, which lets a group take 32, 64 or 128 columns: (heads, run, positions a slot).
+WIDE_TILES = [(32, 1, 1 << 17), (128, 1, 1 << 12), (128, 1, 1 << 17), (16, 64, 1 << 13), (16, 64, 1 << 16), (5, 70, 1 << 16),
+              (40, 33, 1 << 16), (100, 9, 1 << 17), (150, 1, 1 << 17)]
+
+
+def roomier(where, keys):
+    """The same slots with places for `keys` positions, whose pages are not held."""
+    table = where["table"].reshape(-1, where["kept_pages"])
+    each = keys // (where["keys"] // where["kept_pages"])
+    more = np.full((len(table), each - table.shape[1]), 2 ** 31 - 1, np.int32)
+    return dict(keys=keys, table=np.concatenate([table, more], 1).reshape(-1), kept_pages=each)
+
+
+@pytest.mark.parametrize("widths", ["wide", "narrow"])
+@pytest.mark.parametrize("heads,run,keys", WIDE_TILES)
+@pytest.mark.parametrize("back", [None, 30])
+def test_wide_tiles(widths, heads, run, keys, back):
+    rank, rope, nope, _ = WIDTHS[widths]
+    r = rng(heads + run)
+    lengths = [run + 300, run, run + 31, run + 64, run + 1, run + 450, run + 2, run + 99]
+    kept, where = cache(r, lengths, rank + rope, 16)
+    where = roomier(where, keys)
+    counts = np.array([run, 1, max(1, run - 3), run, 1, run, 1, max(1, run // 2)])
+    slots = np.repeat(np.arange(8), counts)
+    positions = np.concatenate([n - c + np.arange(c) for n, c in zip(lengths, counts)])
+    q = dev(r.standard_normal((len(slots), heads, rank + rope)), BF16)
+    kw = dict(rank=rank, scale=(nope + rope) ** -0.5, **({} if back is None else {"back": back}))
+    got = attend(q, kept, slots, positions, where, run=run, max_position=keys - 1, **kw)
+    check_attend(got, q, kept, slots, positions, where, **kw)
+    assert torch.equal(got, attend(q, kept, slots, positions, where, run=run, max_position=keys - 1, **kw))
+    # In another order, a tile of many slots; some rows refused.
+    order = r.permutation(len(slots))[:60]
+    slots, positions, q = slots[order].copy(), positions[order].copy(), q[dev(order)]
+    slots[5], positions[3] = 8, keys
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = attend(q, kept, slots, positions, where, run=run, max_position=keys - 1, status=status, **kw)
+    bad = np.isin(np.arange(len(slots)), [5, 3])
+    assert torch.isnan(got[dev(np.flatnonzero(bad))]).all()
+    assert int(status) == abi.TS_STATUS_PAGE | abi.TS_STATUS_POSITION
+    good = np.flatnonzero(~bad)
+    check_attend(got[dev(good)], q[dev(good)], kept, slots[good], positions[good], where, **kw)
+
+
+@pytest.mark.parametrize("widths", ["wide", "narrow"])
+@pytest.mark.parametrize("heads,run,keys,back", [(8, 16, 1 << 17, None), (16, 64, 1 << 16, None), (3, 90, 1 << 17, None),
+                                                 (40, 33, 1 << 16, None), (16, 2000, 1 << 12, 100)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_wide_tiles_not_finite_in_masked_places(widths, heads, run, keys, back, value):
+    """As with narrow ones: a value that is not finite reaches the rows that see its key alone."""
+    rank, rope, nope, _ = WIDTHS[widths]
+    r = rng(heads + run)
+    kept, where = cache(r, [120 + run, 60], rank + rope, 16)
+    where = roomier(where, keys)
+    slots = np.concatenate([np.zeros(run, int), [1]])
+    positions = np.concatenate([120 + np.arange(run), [59]])
+    d = 37
+    q = r.standard_normal((run + 1, heads, rank + rope))
+    q[..., d] = 0
+    q = dev(q, BF16)
+    kw = dict(rank=rank, scale=0.05, **({} if back is None else {"back": back}))
+    call = dict(kw, run=run, max_position=keys - 1)
+    want = attend(q, kept, slots, positions, where, **call)
+    few = np.unique(np.concatenate([[0, run], r.integers(0, run, 30)]))
+    check_attend(want[dev(few)], q[dev(few)], kept, slots[few], positions[few], where, **kw)
+    for key in (23, 121, 120 + run // 2, 120 + run - 1):
+        sees = (positions - (back or keys) <= key) & (positions >= key) & (slots == 0)
+        x = kept.clone()
+        x[L.kept_row(0, key, **where), d] = value
+        got = attend(q, x, slots, positions, where, **call)
+        assert bool(torch.isnan(got[dev(np.flatnonzero(sees))]).all())
+        others = dev(np.flatnonzero(~sees))
+        assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("widths", ["wide", "narrow"])
+@pytest.mark.parametrize("heads", [5, 16])
+def test_decode_rows_take_weights_in_two_parts(widths, heads):
+    rank, rope, nope, _ = WIDTHS[widths]
+    r = rng(heads)
+    lengths = [900, 1, 333]
+    kept, where = cache(r, lengths, rank + rope, 16)
+    q = dev(r.standard_normal((3, heads, rank + rope)), BF16)
+    slots, positions = np.arange(3), np.array(lengths) - 1
+    kw = dict(rank=rank, scale=(nope + rope) ** -0.5)
+    check_attend(attend(q, kept, slots, positions, where, **kw), q, kept, slots, positions, where, one_part=False, **kw)
+
+
 # --- the expanded form ----------------------------------------------------------------------------
 
 def check_flash(got, q, k, v, r, **kw):
