@@ -205,14 +205,14 @@ int launch(HeadsParams &p, uint32_t heads, void *stream) {
     using T = Tile<XBF16, NW, RW, MT, MN>;
     const auto kernel = linear_heads_kernel<XBF16, NW, RW, MT, MN>;
     constexpr uint32_t kMost = std::max(3 * T::kStage, T::kOut);
-    static const hipError_t attr =
-        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
-    if (attr != hipSuccess) return ts::hip_status(attr, "linear_heads: shared memory attribute");
     p.row_tiles = (p.rows - 1) / T::kRows + 1;
     p.col_tiles = (p.n - 1) / T::kCols + 1;
     const uint64_t all = (uint64_t)p.row_tiles * p.col_tiles * heads;
-    TS_REQUIRE(all <= 0x7ffffff0ull, "linear_heads: %u rows in one launch", p.rows);
+    TS_REQUIRE(all < (1ull << 32) / T::kThreads - 8, "linear_heads: %u rows in one launch", p.rows);
     p.groups = (uint32_t)all;
+    static const hipError_t attr =
+        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (attr != hipSuccess) return ts::hip_status(attr, "linear_heads: shared memory attribute");
     const uint32_t stages = std::min(3u, (p.k - 1) / kChunk + 1);  // (fewer: more groups a CU)
     hipLaunchKernelGGL(kernel, dim3((p.groups + 7) / 8 * 8), dim3(T::kThreads), std::max(stages * T::kStage, T::kOut),
                        (hipStream_t)stream, p);

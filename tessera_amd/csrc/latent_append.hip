@@ -231,7 +231,7 @@ extern "C" int tessera_hip_append_latent(const ts_append_latent_args *a, void *s
     p.head_units = q ? (a->heads + (1u << p.head_shift) - 1) >> p.head_shift : 0;
     p.c_groups = (a->rows - 1) / kWaves + 1;
     const uint64_t all = p.c_groups + ((uint64_t)a->rows * p.head_units + kWaves - 1) / kWaves;
-    TS_REQUIRE(all <= 0x3fffffffull, "append_latent: %u rows in one launch", a->rows);
+    TS_REQUIRE(all < (1ull << 32) / (64 * kWaves), "append_latent: %u rows in one launch", a->rows);
     const auto kernel = a->x_dtype == TS_BF16 ? a->halves ? append_latent_kernel<true, true> : append_latent_kernel<true, false>
                                               : a->halves ? append_latent_kernel<false, true> : append_latent_kernel<false, false>;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)all), dim3(64 * kWaves), 0, (hipStream_t)stream, p);

@@ -845,7 +845,7 @@ extern "C" int tessera_hip_attend_latent(const ts_latent_args *k, void *stream) 
     const ts_rows_args *a = &k->rows;
     if (a->rows == 0) return TS_OK;
     const Plan s = plan(k);
-    TS_REQUIRE((uint64_t)s.tiles * s.blocks <= 0x7fffffffull / 64, "attend_latent: %u rows in one launch", a->rows);
+    TS_REQUIRE(((uint64_t)s.groups + 7) * s.blocks < 1u << 23, "attend_latent: %u rows in one launch", a->rows);  // (2^32 threads)
     const size_t partials = partial_bytes(k, s), need = partials + share_bytes(s);
     if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
         return ts::fail(TS_ERR_WORKSPACE, "attend_latent: workspace of %zu bytes, 16-byte aligned, needed", need);

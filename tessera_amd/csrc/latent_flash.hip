@@ -468,6 +468,6 @@ extern "C" int tessera_hip_flash_latent(const ts_flash_latent_args *a, void *str
     // Whole tiles and a begun one a sequence at most.
     p.tiles = a->rows / kRows + (p.seqs < a->rows ? p.seqs : a->rows);
     const uint64_t groups = (uint64_t)p.tiles * a->heads;
-    TS_REQUIRE(groups <= 0x7fffffffull, "flash_latent: %u rows in one launch", a->rows);
+    TS_REQUIRE(groups < (1ull << 32) / kThreads, "flash_latent: %u rows in one launch", a->rows);
     return wide ? launch<128, 64, 128>(p, (uint32_t)groups, stream) : launch<64, 32, 64>(p, (uint32_t)groups, stream);
 }

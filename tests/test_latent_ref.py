@@ -189,6 +189,13 @@ def test_flash_refusals(over, text):
     _refused("tessera_hip_flash_latent", _flash(**over), text)
 
 
+def test_more_rows_than_one_launch_takes():
+    _refused("tessera_hip_append_latent", _append(rows=1 << 28), b"in one launch")
+    _refused("tessera_hip_linear_heads", _heads(rows=1 << 30), b"in one launch")
+    _refused("tessera_hip_attend_latent", _attend(rows=1 << 27), b"in one launch")
+    _refused("tessera_hip_flash_latent", _flash(rows=1 << 28), b"in one launch")
+
+
 def test_empty_calls_need_no_pointers():
     _no_gpu()
     lib = abi.load()
