@@ -125,7 +125,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     constexpr uint32_t kThreads = 64 * S::kWaves;
     extern __shared__ __attribute__((aligned(16))) char stage[];
     __shared__ uint32_t rows_at[2][128];  // the tile's rows' positions and slots (each wave writes all, the same)
-    __shared__ uint32_t starts[kMaxTiles + 1], words[S::kWaves], odd_met[S::kWaves], found;
+    __shared__ uint32_t starts[kMaxTiles + 1], firsts[2][kWholeTiles], words[S::kWaves], odd_met[S::kWaves], found;
     __shared__ uint16_t from_aside[S::kAside ? S::kOwn : 1][S::kAside ? kThreads : 1];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4, team = wave / WC, mine = wave % WC;
@@ -148,33 +148,29 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
         }
     };
     if (p.partials) {
-        constexpr uint32_t kEach = kMaxTiles / kThreads;
-        uint32_t n[kEach], sum = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; i++) {
-            const uint32_t t = threadIdx.x * kEach + i;
-            n[i] = 0;
+#pragma unroll 1
+        for (uint32_t t = threadIdx.x; t < (p.whole ? kWholeTiles : kMaxTiles); t += kThreads) {
+            uint32_t n = 0;
             if (t < p.tiles) {
                 const uint32_t r0 = t * p.tile_rows, r1 = min(r0 + p.tile_rows, p.rows) - 1;
                 const uint32_t most = min(p.max_position, p.place.keys - 1);
-                const uint32_t p0 = min(p.positions[r0], most), p1 = min(p.positions[r1], most);
+                const uint32_t first = p.positions[r0], slot = p.slots[r0];
+                const uint32_t p0 = min(first, most), p1 = min(p.positions[r1], most);
                 const uint32_t from0 = p0 > p.back ? p0 - p.back : 0, from1 = p1 > p.back ? p1 - p.back : 0;
                 auto units = [](uint32_t lo, uint32_t hi) { return (hi - (lo & ~(kBlock - 1))) / S::kUnit + 1; };
-                n[i] = p.slots[r0] == p.slots[r1] ? units(min(from0, from1), max(p0, p1))
-                                                  : units(from0, p0) + units(from1, p1);
-                n[i] = min(n[i], 1u << 21);
+                n = slot == p.slots[r1] ? units(min(from0, from1), max(p0, p1)) : units(from0, p0) + units(from1, p1);
+                n = min(n, 1u << 21);
+                if (t < kWholeTiles) {
+                    firsts[0][t] = first;
+                    firsts[1][t] = slot;
+                }
             }
-            sum += n[i];
+            starts[t] = n;
         }
+        __syncthreads();
         if (p.whole) {
             // Each tile's keys in as many equal parts as leave none longer than `each`: the shortest `each` (of 16 tried,
             // one a column's lanes) whose parts are no more than the groups.
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; i++) {
-                const uint32_t t = threadIdx.x * kEach + i;
-                if (t < kWholeTiles) starts[t] = n[i];
-            }
-            __syncthreads();
             uint32_t m[kWholeTiles / 64], all = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kWholeTiles / 64; i++) all += m[i] = starts[64 * i + lane];
@@ -209,6 +205,10 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             if (!mine_found) return;
         } else {
             // All tiles' units, one behind the other, in equal runs.
+            constexpr uint32_t kEach = kMaxTiles / kThreads;
+            uint32_t n[kEach], sum = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; i++) sum += n[i] = starts[threadIdx.x * kEach + i];
             const uint32_t upto = wave_upto(sum, lane);
             if (lane == 63) words[wave] = upto;
             __syncthreads();
@@ -246,17 +246,27 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;
     auto fetch = [&]() {
         const uint32_t row0 = tile * p.tile_rows, l0 = again(lane);
+        uint32_t r = row0, h = block * p.block_heads;
+        if (p.tile_rows == 1) {
+            pos = p.whole ? firsts[0][tile] : p.positions[tile];
+            slot = p.whole ? firsts[1][tile] : p.slots[tile];
+            row_pos[0] = row_pos[1] = pos;
+            row_slot[0] = row_slot[1] = slot;
+            const uint32_t c = 16 * mine + (l0 & 15);
+            there = c < p.block_heads && h + c < p.heads;
+            if (there) h += c;
+        } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 2; i++) {
-            const uint32_t r = min(row0 + min(l0 + 64 * i, p.tile_rows - 1), p.rows - 1);
-            row_pos[i] = p.positions[r];
-            row_slot[i] = p.slots[r];
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t r = min(row0 + min(l0 + 64 * i, p.tile_rows - 1), p.rows - 1);
+                row_pos[i] = p.positions[r];
+                row_slot[i] = p.slots[r];
+            }
+            there = column_of(p, row0, block, 16 * mine + (l0 & 15), r, h);
+            if (!there) r = row0, h = 0;
+            pos = p.positions[r];
+            slot = p.slots[r];
         }
-        uint32_t r, h;
-        there = column_of(p, row0, block, 16 * mine + (l0 & 15), r, h);
-        if (!there) r = row0, h = 0;
-        pos = p.positions[r];
-        slot = p.slots[r];
         const uint16_t *at = p.q + ((size_t)r * p.heads + h) * S::kWidth + 8 * (l0 >> 4);
 #pragma unroll
         for (uint32_t j = 0; j < S::kQ; j++) q[j] = *(const bf16x8 *)(at + 32 * j);
@@ -266,14 +276,21 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     // Where the lane's 16 bytes of the wave's loads of a step come from, in their block of 16 rows (LDS holds rows back
     // to back). They repeat after nine loads: in the other block, or (WC = 1) eight rows on, where the XOR differs by 3.
     uint32_t from_at[S::kAside ? 1 : S::kOwn];
+    {
+        constexpr uint32_t kStep = 64 * WC;
+        uint32_t row = (64 * mine + lane) / S::kPieces, piece = (64 * mine + lane) % S::kPieces;
 #pragma unroll S::kAside ? 1 : S::kOwn
-    for (uint32_t i = 0; i < S::kOwn; i++) {
-        const uint32_t g = 64 * ((mine + i * WC) % (S::kParts / 2)) + lane, row = g / S::kPieces;
-        const uint32_t at = row * S::kRow + ((g % S::kPieces) ^ swap_of<S::kPieces>(row)) * 16;
-        if (S::kAside)
-            from_aside[i][threadIdx.x] = (uint16_t)at;
-        else
-            from_at[S::kAside ? 0 : i] = at;
+        for (uint32_t i = 0; i < S::kOwn; i++) {
+            const uint32_t at = row * S::kRow + (piece ^ swap_of<S::kPieces>(row)) * 16;
+            if (S::kAside)
+                from_aside[i][threadIdx.x] = (uint16_t)at;
+            else
+                from_at[S::kAside ? 0 : i] = at;
+            piece += kStep % S::kPieces;
+            row += kStep / S::kPieces;
+            if (piece >= S::kPieces) piece -= S::kPieces, row++;
+            row &= kBlock - 1;
+        }
     }
     // LDS offsets of the lane's operands: K piece grp of row `col`, and V^T d 8 (lane / 2 % 2) + 4 (lane % 2) .. of keys
     // 4 grp + lane / 4 % 4; others by the XOR of their piece.
@@ -327,30 +344,43 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             const uint32_t l0 = again(lane);
             const uint32_t now = __builtin_amdgcn_readfirstlane(
                 rows_at[1][row_waits[0] ? __builtin_ctzll(row_waits[0]) : 64 + __builtin_ctzll(row_waits[1])]);
-            // Keys that some row sees, [lo, hi], and those that all rows see alike, [same_lo, same_hi].
-            uint32_t least[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-#pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
-                const uint32_t row_pos = rows_at[0][64 * i + l0], since = row_pos > p.back ? row_pos - p.back : 0;
-                const bool here = (row_waits[i] >> l0 & 1) && rows_at[1][64 * i + l0] == now;
-                row_waits[i] &= ~__builtin_amdgcn_ballot_w64(here);
-                if (here) {
-                    least[0] = min(least[0], since);
-                    least[1] = min(least[1], ~row_pos);
-                    least[2] = min(least[2], ~since);
-                    least[3] = min(least[3], row_pos);
-                } else if (row_live[i] >> l0 & 1) {
-                    least[2] = least[3] = 0;
-                }
-            }
-            const uint32_t lo = wave_least(least[0]), hi = ~wave_least(least[1]);
-            const uint32_t same_lo = ~wave_least(least[2]), same_hi = wave_least(least[3]);
-            // Those of the wave's columns: [wlo, whi] and [all_lo, all_hi].
+            // Keys that some row sees, [lo, hi], and those that all rows see alike, [same_lo, same_hi]; those of the wave's
+            // columns, [wlo, whi] and [all_lo, all_hi].
             const bool act = wait && slot == now;
             wait = wait && !act;
-            const uint32_t wlo = row16_least(act ? from : 0xffffffffu), whi = ~row16_least(act ? ~pos : 0xffffffffu);
-            const uint32_t all_lo = ~row16_least(act ? ~from : live ? 0u : 0xffffffffu);
-            const uint32_t all_hi = row16_least(act ? pos : live ? 0u : 0xffffffffu);
+            uint32_t lo, hi, same_lo, same_hi, wlo, whi, all_lo, all_hi;
+            if (p.tile_rows == 1) {
+                row_waits[0] = 0;
+                lo = same_lo = all_lo = __builtin_amdgcn_readfirstlane(from);
+                hi = same_hi = all_hi = __builtin_amdgcn_readfirstlane(pos);
+                const bool any = __builtin_amdgcn_ballot_w64(act) != 0;
+                wlo = any ? lo : 0xffffffffu;
+                whi = any ? hi : 0;
+            } else {
+                uint32_t least[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) {
+                    const uint32_t row_pos = rows_at[0][64 * i + l0], since = row_pos > p.back ? row_pos - p.back : 0;
+                    const bool here = (row_waits[i] >> l0 & 1) && rows_at[1][64 * i + l0] == now;
+                    row_waits[i] &= ~__builtin_amdgcn_ballot_w64(here);
+                    if (here) {
+                        least[0] = min(least[0], since);
+                        least[1] = min(least[1], ~row_pos);
+                        least[2] = min(least[2], ~since);
+                        least[3] = min(least[3], row_pos);
+                    } else if (row_live[i] >> l0 & 1) {
+                        least[2] = least[3] = 0;
+                    }
+                }
+                lo = wave_least(least[0]);
+                hi = ~wave_least(least[1]);
+                same_lo = ~wave_least(least[2]);
+                same_hi = wave_least(least[3]);
+                wlo = row16_least(act ? from : 0xffffffffu);
+                whi = ~row16_least(act ? ~pos : 0xffffffffu);
+                all_lo = ~row16_least(act ? ~from : live ? 0u : 0xffffffffu);
+                all_hi = row16_least(act ? pos : live ? 0u : 0xffffffffu);
+            }
             auto differ = [&](uint32_t here, uint32_t n) { return max(here, lo) < same_lo || min(here + n - 1, hi) > same_hi; };
             const uint32_t base0 = lo & ~(kBlock - 1), last = hi / kBlock, np = (hi - base0) / S::kUnit + 1;
             const uint32_t unit0 = pass_unit(a, units, np), unit1 = pass_unit(b, units, np);
