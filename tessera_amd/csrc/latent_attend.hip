@@ -242,6 +242,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     // refused, go along with what is loaded for them.)
     uint32_t row_pos[2], row_slot[2], pos, slot;
     bool there;
+    const uint16_t *q_at;
     bf16x8 q[S::kQ];
     const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;
     auto fetch = [&]() {
@@ -267,9 +268,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             pos = p.positions[r];
             slot = p.slots[r];
         }
-        const uint16_t *at = p.q + ((size_t)r * p.heads + h) * S::kWidth + 8 * (l0 >> 4);
-#pragma unroll
-        for (uint32_t j = 0; j < S::kQ; j++) q[j] = *(const bf16x8 *)(at + 32 * j);
+        q_at = p.q + ((size_t)r * p.heads + h) * S::kWidth + 8 * (l0 >> 4);
     };
     fetch();
 
@@ -328,11 +327,8 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 atomicOr(p.status, slot >= p.place.slot_count ? TS_STATUS_PAGE : TS_STATUS_POSITION);
         }
         const bool live = there && lives(pos, slot);
-        if (qsign)
-#pragma unroll
-            for (uint32_t j = 0; j < S::kQ; j++) q[j] = as_bf16x8(__builtin_bit_cast(u32x4, q[j]) ^ qsign);
         const uint32_t from = pos > p.back ? pos - p.back : 0;
-        bool wait = live;
+        bool wait = live, fresh = true;  // fresh: q is not there yet
         float m = -INFINITY, l = 0.0f;
         f32x4 o[S::kD];
 #pragma unroll
@@ -386,47 +382,49 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             const uint32_t unit0 = pass_unit(a, units, np), unit1 = pass_unit(b, units, np);
             if (unit0 >= unit1) continue;
 
-            // Pages of a round's blocks (the wave's own step's where teams do not meet), asked for a round ahead. (Without
-            // a table a slot is one page.)
-            uint32_t id[S::kIds];
-            const uint32_t first_block = base0 / kBlock + (WC == 1 ? 2 * wave : 0);
-            auto block_at = [&](uint32_t round, uint32_t i) { return min(first_block + round * (S::kUnit / kBlock) + i, last); };
+            // Where the blocks of the rounds from r0 on are held, those of kChunk rounds one a lane, and which are not. (A block
+            // that is not held is the first in the loads, and cleared. Without a table a slot is one page.)
+            constexpr uint32_t kChunk = 64 / S::kIds;
+            uint32_t r0, place;
+            uint64_t lost_of;
             const_u32 *pages = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
-            auto look = [&](uint32_t round, uint32_t (&id)[S::kIds]) {
-                if (p.place.table) {
+            auto look = [&](uint32_t round, bool first) {
+                const uint32_t l0 = again(lane);
+                const uint32_t block = min(base0 / kBlock + (WC == 1 ? 2 * wave : 0) +
+                                               (round + l0 / S::kIds) * (S::kUnit / kBlock) + l0 % S::kIds, last);
+                uint32_t page = now * (p.place.keys / kBlock);
+                if (p.place.table) page = pages[block >> page_blocks];
+                if (first && fresh) {
+                    // q is asked for behind the pages, which the first keys wait for, and before those. (The pages' own wait is
+                    // here, where q's loads are known to be younger.)
 #pragma unroll
-                    for (uint32_t i = 0; i < S::kIds; i++) id[i] = pages[block_at(round, i) >> page_blocks];
+                    for (uint32_t j = 0; j < S::kQ; j++) q[j] = *(const bf16x8 *)(q_at + 32 * j);
+                    asm volatile("; pages" : "+v"(page));
+                    if (qsign)
+#pragma unroll
+                        for (uint32_t j = 0; j < S::kQ; j++) q[j] = as_bf16x8(__builtin_bit_cast(u32x4, q[j]) ^ qsign);
+                    fresh = false;
                 } else {
-#pragma unroll
-                    for (uint32_t i = 0; i < S::kIds; i++) id[i] = now * (p.place.keys / kBlock);
+                    asm volatile("" : "+v"(page));
                 }
+                const bool lost = page >= page_count;
+                place = ((lost ? 0 : page) << page_blocks) + (block & page_mask);
+                lost_of = __builtin_amdgcn_ballot_w64(lost);
+                r0 = round;
             };
             // The blocks of a round that are not held, a bit each.
-            auto gone_of = [&]() {
-                uint32_t gone = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < S::kIds; i++) gone |= id[i] >= page_count ? 1u << i : 0u;
-                return gone;
-            };
+            auto gone_of = [&](uint32_t round) { return (uint32_t)(lost_of >> (round - r0) * S::kIds) & ((1u << S::kIds) - 1); };
             auto issue = [&](uint32_t round, uint32_t slot_of_ring) {
+                uint32_t from[S::kOwn];
+#pragma unroll
+                for (uint32_t i = 0; i < S::kOwn; i++) from[i] = S::kAside ? from_aside[i][threadIdx.x] : from_at[S::kAside ? 0 : i];
                 const uint32_t to = lds_address(stage) + (slot_of_ring * S::kTeams + team) * S::kTile;
                 u32x4 buf[2];
 #pragma unroll
                 for (uint32_t i = 0; i < 2; i++) {
-                    uint32_t page = id[0], block = block_at(round, 0);
-#pragma unroll
-                    for (uint32_t e = 1; e < S::kIds; e++)
-                        if (e == (WC == 1 ? i : 2 * team + i)) {
-                            page = id[e];
-                            block = block_at(round, e);
-                        }
-                    page = page < page_count ? page : 0;  // (one that is not held: page 0, whose rows are cleared)
-                    const uint32_t kept_block = (page << page_blocks) + (block & page_mask);
-                    buf[i] = rows_buffer((const char *)p.kept + (size_t)kept_block * (kBlock * S::kRow));
+                    const uint32_t block = __builtin_amdgcn_readlane(place, (round - r0) * S::kIds + (WC == 1 ? i : 2 * team + i));
+                    buf[i] = rows_buffer((const char *)p.kept + (size_t)block * (kBlock * S::kRow));
                 }
-                uint32_t from[S::kOwn];
-#pragma unroll
-                for (uint32_t i = 0; i < S::kOwn; i++) from[i] = S::kAside ? from_aside[i][threadIdx.x] : from_at[S::kAside ? 0 : i];
 #pragma unroll
                 for (uint32_t i = 0; i < S::kLoads; i++) {
                     const uint32_t part = mine + i * WC;
@@ -583,14 +581,14 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             if (WC == 1) {
                 char *at = stage + team * S::kTile;
                 uint32_t round = unit0;
-                look(round, id);
+                look(round, true);
                 for (; round < unit1; round++) {
                     const uint32_t here = base0 + round * S::kUnit + kKeys * wave;
                     if (here > hi) break;
-                    const uint32_t gone = gone_of();
+                    if (round - r0 == kChunk) look(round, false);
+                    const uint32_t gone = gone_of(round);
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads
                     issue(round, 0);
-                    look(min(round + 1, unit1 - 1), id);
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     if (here < lo || here + (kKeys - 1) > hi || gone) clear(here, at, gone);
                     step(here, at, gone, differ(here, kKeys));
@@ -599,15 +597,10 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                 // kRing - 1 rounds on their way.
                 constexpr uint32_t kLater = (S::kRing - 2) * S::kLeast;
                 uint32_t gone[S::kRing], n = 0;
-                uint32_t first_id[S::kRing][S::kIds];
+                look(unit0, true);
 #pragma unroll
-                for (uint32_t r = 0; r < S::kRing; r++) look(min(unit0 + r, unit1 - 1), first_id[r]);
-#pragma unroll
-                for (uint32_t r = 0; r < S::kRing; r++) {
-#pragma unroll
-                    for (uint32_t i = 0; i < S::kIds; i++) id[i] = first_id[r][i];
-                    if (r + 1 == S::kRing) break;
-                    gone[r] = gone_of();
+                for (uint32_t r = 0; r + 1 < S::kRing; r++) {
+                    gone[r] = gone_of(unit0 + r);
                     if (unit0 + r < unit1) issue(unit0 + r, r);
                 }
                 for (uint32_t round = unit0; round < unit1; round++) {
@@ -615,10 +608,12 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
                     else
                         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    gone[S::kRing - 1] = gone_of();
-                    if (round + S::kRing - 1 < unit1) {
-                        issue(round + S::kRing - 1, (n + S::kRing - 1) % S::kRing);
-                        look(min(round + S::kRing, unit1 - 1), id);
+                    const uint32_t next = round + S::kRing - 1;
+                    gone[S::kRing - 1] = 0;
+                    if (next < unit1) {
+                        if (next - r0 == kChunk) look(next, false);
+                        gone[S::kRing - 1] = gone_of(next);
+                        issue(next, (n + S::kRing - 1) % S::kRing);
                     }
                     const uint32_t here = base0 + round * S::kUnit;
                     const uint32_t at_here = here + team * kKeys, lost = gone[0] >> (2 * team) & 3;
