@@ -278,7 +278,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     {
         constexpr uint32_t kStep = 64 * WC;
         uint32_t row = (64 * mine + lane) / S::kPieces, piece = (64 * mine + lane) % S::kPieces;
-#pragma unroll S::kAside ? 1 : S::kOwn
+#pragma unroll S::kAside ? 3 : S::kOwn
         for (uint32_t i = 0; i < S::kOwn; i++) {
             const uint32_t at = row * S::kRow + (piece ^ swap_of<S::kPieces>(row)) * 16;
             if (S::kAside)
