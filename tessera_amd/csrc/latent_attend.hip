@@ -33,31 +33,34 @@ using namespace latent;
 constexpr uint32_t kKeys = 32;         // keys of a step
 constexpr uint32_t kMaxTiles = 1024;   // row tiles whose keys are shared
 constexpr uint32_t kWholeTiles = 128;  // and those of which each group has one
+constexpr uint32_t kCutRows = 512;     // rows whose tiles are cut where slots change
 constexpr uint32_t kJoinThreads = 256;
 
 struct LatentParams {
     const uint16_t *q, *kept;
     uint16_t *out;
     // Where keys are shared: results of groups for a tile that an earlier group began, then for one that a later
-    // group goes on with, each [groups][blocks] of a tile's columns; and each row tile's groups (first, count).
+    // group goes on with, each [groups][blocks] of a tile's columns; and each row tile's groups and rows (first and count of
+    // both), then how many tiles there are.
     float *partials;
     uint32_t *shares;
     const uint32_t *slots, *positions;
     uint32_t *status;
     Place place;
     uint32_t rows, heads, back, max_position;
-    uint32_t tile_rows, tiles, groups;  // rows a tile, row tiles, and groups a block of heads
+    uint32_t tile_rows, tiles, groups;  // rows a tile, row tiles (cut ones: their most), and groups a block of heads
     int whole;                          // where keys are shared: a group has keys of one tile only
+    int cut;                            // and: a tile's rows are one slot's
     uint32_t block_heads, blocks;       // a row's heads in a tile, and the blocks they make
     float scale;
 };
 
-// Column c's row and head of a tile; false where it has none.
-TS_DEV bool column_of(const LatentParams &p, uint32_t row0, uint32_t block, uint32_t c, uint32_t &r, uint32_t &h) {
+// Column c's row and head of a tile of n rows; false where it has none.
+TS_DEV bool column_of(const LatentParams &p, uint32_t row0, uint32_t n, uint32_t block, uint32_t c, uint32_t &r, uint32_t &h) {
     const uint32_t ri = c / p.block_heads;
     r = row0 + ri;
     h = block * p.block_heads + c % p.block_heads;
-    return ri < p.tile_rows && r < p.rows && h < p.heads;
+    return ri < n && h < p.heads;
 }
 
 // A column's partial result: RANK / 4 times [columns] of four sums, then [columns] maxima and sums.
@@ -125,7 +128,8 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     constexpr uint32_t kThreads = 64 * S::kWaves;
     extern __shared__ __attribute__((aligned(16))) char stage[];
     __shared__ uint32_t rows_at[2][128];  // the tile's rows' positions and slots (each wave writes all, the same)
-    __shared__ uint32_t starts[kMaxTiles + 1], firsts[2][kWholeTiles], words[S::kWaves], odd_met[S::kWaves], found;
+    // (starts: with cut tiles the second half holds their first rows.)
+    __shared__ uint32_t starts[kMaxTiles + 2], firsts[2][kWholeTiles], words[8], odd_met[S::kWaves], found;
     __shared__ uint16_t from_aside[S::kAside ? S::kOwn : 1][S::kAside ? kThreads : 1];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 15, grp = lane >> 4, team = wave / WC, mine = wave % WC;
@@ -141,18 +145,61 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
     auto part = [&](bool some) {
         partial = !some ? nullptr : p.partials + ((size_t)((a ? 0 : p.groups) + u) * p.blocks + block) * part_floats<RANK>(S::kCols);
     };
+    const bool cut = WC > 1 && p.cut;
+    uint32_t tiles = p.tiles;
+    uint32_t *const cuts = starts + kCutRows + 1;
+    auto row_of = [&](uint32_t tile) { return cut ? (uint32_t)__builtin_amdgcn_readfirstlane(cuts[tile]) : tile * p.tile_rows; };
+    auto rows_of = [&](uint32_t tile) {
+        return cut ? (uint32_t)__builtin_amdgcn_readfirstlane(cuts[tile + 1] - cuts[tile])
+                     : min(p.tile_rows, p.rows - tile * p.tile_rows);
+    };
     auto share = [&](uint32_t first, uint32_t count) {
         if (a == 0 && block == 0 && threadIdx.x == 0) {
-            p.shares[2 * tile] = first;
-            p.shares[2 * tile + 1] = count;
+            p.shares[4 * tile] = first;
+            p.shares[4 * tile + 1] = count;
+            p.shares[4 * tile + 2] = row_of(tile);
+            p.shares[4 * tile + 3] = rows_of(tile);
         }
     };
     if (p.partials) {
+        if (cut) {
+            // Tiles begin where the slot changes, where tile_rows rows are full, and every 64 rows (a wave's).
+            constexpr uint32_t kOwn = kCutRows / 64 / S::kWaves;
+            uint64_t begins[kOwn];
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; i++) {
+                const uint32_t r = (wave + i * S::kWaves) * 64 + lane;
+                const uint32_t slot = p.slots[min(r, p.rows - 1)], before = p.slots[min(max(r, 1u) - 1, p.rows - 1)];
+                const uint64_t change = __builtin_amdgcn_ballot_w64(lane == 0 || slot != before);
+                const uint32_t since = lane - (63 - __builtin_clzll(change & (~0ull >> (63 - lane))));
+                begins[i] = __builtin_amdgcn_ballot_w64(r < p.rows && since % p.tile_rows == 0);
+                words[wave + i * S::kWaves] = __builtin_popcountll(begins[i]);
+            }
+            __syncthreads();
+            uint32_t n[kCutRows / 64];
+            tiles = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kCutRows / 64; i++) tiles += n[i] = __builtin_amdgcn_readfirstlane(words[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; i++) {
+                uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(begins[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)begins[i], 0));
+#pragma unroll
+                for (uint32_t e = 0; e < kCutRows / 64; e++)
+                    if (e < wave + i * S::kWaves) at += n[e];
+                if (begins[i] >> lane & 1) cuts[at] = (wave + i * S::kWaves) * 64 + lane;
+            }
+            if (threadIdx.x == 0) {
+                cuts[tiles] = p.rows;
+                if (u == 0 && block == 0) p.shares[4 * p.tiles] = tiles;
+            }
+            __syncthreads();
+        }
 #pragma unroll 1
-        for (uint32_t t = threadIdx.x; t < (p.whole ? kWholeTiles : kMaxTiles); t += kThreads) {
+        for (uint32_t t = threadIdx.x; t < (p.whole ? kWholeTiles : cut ? kCutRows : kMaxTiles); t += kThreads) {
             uint32_t n = 0;
-            if (t < p.tiles) {
-                const uint32_t r0 = t * p.tile_rows, r1 = min(r0 + p.tile_rows, p.rows) - 1;
+            if (t < tiles) {
+                const uint32_t r0 = cut ? cuts[t] : t * p.tile_rows;
+                const uint32_t r1 = (cut ? cuts[t + 1] : min(r0 + p.tile_rows, p.rows)) - 1;
                 const uint32_t most = min(p.max_position, p.place.keys - 1);
                 const uint32_t first = p.positions[r0], slot = p.slots[r0];
                 const uint32_t p0 = min(first, most), p1 = min(p.positions[r1], most);
@@ -175,12 +222,12 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
 #pragma unroll
             for (uint32_t i = 0; i < kWholeTiles / 64; i++) all += m[i] = starts[64 * i + lane];
             all = wave_total(all);
-            const float least = (float)all / (float)p.groups, most = (float)all / (float)(p.groups - p.tiles) + 1.0f;
+            const float least = (float)all / (float)p.groups, most = (float)all / (float)(p.groups - tiles) + 1.0f;
             const float by = __builtin_amdgcn_rcpf(least + (most - least) * (float)col * (1.0f / 15.0f));
             auto parts_of = [](uint32_t n, float by) { return min(max((uint32_t)ceilf((float)n * by), 1u), n); };
             uint32_t parts = 0;
 #pragma unroll 4
-            for (uint32_t t = grp; t < p.tiles; t += 4) parts += parts_of(starts[t], by);
+            for (uint32_t t = grp; t < tiles; t += 4) parts += parts_of(starts[t], by);
             parts = rows4_total(parts);
             const uint64_t fit = __builtin_amdgcn_ballot_w64(parts <= p.groups);
             const float chosen = fit ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), __builtin_ctzll(fit))) : 0.0f;
@@ -188,7 +235,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             bool mine_found = false;
 #pragma unroll
             for (uint32_t i = 0; i < kWholeTiles / 64; i++) {
-                const uint32_t own = 64 * i + lane < p.tiles ? parts_of(m[i], chosen) : 0, upto = before + wave_upto(own, lane);
+                const uint32_t own = 64 * i + lane < tiles ? parts_of(m[i], chosen) : 0, upto = before + wave_upto(own, lane);
                 const uint64_t here = __builtin_amdgcn_ballot_w64(u < upto && u >= upto - own);
                 before = __builtin_amdgcn_readlane(upto, 63);
                 if (!here) continue;
@@ -208,7 +255,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             constexpr uint32_t kEach = kMaxTiles / kThreads;
             uint32_t n[kEach], sum = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kEach; i++) sum += n[i] = starts[threadIdx.x * kEach + i];
+            for (uint32_t i = 0; i < kEach; i++) sum += n[i] = threadIdx.x * kEach + i < tiles ? starts[threadIdx.x * kEach + i] : 0;
             const uint32_t upto = wave_upto(sum, lane);
             if (lane == 63) words[wave] = upto;
             __syncthreads();
@@ -227,12 +274,12 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
 #pragma unroll
             for (uint32_t i = 0; i < kEach; i++) {
                 const uint32_t t = threadIdx.x * kEach + i;
-                if (t >= p.tiles) break;
+                if (t >= tiles) break;
                 starts[t] = at;
                 if (unit >= at && unit < at + n[i]) found = t;
                 at += n[i];
             }
-            if (threadIdx.x == 0) starts[p.tiles] = all;
+            if (threadIdx.x == 0) starts[tiles] = all;
             __syncthreads();
             tile = __builtin_amdgcn_readfirstlane(found);
         }
@@ -240,17 +287,25 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
 
     // A tile's rows, two a lane, for what all waves agree on, and the lane's column. (Columns that are not there, or are
     // refused, go along with what is loaded for them.)
-    uint32_t row_pos[2], row_slot[2], pos, slot;
+    uint32_t row_pos[2], row_slot[2], pos, slot, cut_row, cut_rows;
     bool there;
     const uint16_t *q_at;
-    bf16x8 q[S::kQ];
     const uint32_t qsign = p.scale < 0.0f ? 0x80008000u : 0u;
+    // The tile's first row and rows. (With 16 columns, where registers are fewest, from the tile's number each time.)
+    auto tile_row = [&]() { return WC > 1 ? cut_row : tile * p.tile_rows; };
+    auto tile_rows = [&]() { return WC > 1 ? cut_rows : min(p.tile_rows, p.rows - tile * p.tile_rows); };
+    auto one_row = [&]() { return WC > 1 ? cut_rows == 1 : p.tile_rows == 1; };
     auto fetch = [&]() {
-        const uint32_t row0 = tile * p.tile_rows, l0 = again(lane);
+        const uint32_t l0 = again(lane);
+        if (WC > 1) {
+            cut_row = row_of(tile);
+            cut_rows = rows_of(tile);
+        }
+        const uint32_t row0 = tile_row(), rows = tile_rows();
         uint32_t r = row0, h = block * p.block_heads;
-        if (p.tile_rows == 1) {
-            pos = p.whole ? firsts[0][tile] : p.positions[tile];
-            slot = p.whole ? firsts[1][tile] : p.slots[tile];
+        if (one_row()) {
+            pos = p.whole ? firsts[0][tile] : p.positions[row0];
+            slot = p.whole ? firsts[1][tile] : p.slots[row0];
             row_pos[0] = row_pos[1] = pos;
             row_slot[0] = row_slot[1] = slot;
             const uint32_t c = 16 * mine + (l0 & 15);
@@ -259,11 +314,11 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 2; i++) {
-                const uint32_t r = min(row0 + min(l0 + 64 * i, p.tile_rows - 1), p.rows - 1);
+                const uint32_t r = row0 + min(l0 + 64 * i, rows - 1);
                 row_pos[i] = p.positions[r];
                 row_slot[i] = p.slots[r];
             }
-            there = column_of(p, row0, block, 16 * mine + (l0 & 15), r, h);
+            there = column_of(p, row0, rows, block, 16 * mine + (l0 & 15), r, h);
             if (!there) r = row0, h = 0;
             pos = p.positions[r];
             slot = p.slots[r];
@@ -311,7 +366,6 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             part(a || b < units);
             share(u, (t1 - 1) / each - u + 1);
         }
-        const uint32_t row0 = tile * p.tile_rows;
         auto lives = [&](uint32_t pos, uint32_t slot) { return pos <= p.max_position && holds(p.place, slot, pos); };
         uint64_t row_waits[2], row_live[2];
         {
@@ -320,7 +374,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             for (uint32_t i = 0; i < 2; i++) {
                 rows_at[0][64 * i + l0] = row_pos[i];
                 rows_at[1][64 * i + l0] = row_slot[i];
-                const bool here = 64 * i + l0 < p.tile_rows && row0 + 64 * i + l0 < p.rows;
+                const bool here = 64 * i + l0 < tile_rows();
                 row_waits[i] = row_live[i] = __builtin_amdgcn_ballot_w64(here && lives(row_pos[i], row_slot[i]));
             }
             if (there && !lives(pos, slot) && p.status && a == 0 && team == 0 && l0 < 16)
@@ -328,7 +382,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
         }
         const bool live = there && lives(pos, slot);
         const uint32_t from = pos > p.back ? pos - p.back : 0;
-        bool wait = live, fresh = true;  // fresh: q is not there yet
+        bool wait = live;
         float m = -INFINITY, l = 0.0f;
         f32x4 o[S::kD];
 #pragma unroll
@@ -345,7 +399,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             const bool act = wait && slot == now;
             wait = wait && !act;
             uint32_t lo, hi, same_lo, same_hi, wlo, whi, all_lo, all_hi;
-            if (p.tile_rows == 1) {
+            if (one_row()) {
                 row_waits[0] = 0;
                 lo = same_lo = all_lo = __builtin_amdgcn_readfirstlane(from);
                 hi = same_hi = all_hi = __builtin_amdgcn_readfirstlane(pos);
@@ -385,6 +439,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             // Where the blocks of the rounds from r0 on are held, those of kChunk rounds one a lane, and which are not. (A block
             // that is not held is the first in the loads, and cleared. Without a table a slot is one page.)
             constexpr uint32_t kChunk = 64 / S::kIds;
+            bf16x8 q[S::kQ];
             uint32_t r0, place;
             uint64_t lost_of;
             const_u32 *pages = in_constant<const_u32 *>(p.place.table + (size_t)now * p.place.kept_pages);
@@ -394,7 +449,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                                                (round + l0 / S::kIds) * (S::kUnit / kBlock) + l0 % S::kIds, last);
                 uint32_t page = now * (p.place.keys / kBlock);
                 if (p.place.table) page = pages[block >> page_blocks];
-                if (first && fresh) {
+                if (first) {
                     // q is asked for behind the pages, which the first keys wait for, and before those. (The pages' own wait is
                     // here, where q's loads are known to be younger.)
 #pragma unroll
@@ -403,9 +458,6 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     if (qsign)
 #pragma unroll
                         for (uint32_t j = 0; j < S::kQ; j++) q[j] = as_bf16x8(__builtin_bit_cast(u32x4, q[j]) ^ qsign);
-                    fresh = false;
-                } else {
-                    asm volatile("" : "+v"(page));
                 }
                 const bool lost = page >= page_count;
                 place = ((lost ? 0 : page) << page_blocks) + (block & page_mask);
@@ -683,7 +735,7 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
             }
         };
         uint32_t r, h;
-        if (column_of(p, row0, block, c, r, h)) {
+        if (column_of(p, tile_row(), tile_rows(), block, c, r, h)) {
             if (partial) {
                 float *to = partial + (g * S::kCols + c) * 4;
                 each_of([&](uint32_t d, f32x4 x) { *(f32x4 *)(to + 4 * d * S::kCols * 4) = x; });
@@ -715,12 +767,13 @@ __global__ __launch_bounds__(kJoinThreads) void join_latent_kernel(LatentParams 
     const uint32_t piece = u % (RANK / 64), c0 = u / (RANK / 64) % (columns / 16) * 16;
     u /= RANK / 64 * (columns / 16);
     const uint32_t block = u % p.blocks, tile = u / p.blocks;
-    const uint32_t first = __builtin_amdgcn_readfirstlane(p.shares[2 * tile]);
-    const uint32_t parts = __builtin_amdgcn_readfirstlane(p.shares[2 * tile + 1]);
-    if (parts < 2) return;
+    const u32x4 share = *(const u32x4 *)(p.shares + 4 * tile);
+    const uint32_t tiles = p.cut ? p.shares[4 * p.tiles] : p.tiles;
+    const uint32_t first = __builtin_amdgcn_readfirstlane(share[0]), parts = __builtin_amdgcn_readfirstlane(share[1]);
+    if (tile >= tiles || parts < 2) return;
     const uint32_t c = c0 + (threadIdx.x & 15), quad = piece * 16 + (threadIdx.x >> 4);
     uint32_t r, h;
-    if (!column_of(p, tile * p.tile_rows, block, c, r, h)) return;
+    if (!column_of(p, __builtin_amdgcn_readfirstlane(share[2]), __builtin_amdgcn_readfirstlane(share[3]), block, c, r, h)) return;
     auto part_at = [&](uint32_t j) {
         return p.partials + ((size_t)((j ? 0 : p.groups) + first + j) * p.blocks + block) * part_floats<RANK>(columns);
     };
@@ -761,7 +814,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_latent_kernel(LatentParams 
 
 struct Plan {
     uint32_t columns, block_heads, blocks, tile_rows, tiles, groups;
-    bool shared, whole;
+    bool shared, whole, cut;
 };
 
 // How many columns a group has, and how the keys are divided. A group takes some time for its q, its partial sums and
@@ -770,12 +823,15 @@ struct Plan {
 // 1 x 16 x 4000 18, 22, 23, 29; 1 x 128 x 4000 22, 29, 31, 43; 4 x 128 x 4000 30, 30, 33, 41; 32 x 64 x 4000 65, 55, 45, 46;
 // 32 x 128 x 512 .. 8192 118, 109, 70, 72; 2 x 512 rows of 16 heads x 2500 .. 4600 318, 277, 168, 155.)
 //
-// Rows of a tile that belong to two slots take two passes over keys, one after the other. So a tile has no more rows than
-// a fourth of those that stand together (24 sequences of up to 5 rows, 16 heads, 4000 keys: 48 us with one row a
-// tile, 82 with two to five).
+// Rows of a tile that belong to two slots take two passes over keys, one after the other. So tiles are cut where slots change,
+// which a group looks for among up to kCutRows rows; of more rows, and in 16 columns, a tile has no more than a fourth of those
+// that stand together. (24 sequences of up to 5 rows, 32 heads, 1000 .. 9001 keys: 62 us, with a row a tile 71; 4 heads, 4000
+// keys: 36 and 43; 16 heads with two to five rows a tile and no cuts 82.)
 Plan plan(const ts_latent_args *k) {
     const ts_rows_args *a = &k->rows;
-    constexpr double kStart[4] = {19, 22, 29, 40}, kKey[4] = {0.020, 0.032, 0.033, 0.0565};  // us (512 + 64 values)
+    constexpr double kStart[2][4] = {{19, 22, 29, 40}, {14.5, 19.5, 20, 29}};                // us (512 + 64 values; 256 + 32)
+    constexpr double kKey[2][4] = {{0.020, 0.032, 0.033, 0.0565}, {0.010, 0.016, 0.0165, 0.028}};
+    const uint32_t of = k->rank == 512 ? 0 : 1;
     const uint32_t run = std::max(1u, std::min(k->run, a->rows));
     Plan best = {};
     double least = INFINITY;
@@ -784,22 +840,22 @@ Plan plan(const ts_latent_args *k) {
         s.columns = 16u << i;
         s.block_heads = std::min(a->heads, s.columns);
         s.blocks = (a->heads - 1) / s.block_heads + 1;
-        s.tile_rows = std::max(1u, std::min(run / 4, s.columns / s.block_heads));
-        s.tiles = (a->rows - 1) / s.tile_rows + 1;
-        s.groups = s.tiles;
-        s.shared = s.whole = false;
+        s.tile_rows = std::max(1u, std::min(run, s.columns / s.block_heads));
         const uint32_t at_once = std::max(1u, (k->rank == 512 || s.columns >= 64 ? 256u : 512u) / s.blocks);  // a CU's one or two
         const uint32_t unit = kKeys * (s.columns == 16 ? 4 : s.columns == 128 ? 1 : 2);
         const uint64_t span = std::min<uint64_t>(std::min<uint64_t>((uint64_t)a->max_position + 1, a->keys),
                                                  (uint64_t)a->back + s.tile_rows + kBlock);
-        const uint64_t units = (span + unit - 1) / unit + 1;
-        if (at_once > 1 && s.tiles <= std::min(kMaxTiles, 4 * at_once) && span > unit) {
-            s.groups = (uint32_t)std::min<uint64_t>(at_once, s.tiles * units);
-            s.shared = true;
-            s.whole = s.tiles <= kWholeTiles && 3 * s.tiles <= s.groups;
-        }
-        const double keys = (double)span * s.tiles * s.blocks / 256.0;  // a CU's
-        const double takes = kStart[i] + keys * kKey[i] * a->width / 576.0;
+        auto shared = [&](uint32_t tiles) { return at_once > 1 && tiles <= std::min(kMaxTiles, 4 * at_once) && span > unit; };
+        s.cut = s.columns > 16 && s.tile_rows > 1 && a->rows <= kCutRows && shared(a->rows);
+        if (!s.cut) s.tile_rows = std::max(1u, std::min(run / 4, s.tile_rows));
+        s.tiles = s.cut ? a->rows : (a->rows - 1) / s.tile_rows + 1;
+        // (Cut tiles: as many as full runs make.)
+        const uint32_t tiles = s.cut ? (a->rows * ((run - 1) / s.tile_rows + 1) - 1) / run + 1 : s.tiles;
+        s.shared = shared(s.tiles);
+        s.groups = s.shared ? (uint32_t)std::min<uint64_t>(at_once, s.tiles * ((span + unit - 1) / unit + 1)) : s.tiles;
+        s.whole = s.shared && s.tiles <= kWholeTiles && s.tiles < s.groups && 3 * tiles <= s.groups;
+        const double keys = (double)span * tiles * s.blocks / 256.0;  // a CU's
+        const double takes = kStart[of][i] + keys * kKey[of][i];
         if (takes < least) least = takes, best = s;
     }
     return best;
@@ -808,7 +864,7 @@ Plan plan(const ts_latent_args *k) {
 size_t partial_bytes(const ts_latent_args *k, const Plan &s) {
     return s.shared ? (size_t)s.groups * 2 * s.blocks * s.columns * (k->rank + 2) * sizeof(float) : 0;
 }
-size_t share_bytes(const Plan &s) { return s.shared ? (size_t)s.tiles * 2 * sizeof(uint32_t) : 0; }
+size_t share_bytes(const Plan &s) { return s.shared ? ((size_t)s.tiles * 4 + 1) * sizeof(uint32_t) : 0; }
 
 bool wide(const ts_latent_args *k) { return k->rank == 512 && k->rows.width == 576; }
 bool narrow(const ts_latent_args *k) { return k->rank == 256 && k->rows.width == 288; }
@@ -885,6 +941,7 @@ extern "C" int tessera_hip_attend_latent(const ts_latent_args *k, void *stream) 
     p.tile_rows = s.tile_rows; p.tiles = s.tiles; p.groups = s.groups;
     p.block_heads = s.block_heads; p.blocks = s.blocks;
     p.whole = s.shared && s.whole;
+    p.cut = s.cut;
     p.scale = a->scale;
     return k->rank == 512 ? launch<512, 64>(p, s, stream) : launch<256, 32>(p, s, stream);
 }

@@ -491,6 +491,25 @@ def test_wide_tiles_not_finite_in_masked_places(widths, heads, run, keys, back, 
         assert torch.equal(got[others], want[others])
 
 
+@pytest.mark.parametrize("rows", [2, 63, 64, 65, 130, 512, 513])
+@pytest.mark.parametrize("heads,run", [(16, 5), (32, 2), (5, 9)])
+def test_rows_of_many_short_runs(rows, heads, run):
+    """Runs of any length at any place, as many tiles as may be told from the slots, and more."""
+    rank, rope = 256, 32
+    r = rng(rows + heads)
+    counts = []
+    while sum(counts) < rows:
+        counts.append(min(int(r.integers(1, run + 2)), rows - sum(counts)))
+    lengths = [int(c + r.integers(0, 50)) for c in counts]
+    kept, where = cache(r, lengths, rank + rope, 16)
+    where = roomier(where, 1 << 14)
+    slots = np.repeat(np.arange(len(counts)), counts)
+    positions = np.concatenate([n - c + np.arange(c) for n, c in zip(lengths, counts)])
+    q = dev(r.standard_normal((rows, heads, rank + rope)), BF16)
+    got = attend(q, kept, slots, positions, where, rank=rank, scale=0.1, run=run, max_position=(1 << 14) - 1)
+    check_attend(got, q, kept, slots, positions, where, rank=rank, scale=0.1)
+
+
 @pytest.mark.parametrize("widths", ["wide", "narrow"])
 @pytest.mark.parametrize("heads", [5, 16])
 def test_decode_rows_take_weights_in_two_parts(widths, heads):
