@@ -652,11 +652,14 @@ _BF16 = (torch.bfloat16,)
 def _rows_of(what, name, t, on, dtype, heads=None):
     """The distances (of rows, of heads) of t [rows, heads, width], any of them where there is one row or head."""
     rows, n, width = t.shape
-    if t.get_device() != on or t.dtype is not dtype or (t.stride(2) != 1 and width > 1) or (heads is not None and n != heads):
+    row, head, one = t.stride()
+    if t.get_device() != on or t.dtype is not dtype or (one != 1 and width > 1) or (heads is not None and n != heads):
         raise ValueError(f"{what}: {name} must be [rows, heads, width] of {str(dtype).replace('torch.', '')} on GPU {on}, a "
                          "head's values back to back")
-    head = t.stride(1) if n > 1 else 0
-    row = t.stride(0) if rows > 1 else 0
+    if n <= 1:
+        head = 0
+    if rows <= 1:
+        row = 0
     if row >> 32 or head >> 32:
         raise ValueError(f"{what}: {name} rows or heads more than 2^32 elements apart")
     return row, head
@@ -675,8 +678,10 @@ def append_latent(c, kept, slots, positions, *, keys, rank, gain=None, angles=No
     rows, width = c.shape
     on, x = c.get_device(), c.dtype
     rope = width - rank
-    stride = c.stride(0) if rows > 1 else width
-    if x not in _ROWS or (c.stride(1) != 1 and width > 1) or stride >> 32:
+    stride, one = c.stride()
+    if rows <= 1:
+        stride = width
+    if x not in _ROWS or (one != 1 and width > 1) or stride >> 32:
         raise ValueError("append_latent: c must be rows of f32 or bf16, a row's values back to back")
     if kept.shape[-1] != width:
         raise ValueError(f"append_latent: kept rows of {kept.shape[-1]} values for rows of {width}")
