@@ -232,46 +232,69 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         const uint32_t g = 64 * (x * kWaves + wave) + lane, r = g / kPv;
         vplace[x] = r * p.v_stride * 2 + (g % kPv ^ value_swap<kPv>(r)) * 16;
     }
-    // One step's rows, a KiB a load; keys past the last are the last again.
-    auto issue = [&](uint32_t n, uint32_t slot) {
-        const uint32_t to = lds_address(stage) + slot * kStage;
-        const uint32_t key0 = base + n * kKeys, most = (uint32_t)hi - key0;
-        const auto kbuf = rows_buffer(p.k + (size_t)(q.key0 + key0) * p.k_stride + (size_t)h * p.k_head);
-        const auto vbuf = rows_buffer(p.v + (size_t)(q.key0 + key0) * p.v_stride + (size_t)h * p.v_head);
-        const auto rbuf = rows_buffer(p.r + (size_t)(q.key0 + key0) * p.r_stride);
-        auto loads = [&](auto place) {  // (place(where a row lies, its number, its distance))
-#pragma unroll
-            for (uint32_t x = 0; x < kPartsK; x++)
-                rows_to_lds16(kbuf, to + (x * kWaves + wave) * 1024, place(kplace[x], (x * kWaves + wave) * (64 / kPk), kPk, p.k_stride));
-#pragma unroll
-            for (uint32_t x = 0; x < kPartsR; x++)
-                rows_to_lds16(rbuf, to + kK + (x * kWaves + wave) * 1024, place(rplace[x], (x * kWaves + wave) * (64 / kPr), kPr, p.r_stride));
-#pragma unroll
-            for (uint32_t x = 0; x < kPartsV; x++)
-                rows_to_lds16(vbuf, to + kK + kR + (x * kWaves + wave) * 1024,
-                              place(vplace[x], (x * kWaves + wave) * (64 / kPv), kPv, p.v_stride));
+    // A step's rows, a KiB a load, of which a wave has kLoads; keys past the last are the last again. The vector cache
+    // takes 64 bytes a cycle, so that a step's loads one behind the other keep a wave for 640 cycles: they go between
+    // the products.
+    constexpr uint32_t kLoads = kPartsK + kPartsR + kPartsV;
+    const char *kat = (const char *)(p.k + (size_t)(q.key0 + base) * p.k_stride + (size_t)h * p.k_head);
+    const char *vat = (const char *)(p.v + (size_t)(q.key0 + base) * p.v_stride + (size_t)h * p.v_head);
+    const char *rat = (const char *)(p.r + (size_t)(q.key0 + base) * p.r_stride);
+    uint32_t most = (uint32_t)(hi - base);  // keys behind the step's first
+    auto last = [&]() {
+        if (most >= kKeys - 1) return;
+        auto ends = [&](uint32_t &at, uint32_t row0, uint32_t pieces, uint32_t stride) {
+            const uint32_t row = row0 + again(lane) / pieces;
+            at -= row > most ? (row - most) * stride * 2 : 0;
         };
-        if (most >= kKeys - 1)
-            loads([](uint32_t at, uint32_t, uint32_t, uint32_t) { return at; });
-        else
-            loads([&](uint32_t at, uint32_t row0, uint32_t pieces, uint32_t stride) {
-                const uint32_t row = row0 + again(lane) / pieces;
-                return at - (row > most ? (row - most) * stride * 2 : 0);
-            });
-    };
-
 #pragma unroll
-    for (uint32_t n = 0; n + 1 < kRing; n++)
-        if (n < steps) issue(n, n);
+        for (uint32_t x = 0; x < kPartsK; x++) ends(kplace[x], (x * kWaves + wave) * (64 / kPk), kPk, p.k_stride);
+#pragma unroll
+        for (uint32_t x = 0; x < kPartsR; x++) ends(rplace[x], (x * kWaves + wave) * (64 / kPr), kPr, p.r_stride);
+#pragma unroll
+        for (uint32_t x = 0; x < kPartsV; x++) ends(vplace[x], (x * kWaves + wave) * (64 / kPv), kPv, p.v_stride);
+    };
+    auto onward = [&]() {
+        kat += (size_t)p.k_stride * (2 * kKeys);
+        vat += (size_t)p.v_stride * (2 * kKeys);
+        rat += (size_t)p.r_stride * (2 * kKeys);
+        most -= kKeys;
+        last();
+    };
+    struct Next {
+        u32x4 k, v, r;
+        uint32_t land;
+    };
+    auto rows_to = [&](uint32_t slot) { return Next{rows_buffer(kat), rows_buffer(vat), rows_buffer(rat), lds_address(stage) + slot * kStage}; };
+    auto load = [&](const Next &next, uint32_t x) {
+        if (x < kPartsK)
+            rows_to_lds16(next.k, next.land + (x * kWaves + wave) * 1024, kplace[x]);
+        else if (x < kPartsK + kPartsR)
+            rows_to_lds16(next.r, next.land + kK + ((x - kPartsK) * kWaves + wave) * 1024, rplace[x - kPartsK]);
+        else
+            rows_to_lds16(next.v, next.land + kK + kR + ((x - kPartsK - kPartsR) * kWaves + wave) * 1024,
+                          vplace[x - kPartsK - kPartsR]);
+    };
+    if (steps) {
+        last();
+        const Next next = rows_to(0);
+#pragma unroll
+        for (uint32_t x = 0; x < kLoads; x++) load(next, x);
+    }
     for (uint32_t n = 0, slot = 0; n < steps; n++) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (n + kRing - 1 < steps) issue(n + kRing - 1, (slot + kRing - 1) % kRing);
         char *at = stage + slot * kStage;
-        slot = slot + 1 == kRing ? 0 : slot + 1;
+        slot ^= 1;
+        // (Behind the last step, its rows once more: nobody reads them.)
+        if (n + 1 < steps) onward();
+        const Next next = rows_to(slot);
         const int32_t here = base + (int32_t)(n * kKeys), end = here + (int32_t)kKeys - 1;
         const bool apart = here < same_lo || end > same_hi;  // some key is one row's and not another's, or no key
         const bool work = here <= whi && end >= wlo;
-        if (!apart && !work) continue;
+        if (!apart && !work) {
+#pragma unroll
+            for (uint32_t x = 0; x < kLoads; x++) load(next, x);
+            continue;
+        }
 
         // Half t of the step, 32 keys: its scores, register e key 32 t + 8 (e / 4) + 4 half + e % 4; its softmax; its
         // values. The first half's softmax runs beside the second's scores, the second's beside the first's values, in
@@ -308,8 +331,8 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         };
         // The softmax in kSoft pieces. m moves only when a score passes it by 2^kSlack, so most steps leave the sum and O as
         // they are and no weight passes 2^kSlack.
-        constexpr uint32_t kSoft = 11;
-        float mx, mn, mo, sum;
+        constexpr uint32_t kSoft = 13;
+        float mx, mn, mo, sum, arg[2], weight[2];
         uint32_t w[2][8];
         auto soft = [&](uint32_t t, uint32_t i) {
             if (i < 2) {
@@ -326,12 +349,26 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
                 pinned(mn);
                 pinned(mo);
             } else {
-                const uint32_t e = 2 * (i - 3);
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][e], sl, -mo)), y = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], sl, -mo));
-                sum += x + y;
-                w[t][i - 3] = bf16_pair(x, y);
-                pinned(sum);
-                pinned(w[t][i - 3]);
+                // Pair j's arguments, the pair's before it weights, and those of one more before into the sum: none waits for
+                // another.
+                const uint32_t j = i - 3;
+                if (j >= 2) {
+                    sum += weight[0] + weight[1];
+                    w[t][j - 2] = bf16_pair(weight[0], weight[1]);
+                    pinned(sum);
+                    pinned(w[t][j - 2]);
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 2; e++) {
+                    if (j >= 1 && j < 9) {
+                        weight[e] = __builtin_amdgcn_exp2f(arg[e]);
+                        pinned(weight[e]);
+                    }
+                    if (j < 8) {
+                        arg[e] = fmaf(s[t][2 * j + e], sl, -mo);
+                        pinned(arg[e]);
+                    }
+                }
             }
         };
         // The pieces that belong to product i of n.
@@ -371,7 +408,11 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        scores(0, [](uint32_t) {});
+        scores(0, [&](uint32_t i) {
+#pragma unroll
+            for (uint32_t x = 0; x < kLoads; x++)
+                if (x * kQ / kLoads == i) load(next, x);
+        });
         masked(0);
         scores(1, [&](uint32_t i) { pieces(0, i, kQ); });
         masked(1);
@@ -419,6 +460,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         raised();
         values(1, [](uint32_t) {});
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (!there) return;
     // A row that sees no key is zero.
     const float sum = halves_sum(l), by = pos < 0 ? 0.0f : 1.0f / sum;
@@ -434,10 +476,11 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
 template <uint32_t NOPE, uint32_t ROPE, uint32_t VALUE>
 int launch(const FlashParams &p, uint32_t groups, void *stream) {
     constexpr uint32_t kLds = kRing * kKeys * 2 * (NOPE + ROPE + VALUE);
-    static const hipError_t attr = hipFuncSetAttribute((const void *)flash_latent_kernel<NOPE, ROPE, VALUE>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    const auto kernel = flash_latent_kernel<NOPE, ROPE, VALUE>;
+    static const hipError_t attr =
+        hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return ts::hip_status(attr, "flash_latent: shared memory attribute");
-    hipLaunchKernelGGL((flash_latent_kernel<NOPE, ROPE, VALUE>), dim3(groups), dim3(kThreads), kLds, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), kLds, (hipStream_t)stream, p);
     TS_CHECK_LAUNCH("flash_latent launch");
     return TS_OK;
 }
