@@ -280,20 +280,27 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
 #pragma unroll
         for (uint32_t x = 0; x < kLoads; x++) load(next, x);
     }
-    for (uint32_t n = 0, slot = 0; n < steps; n++) {
+    // The operands' places by their piece; those of a step's buffer are a constant further.
+    uint32_t kx[NOPE / 16], rx[ROPE / 16], vx[kD];
+#pragma unroll
+    for (uint32_t j = 0; j < NOPE / 16; j++) kx[j] = koff ^ 32 * j;
+#pragma unroll
+    for (uint32_t j = 0; j < ROPE / 16; j++) rx[j] = roff ^ 32 * j;
+#pragma unroll
+    for (uint32_t d = 0; d < kD; d++) vx[d] = voff ^ 64 * d;
+    auto step = [&](uint32_t n, auto slot) {
+        char *const at = stage + slot() * kStage;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        char *at = stage + slot * kStage;
-        slot ^= 1;
         // (Behind the last step, its rows once more: nobody reads them.)
         if (n + 1 < steps) onward();
-        const Next next = rows_to(slot);
+        const Next next = rows_to(1 - slot());
         const int32_t here = base + (int32_t)(n * kKeys), end = here + (int32_t)kKeys - 1;
         const bool apart = here < same_lo || end > same_hi;  // some key is one row's and not another's, or no key
         const bool work = here <= whi && end >= wlo;
         if (!apart && !work) {
 #pragma unroll
             for (uint32_t x = 0; x < kLoads; x++) load(next, x);
-            continue;
+            return;
         }
 
         // Half t of the step, 32 keys: its scores, register e key 32 t + 8 (e / 4) + 4 half + e % 4; its softmax; its
@@ -301,11 +308,10 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         // pieces between the products (a wave's instructions issue in order). Operands are read kAhead products ahead.
         f32x16 s[2];
         bf16x8 ring[kAhead + 1];
-        const uint32_t k0 = again(koff), r0 = again(roff), v0 = again(voff);
         auto scores = [&](uint32_t t, auto beside) {
             auto read_k = [&](uint32_t j) {
-                ring[j % (kAhead + 1)] = j < NOPE / 16 ? *(const bf16x8 *)(at + (k0 ^ 32 * j) + t * 32 * (2 * NOPE))
-                                                       : *(const bf16x8 *)(at + (r0 ^ 32 * (j - NOPE / 16)) + t * 32 * (2 * ROPE));
+                ring[j % (kAhead + 1)] = j < NOPE / 16 ? *(const bf16x8 *)(at + t * 32 * (2 * NOPE) + kx[j < NOPE / 16 ? j : 0])
+                                                       : *(const bf16x8 *)(at + t * 32 * (2 * ROPE) + rx[j < NOPE / 16 ? 0 : j - NOPE / 16]);
             };
 #pragma unroll
             for (int e = 0; e < 16; e++) s[t][e] = 0.0f;
@@ -336,10 +342,11 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         uint32_t w[2][8];
         auto soft = [&](uint32_t t, uint32_t i) {
             if (i < 2) {
-                float x = fmaxf(s[t][8 * i], s[t][8 * i + 1]);
+                // (A NaN may come out: the row's sum is one as well.)
+                float x = __builtin_elementwise_maximum(s[t][8 * i], s[t][8 * i + 1]);
 #pragma unroll
-                for (int e = 2; e < 8; e++) x = fmaxf(x, s[t][8 * i + e]);
-                mx = i ? fmaxf(mx, x) : x;
+                for (int e = 2; e < 8; e++) x = __builtin_elementwise_maximum(x, s[t][8 * i + e]);
+                mx = i ? __builtin_elementwise_maximum(mx, x) : x;
                 pinned(mx);
             } else if (i == 2) {
                 mx = halves_max(mx) * sl;
@@ -391,7 +398,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         auto values = [&](uint32_t t, auto beside) {
             // Product i: keys 32 t + 16 (i / kD) .., d 32 (i % kD) .. . (Eight rows on the XOR is the same.)
             auto read_v = [&](uint32_t i) {
-                const char *v = at + (v0 ^ i % kD * 64) + (32 * t + i / kD * 16) * (2 * VALUE);
+                const char *v = at + (32 * t + i / kD * 16) * (2 * VALUE) + vx[i % kD];
                 const u32x2 lo4 = read_vt4(v), hi4 = read_vt4(v + 8 * (2 * VALUE));
                 ring[i % (kAhead + 1)] = as_bf16x8(u32x4{lo4.x, lo4.y, hi4.x, hi4.y});
             };
@@ -459,6 +466,10 @@ __global__ __launch_bounds__(kThreads, 2) void flash_latent_kernel(FlashParams p
         values(0, [&](uint32_t i) { pieces(1, i, 2 * kD); });
         raised();
         values(1, [](uint32_t) {});
+    };
+    for (uint32_t n = 0; n < steps; n += 2) {
+        step(n, [] { return 0u; });
+        if (n + 1 < steps) step(n + 1, [] { return 1u; });
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (!there) return;
