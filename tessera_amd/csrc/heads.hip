@@ -2,10 +2,10 @@
 //
 // 2 n k flops against 2 (n + k) bytes of x and out: at k or n of 128 at most 128 flops a byte, a fifth of what the
 // matrix unit needs for each byte from HBM, so bytes bound it (few rows: the weights'). A chunk of 64 k of a group's rows
-// of x and w, 128 or 256 bytes of each, goes straight to LDS, two chunks ahead of the products: reads of whole lines, where
+// of x and w, 128 or 256 bytes of each, goes straight to LDS, one or two chunks ahead of the products: reads of whole lines, where
 // operands taken from memory as they lie (32 rows, 32 bytes of each) were bound by the vector cache's tags.
 // 1024 rows of 32 heads, 512 -> 128 to f32: 13.5 us, 4.0 TB/s (from memory to registers 27.5 us); 32 rows of 128 heads,
-// 128 -> 512: 5.5 us, 4.0 TB/s (7.6 us); 8192 rows of 16 heads, 512 -> 128: 39 us, 5.2 TB/s. What is left is the start
+// 128 -> 512: 5.5 us, 4.0 TB/s (7.6 us); 8192 rows of 16 heads, 512 -> 128: 34 us, 6.0 TB/s. What is left is the start
 // of each group, before its first chunk has come, and its end; f32 rows are bound by vector work (25 us, 3.5 TB/s).
 #include "common.h"
 
@@ -61,6 +61,7 @@ struct Tile {
     static constexpr uint32_t kXRow = kChunk * (XBF16 ? 2 : 4), kWRow = kChunk * 2;
     static constexpr uint32_t kX = kRows * kXRow, kStage = kX + kCols * kWRow;
     static constexpr uint32_t kXLoads = kX / 1024 / kWaves, kWLoads = kCols * kWRow / 1024 / kWaves;  // a wave's
+    static constexpr uint32_t kStages = MT * MN == 4 && XBF16 ? 2 : 3;  // chunks in LDS: two of the largest leave a CU two groups
     static constexpr uint32_t kOutRow = kCols * 4 + 16, kOut = kRows * kOutRow;
     static_assert(kX % (1024 * kWaves) == 0 && kCols * kWRow % (1024 * kWaves) == 0, "equal loads for all waves");
 };
@@ -145,21 +146,22 @@ __global__ __launch_bounds__(64 * NW * RW, 2) void linear_heads_kernel(HeadsPara
     };
     constexpr uint32_t kLoads = T::kXLoads + T::kWLoads;
     issue(0, 0);
-    if (kChunk < p.k) issue(kChunk, 1);
+    if (T::kStages == 3 && kChunk < p.k) issue(kChunk, 1);
     uint32_t now = 0;
     for (uint32_t k0 = 0; k0 < p.k; k0 += kChunk) {
-        if (k0 + kChunk < p.k)
+        if (T::kStages == 3 && k0 + kChunk < p.k)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (k0 + 2 * kChunk < p.k) issue(k0 + 2 * kChunk, now ? now - 1 : 2);
+        const uint32_t next = k0 + (T::kStages - 1) * kChunk;
+        if (next < p.k) issue(next, now ? now - 1 : T::kStages - 1);
         if (n0 + n1 < p.n) {
             if (k0 + kChunk <= p.k)
                 products(stage + now * T::kStage, kChunk);
             else
                 products(stage + now * T::kStage, p.k - k0);
         }
-        now = now == 2 ? 0 : now + 1;
+        now = now + 1 == T::kStages ? 0 : now + 1;
     }
     // Sums change places in LDS, so that a store has whole rows' columns: register 4 q + i of a lane is column
     // 8 q + 4 half + i of row `col`.
@@ -204,7 +206,7 @@ template <bool XBF16, uint32_t NW, uint32_t RW, uint32_t MT, uint32_t MN>
 int launch(HeadsParams &p, uint32_t heads, void *stream) {
     using T = Tile<XBF16, NW, RW, MT, MN>;
     const auto kernel = linear_heads_kernel<XBF16, NW, RW, MT, MN>;
-    constexpr uint32_t kMost = std::max(3 * T::kStage, T::kOut);
+    constexpr uint32_t kMost = std::max(T::kStages * T::kStage, T::kOut);
     p.row_tiles = (p.rows - 1) / T::kRows + 1;
     p.col_tiles = (p.n - 1) / T::kCols + 1;
     const uint64_t all = (uint64_t)p.row_tiles * p.col_tiles * heads;
@@ -213,7 +215,7 @@ int launch(HeadsParams &p, uint32_t heads, void *stream) {
     static const hipError_t attr =
         hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (attr != hipSuccess) return ts::hip_status(attr, "linear_heads: shared memory attribute");
-    const uint32_t stages = std::min(3u, (p.k - 1) / kChunk + 1);  // (fewer: more groups a CU)
+    const uint32_t stages = std::min(T::kStages, (p.k - 1) / kChunk + 1);  // (fewer: more groups a CU)
     hipLaunchKernelGGL(kernel, dim3((p.groups + 7) / 8 * 8), dim3(T::kThreads), std::max(stages * T::kStage, T::kOut),
                        (hipStream_t)stream, p);
     TS_CHECK_LAUNCH("linear_heads launch");
@@ -261,5 +263,9 @@ extern "C" int tessera_hip_linear_heads(const ts_heads_args *a, void *stream) {
     // of the group's columns: taking them apart is vector work, which waves along the columns would repeat (1024 rows of
     // 32 heads, 512 -> 128: 25 us against 40).
     if (a->n <= 64) return bf16 ? launch<true, 2, 2, 1, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 2>(p, a->heads, stream);
+    // Many rows of bf16: 128 a tile, 64 x 64 a wave, two chunks in LDS (8192 rows of 16 heads, 512 -> 128: 34 us against 39 with 64
+    // rows; 32000 rows, 640 -> 640: 46 against 53; but of one chunk, 2000 rows of 16 heads, 8 -> 640: 19 against 17).
+    if (bf16 && a->k > kChunk && (uint64_t)a->heads * ((a->n - 1) / 128 + 1) * ((a->rows - 1) / 128 + 1) >= 1024)
+        return launch<true, 2, 2, 2, 2>(p, a->heads, stream);
     return bf16 ? launch<true, 4, 1, 2, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 4>(p, a->heads, stream);
 }

@@ -174,6 +174,21 @@ def test_linear_heads(rows, heads, n, k, x, out):
     assert not gap or bool((held[..., n:] == 7.0).all())
 
 
+@pytest.mark.parametrize("rows,heads,n,k", [(1100, 128, 40, 72), (130, 520, 130, 136), (4100, 16, 200, 320)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_linear_heads_of_many_rows(rows, heads, n, k, out):
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(rows, heads, k, generator=g, device="cuda").to(BF16)
+    w = torch.randn(heads, n, k, generator=g, device="cuda").to(BF16)
+    got = rules.linear_heads(x, w, out_dtype=out).double()
+    xd, wd = x.double().transpose(0, 1).contiguous(), w.double().transpose(1, 2).contiguous()
+    want = torch.bmm(xd, wd).transpose(0, 1)
+    size = torch.bmm(xd.abs(), wd.abs()).transpose(0, 1)
+    # k / 16 accumulating products and one more rounding, 2^-21 each, and bf16's half step.
+    limit = (k / 16 + 1) * 2.0 ** -21 * size + (HALF * want.abs() if out is BF16 else 0)
+    assert bool(((got - want).abs() <= limit).all())
+
+
 @pytest.mark.parametrize("x", [F32, BF16])
 def test_linear_heads_not_finite_and_layouts(x):
     """An infinity or NaN reaches its row alone (f32 ones too, though they enter in parts); heads may lie outside rows."""
