@@ -8,11 +8,11 @@
 // their use; V^T comes through the transposing LDS read. Two groups share a CU (all of its LDS: there is none besides
 // the steps'), so that one's softmax runs under the other's products.
 //
-// 4 prompts of 2048 rows, 16 heads of 128 + 64 and 128 values: 115 us, 750 TFLOP/s (132 us before a step's halves took turns
-// and tiles of a head shared an XCD); one of 16384 rows 910 TFLOP/s. The matrix unit is busy for 45% of the cycles and the
-// vector unit for 47%, at the clock of 1.7 GHz that the card then keeps; LDS for a quarter. Small grids are bound by a wave's
-// steps in turn, some 1.5 us each (5 sequences of up to 900 rows, 5 heads of 64 + 32 and 64 values: 25 us; with two teams of
-// waves a group, each with every other step, 22 us, but a row of 16 heads 8.2 us against 7.1 and the large ones 122).
+// 4 prompts of 2048 rows, 16 heads of 128 + 64 and 128 values: 107 us, 800 TFLOP/s (132 us before a step's halves took turns
+// and tiles of a head shared an XCD, 117 with a step's loads before its products); one of 16384 rows 1000 TFLOP/s. The
+// matrix unit is busy for 50% of the cycles and the vector unit for 47%, at the clock of 1.7 GHz that the card then keeps; LDS
+// for a quarter. Small grids are bound by a wave's steps in turn, some 1.4 us each (5 sequences of up to 900 rows, 5 heads of
+// 64 + 32 and 64 values: 25 us; one prompt of 2048 rows and 8 heads 46 us).
 #include "latent.h"
 
 namespace {
