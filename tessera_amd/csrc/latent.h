@@ -17,10 +17,11 @@ TS_DEV uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(ts_lds
 // 16 bytes a lane from `buf` (byte offset `at`, a lane's) straight to LDS: the lane lands at `lds` + 16 lane. Written out,
 // because with the builtin's load on its way the compiler waits for all loads before a transposing read of LDS, whatever
 // it reads. Nothing but LDS (and m0, which nothing else of these kernels uses) is written, and only the caller's own
-// waits (vmcnt) tell when: a barrier after them, before any read.
+// waits (vmcnt) tell when: a barrier after them, before any read. (Five wait states between a vector instruction that writes
+// a scalar register and a load that reads it are the program's to keep, and the compiler does not look into the text.)
 TS_DEV void rows_to_lds16(u32x4 buf, uint32_t lds, uint32_t at) {
 #ifdef __HIP_DEVICE_COMPILE__
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(lds), "v"(at), "s"(buf)
                  : "memory");
 #endif
