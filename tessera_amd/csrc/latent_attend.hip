@@ -17,9 +17,11 @@
 //    512 .. 8192 keys, 64 columns: 70 against 78).
 //
 // 32 sequences of 16 heads, 32000 keys each: 5.3 TB/s, what a copy reaches. 8 prompts' chunks of 512 rows behind 8000 keys,
-// 16 heads: 1050 TFLOP/s; there the LDS reads bound it (a wave's 16 columns read a step's whole rows, 68 KB, for 68 products of
-// 16x16x32; 32 columns a wave do not fit the registers). Short calls are bound by a group's start (positions, pages, q and the
-// first keys come one after the other, 7 us) and by the join (5 us, 13 for 128 columns a group).
+// 16 heads: 1000 to 1050 TFLOP/s. A round of 32 keys and 128 columns takes some 4700 cycles: its loads 600 (the vector cache
+// takes 64 bytes a cycle), scores 1300, softmax 350, values 1300, the barrier 500 and more; the matrix unit is busy for 46% of
+// the cycles, LDS for 48% (a wave's 16 columns read a step's whole rows, 68 KB; 32 columns a wave do not fit the registers), at
+// a clock of 1.9 GHz. Short calls are bound by a group's start (positions, pages, q and the first keys come one after the
+// other, 7 us) and by the join (5 us, 22 for the chunks' 128 columns).
 #include <algorithm>
 
 #include "kept8_attend.h"
