@@ -6,7 +6,7 @@
 // operands taken from memory as they lie (32 rows, 32 bytes of each) were bound by the vector cache's tags.
 // 1024 rows of 32 heads, 512 -> 128 to f32: 13.5 us, 4.0 TB/s (from memory to registers 27.5 us); 32 rows of 128 heads,
 // 128 -> 512: 5.5 us, 4.0 TB/s (7.6 us); 8192 rows of 16 heads, 512 -> 128: 34 us, 6.0 TB/s. What is left is the start
-// of each group, before its first chunk has come, and its end; f32 rows are bound by vector work (25 us, 3.5 TB/s).
+// of each group, before its first chunk has come, and its end; f32 rows are bound by three products for one and the vector work before them (24 us, 3.7 TB/s).
 #include "common.h"
 
 #include <algorithm>
@@ -61,7 +61,7 @@ struct Tile {
     static constexpr uint32_t kXRow = kChunk * (XBF16 ? 2 : 4), kWRow = kChunk * 2;
     static constexpr uint32_t kX = kRows * kXRow, kStage = kX + kCols * kWRow;
     static constexpr uint32_t kXLoads = kX / 1024 / kWaves, kWLoads = kCols * kWRow / 1024 / kWaves;  // a wave's
-    static constexpr uint32_t kStages = MT * MN == 4 && XBF16 ? 2 : 3;  // chunks in LDS: two of the largest leave a CU two groups
+    static constexpr uint32_t kStages = NW == 2 && MN == 2 ? 2 : 3;  // chunks in LDS: two of the largest leave a CU two groups
     static constexpr uint32_t kOutRow = kCols * 4 + 16, kOut = kRows * kOutRow;
     static_assert(kX % (1024 * kWaves) == 0 && kCols * kWRow % (1024 * kWaves) == 0, "equal loads for all waves");
 };
@@ -259,13 +259,13 @@ extern "C" int tessera_hip_linear_heads(const ts_heads_args *a, void *stream) {
             return bf16 ? launch<true, 2, 1, 1, 1>(p, a->heads, stream) : launch<false, 2, 1, 1, 1>(p, a->heads, stream);
         return bf16 ? launch<true, 4, 1, 1, 1>(p, a->heads, stream) : launch<false, 4, 1, 1, 1>(p, a->heads, stream);
     }
-    // 64 columns have a tile of their own (1000 rows of 16 heads, 256 -> 64: 5.3 us against 6.2). A wave of f32 rows has all
-    // of the group's columns: taking them apart is vector work, which waves along the columns would repeat (1024 rows of
-    // 32 heads, 512 -> 128: 25 us against 40).
+    // 64 columns have a tile of their own (1000 rows of 16 heads, 256 -> 64: 5.3 us against 6.2).
     if (a->n <= 64) return bf16 ? launch<true, 2, 2, 1, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 2>(p, a->heads, stream);
     // Many rows of bf16: 128 a tile, 64 x 64 a wave, two chunks in LDS (8192 rows of 16 heads, 512 -> 128: 34 us against 39 with 64
     // rows; 32000 rows, 640 -> 640: 46 against 53; but of one chunk, 2000 rows of 16 heads, 8 -> 640: 19 against 17).
     if (bf16 && a->k > kChunk && (uint64_t)a->heads * ((a->n - 1) / 128 + 1) * ((a->rows - 1) / 128 + 1) >= 1024)
         return launch<true, 2, 2, 2, 2>(p, a->heads, stream);
-    return bf16 ? launch<true, 4, 1, 2, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 4>(p, a->heads, stream);
+    // f32 rows are taken apart by each wave that reads them, and are twice the bytes in LDS: two waves along the columns and
+    // two chunks (1024 rows of 32 heads, 512 -> 128: 23.6 us; one wave along them and a group a CU 24.8, four 29.5).
+    return bf16 ? launch<true, 4, 1, 2, 1>(p, a->heads, stream) : launch<false, 2, 2, 1, 2>(p, a->heads, stream);
 }
