@@ -737,6 +737,8 @@ def linear_heads(x, w, *, out=None, out_dtype=torch.float32):
     w_head = w.stride(0) if heads > 1 else 0
     if out is None:
         out = x.new_empty(rows, heads, n, dtype=out_dtype)
+    elif rows and out.data_ptr() == x.data_ptr():
+        raise ValueError("linear_heads: out lies where x does")
     o_row, o_head = _rows_of(what, "out", out, on, out.dtype, heads)
     if on < 0 or dtype not in _ROWS or out.dtype not in _ROWS or out.shape != (rows, heads, n):
         raise ValueError(f"linear_heads: x and out [rows, heads, *] must be f32 or bf16 on a GPU, out {[rows, heads, n]}")
@@ -765,6 +767,8 @@ def attend_latent(q, kept, slots, positions, *, keys, rank, scale, table=None, k
         out = q.new_empty(rows, heads, rank)
     elif out.shape != (rows, heads, rank):
         raise ValueError(f"attend_latent: out must be {[rows, heads, rank]}")
+    elif rows and out.data_ptr() == q.data_ptr():
+        raise ValueError("attend_latent: out lies where q does")
     bf16 = torch.bfloat16
     if not (on >= 0 and kept.get_device() == slots.get_device() == positions.get_device() == out.get_device() == on
             and q.dtype is bf16 and kept.dtype is bf16 and out.dtype is bf16 and slots.dtype in _INTS
@@ -817,6 +821,8 @@ def flash_latent(q, k, v, r, *, scale, first=None, key_first=None, back=abi.U32_
         out = q.new_empty(rows, heads, value)
     elif out.shape != (rows, heads, value):
         raise ValueError(f"flash_latent: out must be {[rows, heads, value]}")
+    elif rows and out.data_ptr() == q.data_ptr():
+        raise ValueError("flash_latent: out lies where q does")
     if first is None and key_first is not None:
         raise ValueError("flash_latent: key_first without first")
     seqs = 1 if first is None else first.numel() - 1

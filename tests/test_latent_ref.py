@@ -242,3 +242,12 @@ def test_python_refuses_before_any_launch():
         rules.flash_latent(t(3, 4, 192), t(5, 4, 128), t(5, 4, 128), t(5, 64), scale=1.0, key_first=t(2, d=torch.int32))
     with pytest.raises(ValueError, match="not on a GPU"):
         rules.flash_latent(t(3, 4, 192), t(5, 4, 128), t(5, 4, 128), t(5, 64), scale=1.0)
+    x = t(3, 4, 64)
+    with pytest.raises(ValueError, match="out lies where x"):
+        rules.linear_heads(x, t(4, 64, 64), out=x)
+    x = t(3, 4, 576)
+    with pytest.raises(ValueError, match="out lies where q"):
+        rules.attend_latent(x, t(64, 576), i, i, keys=64, rank=512, scale=1.0, out=x.flatten()[:3 * 4 * 512].view(3, 4, 512))
+    x = t(3, 4, 192)
+    with pytest.raises(ValueError, match="out lies where q"):
+        rules.flash_latent(x, t(5, 4, 128), t(5, 4, 128), t(5, 64), scale=1.0, out=x.flatten()[:3 * 4 * 128].view(3, 4, 128))
