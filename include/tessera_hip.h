@@ -475,7 +475,7 @@ size_t tessera_hip_attend_latent_workspace(const ts_latent_args *a);
  *    a sequence whose bounds do not ascend or pass `rows` or `key_rows`, are left as they were.
  *  - Infinities and NaN reach the rows that see them alone. */
 typedef struct {
-    const void *q;             /* [rows, heads, nope + rope] bf16: rows q_stride apart, a row's heads back to back */
+    const void *q;             /* [rows, heads, nope + rope] bf16: rows q_stride apart (0: one row, for all), a row's heads back to back */
     const void *k, *v;         /* [key_rows, heads, nope], [key_rows, heads, value] bf16: rows *_stride, heads *_head apart */
     const void *r;             /* [key_rows, rope] bf16, r_stride apart */
     void *out;                 /* [rows, heads, value] bf16 */

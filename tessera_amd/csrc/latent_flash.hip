@@ -507,7 +507,7 @@ extern "C" int tessera_hip_flash_latent(const ts_flash_latent_args *a, void *str
     TS_REQUIRE(a->rows <= 1u << 28 && a->key_rows <= 1u << 28, "flash_latent: %u rows, %u keys", a->rows, a->key_rows);
     TS_REQUIRE(a->seqs <= 1u << 20 && (a->first || a->seqs <= 1), "flash_latent: %u sequences without their bounds", a->seqs);
     TS_REQUIRE(a->first || !a->key_first, "flash_latent: bounds of the keys without those of the rows");
-    TS_REQUIRE(a->q_stride >= a->heads * (a->nope + a->rope) && a->q_stride % 8 == 0,
+    TS_REQUIRE((a->q_stride == 0 || a->q_stride >= a->heads * (a->nope + a->rope)) && a->q_stride % 8 == 0,
                "flash_latent: q rows %u apart must hold %u heads and be whole 16-byte pieces", a->q_stride, a->heads);
     TS_REQUIRE(a->k_stride % 8 == 0 && a->k_head % 8 == 0 && a->v_stride % 8 == 0 && a->v_head % 8 == 0 && a->r_stride % 8 == 0,
                "flash_latent: rows and heads of k, v and r must be whole 16-byte pieces apart");

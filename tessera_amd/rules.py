@@ -835,7 +835,7 @@ def flash_latent(q, k, v, r, *, scale, first=None, key_first=None, back=abi.U32_
         _checked(what, on, ("out", out, _BF16, -1), ("first", first, _INTS, -1), ("key_first", key_first, _INTS, seqs + 1))
     a = abi.FlashLatentArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.data_ptr(), out.data_ptr(),
                             None if first is None else first.data_ptr(), None if key_first is None else key_first.data_ptr(),
-                            rows, key_rows, seqs, heads, nope, rope, value, q_row or heads * width, k_row, k_head, v_row,
+                            rows, key_rows, seqs, heads, nope, rope, value, q_row, k_row, k_head, v_row,
                             v_head, r_row, back, scale)
     _call_on(on, abi.load().tessera_hip_flash_latent, a)
     return out
