@@ -410,7 +410,8 @@ typedef struct {
     const float *gain;             /* [rank] or NULL */
     const float *rope_table;       /* [rope_rows][rope / 2][2] (cos, sin), or NULL */
     void *q_out;                   /* [rows, heads, rope]: rows q_out_stride, heads q_out_head apart; may be q
-                                      where both are laid out alike and of one type */
+                                      where both are laid out alike and of one type. No two pieces meet: a row's
+                                      heads before the next row, or a head's rows before the next head */
     void *kept;
     void *c_out, *r_out;           /* bf16 [rows, rank], [rows, rope], either or both NULL */
     const uint32_t *slots, *positions; /* [rows] */
@@ -436,7 +437,8 @@ int tessera_hip_append_latent(const ts_append_latent_args *a, void *stream);
 typedef struct {
     const void *x;      /* [rows, heads, k]: rows x_stride, heads x_head elements apart, whole 16-byte pieces */
     const void *w;      /* [heads, n, k] bf16: heads w_head apart (a multiple of 8), a head's rows back to back */
-    void *out;          /* [rows, heads, n]: rows out_stride, heads out_head elements apart */
+    void *out;          /* [rows, heads, n]: rows out_stride, heads out_head elements apart, no two of a head's n meeting
+                           (a row's heads before the next row, or a head's rows before the next head) */
     uint32_t rows, heads, n;
     uint32_t k;         /* a multiple of 8 */
     uint32_t x_stride, x_head, out_stride, out_head;

@@ -37,6 +37,14 @@ int hip_status(hipError_t e, const char *what);
 
 inline bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
+// Whether the pieces of `width` values at r * row + h * head lie beside one another: heads within rows, or rows within heads.
+inline bool beside(uint64_t rows, uint64_t row, uint64_t heads, uint64_t head, uint64_t width) {
+    auto within = [&](uint64_t n, uint64_t step, uint64_t outer, uint64_t outer_step) {
+        return (n <= 1 || step >= width) && (outer <= 1 || outer_step >= (n > 1 ? (n - 1) * step : 0) + width);
+    };
+    return within(heads, head, rows, row) || within(rows, row, heads, head);
+}
+
 // A product's stage chain (ts_linear_args.after), checked (map.hip): an empty chain
 // when after is NULL; refused with TS_AFTER_ADD or TS_AFTER_ARGMAX, or with operands
 // that repeat.

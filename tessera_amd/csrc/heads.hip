@@ -237,7 +237,7 @@ extern "C" int tessera_hip_linear_heads(const ts_heads_args *a, void *stream) {
                "linear_heads: x's rows and heads and w's heads must be whole 16-byte pieces apart");
     TS_REQUIRE(a->heads == 1 || a->w_head >= (uint64_t)a->n * a->k, "linear_heads: heads of w %llu apart",
                (unsigned long long)a->w_head);
-    TS_REQUIRE((a->heads == 1 || a->out_head >= a->n) && (a->rows <= 1 || a->out_stride >= a->n),
+    TS_REQUIRE(ts::beside(a->rows, a->out_stride, a->heads, a->out_head, a->n),
                "linear_heads: out's rows %u and heads %u apart meet", a->out_stride, a->out_head);
     TS_REQUIRE(ts::aligned(a->x, 16) && ts::aligned(a->w, 16), "linear_heads: x and w must be 16-byte aligned");
     const uint32_t size = a->out_dtype == TS_F32 ? 4 : 2;

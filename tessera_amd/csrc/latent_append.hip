@@ -212,6 +212,8 @@ extern "C" int tessera_hip_append_latent(const ts_append_latent_args *a, void *s
                        a->q_out_head % out_unit == 0,
                    "append_latent: q's rows and heads must be whole 16-byte pieces apart");
         TS_REQUIRE(a->q_out_head >= a->rope || a->heads == 1, "append_latent: q out's heads %u apart", a->q_out_head);
+        TS_REQUIRE(ts::beside(a->rows, a->q_out_stride, a->heads, a->q_out_head, a->rope),
+                   "append_latent: q out's rows %u and heads %u apart meet", a->q_out_stride, a->q_out_head);
         TS_REQUIRE(ts::aligned(a->q, 16) && ts::aligned(a->q_out, 16), "append_latent: q must be 16-byte aligned");
         TS_REQUIRE(a->q_out != a->q || (a->q_out_dtype == a->x_dtype && a->q_stride == a->q_out_stride &&
                                         a->q_head == a->q_out_head),

@@ -22,3 +22,20 @@ def test_flash_of_broadcast_rows(widths):
     check_flash(got, *many, first=[0, 150], key_first=[0, 170], scale=0.1)
     one = rules.flash_latent(q, *many[1:], scale=0.1)  # (a row by itself has no distance either)
     assert torch.equal(one, got[149:])
+
+
+def test_append_with_heads_outside_rows():
+    """q_out [heads, rows, rope] seen as [rows, heads, rope]; rows that lie on one another are refused."""
+    r = rng(22)
+    n, rank, rope, heads = 11, 256, 32, 5
+    c, q = dev(r.standard_normal((n, rank + rope)), F32), dev(r.standard_normal((n, heads, rope)), F32)
+    angles, i = rules.rope_table(64, 1e4, width=rope), torch.arange(n, dtype=torch.int32, device="cuda")
+    kept = torch.zeros(64, rank + rope, dtype=BF16, device="cuda")
+    kw = dict(keys=64, rank=rank, angles=angles, q=q)
+    want = rules.append_latent(c, kept, i * 0, i, **kw)
+    out = torch.zeros(heads, n, rope, device="cuda").transpose(0, 1)
+    assert torch.equal(rules.append_latent(c, kept, i * 0, i, q_out=out, **kw), want)
+    for bad in (torch.zeros(1, heads, rope, device="cuda").expand(n, -1, -1),
+                torch.zeros(n * heads * rope, device="cuda").as_strided((n, heads, rope), (rope, rope, 1))):
+        with pytest.raises(abi.HipError, match="meet"):
+            rules.append_latent(c, kept, i * 0, i, q_out=bad, **kw)
