@@ -629,7 +629,10 @@ __global__ __launch_bounds__((64 * Shape<RANK, ROPE, WC>::kWaves), 2) void atten
                     const uint32_t row = g / S::kPieces, key = here + row;
                     if (key < lo || key > hi || gone >> (row / kBlock) & 1) *(u32x4 *)(at + g * 16) = u32x4{0, 0, 0, 0};
                 }
-                if (gone && p.status && lane == 0) atomicOr(p.status, TS_STATUS_PAGE);
+                // (Rows that stand apart may leave keys of the pass that none of them sees.)
+                if (gone && p.status && act && ((gone & 1 && here <= pos && here + (kBlock - 1) >= from) ||
+                                                (gone & 2 && here + kBlock <= pos && here + (kKeys - 1) >= from)))
+                    atomicOr(p.status, TS_STATUS_PAGE);
             };
 
             if (WC == 1) {

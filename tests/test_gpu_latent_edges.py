@@ -39,3 +39,39 @@ def test_append_with_heads_outside_rows():
                 torch.zeros(n * heads * rope, device="cuda").as_strided((n, heads, rope), (rope, rope, 1))):
         with pytest.raises(abi.HipError, match="meet"):
             rules.append_latent(c, kept, i * 0, i, q_out=bad, **kw)
+
+
+# Rows of one slot far apart, whose windows leave keys between them that no row sees: (heads, run, rows), which
+# take 16, 32, 64 and 128 columns a group with `back` 700 and 8192 positions a slot.
+APART = [(2, 16, 16), (2, 5, 80), (2, 5, 500), (8, 5, 500), (40, 3, 300), (40, 64, 512)]
+
+
+def two_windows(r, rows, width, page=16, back=700, keys=8192):
+    """Positions near 800 and near 6000 in turn, and kept rows whose table holds the pages of their windows alone."""
+    positions = np.where(np.arange(rows) % 2 == 0, 800, 6000) + np.arange(rows) // 2 % 40
+    seen = np.zeros(keys // page, bool)
+    for p in set(positions):
+        seen[(p - back) // page:p // page + 1] = True
+    held = np.flatnonzero(seen)
+    table = np.full(len(seen), 2 ** 31 - 1, np.int32)
+    table[held] = r.permutation(len(held))
+    kept = dev(r.standard_normal((len(held) * page, width)), BF16)
+    return positions, kept, dict(keys=keys, table=table, kept_pages=len(seen), page=page)
+
+
+@pytest.mark.parametrize("widths", ["wide", "narrow"])
+@pytest.mark.parametrize("heads,run,rows", APART)
+def test_pages_between_windows_need_not_be_held(widths, heads, run, rows):
+    """A page that no row sees is no row's refusal, wherever the rows that share its loads stand."""
+    rank, rope, nope, _ = WIDTHS[widths]
+    r = rng(rows + heads)
+    positions, kept, where = two_windows(r, rows, rank + rope)
+    q = dev(r.standard_normal((rows, heads, rank + rope)), BF16)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kw = dict(rank=rank, scale=(nope + rope) ** -0.5, back=700)
+    got = attend(q, kept, np.zeros(rows, int), positions, where, run=run, max_position=8191, status=status, **kw)
+    few = np.unique(np.concatenate([np.arange(6), r.integers(0, rows, 20)]))
+    check_attend(got[dev(few)], q[dev(few)], kept, np.zeros(len(few), int), positions[few], where, **kw)
+    assert int(status) == 0
+    finite = bool(torch.isfinite(got).all())
+    assert finite
