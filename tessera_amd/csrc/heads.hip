@@ -71,6 +71,7 @@ __global__ __launch_bounds__(64 * NW * RW, 2) void linear_heads_kernel(HeadsPara
     using T = Tile<XBF16, NW, RW, MT, MN>;
     constexpr uint32_t kWaves = T::kWaves;
     extern __shared__ __attribute__((aligned(16))) char stage[];
+    __shared__ uint32_t odd_met[XBF16 ? 1 : kWaves];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t col = lane & 31, half = lane >> 5;
     // Groups go to the eight XCDs in turn: those of a head, which read the same x or w, belong to one.
@@ -165,6 +166,16 @@ __global__ __launch_bounds__(64 * NW * RW, 2) void linear_heads_kernel(HeadsPara
     }
     // Sums change places in LDS, so that a store has whole rows' columns: register 4 q + i of a lane is column
     // 8 q + 4 half + i of row `col`.
+    if (!XBF16) {
+        float odd = 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+        for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+            for (uint32_t j = 0; j < MN; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) odd = fmaf(acc[m][j][i], 0.0f, odd);
+        odd_met[wave] = __builtin_amdgcn_ballot_w64(odd != odd) != 0;
+    }
     lds_barrier();
 #pragma unroll
     for (uint32_t m = 0; m < MT; m++)
@@ -199,6 +210,31 @@ __global__ __launch_bounds__(64 * NW * RW, 2) void linear_heads_kernel(HeadsPara
             else
                 ((float *)p.out)[at] = v;
         }
+    }
+    if (XBF16) return;
+    // A sum of parts may be NaN only because one of them is 0 and its weight infinite: those are summed anew, of whole values.
+    uint32_t any = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; i++) any |= __builtin_amdgcn_readfirstlane(odd_met[i]);
+    if (!any) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores of the same places
+    lds_barrier();
+#pragma unroll 1
+    for (uint32_t e = threadIdx.x; e < T::kRows * T::kCols; e += T::kThreads) {
+        const uint32_t row = e / T::kCols, n = e % T::kCols;
+        if (r0 + row >= p.rows || n0 + n >= p.n) continue;
+        float v = *(const float *)(stage + row * T::kOutRow + n * 4);
+        if (v == v) continue;
+        const float *a = (const float *)p.x + (uint64_t)(r0 + row) * p.x_stride + (uint64_t)h * p.x_head;
+        const uint16_t *b = p.w + h * p.w_head + (uint64_t)(n0 + n) * p.k;
+        v = 0.0f;
+#pragma unroll 1
+        for (uint32_t k = 0; k < p.k && v == v; k++) v = fmaf(a[k], lo_bf16(b[k]), v);
+        const uint64_t at = out + (uint64_t)(r0 + row) * p.out_stride + n;
+        if (p.out_bf16)
+            ((uint16_t *)p.out)[at] = bf16_bits(v);
+        else
+            ((float *)p.out)[at] = v;
     }
 }
 

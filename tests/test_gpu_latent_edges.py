@@ -75,3 +75,25 @@ def test_pages_between_windows_need_not_be_held(widths, heads, run, rows):
     assert int(status) == 0
     finite = bool(torch.isfinite(got).all())
     assert finite
+
+
+@pytest.mark.parametrize("rows,heads,n,k", [(5, 3, 130, 72), (40, 40, 200, 136), (100, 3, 40, 72), (100, 2, 130, 200)])
+@pytest.mark.parametrize("x", [F32, BF16])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_linear_heads_of_weights_that_are_not_finite(rows, heads, n, k, x, out):
+    """An infinite weight makes its outputs infinite, but where x is 0 or the signs of two of them differ; NaN makes them NaN."""
+    r = rng(rows + n)
+    xs, w = r.standard_normal((rows, heads, k)), dev(r.standard_normal((heads, n, k)), BF16)
+    xs[:, :, 9] = np.where(np.arange(rows)[:, None] % 2 == 0, 1.5, -2.0)  # (8 bits: the lower parts of an f32 are 0)
+    xs[3, :, 9] = 0.0
+    xs = dev(xs, x)
+    want = f64(rules.linear_heads(xs, w, out_dtype=out))
+    w[:, 1, 9], w[0, 3, 9], w[1, n - 1, 70], w[0, 5, 1] = float("inf"), -float("inf"), float("inf"), float("nan")
+    w[1, 7, 8], w[1, 7, 9] = float("inf"), -float("inf")
+    a, b = f64(xs), f64(w)
+    with np.errstate(invalid="ignore"):
+        bad = np.einsum("rhk,hnk->rhn", a, b)
+    got = f64(rules.linear_heads(xs, w, out_dtype=out))
+    odd = ~np.isfinite(bad)
+    assert np.array_equal(got[odd], bad[odd], equal_nan=True) and np.array_equal(got[~odd], want[~odd])
+    assert np.isinf(bad).sum() > rows and np.isnan(bad[3, 0, 1]) and np.isnan(bad[:, 0, 5]).all()
