@@ -147,7 +147,21 @@ __global__ __launch_bounds__(64 * kWaves) void append_latent_kernel(LatentRows p
         for (uint32_t i = 0; i < kPasses; i++)
 #pragma unroll
             for (int k = 0; k < 8; k++) sum = fmaf(v[i][k], v[i][k], sum);
-        const float by = 1.0f / sqrtf(wave_sum(sum) / (float)p.rank + p.eps);
+        sum = wave_sum(sum);
+        float by = 1.0f / sqrtf(sum / (float)p.rank + p.eps);
+        if (sum == INFINITY) {
+            // Squares past f32's range: those of the values by 2^-72 hold, and half of it goes to the values (a root of 2^59 or
+            // more takes what that makes subnormal to 0). A value that is infinite still makes the others 0 and itself NaN.
+            sum = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < kPasses; i++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    v[i][k] *= 0x1p-36f;
+                    sum = fmaf(v[i][k] * 0x1p-36f, v[i][k] * 0x1p-36f, sum);
+                }
+            by = 0x1p-36f / sqrtf(wave_sum(sum) / (float)p.rank + p.eps * 0x1p-72f * 0x1p-72f);
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kPasses; i++) {
             const uint32_t d = 512 * i + 8 * lane;

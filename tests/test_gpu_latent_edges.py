@@ -97,3 +97,28 @@ def test_linear_heads_of_weights_that_are_not_finite(rows, heads, n, k, x, out):
     odd = ~np.isfinite(bad)
     assert np.array_equal(got[odd], bad[odd], equal_nan=True) and np.array_equal(got[~odd], want[~odd])
     assert np.isinf(bad).sum() > rows and np.isnan(bad[3, 0, 1]) and np.isnan(bad[:, 0, 5]).all()
+
+
+@pytest.mark.parametrize("x", [F32, BF16])
+@pytest.mark.parametrize("rank", [512, 1024, 8])
+def test_append_of_rows_past_the_range_of_their_squares(x, rank):
+    """A finite row is normed whatever its size: squares of values from 2^64 on (or their sum) pass f32's range."""
+    r = rng(rank)
+    rope, n = 32, 6
+    c = r.standard_normal((n, rank + rope))
+    c[1] *= 2.0 ** 66
+    c[2] *= 2.0 ** 122
+    c[3, :rank] = 2.0 ** 63 * np.sign(c[3, :rank])  # (each square holds, their sum does not)
+    c[4, :rank] = 0
+    c[4, 5] = -3e38
+    c[5, 3] = np.inf
+    c = dev(c, x)
+    gain = dev(1 + 0.1 * r.standard_normal(rank), F32)
+    kept = torch.zeros(16, rank + rope, dtype=BF16, device="cuda")
+    i = torch.arange(n, dtype=torch.int32, device="cuda")
+    rules.append_latent(c, kept, i * 0, i, keys=16, rank=rank, gain=gain, eps=1e-5)
+    want = L.normed(f64(c)[:5, :rank], f64(gain), 1e-5)
+    # As check_append's: (rank + 8) steps of f32 and the rounding to bf16.
+    assert np.all(np.abs(f64(kept)[:5, :rank] - want) <= np.abs(want) * ((rank + 8) * 2.0 ** -24 + HALF))
+    got = f64(kept)[5, :rank]
+    assert np.isnan(got[3]) and not np.delete(got, 3).any()
