@@ -390,7 +390,7 @@ size_t tessera_hip_attend_kept8_workspace(const ts_kept8_args *a);
  * keys and values of the latents, for prompts.
  * The reference describes such a model (engine/models) but has no kernel for it; it composes the
  * expanded form of separate stages. No output of these calls overlaps an input (append's q_out may be
- * its q).
+ * its q, laid out alike) or another output; parts of the same wider rows may be one's input and output.
  * ------------------------------------------------------------------------- */
 
 /* New rows into the kept rows: c's first `rank` values through RmsNorm (gain, or not where it is

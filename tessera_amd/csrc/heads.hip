@@ -7,9 +7,10 @@
 // 1024 rows of 32 heads, 512 -> 128 to f32: 13.5 us, 4.0 TB/s (from memory to registers 27.5 us); 32 rows of 128 heads,
 // 128 -> 512: 5.5 us, 4.0 TB/s (7.6 us); 8192 rows of 16 heads, 512 -> 128: 34 us, 6.0 TB/s. What is left is the start
 // of each group, before its first chunk has come, and its end; f32 rows are bound by three products for one and the vector work before them (24 us, 3.7 TB/s).
-#include "common.h"
-
 #include <algorithm>
+
+#include "common.h"
+#include "places.h"
 
 namespace {
 
@@ -238,15 +239,25 @@ __global__ __launch_bounds__(64 * NW * RW, 2) void linear_heads_kernel(HeadsPara
     }
 }
 
+int out_apart(const ts_heads_args *a) {
+    const uint64_t x = a->x_dtype == TS_F32 ? 4 : 2, out = a->out_dtype == TS_F32 ? 4 : 2;
+    return ts::outputs_apart("linear_heads",
+                             {{"out", a->out, a->n * out, a->rows, a->out_stride * out, a->heads, a->out_head * out}},
+                             {{"x", a->x, a->k * x, a->rows, a->x_stride * x, a->heads, a->x_head * x},
+                              {"w", a->w, 2ull * a->n * a->k, a->heads, 2ull * a->w_head}});
+}
+
 template <bool XBF16, uint32_t NW, uint32_t RW, uint32_t MT, uint32_t MN>
-int launch(HeadsParams &p, uint32_t heads, void *stream) {
+int launch(HeadsParams &p, const ts_heads_args *a, void *stream) {
     using T = Tile<XBF16, NW, RW, MT, MN>;
     const auto kernel = linear_heads_kernel<XBF16, NW, RW, MT, MN>;
     constexpr uint32_t kMost = std::max(T::kStages * T::kStage, T::kOut);
     p.row_tiles = (p.rows - 1) / T::kRows + 1;
     p.col_tiles = (p.n - 1) / T::kCols + 1;
-    const uint64_t all = (uint64_t)p.row_tiles * p.col_tiles * heads;
+    const uint64_t all = (uint64_t)p.row_tiles * p.col_tiles * a->heads;
     TS_REQUIRE(all < (1ull << 32) / T::kThreads - 8, "linear_heads: %u rows in one launch", p.rows);
+    const int rc = out_apart(a);
+    if (rc) return rc;
     p.groups = (uint32_t)all;
     static const hipError_t attr =
         hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
@@ -292,16 +303,16 @@ extern "C" int tessera_hip_linear_heads(const ts_heads_args *a, void *stream) {
     // 128 would leave CUs without a group (1 row, 16 heads, 128 -> 512: 3.9 us against 4.6).
     if (a->rows <= 64) {
         if ((uint64_t)a->heads * ((a->n - 1) / 128 + 1) * ((a->rows - 1) / 32 + 1) < 256)
-            return bf16 ? launch<true, 2, 1, 1, 1>(p, a->heads, stream) : launch<false, 2, 1, 1, 1>(p, a->heads, stream);
-        return bf16 ? launch<true, 4, 1, 1, 1>(p, a->heads, stream) : launch<false, 4, 1, 1, 1>(p, a->heads, stream);
+            return bf16 ? launch<true, 2, 1, 1, 1>(p, a, stream) : launch<false, 2, 1, 1, 1>(p, a, stream);
+        return bf16 ? launch<true, 4, 1, 1, 1>(p, a, stream) : launch<false, 4, 1, 1, 1>(p, a, stream);
     }
     // 64 columns have a tile of their own (1000 rows of 16 heads, 256 -> 64: 5.3 us against 6.2).
-    if (a->n <= 64) return bf16 ? launch<true, 2, 2, 1, 1>(p, a->heads, stream) : launch<false, 1, 4, 1, 2>(p, a->heads, stream);
+    if (a->n <= 64) return bf16 ? launch<true, 2, 2, 1, 1>(p, a, stream) : launch<false, 1, 4, 1, 2>(p, a, stream);
     // Many rows of bf16: 128 a tile, 64 x 64 a wave, two chunks in LDS (8192 rows of 16 heads, 512 -> 128: 34 us against 39 with 64
     // rows; 32000 rows, 640 -> 640: 46 against 53; but of one chunk, 2000 rows of 16 heads, 8 -> 640: 19 against 17).
     if (bf16 && a->k > kChunk && (uint64_t)a->heads * ((a->n - 1) / 128 + 1) * ((a->rows - 1) / 128 + 1) >= 1024)
-        return launch<true, 2, 2, 2, 2>(p, a->heads, stream);
+        return launch<true, 2, 2, 2, 2>(p, a, stream);
     // f32 rows are taken apart by each wave that reads them, and are twice the bytes in LDS: two waves along the columns and
     // two chunks (1024 rows of 32 heads, 512 -> 128: 23.6 us; one wave along them and a group a CU 24.8, four 29.5).
-    return bf16 ? launch<true, 4, 1, 2, 1>(p, a->heads, stream) : launch<false, 2, 2, 1, 2>(p, a->heads, stream);
+    return bf16 ? launch<true, 4, 1, 2, 1>(p, a, stream) : launch<false, 2, 2, 1, 2>(p, a, stream);
 }

@@ -10,6 +10,7 @@
 // 512 + 64 values with 16 heads' q parts in 16.6 us, 4.3 TB/s; few rows the chain of place, row, angles and store (one row
 // 2.5 us, 128 f32 rows with 128 heads 4.7 us, 1.4 TB/s).
 #include "kept8.h"
+#include "places.h"
 
 namespace {
 
@@ -250,6 +251,23 @@ extern "C" int tessera_hip_append_latent(const ts_append_latent_args *a, void *s
     p.c_groups = (a->rows - 1) / kWaves + 1;
     const uint64_t all = p.c_groups + ((uint64_t)a->rows * p.head_units + kWaves - 1) / kWaves;
     TS_REQUIRE(all < (1ull << 32) / (64 * kWaves), "append_latent: %u rows in one launch", a->rows);
+    const uint64_t size = a->x_dtype == TS_F32 ? 4 : 2, out = a->q_out_dtype == TS_F32 ? 4 : 2, width = a->rank + a->rope;
+    const uint64_t held = a->kept_table ? (uint64_t)a->pages * a->page : (uint64_t)a->slot_count * a->keys;
+    const uint32_t heads = q ? a->heads : 0;
+    rc = ts::outputs_apart(
+        "append_latent",
+        {{"q_out", a->q_out, a->rope * out, a->rows, a->q_out_stride * out, heads, a->q_out_head * out},
+         {"c_out", a->c_out, (uint64_t)a->rows * a->rank * 2},
+         {"r_out", a->r_out, (uint64_t)a->rows * a->rope * 2},
+         {"kept", a->kept, held * width * 2}},
+        {{"c", a->c, width * size, a->rows, a->c_stride * size},
+         {"q", a->q_out == a->q ? nullptr : a->q, a->rope * size, a->rows, a->q_stride * size, heads, a->q_head * size},
+         {"gain", a->gain, (uint64_t)a->rank * 4},
+         {"the angle table", a->rope_table, (uint64_t)a->rope_rows * a->rope * 4},
+         {"slots", a->slots, (uint64_t)a->rows * 4},
+         {"positions", a->positions, (uint64_t)a->rows * 4},
+         {"the page table", a->kept_table, (uint64_t)a->slot_count * a->kept_pages * 4}});
+    if (rc) return rc;
     const auto kernel = a->x_dtype == TS_BF16 ? a->halves ? append_latent_kernel<true, true> : append_latent_kernel<true, false>
                                               : a->halves ? append_latent_kernel<false, true> : append_latent_kernel<false, false>;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)all), dim3(64 * kWaves), 0, (hipStream_t)stream, p);

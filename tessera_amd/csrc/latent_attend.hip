@@ -26,6 +26,7 @@
 
 #include "kept8_attend.h"
 #include "latent.h"
+#include "places.h"
 
 namespace {
 
@@ -935,6 +936,15 @@ extern "C" int tessera_hip_attend_latent(const ts_latent_args *k, void *stream) 
     const size_t partials = partial_bytes(k, s), need = partials + share_bytes(s);
     if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
         return ts::fail(TS_ERR_WORKSPACE, "attend_latent: workspace of %zu bytes, 16-byte aligned, needed", need);
+    const uint64_t of = (uint64_t)a->rows * a->heads * 2, held = a->kept_table ? (uint64_t)k->pages * a->page : (uint64_t)k->slot_count * a->keys;
+    const int over = ts::outputs_apart("attend_latent", {{"out", a->out, of * k->rank}},
+                                       {{"q", a->q, of * a->width},
+                                        {"kept", a->k, held * a->width * 2},
+                                        {"slots", a->slots, (uint64_t)a->rows * 4},
+                                        {"positions", a->positions, (uint64_t)a->rows * 4},
+                                        {"the page table", a->kept_table, (uint64_t)k->slot_count * a->kept_pages * 4},
+                                        {"the workspace", a->workspace, need}});
+    if (over) return over;
     LatentParams p;
     p.q = (const uint16_t *)a->q; p.kept = (const uint16_t *)a->k; p.out = (uint16_t *)a->out;
     p.partials = need ? (float *)a->workspace : nullptr;

@@ -14,6 +14,7 @@
 // for a quarter. Small grids are bound by a wave's steps in turn, some 1.4 us each (5 sequences of up to 900 rows, 5 heads of
 // 64 + 32 and 64 values: 25 us; one prompt of 2048 rows and 8 heads 46 us).
 #include "latent.h"
+#include "places.h"
 
 namespace {
 
@@ -529,5 +530,14 @@ extern "C" int tessera_hip_flash_latent(const ts_flash_latent_args *a, void *str
     p.tiles = a->rows / kRows + (p.seqs < a->rows ? p.seqs : a->rows);
     const uint64_t groups = (uint64_t)p.tiles * a->heads;
     TS_REQUIRE(groups < (1ull << 32) / kThreads, "flash_latent: %u rows in one launch", a->rows);
+    const uint64_t bounds = a->first ? ((uint64_t)a->seqs + 1) * 4 : 0;
+    const int over = ts::outputs_apart("flash_latent", {{"out", a->out, (uint64_t)a->rows * a->heads * a->value * 2}},
+                                       {{"q", a->q, 2ull * a->heads * (a->nope + a->rope), a->rows, 2ull * a->q_stride},
+                                        {"k", a->k, 2ull * a->nope, a->key_rows, 2ull * a->k_stride, a->heads, 2ull * a->k_head},
+                                        {"v", a->v, 2ull * a->value, a->key_rows, 2ull * a->v_stride, a->heads, 2ull * a->v_head},
+                                        {"r", a->r, 2ull * a->rope, a->key_rows, 2ull * a->r_stride},
+                                        {"first", a->first, bounds},
+                                        {"key_first", a->key_first, bounds}});
+    if (over) return over;
     return wide ? launch<128, 64, 128>(p, (uint32_t)groups, stream) : launch<64, 32, 64>(p, (uint32_t)groups, stream);
 }
