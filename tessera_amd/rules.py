@@ -817,6 +817,8 @@ def flash_latent(q, k, v, r, *, scale, first=None, key_first=None, back=abi.U32_
     if r.shape != (key_rows, rope) or r.get_device() != on or r.dtype is not bf16 or (r.stride(1) != 1 and rope > 1):
         raise ValueError(f"flash_latent: r must be bf16 {[key_rows, rope]} on GPU {on}, a row's values back to back")
     r_row = r.stride(0) if key_rows > 1 else 0
+    if r_row >> 32:
+        raise ValueError("flash_latent: r rows more than 2^32 elements apart")
     if out is None:
         out = q.new_empty(rows, heads, value)
     elif out.shape != (rows, heads, value):

@@ -125,3 +125,12 @@ def test_parts_of_the_same_rows(x_stride, x_head, out_stride, out_head, first, t
     a.x_stride, a.x_head, a.out_stride, a.out_head = x_stride, x_head, out_stride, out_head
     code = getattr(abi.load(), fn)(C.byref(a), None)
     assert code not in (abi.TS_OK, abi.TS_ERR_ARG) if taken else code == abi.TS_ERR_ARG
+
+
+def test_flash_refuses_key_parts_too_far_apart(called):
+    """A distance that 32 bits do not hold is refused, not cut."""
+    q, kv = t(3, 4, 192), t(2, 4, 256)
+    r = torch.empty((1 << 32) + 64, dtype=BF16, device="meta").as_subclass(OnGpu).as_strided((2, 64), (1 << 32, 1))
+    with pytest.raises(ValueError, match="2\\^32 elements apart"):
+        rules.flash_latent(q, kv[..., :128], kv[..., 128:], r, scale=1.0)
+    assert not called
