@@ -122,3 +122,25 @@ def test_append_of_rows_past_the_range_of_their_squares(x, rank):
     assert np.all(np.abs(f64(kept)[:5, :rank] - want) <= np.abs(want) * ((rank + 8) * 2.0 ** -24 + HALF))
     got = f64(kept)[5, :rank]
     assert np.isnan(got[3]) and not np.delete(got, 3).any()
+
+
+# More than 64 rows and columns over several chunks of 64 k, whole and begun: two buffers of f32 x, three of bf16.
+@pytest.mark.parametrize("rows,heads,n,k", [(65, 3, 130, 72), (100, 2, 129, 136), (200, 4, 335, 328), (97, 32, 128, 512), (129, 2, 65, 128),
+                                            (190, 1, 200, 192), (70, 5, 257, 640), (128, 2, 128, 1000)])
+@pytest.mark.parametrize("x", [F32, BF16])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_linear_heads_of_many_chunks(rows, heads, n, k, x, out):
+    """The bound of the products a head: k / 16 accumulating steps and one more at 2^-21 each of the sum of |x w|, three
+    times as many of f32 x, whose parts drop 2^-24; then half a step of bf16."""
+    r = rng(rows + n + k)
+    gap = 8 if n % 2 else 0
+    xs = dev(r.standard_normal((rows, heads, k + 8)), x)[..., :k]
+    w = dev(r.standard_normal((heads, n, k)) / 8, BF16)
+    held = torch.full((rows, heads, n + gap), 7.0, dtype=out, device="cuda")
+    got = rules.linear_heads(xs, w, out=held[..., :n])
+    a, b = f64(xs), f64(w)
+    want, size = (np.matmul(p.transpose(1, 0, 2), q.transpose(0, 2, 1)).transpose(1, 0, 2) for p, q in ((a, b), (np.abs(a), np.abs(b))))
+    steps = (k / 16 + 1) * (3 if x == F32 else 1)
+    limit = size * (steps * 2.0 ** -21 + 2.0 ** -24) + (HALF * np.abs(want) if out == BF16 else 0)
+    assert np.all(np.abs(f64(got) - want) <= limit)
+    assert bool((held[..., n:] == 7.0).all())
