@@ -144,3 +144,54 @@ def test_linear_heads_of_many_chunks(rows, heads, n, k, x, out):
     limit = size * (steps * 2.0 ** -21 + 2.0 ** -24) + (HALF * np.abs(want) if out == BF16 else 0)
     assert np.all(np.abs(f64(got) - want) <= limit)
     assert bool((held[..., n:] == 7.0).all())
+
+
+# (heads, run, rows, positions a slot), which take 16, 32, 64 and 128 columns a group: keys of few tiles in whole parts and in
+# equal runs, tiles cut where the slot changes, several blocks of heads, groups that each have a tile alone.
+LOST = [(16, 1, 6, 1 << 13), (16, 1, 300, 1 << 13), (2, 16, 32, 1 << 13), (32, 1, 6, 1 << 17), (32, 1, 300, 1 << 13), (2, 3, 6, 1 << 17),
+        (8, 16, 640, 1 << 13), (64, 1, 300, 1 << 13), (150, 1, 6, 1 << 17), (8, 5, 10, 1 << 17), (5, 33, 500, 1 << 13), (16, 16, 640, 1 << 13),
+        (128, 1, 6, 1 << 17), (128, 1, 300, 1 << 13), (40, 3, 9, 1 << 17), (16, 33, 528, 1 << 13), (32, 33, 528, 1 << 13),
+        (1024, 1, 300, 1 << 13)]
+
+
+@pytest.mark.parametrize("widths", ["wide", "narrow"])
+@pytest.mark.parametrize("heads,run,rows,keys", LOST)
+@pytest.mark.parametrize("back", [None, 3000])
+def test_lost_pages(widths, heads, run, rows, keys, back):
+    """A page that is not held makes the rows that see its keys NaN, and sets the bit; the rows beside them, of shorter and of
+    other sequences over the same pages, keep their bits. Pages at the start, at the end, in either block of a step, behind
+    the blocks that are looked up at once (16 or 32 rounds)."""
+    rank, rope, nope, _ = WIDTHS[widths]
+    r = rng(rows + heads)
+    n, page = 5000, 16
+    held = -(-n // page)
+    table = np.full((3, keys // page), 2 ** 31 - 1, np.int32)
+    table[:, :held] = r.permutation(held)
+    where = dict(keys=keys, kept_pages=keys // page, page=page)
+    kept = dev(r.standard_normal((held * page, rank + rope)), BF16)
+    index = np.arange(rows) // run
+    starts = np.where(np.arange(index[-1] + 1) % 5 == 3, r.integers(0, 200, index[-1] + 1), r.integers(3800, n - run + 1, index[-1] + 1))
+    starts[0] = n - run
+    positions = starts[index] + np.arange(rows) % run
+    slots = np.where(index % 3 == 2, 1 + index % 2, 0)
+    q = dev(r.standard_normal((rows, heads, rank + rope)), BF16)
+    kw = dict(rank=rank, scale=(nope + rope) ** -0.5, **({} if back is None else {"back": back}))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    call = dict(kw, run=run, max_position=keys - 1, status=status)
+    want = attend(q, kept, slots, positions, dict(where, table=table.reshape(-1)), **call)
+    few = np.unique([0, rows - 1, rows // 2])
+    check_attend(want[dev(few)], q[dev(few)], kept, slots[few], positions[few], dict(where, table=table.reshape(-1)), **kw)
+    assert int(status) == 0
+    last = int(positions[slots == 0].max()) // page
+    for lost in ([0], [1], [150], [151], [255, 256, 257], [last - 1], [last]):
+        fewer = table.copy()
+        fewer[0, lost] = held
+        sees = np.zeros(rows, bool)
+        for b in lost:
+            sees |= (slots == 0) & (positions >= b * page) & (positions - (keys if back is None else back) <= b * page + page - 1)
+        status.zero_()
+        got = attend(q, kept, slots, positions, dict(where, table=fewer.reshape(-1)), **call)
+        assert bool(torch.isnan(got[dev(np.flatnonzero(sees))]).all()), lost
+        others = dev(np.flatnonzero(~sees))
+        same = torch.equal(got[others], want[others])
+        assert same and int(status) == (abi.TS_STATUS_PAGE if sees.any() else 0), lost
