@@ -195,3 +195,43 @@ def test_lost_pages(widths, heads, run, rows, keys, back):
         others = dev(np.flatnonzero(~sees))
         same = torch.equal(got[others], want[others])
         assert same and int(status) == (abi.TS_STATUS_PAGE if sees.any() else 0), lost
+
+
+def flash_forms(q, k, v, r, *, scale, first, key_first, back):
+    """latent_ref.flash on the GPU, in 64 bits, a head of a sequence at once."""
+    out, size = (torch.full((*q.shape[:2], v.shape[-1]), float("nan"), dtype=torch.float64, device="cuda") for _ in range(2))
+    spread = torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda")
+    for a, b, ka, kb in zip(first[:-1], first[1:], key_first[:-1], key_first[1:]):
+        pos = (kb - ka) - (b - a) + torch.arange(b - a, device="cuda")[:, None]
+        key = torch.arange(kb - ka, device="cuda")
+        sees = (key <= pos) & (key >= pos - back)
+        for h in range(q.shape[1]):
+            x, rows, vv = q[a:b, h].double(), torch.cat([k[ka:kb, h], r[ka:kb]], -1).double().T.contiguous(), v[ka:kb, h].double()
+            w = torch.softmax((x @ rows * scale).masked_fill(~sees, -float("inf")), -1).nan_to_num(0.0)
+            out[a:b, h], size[a:b, h] = w @ vv, w @ vv.abs()
+            spread[a:b, h] = ((x.abs() @ rows.abs()) * sees).amax(-1) * abs(scale)
+    return out.cpu().numpy(), size.cpu().numpy(), spread.cpu().numpy()
+
+
+@pytest.mark.parametrize("rows,more", [([8300], [0]), ([4100, 5300], [77, 0]), ([90, 9000, 40], [0, 300, 9]), ([600] * 15, [0] * 15),
+                                       ([2000, 7000], [-1000, 0])])
+@pytest.mark.parametrize("widths,heads", [("narrow", 1), ("narrow", 8), ("wide", 2)])
+@pytest.mark.parametrize("back", [None, 40])
+def test_flash_of_long_sequences(rows, more, widths, heads, back):
+    """More than the 64 tiles that are ordered at once, of a sequence or a few: every row is written, once and rightly."""
+    _, rope, nope, value = WIDTHS[widths]
+    keys = [a + b for a, b in zip(rows, more)]
+    first, key_first = np.concatenate([[0], np.cumsum(rows)]), np.concatenate([[0], np.cumsum(keys)])
+    g = torch.Generator(device="cuda").manual_seed(sum(rows))
+    new = lambda *s: torch.randn(s, generator=g, device="cuda").to(BF16)  # noqa: E731
+    behind = 50
+    q, k, v, r = new(first[-1] + behind, heads, nope + rope), new(key_first[-1], heads, nope), new(key_first[-1], heads, value), new(key_first[-1], rope)
+    out = torch.full((len(q), heads, value), 7.0, dtype=BF16, device="cuda")
+    kw = dict(scale=(nope + rope) ** -0.5, **({} if back is None else {"back": back}))
+    got = rules.flash_latent(q, k, v, r, first=ints(first), key_first=ints(key_first), out=out, **kw)
+    assert bool((got[first[-1]:] == 7.0).all())
+    want, size, spread = flash_forms(q, k, v, r, first=first, key_first=key_first, scale=kw["scale"], back=1 << 30 if back is None else back)
+    got, want, size, spread = f64(got)[:first[-1]], want[:first[-1]], size[:first[-1]], spread[:first[-1]]
+    # (latent_ref.bound's 2^-14 is of 128 steps of 64 keys; 2^-13 more for up to 256.)
+    limit = L.bound(want, size, spread, (nope + rope) / 16 + 1, HALF) + 2.0 ** -13 * size
+    assert np.all(np.abs(got - want) <= limit)
