@@ -10,11 +10,12 @@
 //    the end. With WC = 1 each wave streams keys of its own and waits for no other.
 //  * Keys are dealt to the groups, the tiles' one behind the other, so that groups end together however the sequences
 //    differ in length; a tile that several groups have is joined by a second kernel. Few tiles: each in equal parts of
-//    its own, a group one of them, which spares groups a second start (24 sequences of up to 5 rows, 32 heads, 1000 ..
-//    9001 keys: 84 us against 97).
-//  * A weight enters the product in two bf16 parts with 16 columns, which leave the matrix unit time for it, in one else
-//    (24 sequences of up to 5 rows, 32 heads, 1000 .. 9001 keys, 32 columns: 75 us against 82; 32 sequences of 128 heads,
-//    512 .. 8192 keys, 64 columns: 70 against 78).
+//    its own, a group one of them, which spares groups a second start (24 sequences of 3 to 5 rows, 32 heads, 1000 ..
+//    9001 keys: 73 us against 81; 32 sequences of 16 heads, 512 .. 8192 keys: 48 against 54).
+//  * A weight enters the product in two bf16 parts with 16 columns, which leave the matrix unit time for it, in one else. Two
+//    there would bring the error against 64 bits (2-norm) from 2.0e-3 to 1.66e-3, the output's own rounding, and take 48 us for
+//    46 with 32 columns (32 sequences of 32 heads, 4000 keys), 77 for 70 with 64 (32 sequences of 128 heads, 512 .. 8192 keys;
+//    24 x 5 drafts of 32 heads 70 for 65), 191 for 149 with 128 (two chunks of 512 rows, 16 heads, 2500 and 4600 keys).
 //
 // 32 sequences of 16 heads, 32000 keys each: 5.3 TB/s, what a copy reaches. 8 prompts' chunks of 512 rows behind 8000 keys,
 // 16 heads: 1000 to 1050 TFLOP/s. A round of 32 keys and 128 columns takes some 4700 cycles: its loads 600 (the vector cache
@@ -825,14 +826,21 @@ struct Plan {
 
 // How many columns a group has, and how the keys are divided. A group takes some time for its q, its partial sums and
 // their share of the join, and some for each key it reads; both grow with its columns, a key's less than they do. Of 16, 32,
-// 64 and 128 columns those are taken whose groups are done first. (us, sequences x heads x keys; 16, 32, 64, 128 columns:
-// 1 x 16 x 4000 18, 22, 23, 29; 1 x 128 x 4000 22, 29, 31, 43; 4 x 128 x 4000 30, 30, 33, 41; 32 x 64 x 4000 65, 55, 45, 46;
-// 32 x 128 x 512 .. 8192 118, 109, 70, 72; 2 x 512 rows of 16 heads x 2500 .. 4600 318, 277, 168, 155.)
+// 64 and 128 columns those are taken whose groups are done first. The constants are times of the kernels' earlier forms, a key's
+// of 256 + 32 values half the others'; as the kernels are (us of graph replays, about 5 of them the graph's; sequences x heads x
+// keys; 16, 32, 64, 128 columns):
+//   512 + 64: 1 x 16 x 4000 23, 26, 26, 32; 1 x 128 x 4000 26, 32, 35, 47; 4 x 128 x 4000 32, 32, 37, 46; 32 x 64 x 4000 59, 54,
+//   49, 50; 32 x 128 x 512 .. 8192 138, 97, 70, 72; 2 x 512 rows of 16 heads x 2500, 4600 322, 241, 164, 150; the last two with
+//   a window of 1000 54, 47, 39, 47 and 124, 98, 65, 74.
+//   256 + 32: 18, 22, 22, 29; 21, 27, 27, 38; 24, 31, 30, 36; 34, 34, 34, 37; 58, 47, 46, 46; 130, 105, 99, 93; 35, 30, 29, 32
+//   and 53, 42, 40, 50.
+// Of 38 shapes the columns taken are within 10% of the best, but for drafts of 24 x 3 to 5 rows: of 16 heads x 4000 keys 73
+// (16 columns) for 47 (64), and 256 + 32 values, 32 heads, a window of 1000 34 (16) for 29 (32).
 //
 // Rows of a tile that belong to two slots take two passes over keys, one after the other. So tiles are cut where slots change,
 // which a group looks for among up to kCutRows rows; of more rows, and in 16 columns, a tile has no more than a fourth of those
-// that stand together. (24 sequences of up to 5 rows, 32 heads, 1000 .. 9001 keys: 62 us, with a row a tile 71; 4 heads, 4000
-// keys: 36 and 43; 16 heads with two to five rows a tile and no cuts 82.)
+// that stand together. (24 sequences of 3 to 5 rows, 32 heads, 1000 .. 9001 keys: 73 us, with a row a tile 98; 4 heads, 4000
+// keys: 43 and 70.)
 Plan plan(const ts_latent_args *k) {
     const ts_rows_args *a = &k->rows;
     constexpr double kStart[2][4] = {{19, 22, 29, 40}, {14.5, 19.5, 20, 29}};                // us (512 + 64 values; 256 + 32)
@@ -936,7 +944,8 @@ extern "C" int tessera_hip_attend_latent(const ts_latent_args *k, void *stream) 
     const size_t partials = partial_bytes(k, s), need = partials + share_bytes(s);
     if (need && (!a->workspace || a->workspace_bytes < need || !ts::aligned(a->workspace, 16)))
         return ts::fail(TS_ERR_WORKSPACE, "attend_latent: workspace of %zu bytes, 16-byte aligned, needed", need);
-    const uint64_t of = (uint64_t)a->rows * a->heads * 2, held = a->kept_table ? (uint64_t)k->pages * a->page : (uint64_t)k->slot_count * a->keys;
+    const uint64_t of = (uint64_t)a->rows * a->heads * 2;
+    const uint64_t held = a->kept_table ? (uint64_t)k->pages * a->page : (uint64_t)k->slot_count * a->keys;
     const int over = ts::outputs_apart("attend_latent", {{"out", a->out, of * k->rank}},
                                        {{"q", a->q, of * a->width},
                                         {"kept", a->k, held * a->width * 2},

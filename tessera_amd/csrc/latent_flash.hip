@@ -12,7 +12,9 @@
 // and tiles of a head shared an XCD, 117 with a step's loads before its products); one of 16384 rows 1000 TFLOP/s. The
 // matrix unit is busy for 50% of the cycles and the vector unit for 47%, at the clock of 1.7 GHz that the card then keeps; LDS
 // for a quarter. Small grids are bound by a wave's steps in turn, some 1.4 us each (5 sequences of up to 900 rows, 5 heads of
-// 64 + 32 and 64 values: 25 us; one prompt of 2048 rows and 8 heads 46 us).
+// 64 + 32 and 64 values: 25 us; one prompt of 2048 rows and 8 heads 46 us). Weights enter their product in one bf16 part: two bring
+// the error against 64 bits (2-norm) from 2.1e-3 (2.3e-3 with 64 values) to the output's own rounding, 1.6e-3, and take the 4
+// prompts from 108 to 134 us, the 5 sequences from 28 to 31 (graph replays).
 #include "latent.h"
 #include "places.h"
 

@@ -667,7 +667,7 @@ def _rows_of(what, name, t, on, dtype, heads=None):
 
 def append_latent(c, kept, slots, positions, *, keys, rank, gain=None, angles=None, halves=True, eps=1e-6, q=None,
                   q_out=None, c_out=None, r_out=None, table=None, kept_pages=0, page=16, status=None):
-    """New rows of latent attention: c [rows, rank + rope] (f32 or bf16; rows any distance apart), its latent through
+    """New rows of latent attention: c [rows, rank + rope] (f32 or bf16; rows a row or more apart), its latent through
     RmsNorm (with `gain` [rank]) and its last `rope` values through the rotation (with `angles`, rope_table's of width
     `rope`, at least `keys` positions, or any scaled ones of its shape) into kept [*, rank + rope] bf16. q [rows, heads,
     rope] (a view of wider heads serves) is rotated to q_out (a view too, f32 or bf16; made in q's type if not given).
@@ -727,8 +727,8 @@ def append_latent(c, kept, slots, positions, *, keys, rank, gain=None, angles=No
 
 def linear_heads(x, w, *, out=None, out_dtype=torch.float32):
     """A product a head: out[r, h] = w[h] x[r, h]. x [rows, heads, k] f32 or bf16 and out [rows, heads, n] f32 or bf16
-    may be views of wider rows and heads; w [heads, n, k] bf16, heads any distance apart. (q into the latent space with
-    w [heads, rank, nope], latent sums out of it with w [heads, value, rank].)"""
+    may be views of wider rows and heads (no two of out's pieces meet); w [heads, n, k] bf16, heads n k or more apart. (q
+    into the latent space with w [heads, rank, nope], latent sums out of it with w [heads, value, rank].)"""
     what = "linear_heads"
     on, dtype = x.get_device(), x.dtype
     rows, heads, k = x.shape
@@ -799,7 +799,7 @@ def attend_latent(q, kept, slots, positions, *, keys, rank, scale, table=None, k
 def flash_latent(q, k, v, r, *, scale, first=None, key_first=None, back=abi.U32_MAX, out=None):
     """The expanded form of latent attention over whole sequences packed back to back, causal, ends aligned (a row of a
     sequence of n rows and m keys stands at m - n + its number) and with a window of `back` keys before its own: q [rows,
-    heads, nope + rope] bf16 (rows any distance apart), k [keys, heads, nope] and v [keys, heads, value] bf16 (views of
+    heads, nope + rope] bf16 (rows a row or more apart, or one broadcast row), k [keys, heads, nope] and v [keys, heads, value] bf16 (views of
     one product's rows serve), r [keys, rope] bf16: the keys' rotated part, all heads'. first [seqs + 1]: each sequence's
     first row, then the end (None: one sequence); key_first: the same of the keys (None: first's). Returns out [rows,
     heads, value] bf16; rows outside the sequences are left as they were, rows that see no key are zero."""
